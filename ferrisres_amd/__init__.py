@@ -23,6 +23,8 @@ GEMV_SPLIT_AUTO, GEMV_SPLIT_ALWAYS, GEMV_SPLIT_NEVER = 0, 1, 2
 FFN_AUTO, FFN_ONE_LAUNCH, FFN_TWO_LAUNCH = 0, 1, 2
 MOE_TERNARY_MOE_LAYER, MOE_CPU_MOE_LAYER = 0, 1
 QUANT_ABSMEAN, QUANT_STE = 0, 1
+FP8_E4M3, FP8_E5M2 = 0, 1
+FP8_ROWS, FP8_COLS, FP8_TILES, FP8_TILES_T = 0, 1, 2, 3
 
 _STATUS = {
     0: "Ok", 1: "Gpu", 2: "Shape", 3: "Device", 4: "Shader", 5: "OOM", 6: "Unsupported",
@@ -47,6 +49,14 @@ class MoeLora(ctypes.Structure):
                 ("a_gate", ctypes.c_void_p), ("b_gate", ctypes.c_void_p),
                 ("a_up", ctypes.c_void_p), ("b_up", ctypes.c_void_p),
                 ("a_down", ctypes.c_void_p), ("b_down", ctypes.c_void_p)]
+
+
+class _MoeRowsC(ctypes.Structure):
+    """frx_moe_rows (include/frx_ternary.h)."""
+    _fields_ = [("T", ctypes.c_uint32), ("top_k", ctypes.c_uint32), ("E", ctypes.c_uint32),
+                ("align", ctypes.c_uint32), ("R", ctypes.c_uint32), ("offsets", ctypes.c_void_p),
+                ("row_of", ctypes.c_void_p), ("slot_of", ctypes.c_void_p)]
+
 
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _f32p = ctypes.POINTER(ctypes.c_float)
@@ -95,6 +105,18 @@ _SIGS = {
     "frx_dequantize_ternary_blocked": (_int, [_vp, _vp, _vp, _sz, _u32, _vp]),
     "frx_prune_sparse24": (_int, [_vp, _vp, _int, _u32, _u32, _int, _vp, _vp, _vp, _vp]),
     "frx_ternary_linear_group": (_int, [_vp, _vp, _int, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _int]),
+    "frx_fp8_quantize": (_int, [_vp, _vp, _int, _u32, _u32, _sz, _int, _int, _vp, _sz, _vp]),
+    "frx_fp8_linear": (_int, [_vp, _vp, _sz, _int, _vp, _vp, _sz, _vp, _u32, _vp, _int, _u32, _u32, _u32]),
+    "frx_fp8_linear_act": (_int, [_vp, _vp, _int, _vp, _sz, _vp, _vp, _int, _u32, _u32, _u32]),
+    "frx_fp8_linear_grouped": (_int, [_vp, _vp, _sz, _int, _vp, _vp, _sz, _vp, _vp, _u32, _vp, _int, _u32, _u32,
+                                      _u32]),
+    "frx_fp8_grad_weight_grouped": (_int, [_vp, _vp, _sz, _int, _vp, _vp, _sz, _vp, _vp, _u32, _vp, _int, _u32, _u32,
+                                           _u32]),
+    "frx_moe_rows_capacity": (_sz, [_u32, _u32, _u32, _u32]),
+    "frx_moe_sort": (_int, [_vp, _vp, _vp]),
+    "frx_moe_dispatch": (_int, [_vp, _vp, _sz, _vp, _vp]),
+    "frx_moe_combine": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _int, _u32]),
+    "frx_moe_combine_backward": (_int, [_vp, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _u32]),
     "frx_set_gemv_split": (_int, [_vp, _int]),
     "frx_workspace_stats": (_int, [_vp, ctypes.POINTER(_sz), ctypes.POINTER(_sz), ctypes.POINTER(_u32)]),
     "frx_release_retired": (_int, [_vp]),
@@ -268,6 +290,94 @@ def _ptr(t):
     if isinstance(t, int):
         return _vp(t)
     return _vp(t.data_ptr())
+
+
+def _fp8_code(t) -> int:
+    import torch
+    if t.dtype == torch.float8_e4m3fn:
+        return FP8_E4M3
+    if t.dtype == torch.float8_e5m2:
+        return FP8_E5M2
+    raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2, got {t.dtype}")
+
+
+def _rows2(t, name):
+    """(rows, columns, row stride in elements) of a 2-D tensor with unit
+    column stride."""
+    if t.dim() != 2:
+        raise _shape_err(f"{name} must be 2-D, got shape {tuple(t.shape)}")
+    m, n = t.shape
+    if n > 1 and t.stride(1) != 1:
+        raise _shape_err(f"{name} must have unit column stride, got strides {t.stride()}")
+    return m, n, t.stride(0) if m > 1 else max(t.stride(0), n)
+
+
+def _dense(t, shape, dtype, name):
+    """The tensor is contiguous and has this shape and dtype (None: any)."""
+    if tuple(t.shape) != tuple(shape):
+        raise _shape_err(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise _shape_err(f"{name} must be contiguous")
+
+
+def _per_expert(ts, E, shape, dtype, name, rows=False):
+    """(array of E device addresses, row stride) of a stacked tensor [E, ...]
+    or a list of E tensors; rows: 2-D with unit column stride, all of one row
+    stride, else contiguous."""
+    if len(ts) != E:
+        raise _shape_err(f"{name} holds {len(ts)} experts, expected {E}")
+    stacked = hasattr(ts, "dim")
+    each = [ts[0]] if stacked else ts
+    ld = None
+    for t in each:
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if rows:
+            m, n, stride = _rows2(t, name)
+            if (m, n) != tuple(shape):
+                raise _shape_err(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+            if ld not in (None, stride):
+                raise _shape_err(f"{name}: the experts' row strides differ")
+            ld = stride
+        else:
+            _dense(t, shape, dtype, name)
+    if stacked:
+        base, step = ts.data_ptr(), ts.stride(0) * ts.element_size()
+        return (_vp * E)(*[base + e * step for e in range(E)]), ld
+    return (_vp * E)(*[t.data_ptr() for t in ts]), ld
+
+
+class MoeRows:
+    """frx_moe_rows over int32 device tensors: offsets [E + 1], row_of [T]
+    [top_k] and slot_of [R], filled by Context.moe_sort (-1 for none). The
+    rows there is room for, R, are at least MoeRows.capacity(...)."""
+
+    def __init__(self, E: int, align: int, offsets, row_of, slot_of):
+        import torch
+        if row_of.dim() != 2:
+            raise _shape_err(f"row_of must be 2-D, got shape {tuple(row_of.shape)}")
+        self.T, self.top_k = (int(d) for d in row_of.shape)
+        self.E, self.align, self.R = int(E), int(align), int(slot_of.numel())
+        _dense(offsets, (self.E + 1,), torch.int32, "offsets")
+        _dense(row_of, (self.T, self.top_k), torch.int32, "row_of")
+        _dense(slot_of, (self.R,), torch.int32, "slot_of")
+        self.offsets, self.row_of, self.slot_of = offsets, row_of, slot_of
+        self._c = _MoeRowsC(self.T, self.top_k, self.E, self.align, self.R, offsets.data_ptr(), row_of.data_ptr(),
+                            slot_of.data_ptr())
+        self._p = ctypes.addressof(self._c)
+
+    @staticmethod
+    def capacity(T: int, top_k: int, E: int, align: int = 1) -> int:
+        return int(lib().frx_moe_rows_capacity(T, top_k, E, align))
+
+    @classmethod
+    def empty(cls, T: int, top_k: int, E: int, align: int = 1, device="cuda:0"):
+        """Rows for T tokens of top_k routes, on newly allocated tensors."""
+        import torch
+        new = lambda *s: torch.empty(s, dtype=torch.int32, device=device)  # noqa: E731
+        return cls(E, align, new(E + 1), new(T, top_k), new(cls.capacity(T, top_k, E, align)))
 
 
 class DeviceBuffer:
@@ -528,6 +638,149 @@ class Context:
         _check(lib().frx_prune_sparse24(self._h, _ptr(w), _dtype_code(w), N, K, int(per_row), _ptr(patterns),
                                         _ptr(signs), _ptr(meta), _ptr(scale)), self._h)
         return patterns, signs, meta, scale
+
+    # 8-bit floating-point linears; codes are float8 tensors.
+    def fp8_quantize(self, x, blocks: int, q, scale):
+        """frx_fp8_quantize: codes (q's dtype) and scales of x [M][K] (f32 or
+        bf16, any row stride) in blocks FP8_ROWS, FP8_COLS, FP8_TILES or
+        FP8_TILES_T. q [M][K] (COLS, TILES_T: [K][M]) with its columns rounded
+        up to a multiple of 16, any row stride that is one too."""
+        import torch
+        M, K, ldx = _rows2(x, "x")
+        turned = blocks in (FP8_COLS, FP8_TILES_T)
+        r, c = (K, M) if turned else (M, K)
+        qr, qc, ldq = _rows2(q, "q")
+        if (qr, qc) != (r, (c + 15) // 16 * 16):
+            raise _shape_err(f"q has shape {tuple(q.shape)}, expected {(r, (c + 15) // 16 * 16)}")
+        sr = (r + 127) // 128 if blocks in (FP8_TILES, FP8_TILES_T) else r
+        _dense(scale, (sr, (c + 127) // 128), torch.float32, "scale")
+        _check(lib().frx_fp8_quantize(self._h, x.data_ptr(), _dtype_code(x), M, K, ldx, blocks, _fp8_code(q),
+                                      q.data_ptr(), ldq, scale.data_ptr()), self._h)
+        return q, scale
+
+    def fp8_linear(self, a, sa, b, sb, y):
+        """frx_fp8_linear: y [M][N] = a b^T with block scales. a [M][K] codes,
+        sa [M][ceil(K/128)]; b [N][K] e4m3 codes, sb [ceil(N/128)] or [N] rows
+        of ceil(K/128) scales."""
+        import torch
+        M, K, lda = _rows2(a, "a")
+        N, kb_, ldb = _rows2(b, "b")
+        if kb_ != K:
+            raise _shape_err(f"b has {kb_} columns, a {K}")
+        if b.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"b must be float8_e4m3fn, got {b.dtype}")
+        kb = (K + 127) // 128
+        _dense(sa, (M, kb), torch.float32, "sa")
+        b_rows = 1 if sb.shape[0] == N else 128
+        _dense(sb, (N if b_rows == 1 else (N + 127) // 128, kb), torch.float32, "sb")
+        _dense(y, (M, N), None, "y")
+        _check(lib().frx_fp8_linear(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(), b.data_ptr(), ldb,
+                                    sb.data_ptr(), b_rows, y.data_ptr(), _dtype_code(y), M, K, N), self._h)
+        return y
+
+    def fp8_linear_act(self, x, b, sb, y):
+        """frx_fp8_linear_act: y = x w^T for f32 or bf16 x [M][K], quantised on
+        the way, and FP8_TILES weights b [N][K], sb [ceil(N/128)][ceil(K/128)]."""
+        import torch
+        M, K = x.shape
+        N, kb_, ldb = _rows2(b, "b")
+        if kb_ != K:
+            raise _shape_err(f"b has {kb_} columns, x {K}")
+        if b.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"b must be float8_e4m3fn, got {b.dtype}")
+        _dense(x, (M, K), None, "x")
+        _dense(sb, ((N + 127) // 128, (K + 127) // 128), torch.float32, "sb")
+        _dense(y, (M, N), None, "y")
+        _check(lib().frx_fp8_linear_act(self._h, x.data_ptr(), _dtype_code(x), b.data_ptr(), ldb, sb.data_ptr(),
+                                        y.data_ptr(), _dtype_code(y), M, K, N), self._h)
+        return y
+
+    def fp8_linear_grouped(self, a, sa, b, sb, offsets, y):
+        """frx_fp8_linear_grouped: rows offsets[e] to offsets[e + 1] of a [R][K]
+        times expert e's codes b[e] [N][K], sb[e] [ceil(N/128)][ceil(K/128)]
+        (stacked tensors, or lists of E)."""
+        import torch
+        R, K, lda = _rows2(a, "a")
+        E, kb = int(offsets.numel()) - 1, (K + 127) // 128
+        N = int(y.shape[1]) if y.dim() == 2 else 0
+        _dense(offsets, (E + 1,), torch.int32, "offsets")
+        _dense(sa, (R, kb), torch.float32, "sa")
+        bp, ldb = _per_expert(b, E, (N, K), torch.float8_e4m3fn, "b", rows=True)
+        sp, _ = _per_expert(sb, E, ((N + 127) // 128, kb), torch.float32, "sb")
+        _dense(y, (R, N), None, "y")
+        _check(lib().frx_fp8_linear_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(), bp, ldb, sp,
+                                            offsets.data_ptr(), E, y.data_ptr(), _dtype_code(y), R, K, N), self._h)
+        return y
+
+    def fp8_grad_weight_grouped(self, a, sa, b, sb, offsets, dw):
+        """frx_fp8_grad_weight_grouped: dw[e] [N][K] = the sum over expert e's
+        rows of dy (a [N][R], FP8_COLS) times x (b [K][R], FP8_COLS)."""
+        import torch
+        N, R, lda = _rows2(a, "a")
+        K, r_, ldb = _rows2(b, "b")
+        if r_ != R:
+            raise _shape_err(f"b has {r_} columns, a {R}")
+        if b.dtype != torch.float8_e4m3fn:
+            raise TypeError(f"b must be float8_e4m3fn, got {b.dtype}")
+        E, rb = int(offsets.numel()) - 1, (R + 127) // 128
+        _dense(offsets, (E + 1,), torch.int32, "offsets")
+        _dense(sa, (N, rb), torch.float32, "sa")
+        _dense(sb, (K, rb), torch.float32, "sb")
+        dp, _ = _per_expert(dw, E, (N, K), dw[0].dtype, "dw")
+        _check(lib().frx_fp8_grad_weight_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
+                                                 b.data_ptr(), ldb, sb.data_ptr(), offsets.data_ptr(), E, dp,
+                                                 _dtype_code(dw[0]), R, N, K), self._h)
+        return dw
+
+    # Tokens sorted by expert, and back.
+    def moe_sort(self, topk_idx, rows: MoeRows):
+        """frx_moe_sort: fills rows from topk_idx [T][top_k] int32 (an index
+        outside [0, E) goes nowhere)."""
+        import torch
+        _dense(topk_idx, (rows.T, rows.top_k), torch.int32, "topk_idx")
+        _check(lib().frx_moe_sort(self._h, topk_idx.data_ptr(), rows._p), self._h)
+        return rows
+
+    def moe_dispatch(self, x, rows: MoeRows, xs):
+        """frx_moe_dispatch: xs [R][...] = each row's token of x [T][...], for
+        rows of any type whose bytes are a multiple of 4."""
+        _dense(x, (rows.T, *x.shape[1:]), None, "x")
+        _dense(xs, (rows.R, *x.shape[1:]), x.dtype, "xs")
+        _check(lib().frx_moe_dispatch(self._h, x.data_ptr(), x.numel() // rows.T * x.element_size(), rows._p,
+                                      xs.data_ptr()), self._h)
+        return xs
+
+    def moe_combine(self, ys, rows: MoeRows, w, y):
+        """frx_moe_combine: y [T][H] = the sum of each token's rows of ys [R]
+        [H], times w [T][top_k] f32 (None: every weight 1)."""
+        import torch
+        H = int(y.shape[-1])
+        _dense(ys, (rows.R, H), None, "ys")
+        _dense(y, (rows.T, H), None, "y")
+        if w is not None:
+            _dense(w, (rows.T, rows.top_k), torch.float32, "w")
+        _check(lib().frx_moe_combine(self._h, ys.data_ptr(), _dtype_code(ys), rows._p, w if w is None else w.data_ptr(),
+                                     y.data_ptr(), _dtype_code(y), H), self._h)
+        return y
+
+    def moe_combine_backward(self, dy, ys, rows: MoeRows, w, dys, dw):
+        """frx_moe_combine_backward: dys [R][H] and dw [T][top_k] f32 of
+        moe_combine for dy [T][H]; ys and dw may both be None, w too."""
+        import torch
+        H = int(dy.shape[-1])
+        _dense(dy, (rows.T, H), None, "dy")
+        _dense(dys, (rows.R, H), None, "dys")
+        if (ys is None) != (dw is None):
+            raise _shape_err("ys and dw come together")
+        if ys is not None:
+            _dense(ys, (rows.R, H), dys.dtype, "ys")
+            _dense(dw, (rows.T, rows.top_k), torch.float32, "dw")
+        if w is not None:
+            _dense(w, (rows.T, rows.top_k), torch.float32, "w")
+        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        _check(lib().frx_moe_combine_backward(self._h, dy.data_ptr(), _dtype_code(dy), ptr(ys), _dtype_code(dys),
+                                              rows._p, ptr(w), dys.data_ptr(), ptr(dw), H), self._h)
+        return dys, dw
 
     def set_gemv_split(self, mode: int):
         """frx_set_gemv_split: GEMV_SPLIT_AUTO, _ALWAYS or _NEVER (the

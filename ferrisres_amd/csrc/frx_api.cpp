@@ -96,6 +96,8 @@ struct frx_ctx {
   size_t xpl_ws_bytes = 0;
   void *spp_ws = nullptr;  // 2:4 metadata in its prepared form (GEMM above a few tokens)
   size_t spp_ws_bytes = 0;
+  void *q8_ws = nullptr;  // 8-bit codes and scales of frx_fp8_linear_act's activations
+  size_t q8_ws_bytes = 0;
   unsigned *sk_cnt = nullptr;  // its per-row-tile arrival counters (zero between launches)
   int gemv_split = FRX_GEMV_SPLIT_AUTO;
   unsigned *ffn_bar = nullptr;  // grid-barrier words of the one-launch FFN
@@ -199,6 +201,7 @@ void frx_destroy(frx_ctx *ctx) {
   if (ctx->gk_ws) (void)hipFree(ctx->gk_ws);
   if (ctx->xpl_ws) (void)hipFree(ctx->xpl_ws);
   if (ctx->spp_ws) (void)hipFree(ctx->spp_ws);
+  if (ctx->q8_ws) (void)hipFree(ctx->q8_ws);
   if (ctx->sk_cnt) (void)hipFree(ctx->sk_cnt);
   if (ctx->ffn_bar) (void)hipFree(ctx->ffn_bar);
   for (void *p : ctx->retired) (void)hipFree(p);
@@ -1500,6 +1503,238 @@ frx_status frx_prune_sparse24(frx_ctx *ctx, const void *w, frx_dtype wt, uint32_
   const hipError_t e = frx::launch_prune_sparse24(w, wt == FRX_BF16, (int)N, (int)K, per_row != 0, patterns, signs,
                                                   meta, scale, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "2:4 prune launch");
+  return FRX_OK;
+}
+
+// ---- 8-bit floating-point linears ---------------------------------------------
+
+static bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+static bool is_dtype(frx_dtype t) { return t == FRX_F32 || t == FRX_BF16; }
+static size_t dtype_bytes(frx_dtype t) { return t == FRX_BF16 ? 2 : 4; }
+constexpr uint32_t kMaxDim = 0x7FFFFF00u;
+// a tile of 256 rows is addressed by 32-bit offsets
+constexpr size_t kMaxCodeLd = (size_t)1 << 23;
+
+frx_status frx_fp8_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t M, uint32_t K, size_t ldx,
+                            frx_fp8_blocks blocks, frx_fp8 code, uint8_t *q, size_t ldq, float *scale) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (!x || !q || !scale) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (M == 0 || K == 0) return fail(ctx, FRX_ERR_SHAPE, "empty shape M=%u K=%u", M, K);
+  if (!is_dtype(xt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (blocks != FRX_FP8_ROWS && blocks != FRX_FP8_COLS && blocks != FRX_FP8_TILES && blocks != FRX_FP8_TILES_T)
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "unknown blocks %d", (int)blocks);
+  if (code != FRX_FP8_E4M3 && code != FRX_FP8_E5M2) return fail(ctx, FRX_ERR_UNSUPPORTED, "unknown code %d", (int)code);
+  if (M > kMaxDim || K > kMaxDim) return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u too large", M, K);
+  if (ldx < K) return fail(ctx, FRX_ERR_SHAPE, "ldx=%zu is less than K=%u", ldx, K);
+  const uint32_t len = blocks == FRX_FP8_COLS || blocks == FRX_FP8_TILES_T ? M : K;
+  if (ldq % 16 != 0 || ldq < len)
+    return fail(ctx, FRX_ERR_SHAPE, "ldq=%zu must be a multiple of 16 that holds %u codes", ldq, len);
+  if (!aligned_to(x, dtype_bytes(xt)) || !aligned_to(q, 16) || !aligned_to(scale, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "x and scale must be aligned to their elements, q to 16 bytes");
+  const size_t kb = (K + 127) / 128, mb = (M + 127) / 128;
+  if ((blocks == FRX_FP8_ROWS ? ((size_t)M * kb + 15) / 16 : kb * mb) > 0x7FFFFFFFu)
+    return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
+  const hipError_t e = frx::launch_fp8_quantize(x, xt == FRX_BF16, M, K, ldx, (int)blocks, code == FRX_FP8_E5M2, q,
+                                                ldq, scale, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp8 quantise launch");
+  return FRX_OK;
+}
+
+// What the three products ask of their operands: rows of a and of b, K columns.
+static frx_status check_fp8(frx_ctx *ctx, const void *a, size_t lda, frx_fp8 at, const void *sa, size_t ldb,
+                            frx_dtype yt, uint32_t M, uint32_t K, uint32_t N) {
+  if (!a || !sa) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (M == 0 || K == 0 || N == 0) return fail(ctx, FRX_ERR_SHAPE, "empty shape M=%u K=%u N=%u", M, K, N);
+  if (at != FRX_FP8_E4M3 && at != FRX_FP8_E5M2) return fail(ctx, FRX_ERR_UNSUPPORTED, "unknown code %d", (int)at);
+  if (!is_dtype(yt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (K % 16 != 0) return fail(ctx, FRX_ERR_SHAPE, "%u columns of codes must be a multiple of 16", K);
+  if (lda % 16 != 0 || ldb % 16 != 0 || lda < K || ldb < K || lda > kMaxCodeLd || ldb > kMaxCodeLd)
+    return fail(ctx, FRX_ERR_SHAPE, "lda=%zu and ldb=%zu must be multiples of 16 from %u to 2^23", lda, ldb, K);
+  if (M > kMaxDim || N > kMaxDim || (size_t)((M + 31) / 32) * ((N + 63) / 64) > 0x3FFFFFFFu)
+    return fail(ctx, FRX_ERR_SHAPE, "M=%u N=%u too large", M, N);
+  if (!aligned_to(a, 16) || !aligned_to(sa, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "codes must be 16-byte aligned, scales 4-byte");
+  return FRX_OK;
+}
+
+// b and y of one product.
+static frx_status check_fp8_side(frx_ctx *ctx, const void *b, const void *sb, const void *y, frx_dtype yt) {
+  if (!b || !sb || !y) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (!aligned_to(b, 16) || !aligned_to(sb, 4) || !aligned_to(y, dtype_bytes(yt)))
+    return fail(ctx, FRX_ERR_SHAPE, "codes must be 16-byte aligned, scales and y aligned to their elements");
+  return FRX_OK;
+}
+
+static frx_status fp8_run(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa, const uint8_t *b,
+                          size_t ldb, const float *sb, uint32_t b_rows, void *y, frx_dtype yt, uint32_t M, uint32_t K,
+                          uint32_t N) {
+  frx::Fp8Plan plan = frx::fp8_plan(M, K, N, ctx->cus);
+  const size_t need = frx::fp8_part_bytes(M, N, plan);
+  if (need && !may_grow(ctx, ctx->gk_ws_bytes, need)) {
+    plan.S = 1;  // a first call under capture: whole K
+    plan.per = (int)((K + 127) / 128);
+  } else if (need) {
+    const frx_status st = ensure_buffer(ctx, &ctx->gk_ws, &ctx->gk_ws_bytes, need, "fp8 split workspace allocation");
+    if (st != FRX_OK) return st;
+  }
+  const hipError_t e = frx::launch_fp8_linear(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, (int)b_rows, y,
+                                              yt == FRX_BF16, M, K, N, plan, reinterpret_cast<float *>(ctx->gk_ws),
+                                              ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp8 linear launch");
+  return FRX_OK;
+}
+
+frx_status frx_fp8_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa, const uint8_t *b,
+                          size_t ldb, const float *sb, uint32_t b_rows, void *y, frx_dtype yt, uint32_t M, uint32_t K,
+                          uint32_t N) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if ((st = check_fp8(ctx, a, lda, at, sa, ldb, yt, M, K, N)) != FRX_OK) return st;
+  if ((st = check_fp8_side(ctx, b, sb, y, yt)) != FRX_OK) return st;
+  if (b_rows != 1 && b_rows != 128) return fail(ctx, FRX_ERR_UNSUPPORTED, "b_rows=%u must be 1 or 128", b_rows);
+  return fp8_run(ctx, a, lda, at, sa, b, ldb, sb, b_rows, y, yt, M, K, N);
+}
+
+frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
+                              const float *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  // x takes the codes' place in the checks; its own alignment is its element's
+  if (!x) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (!is_dtype(xt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (!aligned_to(x, dtype_bytes(xt))) return fail(ctx, FRX_ERR_SHAPE, "x must be aligned to its elements");
+  if ((st = check_fp8(ctx, b, K, FRX_FP8_E4M3, sb, ldb, yt, M, K, N)) != FRX_OK) return st;
+  if ((st = check_fp8_side(ctx, b, sb, y, yt)) != FRX_OK) return st;
+  const size_t kb = (K + 127) / 128, codes = a256((size_t)M * K), need = codes + (size_t)M * kb * 4;
+  if (((size_t)M * kb + 15) / 16 > 0x7FFFFFFFu) return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
+  if (!may_grow(ctx, ctx->q8_ws_bytes, need))
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "the first call at this size allocates and cannot be captured into a graph");
+  if ((st = ensure_buffer(ctx, &ctx->q8_ws, &ctx->q8_ws_bytes, need, "fp8 activation workspace allocation")) != FRX_OK)
+    return st;
+  uint8_t *q = static_cast<uint8_t *>(ctx->q8_ws);
+  float *sa = reinterpret_cast<float *>(q + codes);
+  const hipError_t e = frx::launch_fp8_quantize(x, xt == FRX_BF16, M, K, K, FRX_FP8_ROWS, 0, q, K, sa, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp8 quantise launch");
+  return fp8_run(ctx, q, K, FRX_FP8_E4M3, sa, b, ldb, sb, 128, y, yt, M, K, N);
+}
+
+frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
+                                  const uint8_t *const *b, size_t ldb, const float *const *sb,
+                                  const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R, uint32_t K,
+                                  uint32_t N) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (E == 0 || E > (uint32_t)frx::FP8_MAXE) return fail(ctx, FRX_ERR_SHAPE, "E=%u must be in [1, %d]", E, frx::FP8_MAXE);
+  if (!b || !sb || !offsets) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if ((st = check_fp8(ctx, a, lda, at, sa, ldb, yt, R, K, N)) != FRX_OK) return st;
+  for (uint32_t e = 0; e < E; e++)
+    if ((st = check_fp8_side(ctx, b[e], sb[e], y, yt)) != FRX_OK) return st;
+  if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
+  const hipError_t e = frx::launch_fp8_grouped(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, offsets, (int)E, y,
+                                               yt == FRX_BF16, R, K, N, ctx->cus, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp8 grouped linear launch");
+  return FRX_OK;
+}
+
+frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
+                                       const uint8_t *b, size_t ldb, const float *sb, const uint32_t *offsets,
+                                       uint32_t E, void *const *dw, frx_dtype yt, uint32_t R, uint32_t N, uint32_t K) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (E == 0 || E > (uint32_t)frx::FP8_MAXE) return fail(ctx, FRX_ERR_SHAPE, "E=%u must be in [1, %d]", E, frx::FP8_MAXE);
+  if (!dw || !offsets) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if ((st = check_fp8(ctx, a, lda, at, sa, ldb, yt, N, R, K)) != FRX_OK) return st;
+  for (uint32_t e = 0; e < E; e++)
+    if ((st = check_fp8_side(ctx, b, sb, dw[e], yt)) != FRX_OK) return st;
+  if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
+  const hipError_t e = frx::launch_fp8_grad_weight(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, offsets, (int)E, dw,
+                                                   yt == FRX_BF16, R, N, K, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp8 weight gradient launch");
+  return FRX_OK;
+}
+
+// ---- tokens sorted by expert, and back ------------------------------------------
+
+size_t frx_moe_rows_capacity(uint32_t T, uint32_t top_k, uint32_t E, uint32_t align) {
+  if (align == 0) return 0;
+  const size_t n = (size_t)T * top_k + (size_t)E * (align - 1);
+  return (n + align - 1) / align * align;
+}
+
+static frx_status check_rows(frx_ctx *ctx, const frx_moe_rows *r, frx::RouteRows *out) {
+  if (!r || !r->offsets || !r->row_of || !r->slot_of) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (r->T == 0) return fail(ctx, FRX_ERR_SHAPE, "no tokens");
+  if (r->E == 0 || r->E > 64 || r->top_k == 0 || r->top_k > 64)
+    return fail(ctx, FRX_ERR_SHAPE, "E=%u and top_k=%u must be in [1, 64]", r->E, r->top_k);
+  if (r->align == 0 || r->align > 128 || (r->align & (r->align - 1)))
+    return fail(ctx, FRX_ERR_SHAPE, "align=%u must be a power of two up to 128", r->align);
+  const size_t need = frx_moe_rows_capacity(r->T, r->top_k, r->E, r->align);
+  if (need > 0x3FFFFFFFu || r->R > 0x3FFFFFFFu) return fail(ctx, FRX_ERR_SHAPE, "T=%u R=%u too large", r->T, r->R);
+  if (r->R < need) return fail(ctx, FRX_ERR_SHAPE, "R=%u holds fewer than the %zu rows there may be", r->R, need);
+  if (!aligned_to(r->offsets, 4) || !aligned_to(r->row_of, 4) || !aligned_to(r->slot_of, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "the index arrays must be 4-byte aligned");
+  *out = {(int)r->T, (int)r->top_k, (int)r->E, (int)r->align, (int)r->R, r->offsets, r->row_of, r->slot_of};
+  return FRX_OK;
+}
+
+frx_status frx_moe_sort(frx_ctx *ctx, const uint32_t *topk_idx, const frx_moe_rows *rows) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  frx::RouteRows r;
+  if (!topk_idx || !aligned_to(topk_idx, 4)) return fail(ctx, FRX_ERR_SHAPE, "topk_idx is null or unaligned");
+  if ((st = check_rows(ctx, rows, &r)) != FRX_OK) return st;
+  const hipError_t e = frx::launch_route_sort(topk_idx, r, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "sort launch");
+  return FRX_OK;
+}
+
+frx_status frx_moe_dispatch(frx_ctx *ctx, const void *x, size_t row_bytes, const frx_moe_rows *rows, void *xs) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  frx::RouteRows r;
+  if (!x || !xs) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (row_bytes == 0 || row_bytes % 4 != 0 || row_bytes > ((size_t)1 << 30))
+    return fail(ctx, FRX_ERR_SHAPE, "row_bytes=%zu must be a positive multiple of 4", row_bytes);
+  if (!aligned_to(x, 4) || !aligned_to(xs, 4)) return fail(ctx, FRX_ERR_SHAPE, "x and xs must be 4-byte aligned");
+  if ((st = check_rows(ctx, rows, &r)) != FRX_OK) return st;
+  const hipError_t e = frx::launch_route_dispatch(x, row_bytes, r, xs, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "dispatch launch");
+  return FRX_OK;
+}
+
+frx_status frx_moe_combine(frx_ctx *ctx, const void *ys, frx_dtype st_, const frx_moe_rows *rows, const float *w,
+                           void *y, frx_dtype yt, uint32_t H) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  frx::RouteRows r;
+  if (!ys || !y) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (!is_dtype(st_) || !is_dtype(yt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (H == 0 || H > (1u << 28)) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^28]", H);
+  if (!aligned_to(ys, dtype_bytes(st_)) || !aligned_to(y, dtype_bytes(yt)) || !aligned_to(w, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "ys, y and w must be aligned to their elements");
+  if ((st = check_rows(ctx, rows, &r)) != FRX_OK) return st;
+  const hipError_t e = frx::launch_route_combine(ys, st_ == FRX_BF16, r, w, y, yt == FRX_BF16, H, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "combine launch");
+  return FRX_OK;
+}
+
+frx_status frx_moe_combine_backward(frx_ctx *ctx, const void *dy, frx_dtype dt, const void *ys, frx_dtype st_,
+                                    const frx_moe_rows *rows, const float *w, void *dys, float *dw, uint32_t H) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  frx::RouteRows r;
+  if (!dy || !dys) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (!ys != !dw) return fail(ctx, FRX_ERR_SHAPE, "ys and dw come together");
+  if (!is_dtype(dt) || !is_dtype(st_)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (H == 0 || H > (1u << 28)) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^28]", H);
+  if (!aligned_to(dy, dtype_bytes(dt)) || !aligned_to(ys, dtype_bytes(st_)) || !aligned_to(dys, dtype_bytes(st_)) ||
+      !aligned_to(w, 4) || !aligned_to(dw, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "dy, ys, dys, w and dw must be aligned to their elements");
+  if ((st = check_rows(ctx, rows, &r)) != FRX_OK) return st;
+  const hipError_t e = frx::launch_route_combine_backward(dy, dt == FRX_BF16, ys, st_ == FRX_BF16, r, w, dys, dw, H,
+                                                          ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "combine gradient launch");
   return FRX_OK;
 }
 

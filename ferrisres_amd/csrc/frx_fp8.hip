@@ -1,0 +1,257 @@
+// frx_fp8.hip — launches of the 8-bit floating-point linears (engine: frx_fp8.hpp).
+#include "frx_fp8.hpp"
+
+namespace frx {
+
+namespace {
+
+// Dense product. parts != 0: slice blockIdx.z of K into fp32 part z.
+struct DenseArgs {
+  const uint8_t *a, *b;
+  const float *sa, *sb;
+  void *y;
+  float *part;
+  size_t lda, ldb;
+  uint32_t M, K, N;
+  int per;  // per: blocks of 128 in a slice
+};
+
+// Whether rows of n elements from y on are whole aligned quads.
+template <typename YT>
+__device__ __forceinline__ bool quads(const void *y, uint32_t n) {
+  return ((reinterpret_cast<uintptr_t>(y) & (4 * sizeof(YT) - 1)) | (n & 3)) == 0;
+}
+
+template <bool BR1>
+__device__ __forceinline__ void fill_operands(Fp8Operands &o, const uint8_t *a, size_t lda, const float *sa,
+                                              const uint8_t *b, size_t ldb, const float *sb, uint32_t m0, uint32_t mr,
+                                              uint32_t n0, uint32_t nr, uint32_t K) {
+  const uint32_t kbs = (K + 127) >> 7;
+  o.a = a + (size_t)m0 * lda;
+  o.b = b + (size_t)n0 * ldb;
+  o.sa = sa + (size_t)m0 * kbs;
+  o.sb = sb + (size_t)(BR1 ? n0 : n0 >> 7) * kbs;
+  o.lda = (uint32_t)lda;
+  o.ldb = (uint32_t)ldb;
+  o.sa_ld = o.sb_ld = kbs;
+  o.a_rows = (int)mr;
+  o.b_rows = (int)nr;
+  o.b_first = (int)(n0 & 127);
+  o.K = (int)K;
+}
+
+template <int BM, int BN, int WM, int WN, bool E5M2, bool BR1, typename YT>
+__global__ __launch_bounds__(WM *WN * 64) void fp8_dense_kernel(const DenseArgs p) {
+  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, BR1, sizeof(YT) == 4>;
+  extern __shared__ __align__(16) uint32_t lds[];
+  const uint32_t mts = (p.M + BM - 1) / BM;
+  const uint32_t nt = blockIdx.x / mts, mt = blockIdx.x - nt * mts;
+  const uint32_t m0 = mt * BM, n0 = nt * BN;
+  Fp8Operands o;
+  fill_operands<BR1>(o, p.a, p.lda, p.sa, p.b, p.ldb, p.sb, m0, min((uint32_t)BM, p.M - m0), n0,
+                                   min((uint32_t)BN, p.N - n0), p.K);
+  const int kbs = (int)((p.K + 127) >> 7);
+  o.kb0 = p.part ? (int)blockIdx.z * p.per : 0;
+  o.kb1 = p.part ? min(o.kb0 + p.per, kbs) : kbs;
+  f32x4 acc[Tile::FN][Tile::FM];
+  Tile::run(lds, o, acc);
+  const size_t at = (size_t)m0 * p.N + n0;
+  if (p.part) Tile::template store<float>(acc, p.part + (size_t)blockIdx.z * p.M * p.N + at, p.N, o.a_rows, o.b_rows, (p.N & 3) == 0);
+  else Tile::template store<YT>(acc, (YT *)p.y + at, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
+}
+
+// Rows sorted by expert: blockIdx.x runs over the tiles of all experts (each
+// expert's rows in tiles of their own; workgroups past the last tile end).
+struct GroupArgs {
+  const uint8_t *a;
+  const float *sa;
+  void *y;
+  const uint32_t *offsets;
+  size_t lda, ldb;
+  uint32_t R, K, N;
+  int E;
+  const uint8_t *b[FP8_MAXE];
+  const float *sb[FP8_MAXE];
+};
+
+// Expert e's rows [first, end), kept inside the R rows there are.
+__device__ __forceinline__ void expert_rows(const uint32_t *offsets, int e, uint32_t R, uint32_t &first,
+                                            uint32_t &end) {
+  first = min(offsets[e], R);
+  end = max(min(offsets[e + 1], R), first);
+}
+
+template <int BM, int BN, int WM, int WN, bool E5M2, typename YT>
+__global__ __launch_bounds__(WM *WN * 64) void fp8_grouped_kernel(const GroupArgs p) {
+  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, false, sizeof(YT) == 4>;
+  extern __shared__ __align__(16) uint32_t lds[];
+  const uint32_t nts = (p.N + BN - 1) / BN;
+  const uint32_t mt = blockIdx.x / nts, nt = blockIdx.x - mt * nts;
+  // lane e: expert e's tiles; the expert whose running count passes mt
+  const int lane = threadIdx.x & 63;
+  uint32_t first = 0, end = 0;
+  if (lane < p.E) expert_rows(p.offsets, lane, p.R, first, end);
+  const uint32_t tiles = (end - first + BM - 1) / BM;
+  uint32_t incl = tiles;
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t v = (uint32_t)__shfl_up((int)incl, s);
+    if (lane >= s) incl += v;
+  }
+  const unsigned long long past = __ballot(lane < p.E && incl > mt);
+  if (past == 0) return;
+  const int e = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+  const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(incl - tiles), e);
+  const uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)first, e);
+  const uint32_t z = (uint32_t)__builtin_amdgcn_readlane((int)end, e);
+  const uint32_t m0 = f + (mt - before) * BM, n0 = nt * BN;
+  Fp8Operands o;
+  fill_operands<false>(o, p.a, p.lda, p.sa, p.b[e], p.ldb, p.sb[e], m0, min((uint32_t)BM, z - m0), n0,
+                                     min((uint32_t)BN, p.N - n0), p.K);
+  o.kb0 = 0;
+  o.kb1 = (int)((p.K + 127) >> 7);
+  f32x4 acc[Tile::FN][Tile::FM];
+  Tile::run(lds, o, acc);
+  const size_t at = (size_t)m0 * p.N + n0;
+  Tile::template store<YT>(acc, (YT *)p.y + at, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
+}
+
+// Weight gradients: expert blockIdx.z sums over the blocks of its rows. Here
+// the engine's tokens are dw's rows (dy's columns) and its weight rows x's
+// columns.
+struct GradArgs {
+  const uint8_t *a, *b;
+  const float *sa, *sb;
+  const uint32_t *offsets;
+  size_t lda, ldb;
+  uint32_t R, N, K;
+  void *dw[FP8_MAXE];
+};
+
+template <int BM, int BN, int WM, int WN, bool E5M2, typename YT>
+__global__ __launch_bounds__(WM *WN * 64) void fp8_grad_kernel(const GradArgs p) {
+  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, true, sizeof(YT) == 4>;
+  extern __shared__ __align__(16) uint32_t lds[];
+  const uint32_t mts = (p.N + BM - 1) / BM;
+  const uint32_t nt = blockIdx.x / mts, mt = blockIdx.x - nt * mts;
+  const uint32_t m0 = mt * BM, n0 = nt * BN;
+  const int e = blockIdx.y;
+  uint32_t first, end;
+  expert_rows(p.offsets, e, p.R, first, end);
+  Fp8Operands o;
+  fill_operands<true>(o, p.a, p.lda, p.sa, p.b, p.ldb, p.sb, m0, min((uint32_t)BM, p.N - m0), n0,
+                                    min((uint32_t)BN, p.K - n0), p.R);
+  o.kb0 = (int)(first >> 7);
+  o.kb1 = (int)((end + 127) >> 7);
+  f32x4 acc[Tile::FN][Tile::FM];
+  Tile::run(lds, o, acc);
+  const size_t at = (size_t)m0 * p.K + n0;
+  YT *dw = static_cast<YT *>(p.dw[e]);
+  Tile::template store<YT>(acc, dw + at, p.K, o.a_rows, o.b_rows, quads<YT>(dw, p.K));
+}
+
+// y = the parts added in order.
+template <typename YT>
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float *__restrict__ part, int S, size_t n,
+                                                       YT *__restrict__ y) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float v = part[i];
+  for (int s = 1; s < S; s++) v += part[(size_t)s * n + i];
+  if constexpr (sizeof(YT) == 4) y[i] = v;
+  else y[i] = (uint16_t)bf16_rne_nb(v);
+}
+
+template <typename K, typename A>
+hipError_t go(K kernel, int lds, std::atomic<uint64_t> &done, dim3 grid, int nt, hipStream_t stream, const A &args) {
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), lds, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, grid, dim3(nt), lds, stream, args);
+  return hipGetLastError();
+}
+
+template <int BM, int BN, int WM, int WN, bool E5M2, bool BR1, typename YT>
+hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, BR1, sizeof(YT) == 4>;
+  const size_t tiles = (size_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  return go(fp8_dense_kernel<BM, BN, WM, WN, E5M2, BR1, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, 1, S),
+            Tile::NT, stream, p);
+}
+
+template <bool E5M2, bool BR1, typename YT>
+hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
+  return dense_go<128, 128, 2, 2, E5M2, BR1, YT>(p, S, stream);
+}
+
+// fn<E5M2, BR1 or none, YT>(args) for run-time choices of them.
+template <typename YT>
+hipError_t dense_any(int e5m2, int b_rows, int tile, const DenseArgs &p, int S, hipStream_t stream) {
+  if (b_rows == 1) return e5m2 ? dense_tile<true, true, YT>(tile, p, S, stream) : dense_tile<false, true, YT>(tile, p, S, stream);
+  return e5m2 ? dense_tile<true, false, YT>(tile, p, S, stream) : dense_tile<false, false, YT>(tile, p, S, stream);
+}
+
+template <int BM, int BN, bool E5M2, typename YT>
+hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  using Tile = Fp8Tile<BM, BN, 2, 2, E5M2, false, sizeof(YT) == 4>;
+  const size_t tiles = ((size_t)(p.R + BM - 1) / BM + p.E) * ((p.N + BN - 1) / BN);
+  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  return go(fp8_grouped_kernel<BM, BN, 2, 2, E5M2, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles), Tile::NT, stream,
+            p);
+}
+
+template <int BM, int BN, bool E5M2, typename YT>
+hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  using Tile = Fp8Tile<BM, BN, 2, 2, E5M2, true, sizeof(YT) == 4>;
+  const size_t tiles = (size_t)((p.N + BM - 1) / BM) * ((p.K + BN - 1) / BN);
+  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  return go(fp8_grad_kernel<BM, BN, 2, 2, E5M2, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, (unsigned)E),
+            Tile::NT, stream, p);
+}
+
+}  // namespace
+
+Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
+  return {FP8_T_128, 1, (int)((K + 127) / 128)};
+}
+
+size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p) { return p.S > 1 ? (size_t)p.S * M * N * 4 : 0; }
+
+hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
+                             const float *sb, int b_rows, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
+                             const Fp8Plan &plan, float *part, hipStream_t stream) {
+  const DenseArgs p = {a, b, sa, sb, y, plan.S > 1 ? part : nullptr, lda, ldb, M, K, N, plan.per};
+  const hipError_t e = yt_bf16 ? dense_any<uint16_t>(e5m2, b_rows, plan.tile, p, plan.S, stream)
+                               : dense_any<float>(e5m2, b_rows, plan.tile, p, plan.S, stream);
+  if (e != hipSuccess || plan.S == 1) return e;
+  const size_t n = (size_t)M * N;
+  const dim3 grid((unsigned)((n + 255) / 256));
+  if (yt_bf16) hipLaunchKernelGGL(fp8_join_kernel<uint16_t>, grid, dim3(256), 0, stream, part, plan.S, n, (uint16_t *)y);
+  else hipLaunchKernelGGL(fp8_join_kernel<float>, grid, dim3(256), 0, stream, part, plan.S, n, (float *)y);
+  return hipGetLastError();
+}
+
+hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *const *b,
+                              size_t ldb, const float *const *sb, const uint32_t *offsets, int E, void *y,
+                              int yt_bf16, uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream) {
+  GroupArgs p = {a, sa, y, offsets, lda, ldb, R, K, N, E, {}, {}};
+  for (int e = 0; e < E; e++) {
+    p.b[e] = b[e];
+    p.sb[e] = sb[e];
+  }
+  if (yt_bf16) return e5m2 ? grouped_go<64, 128, true, uint16_t>(p, stream) : grouped_go<64, 128, false, uint16_t>(p, stream);
+  return e5m2 ? grouped_go<64, 128, true, float>(p, stream) : grouped_go<64, 128, false, float>(p, stream);
+}
+
+hipError_t launch_fp8_grad_weight(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b,
+                                  size_t ldb, const float *sb, const uint32_t *offsets, int E, void *const *dw,
+                                  int yt_bf16, uint32_t R, uint32_t N, uint32_t K, hipStream_t stream) {
+  GradArgs p = {a, b, sa, sb, offsets, lda, ldb, R, N, K, {}};
+  for (int e = 0; e < E; e++) p.dw[e] = dw[e];
+  if (yt_bf16) return e5m2 ? grad_go<128, 128, true, uint16_t>(p, E, stream) : grad_go<128, 128, false, uint16_t>(p, E, stream);
+  return e5m2 ? grad_go<128, 128, true, float>(p, E, stream) : grad_go<128, 128, false, float>(p, E, stream);
+}
+
+}  // namespace frx

@@ -336,4 +336,41 @@ hipError_t launch_moe(const void *x, int xt_bf16, const void *router,
                       uint32_t *topk_idx, float *topk_w, const MoeWorkspace &ws,
                       int routing, const MoeLora &lora, hipStream_t stream);
 
+// ---- 8-bit floating-point linears (frx_fp8.hip, frx_fp8_quant.hip) ----------
+constexpr int FP8_MAXE = 64;
+enum { FRXQ_ROWS = 0, FRXQ_COLS = 1, FRXQ_TILES = 2, FRXQ_TILES_T = 3 };  // frx_fp8_blocks
+// blocks: frx_fp8_blocks; e5m2: 0 e4m3, 1 e5m2
+hipError_t launch_fp8_quantize(const void *x, int xt_bf16, uint32_t M, uint32_t K, size_t ldx, int blocks, int e5m2,
+                               uint8_t *q, size_t ldq, float *scale, hipStream_t stream);
+// y = a b^T with block scales (frx_fp8_linear). S > 1: K in S slices of `per`
+// blocks of 128, fp32 parts [S][M][N] in part, added in order.
+struct Fp8Plan {
+  int tile;     // FP8_T_*
+  int S, per;   // K slices, blocks of 128 in each
+};
+enum { FP8_T_256 = 0, FP8_T_128 = 1, FP8_T_64 = 2, FP8_T_32 = 3 };
+Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int cus);
+size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p);
+hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
+                             const float *sb, int b_rows, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
+                             const Fp8Plan &plan, float *part, hipStream_t stream);
+hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *const *b,
+                              size_t ldb, const float *const *sb, const uint32_t *offsets, int E, void *y,
+                              int yt_bf16, uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream);
+hipError_t launch_fp8_grad_weight(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b,
+                                  size_t ldb, const float *sb, const uint32_t *offsets, int E, void *const *dw,
+                                  int yt_bf16, uint32_t R, uint32_t N, uint32_t K, hipStream_t stream);
+
+// ---- tokens sorted by expert, and back (frx_route.hip) -----------------------
+struct RouteRows {
+  int T, top_k, E, align, R;
+  uint32_t *offsets, *row_of, *slot_of;
+};
+hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, hipStream_t stream);
+hipError_t launch_route_dispatch(const void *x, size_t row_bytes, const RouteRows &r, void *xs, hipStream_t stream);
+hipError_t launch_route_combine(const void *ys, int st_bf16, const RouteRows &r, const float *w, void *y, int yt_bf16,
+                                uint32_t H, hipStream_t stream);
+hipError_t launch_route_combine_backward(const void *dy, int dt_bf16, const void *ys, int st_bf16, const RouteRows &r,
+                                         const float *w, void *dys, float *dw, uint32_t H, hipStream_t stream);
+
 }  // namespace frx

@@ -289,6 +289,149 @@ frx_status frx_moe_ternary_ffn(
     uint32_t H, uint32_t I, uint32_t E, uint32_t top_k, frx_activation act,
     void *y, frx_dtype yt, uint32_t *topk_idx, float *topk_w);
 
+/* ---- 8-bit floating-point linear, a scale for each block of 128 ---------------
+ * No counterpart in the reference. For the layers beside the ternary ones that
+ * keep more than 1.58 bits (attention projections before conversion, the
+ * output head, shared or sensitive experts), and for the training of either.
+ * Codes are OCP e4m3 or e5m2 bytes; every 128 of them along the axis that a
+ * product sums over share one f32 scale, and a code stands for scale * code. */
+typedef enum frx_fp8 {
+  FRX_FP8_E4M3 = 0, /* largest value 448 */
+  FRX_FP8_E5M2 = 1, /* largest value 57344 */
+  FRX_FP8_RANGE_ = 0x7fffffff
+} frx_fp8;
+
+/* Which blocks share a scale, and which way the codes lie (kb = ceil(K / 128),
+ * mb = ceil(M / 128)). */
+typedef enum frx_fp8_blocks {
+  FRX_FP8_ROWS = 0,    /* 1 x 128:   q [M][ldq], scale [M][kb] (activations) */
+  FRX_FP8_COLS = 1,    /* 128 x 1, transposed: q [K][ldq], scale [K][mb] (both operands of
+                          a weight gradient, whose sums run over the tokens) */
+  FRX_FP8_TILES = 2,   /* 128 x 128: q [M][ldq], scale [mb][kb] (weights) */
+  FRX_FP8_TILES_T = 3, /* the codes of FRX_FP8_TILES transposed: q [K][ldq], scale [kb][mb]
+                          (weights in the gradient of the activations) */
+  FRX_FP8_BLOCKS_RANGE_ = 0x7fffffff
+} frx_fp8_blocks;
+
+/* Codes and scales of x [M][K] (f32 or bf16, row stride ldx >= K elements).
+ * For each block: scale = max(amax * f32(1 / top), 2^-126), top = 448 or
+ * 57344; code = the product x * f32(1 / scale) rounded to nearest even. Each
+ * of these is one f32 rounding, so codes and scales are reproducible bit for
+ * bit. amax is the largest magnitude of the block; a NaN or an infinity in
+ * a block becomes its scale (and NaN codes), so that it reaches every product
+ * it belongs to. A block at an edge has fewer values.
+ * ldq: bytes between rows of q, a multiple of 16 and at least the row length
+ * (K; COLS and TILES_T: M) rounded up to 16; the codes from there to that
+ * multiple are written as zeros, which is how a row length of any size enters
+ * frx_fp8_linear. Bytes past it are left as they were. q 16-byte aligned, x
+ * and scale aligned to their elements. M, K >= 1. Stream-ordered, no
+ * allocation. */
+frx_status frx_fp8_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t M, uint32_t K,
+                            size_t ldx, frx_fp8_blocks blocks, frx_fp8 code, uint8_t *q, size_t ldq,
+                            float *scale);
+
+/* y[m][n] = sum_b sa[m][b] * sb[n / b_rows][b] * sum_{k in block b} a[m][k] * b[n][k]
+ *   a [M][lda] codes of type at, sa [M][ceil(K / 128)]; b [N][ldb] e4m3 codes,
+ *   sb [ceil(N / b_rows)][ceil(K / 128)], b_rows = 128 (FRX_FP8_TILES) or 1
+ *   (FRX_FP8_ROWS / _COLS); y [M][N] yt. The three products of a layer:
+ *     y  = x w^T:   a = x ROWS,    b = w TILES
+ *     dx = dy w:    a = dy ROWS,   b = w TILES_T   (M x N times N x K)
+ *     dw = dy^T x:  a = dy COLS,   b = x COLS      (sums over the tokens, rounded
+ *                                  up to 16: the quantiser's zero codes)
+ * Sums in fp32: a block's 128 products on the matrix pipe, then the blocks in
+ * order, each times its two scales; one rounding to yt at the end. Requires
+ * K % 16 == 0, lda and ldb multiples of 16 and >= K, a and b 16-byte aligned,
+ * M, N >= 1; y aligned to its element. Few rows, or few tiles, split K over
+ * workgroups: fp32 parts in a context workspace (allocated on the first call
+ * at a larger size; a call under graph capture that would have to allocate
+ * runs unsplit), added in order. */
+frx_status frx_fp8_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
+                          const uint8_t *b, size_t ldb, const float *sb, uint32_t b_rows, void *y,
+                          frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
+
+/* y = x w^T for activations x [M][K] (f32 or bf16, contiguous): frx_fp8_quantize
+ * (ROWS, e4m3) and frx_fp8_linear (b_rows = 128) in one call, with the codes in
+ * a context workspace (which must be there before a graph capture:
+ * FRX_ERR_UNSUPPORTED otherwise), and the two calls' result bit for bit. */
+frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
+                              const float *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
+
+/* The product over rows sorted by expert (frx_moe_sort): row r of a, of expert
+ * e where offsets[e] <= r < offsets[e + 1], times the codes b[e] (b_rows = 128).
+ *   a [R][lda], sa [R][ceil(K / 128)]; b[e] [N][ldb] e4m3, sb[e] [ceil(N / 128)]
+ *   [ceil(K / 128)] (host arrays of E device pointers); offsets [E + 1] u32 on
+ *   the device, ascending; y [R][N]. Rows from offsets[E] on are neither read
+ *   nor written. 1 <= E <= 64; otherwise as frx_fp8_linear. No allocation. */
+frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
+                                  const uint8_t *const *b, size_t ldb, const float *const *sb,
+                                  const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R,
+                                  uint32_t K, uint32_t N);
+
+/* Gradients of the experts' weights: for each expert e
+ *   dw[e][n][k] = sum over its rows r of dy[r][n] * x[r][k]
+ * from both operands in FRX_FP8_COLS over the sorted rows (blocks of 128 rows):
+ *   a [N][lda] codes of type at (dy), sa [N][ceil(R / 128)]; b [K][ldb] e4m3
+ *   codes (x), sb [K][ceil(R / 128)]; offsets [E + 1] as above, multiples of 128
+ *   (a sort with align = 128); dw[e] [N][K] yt (host array of E device
+ *   pointers; zeros for an expert without rows). R % 16 == 0, 1 <= E <= 64. No
+ *   allocation. */
+frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at,
+                                       const float *sa, const uint8_t *b, size_t ldb, const float *sb,
+                                       const uint32_t *offsets, uint32_t E, void *const *dw, frx_dtype yt,
+                                       uint32_t R, uint32_t N, uint32_t K);
+
+/* ---- tokens sorted by expert, and back ----------------------------------------
+ * What frx_moe_ternary_ffn does inside around its ternary experts, for callers
+ * with experts of another kind, and its gradients. A route is a pair (token t,
+ * choice j), slot t * top_k + j; sorted, each expert's routes are consecutive
+ * rows in the order of their slots, and every expert's segment starts at a
+ * multiple of align rows. */
+typedef struct frx_moe_rows {
+  uint32_t T, top_k, E; /* 1 <= top_k <= 64, 1 <= E <= 64 */
+  uint32_t align;       /* 1 to 128, a power of two */
+  uint32_t R;           /* rows there is room for: at least frx_moe_rows_capacity */
+  uint32_t *offsets;    /* [E + 1] first row of each expert; offsets[E]: the end */
+  uint32_t *row_of;     /* [T][top_k] row of each route; 0xFFFFFFFF: it goes nowhere */
+  uint32_t *slot_of;    /* [R] slot of each row; 0xFFFFFFFF: a row of no route (between
+                           segments, and from offsets[E] on) */
+} frx_moe_rows;
+
+/* T * top_k + E * (align - 1), rounded up to align. */
+size_t frx_moe_rows_capacity(uint32_t T, uint32_t top_k, uint32_t E, uint32_t align);
+
+/* Fills offsets, row_of and slot_of (device arrays) from topk_idx [T][top_k]
+ * u32 (frx_moe_ternary_ffn's layout). An index >= E goes nowhere (a padding
+ * token, a dropped route); an index may occur twice in a token, as two routes.
+ * From a few thousand routes on the counts live in a context workspace (grown
+ * on the first call at a larger size; under graph capture a call that finds
+ * none sorts in one workgroup). */
+frx_status frx_moe_sort(frx_ctx *ctx, const uint32_t *topk_idx, const frx_moe_rows *rows);
+
+/* xs[row_of[t][j]] = x[t] for rows of row_bytes bytes of any type (activations,
+ * or codes, or their scales). Rows of no route before offsets[E] become zeros;
+ * rows from there on are left as they were. x [T] and xs [R] rows, 4-byte
+ * aligned, row_bytes a multiple of 4. Its gradient is frx_moe_combine without
+ * weights. */
+frx_status frx_moe_dispatch(frx_ctx *ctx, const void *x, size_t row_bytes, const frx_moe_rows *rows, void *xs);
+
+/* y[t] = sum_j w[t][j] * ys[row_of[t][j]], in the order of j from 0, each product and
+ * addition one f32 rounding, one rounding to yt at the end; a route that goes
+ * nowhere adds nothing (whatever its weight), a token without routes gets zeros. ys [R][H]
+ * st, y [T][H] yt, w [T][top_k] f32 or NULL (every weight 1). H >= 1. */
+frx_status frx_moe_combine(frx_ctx *ctx, const void *ys, frx_dtype st, const frx_moe_rows *rows,
+                           const float *w, void *y, frx_dtype yt, uint32_t H);
+
+/* The gradients of frx_moe_combine for dy [T][H] (dt):
+ *   dys[row_of[t][j]] = w[t][j] * dy[t]  ([R][H] st; rows of no route as in
+ *                                         frx_moe_dispatch)
+ *   dw[t][j] = sum_h dy[t][h] * ys[row_of[t][j]][h]  ([T][top_k] f32, 0 for a
+ *                                         route that goes nowhere)
+ * ys and dw may both be NULL (no gradient of the weights), w may be NULL
+ * (every weight 1). */
+frx_status frx_moe_combine_backward(frx_ctx *ctx, const void *dy, frx_dtype dt, const void *ys,
+                                    frx_dtype st, const frx_moe_rows *rows, const float *w, void *dys,
+                                    float *dw, uint32_t H);
+
 /* ---- gated pair (first half of the dense FFN) -------------------------------
  * Replaces the gate and up gpu_ternary_matmul_vram calls plus the host
  * activation and product of the dense FFN branch
