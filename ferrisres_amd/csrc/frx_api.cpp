@@ -1606,6 +1606,13 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
   if (!aligned_to(x, dtype_bytes(xt))) return fail(ctx, FRX_ERR_SHAPE, "x must be aligned to its elements");
   if ((st = check_fp8(ctx, b, K, FRX_FP8_E4M3, sb, ldb, yt, M, K, N)) != FRX_OK) return st;
   if ((st = check_fp8_side(ctx, b, sb, y, yt)) != FRX_OK) return st;
+  const frx::Fp8Plan plan = frx::fp8_plan(M, K, N, ctx->cus);
+  if (plan.tile == frx::FP8_T_SKINNY && frx::fp8_act_fits(M, K)) {
+    const hipError_t e = frx::launch_fp8_linear_act(x, xt == FRX_BF16, b, ldb, sb, y, yt == FRX_BF16, M, K, N, plan,
+                                                    ctx->stream);
+    if (e != hipSuccess) return hip_fail(ctx, e, "fp8 linear launch");
+    return FRX_OK;
+  }
   const size_t kb = (K + 127) / 128, codes = a256((size_t)M * K), need = codes + (size_t)M * kb * 4;
   if (((size_t)M * kb + 15) / 16 > 0x7FFFFFFFu) return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
   if (!may_grow(ctx, ctx->q8_ws_bytes, need))

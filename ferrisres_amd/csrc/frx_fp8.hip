@@ -1,5 +1,5 @@
 // frx_fp8.hip — launches of the 8-bit floating-point linears (engine: frx_fp8.hpp).
-#include "frx_fp8.hpp"
+#include "frx_fp8_skinny.hpp"
 
 namespace frx {
 
@@ -81,31 +81,43 @@ __device__ __forceinline__ void expert_rows(const uint32_t *offsets, int e, uint
   end = max(min(offsets[e + 1], R), first);
 }
 
+// The expert of tile mt when every expert's rows are cut into tiles of BM, and
+// the tile's first row and its expert's last + 1; -1 past the last tile.
+// Lane e counts expert e's tiles; the expert is the first whose running count
+// passes mt.
+template <int BM>
+__device__ __forceinline__ int expert_tile(const uint32_t *offsets, int E, uint32_t R, uint32_t mt, uint32_t &m0,
+                                           uint32_t &end) {
+  const int lane = threadIdx.x & 63;
+  uint32_t first = 0, last = 0;
+  if (lane < E) expert_rows(offsets, lane, R, first, last);
+  const uint32_t tiles = (last - first + BM - 1) / BM;
+  uint32_t incl = tiles;
+  for (int s = 1; s < 64; s <<= 1) {
+    const uint32_t v = (uint32_t)__shfl_up((int)incl, s);
+    if (lane >= s) incl += v;
+  }
+  const unsigned long long past = __ballot(lane < E && incl > mt);
+  if (past == 0) return -1;
+  const int e = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+  const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(incl - tiles), e);
+  m0 = (uint32_t)__builtin_amdgcn_readlane((int)first, e) + (mt - before) * BM;
+  end = (uint32_t)__builtin_amdgcn_readlane((int)last, e);
+  return e;
+}
+
 template <int BM, int BN, int WM, int WN, bool E5M2, typename YT>
 __global__ __launch_bounds__(WM *WN * 64) void fp8_grouped_kernel(const GroupArgs p) {
   using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, false, sizeof(YT) == 4>;
   extern __shared__ __align__(16) uint32_t lds[];
   const uint32_t nts = (p.N + BN - 1) / BN;
   const uint32_t mt = blockIdx.x / nts, nt = blockIdx.x - mt * nts;
-  // lane e: expert e's tiles; the expert whose running count passes mt
-  const int lane = threadIdx.x & 63;
-  uint32_t first = 0, end = 0;
-  if (lane < p.E) expert_rows(p.offsets, lane, p.R, first, end);
-  const uint32_t tiles = (end - first + BM - 1) / BM;
-  uint32_t incl = tiles;
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint32_t v = (uint32_t)__shfl_up((int)incl, s);
-    if (lane >= s) incl += v;
-  }
-  const unsigned long long past = __ballot(lane < p.E && incl > mt);
-  if (past == 0) return;
-  const int e = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
-  const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(incl - tiles), e);
-  const uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)first, e);
-  const uint32_t z = (uint32_t)__builtin_amdgcn_readlane((int)end, e);
-  const uint32_t m0 = f + (mt - before) * BM, n0 = nt * BN;
+  uint32_t m0, end;
+  const int e = expert_tile<BM>(p.offsets, p.E, p.R, mt, m0, end);
+  if (e < 0) return;
+  const uint32_t n0 = nt * BN;
   Fp8Operands o;
-  fill_operands<false>(o, p.a, p.lda, p.sa, p.b[e], p.ldb, p.sb[e], m0, min((uint32_t)BM, z - m0), n0,
+  fill_operands<false>(o, p.a, p.lda, p.sa, p.b[e], p.ldb, p.sb[e], m0, min((uint32_t)BM, end - m0), n0,
                                      min((uint32_t)BN, p.N - n0), p.K);
   o.kb0 = 0;
   o.kb1 = (int)((p.K + 127) >> 7);
@@ -115,7 +127,28 @@ __global__ __launch_bounds__(WM *WN * 64) void fp8_grouped_kernel(const GroupArg
   Tile::template store<YT>(acc, (YT *)p.y + at, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
 }
 
-// Weight gradients: expert blockIdx.z sums over the blocks of its rows. Here
+template <int RT, bool E5M2, bool BR1, typename XT, typename YT>
+__global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_kernel(const Fp8Skinny p) {
+  extern __shared__ __align__(16) uint32_t lds[];
+  fp8_skinny<RT, E5M2, BR1, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
+}
+
+// Sorted rows in tiles of 16 (decode batches: a few rows of each expert).
+template <int RT, bool E5M2, typename YT>
+__global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_grouped_kernel(const GroupArgs p) {
+  extern __shared__ __align__(16) uint32_t lds[];
+  const uint32_t nts = (p.N + 16 * RT - 1) / (16 * RT);
+  const uint32_t mt = blockIdx.x / nts, nt = blockIdx.x - mt * nts;
+  uint32_t m0, end;
+  const int e = expert_tile<16>(p.offsets, p.E, p.R, mt, m0, end);
+  if (e < 0) return;
+  const uint32_t kbs = (p.K + 127) >> 7;
+  const Fp8Skinny q = {p.a + (size_t)m0 * p.lda, p.sa + (size_t)m0 * kbs, p.b[e], p.sb[e],
+                       static_cast<YT *>(p.y) + (size_t)m0 * p.N, p.lda, p.ldb, min(16u, end - m0), p.K, p.N, 0};
+  fp8_skinny<RT, E5M2, false, uint8_t, YT>(q, nt * 16 * RT, reinterpret_cast<f32x4 *>(lds));
+}
+
+// Weight gradients: expert blockIdx.y sums over the blocks of its rows. Here
 // the engine's tokens are dw's rows (dy's columns) and its weight rows x's
 // columns.
 struct GradArgs {
@@ -179,6 +212,32 @@ hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
             Tile::NT, stream, p);
 }
 
+template <int RT, bool E5M2, bool BR1, typename XT, typename YT>
+hipError_t skinny_rt(const Fp8Skinny &p, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int most = (int)fp8_skinny_red_bytes(RT) + (sizeof(XT) == 1 ? 0 : (int)FP8_ACT_MAX_BYTES);
+  const auto kernel = fp8_skinny_kernel<RT, E5M2, BR1, XT, YT>;
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), most, done);
+  if (e != hipSuccess) return e;
+  const size_t lds = fp8_skinny_red_bytes(RT) + (sizeof(XT) == 1 ? 0 : fp8_skinny_act_bytes(p.M, p.K));
+  hipLaunchKernelGGL(kernel, dim3((p.N + 16 * RT - 1) / (16 * RT)), dim3(FP8_SK_WAVES * 64), lds, stream, p);
+  return hipGetLastError();
+}
+
+template <bool E5M2, bool BR1, typename XT, typename YT>
+hipError_t skinny_go(int rt, const Fp8Skinny &p, hipStream_t stream) {
+  if (rt == 4) return skinny_rt<4, E5M2, BR1, XT, YT>(p, stream);
+  if (rt == 3) return skinny_rt<3, E5M2, BR1, XT, YT>(p, stream);
+  if (rt == 2) return skinny_rt<2, E5M2, BR1, XT, YT>(p, stream);
+  return skinny_rt<1, E5M2, BR1, XT, YT>(p, stream);
+}
+
+template <typename YT>
+hipError_t skinny_any(int e5m2, int b_rows, int rt, const Fp8Skinny &p, hipStream_t stream) {
+  if (b_rows == 1) return e5m2 ? skinny_go<true, true, uint8_t, YT>(rt, p, stream) : skinny_go<false, true, uint8_t, YT>(rt, p, stream);
+  return e5m2 ? skinny_go<true, false, uint8_t, YT>(rt, p, stream) : skinny_go<false, false, uint8_t, YT>(rt, p, stream);
+}
+
 template <bool E5M2, bool BR1, typename YT>
 hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
   return dense_go<128, 128, 2, 2, E5M2, BR1, YT>(p, S, stream);
@@ -214,6 +273,20 @@ hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
 }  // namespace
 
 Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
+  if (M <= 16) {
+    // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
+    const uint32_t tiles = (N + 15) / 16;
+    int best = 1;
+    uint32_t least = ~0u;
+    for (int rt = 1; rt <= 4; rt++) {
+      const uint32_t wgs = (tiles + rt - 1) / rt, rounds = (wgs + cus - 1) / cus * rt;
+      if (rounds <= least) {
+        least = rounds;
+        best = rt;
+      }
+    }
+    return {FP8_T_SKINNY, 1, best};
+  }
   return {FP8_T_128, 1, (int)((K + 127) / 128)};
 }
 
@@ -222,6 +295,11 @@ size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p) { return p.S > 1
 hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
                              const float *sb, int b_rows, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
                              const Fp8Plan &plan, float *part, hipStream_t stream) {
+  if (plan.tile == FP8_T_SKINNY) {
+    const Fp8Skinny p = {a, sa, b, sb, y, lda, ldb, M, K, N, 0};
+    return yt_bf16 ? skinny_any<uint16_t>(e5m2, b_rows, plan.per, p, stream)
+                   : skinny_any<float>(e5m2, b_rows, plan.per, p, stream);
+  }
   const DenseArgs p = {a, b, sa, sb, y, plan.S > 1 ? part : nullptr, lda, ldb, M, K, N, plan.per};
   const hipError_t e = yt_bf16 ? dense_any<uint16_t>(e5m2, b_rows, plan.tile, p, plan.S, stream)
                                : dense_any<float>(e5m2, b_rows, plan.tile, p, plan.S, stream);
@@ -233,6 +311,22 @@ hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float
   return hipGetLastError();
 }
 
+bool fp8_act_fits(uint32_t M, uint32_t K) {
+  return M <= FP8_ACT_MAX_M && fp8_skinny_act_bytes(M, K) <= FP8_ACT_MAX_BYTES;
+}
+
+hipError_t launch_fp8_linear_act(const void *x, int xt_bf16, const uint8_t *b, size_t ldb, const float *sb, void *y,
+                                 int yt_bf16, uint32_t M, uint32_t K, uint32_t N, const Fp8Plan &plan,
+                                 hipStream_t stream) {
+  const int vec = ((reinterpret_cast<uintptr_t>(x) | (size_t)K * (xt_bf16 ? 2 : 4)) & 15) == 0;
+  const Fp8Skinny p = {x, nullptr, b, sb, y, K, ldb, M, K, N, vec};
+  if (xt_bf16)
+    return yt_bf16 ? skinny_go<false, false, uint16_t, uint16_t>(plan.per, p, stream)
+                   : skinny_go<false, false, uint16_t, float>(plan.per, p, stream);
+  return yt_bf16 ? skinny_go<false, false, float, uint16_t>(plan.per, p, stream)
+                 : skinny_go<false, false, float, float>(plan.per, p, stream);
+}
+
 hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *const *b,
                               size_t ldb, const float *const *sb, const uint32_t *offsets, int E, void *y,
                               int yt_bf16, uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream) {
@@ -240,6 +334,20 @@ hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const floa
   for (int e = 0; e < E; e++) {
     p.b[e] = b[e];
     p.sb[e] = sb[e];
+  }
+  if (R <= 8u * (uint32_t)E) {
+    const size_t tiles = ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16);
+    if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)tiles), block(FP8_SK_WAVES * 64);
+    constexpr int lds = (int)fp8_skinny_red_bytes(1);
+    if (yt_bf16) {
+      if (e5m2) hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, true, uint16_t>), grid, block, lds, stream, p);
+      else hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, false, uint16_t>), grid, block, lds, stream, p);
+    } else {
+      if (e5m2) hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, true, float>), grid, block, lds, stream, p);
+      else hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, false, float>), grid, block, lds, stream, p);
+    }
+    return hipGetLastError();
   }
   if (yt_bf16) return e5m2 ? grouped_go<64, 128, true, uint16_t>(p, stream) : grouped_go<64, 128, false, uint16_t>(p, stream);
   return e5m2 ? grouped_go<64, 128, true, float>(p, stream) : grouped_go<64, 128, false, float>(p, stream);

@@ -10,53 +10,12 @@
 //
 // Bound by memory: 2 or 4 bytes in and 1 out per value, about 4 VALU ops per
 // value (mask, max, multiply, half a conversion).
-#include "frx_device.hpp"
+#include "frx_fp8_codes.hpp"
 #include "frx_internal.hpp"
 
 namespace frx {
 
 namespace {
-
-constexpr uint32_t kMag = 0x7FFFFFFFu;
-
-template <bool E5M2>
-__device__ __forceinline__ float fp8_scale(uint32_t amax_bits) {
-  const float s = __uint_as_float(amax_bits) * (E5M2 ? 1.0f / 57344.0f : 1.0f / 448.0f);
-  return s < 0x1p-126f ? 0x1p-126f : s;  // a NaN stays
-}
-
-// Four values as four codes (round to nearest even).
-template <bool E5M2>
-__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d) {
-  if constexpr (E5M2) {
-    const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true);
-  } else {
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
-  }
-}
-
-__device__ __forceinline__ float ld1(const float *p) { return *p; }
-__device__ __forceinline__ float ld1(const uint16_t *p) { return bf16_to_f32(*p); }
-
-// Eight consecutive values (16-byte aligned).
-__device__ __forceinline__ void ld8v(const float *p, float (&v)[8]) {
-  const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    v[i] = a[i];
-    v[4 + i] = b[i];
-  }
-}
-__device__ __forceinline__ void ld8v(const uint16_t *p, float (&v)[8]) {
-  const u32x4 a = *reinterpret_cast<const u32x4 *>(p);
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    v[2 * i] = __uint_as_float(a[i] << 16);
-    v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
-  }
-}
 
 // 1 x 128 blocks: 16 lanes a block, 8 values a lane (a wave reads 1 KB of
 // bf16, 2 KB of f32 in a row of x); the 16 lanes agree on amax with four
@@ -77,17 +36,9 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const XT *__restrict__ x,
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = k + i < K ? ld1(src + i) : 0.0f;
   }
-  uint32_t mx = 0;
-#pragma unroll
-  for (int i = 0; i < 8; i++) mx = max(mx, __float_as_uint(v[i]) & kMag);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) mx = max(mx, (uint32_t)__shfl_xor((int)mx, o));
-  const float s = fp8_scale<E5M2>(mx);
-  const float inv = 1.0f / s;
+  u32x2 c;
+  const float s = fp8_block_codes<E5M2>(v, c);
   if (k < ((K + 15) & ~15u)) {
-    u32x2 c;
-    c.x = fp8_pack4<E5M2>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-    c.y = fp8_pack4<E5M2>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
     // a value past K has no code of its block, whatever its scale
     if (k + 8 > K) {
       const uint32_t n = k < K ? K - k : 0;
@@ -143,7 +94,7 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const XT *__restrict__ x,
 #pragma unroll
   for (int i = 0; i < 32; i++)
 #pragma unroll
-    for (int c = 0; c < 2; c++) mx[c] = max(mx[c], __float_as_uint(v[i][c]) & kMag);
+    for (int c = 0; c < 2; c++) mx[c] = max(mx[c], __float_as_uint(v[i][c]) & FP8_MAG);
   if constexpr (BLOCKS == FRXQ_COLS) {
     red[wave][2 * lane] = mx[0];
     red[wave][2 * lane + 1] = mx[1];

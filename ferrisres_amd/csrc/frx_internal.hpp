@@ -346,14 +346,24 @@ hipError_t launch_fp8_quantize(const void *x, int xt_bf16, uint32_t M, uint32_t 
 // blocks of 128, fp32 parts [S][M][N] in part, added in order.
 struct Fp8Plan {
   int tile;     // FP8_T_*
-  int S, per;   // K slices, blocks of 128 in each
+  int S, per;   // K slices, blocks of 128 in each (FP8_T_SKINNY: 1, 16-row tiles of a workgroup)
 };
-enum { FP8_T_256 = 0, FP8_T_128 = 1, FP8_T_64 = 2, FP8_T_32 = 3 };
+enum { FP8_T_256 = 0, FP8_T_128 = 1, FP8_T_64 = 2, FP8_T_32 = 3, FP8_T_SKINNY = 4 };
 Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int cus);
 size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p);
 hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
                              const float *sb, int b_rows, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
                              const Fp8Plan &plan, float *part, hipStream_t stream);
+// x f32 or bf16 [M][K], quantised on the way (FP8_T_SKINNY plans whose
+// activations fit: fp8_act_fits). Every workgroup makes the codes for itself,
+// which pays while they are few (11008 x 4096, us, one launch / quantiser and
+// product: 1 token 13.1 / 14.8, 4 tokens 14.2 / 14.3).
+constexpr uint32_t FP8_ACT_MAX_M = 4;
+constexpr size_t FP8_ACT_MAX_BYTES = 64 << 10;
+bool fp8_act_fits(uint32_t M, uint32_t K);
+hipError_t launch_fp8_linear_act(const void *x, int xt_bf16, const uint8_t *b, size_t ldb, const float *sb, void *y,
+                                 int yt_bf16, uint32_t M, uint32_t K, uint32_t N, const Fp8Plan &plan,
+                                 hipStream_t stream);
 hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *const *b,
                               size_t ldb, const float *const *sb, const uint32_t *offsets, int E, void *y,
                               int yt_bf16, uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream);

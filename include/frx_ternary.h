@@ -350,9 +350,10 @@ frx_status frx_fp8_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at
                           frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
 
 /* y = x w^T for activations x [M][K] (f32 or bf16, contiguous): frx_fp8_quantize
- * (ROWS, e4m3) and frx_fp8_linear (b_rows = 128) in one call, with the codes in
- * a context workspace (which must be there before a graph capture:
- * FRX_ERR_UNSUPPORTED otherwise), and the two calls' result bit for bit. */
+ * (ROWS, e4m3) and frx_fp8_linear (b_rows = 128) in one call, with the two
+ * calls' result bit for bit. Up to 4 tokens (of 16000 columns together) it
+ * is one launch, the codes in LDS; above, they lie in a context workspace (which
+ * must be there before a graph capture: FRX_ERR_UNSUPPORTED otherwise). */
 frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
                               const float *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
 
