@@ -9,6 +9,7 @@ and passes torch device tensors as raw pointers.
 """
 from __future__ import annotations
 
+import array
 import ctypes
 import os
 
@@ -240,11 +241,22 @@ def sparse24_cpu_to_gpu(patterns: np.ndarray, signs: np.ndarray, n: int, k: int)
 
 # ---- device context ----------------------------------------------------------
 
+_torch = None  # the torch module, imported by the first call that takes tensors
+
+
+def _tt():
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    return _torch
+
+
 def _dtype_code(t) -> int:
-    import torch
-    if t.dtype == torch.float32:
+    torch = _torch or _tt()
+    if t.dtype is torch.float32:
         return FRX_F32
-    if t.dtype == torch.bfloat16:
+    if t.dtype is torch.bfloat16:
         return FRX_BF16
     raise TypeError(f"unsupported dtype {t.dtype}")
 
@@ -293,10 +305,10 @@ def _ptr(t):
 
 
 def _fp8_code(t) -> int:
-    import torch
-    if t.dtype == torch.float8_e4m3fn:
+    torch = _torch or _tt()
+    if t.dtype is torch.float8_e4m3fn:
         return FP8_E4M3
-    if t.dtype == torch.float8_e5m2:
+    if t.dtype is torch.float8_e5m2:
         return FP8_E5M2
     raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2, got {t.dtype}")
 
@@ -304,34 +316,46 @@ def _fp8_code(t) -> int:
 def _rows2(t, name):
     """(rows, columns, row stride in elements) of a 2-D tensor with unit
     column stride."""
-    if t.dim() != 2:
+    if len(t.shape) != 2:
         raise _shape_err(f"{name} must be 2-D, got shape {tuple(t.shape)}")
     m, n = t.shape
-    if n > 1 and t.stride(1) != 1:
+    ld, col = t.stride()
+    if n > 1 and col != 1:
         raise _shape_err(f"{name} must have unit column stride, got strides {t.stride()}")
-    return m, n, t.stride(0) if m > 1 else max(t.stride(0), n)
+    return m, n, ld if m > 1 else max(ld, n)
 
 
 def _dense(t, shape, dtype, name):
     """The tensor is contiguous and has this shape and dtype (None: any)."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise _shape_err(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
     if not t.is_contiguous():
         raise _shape_err(f"{name} must be contiguous")
 
 
 def _per_expert(ts, E, shape, dtype, name, rows=False):
-    """(array of E device addresses, row stride) of a stacked tensor [E, ...]
+    """(array.array of E device addresses, row stride) of a stacked tensor [E, ...]
     or a list of E tensors; rows: 2-D with unit column stride, all of one row
     stride, else contiguous."""
     if len(ts) != E:
         raise _shape_err(f"{name} holds {len(ts)} experts, expected {E}")
-    stacked = hasattr(ts, "dim")
-    each = [ts[0]] if stacked else ts
+    if hasattr(ts, "dim"):  # stacked
+        if ts.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {ts.dtype}")
+        if tuple(ts.shape[1:]) != tuple(shape):
+            raise _shape_err(f"{name} has shape {tuple(ts.shape)}, expected {(E, *shape)}")
+        step, ld, col = ts.stride()
+        m, n = shape
+        if (n > 1 and col != 1) or (m > 1 and ld < n) or (not rows and m > 1 and ld != n):
+            raise _shape_err(f"{name} must have {'unit column stride' if rows else 'contiguous experts'}, got strides "
+                             f"{ts.stride()}")
+        base, step = ts.data_ptr(), step * ts.element_size()
+        at = array.array("Q", range(base, base + E * step, step) if step else [base] * E)
+        return at, ld if m > 1 else max(ld, n)
     ld = None
-    for t in each:
+    for t in ts:
         if t.dtype != dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
         if rows:
@@ -343,10 +367,7 @@ def _per_expert(ts, E, shape, dtype, name, rows=False):
             ld = stride
         else:
             _dense(t, shape, dtype, name)
-    if stacked:
-        base, step = ts.data_ptr(), ts.stride(0) * ts.element_size()
-        return (_vp * E)(*[base + e * step for e in range(E)]), ld
-    return (_vp * E)(*[t.data_ptr() for t in ts]), ld
+    return array.array("Q", [t.data_ptr() for t in ts]), ld
 
 
 class MoeRows:
@@ -645,7 +666,7 @@ class Context:
         bf16, any row stride) in blocks FP8_ROWS, FP8_COLS, FP8_TILES or
         FP8_TILES_T. q [M][K] (COLS, TILES_T: [K][M]) with its columns rounded
         up to a multiple of 16, any row stride that is one too."""
-        import torch
+        torch = _torch or _tt()
         M, K, ldx = _rows2(x, "x")
         turned = blocks in (FP8_COLS, FP8_TILES_T)
         r, c = (K, M) if turned else (M, K)
@@ -662,7 +683,7 @@ class Context:
         """frx_fp8_linear: y [M][N] = a b^T with block scales. a [M][K] codes,
         sa [M][ceil(K/128)]; b [N][K] e4m3 codes, sb [ceil(N/128)] or [N] rows
         of ceil(K/128) scales."""
-        import torch
+        torch = _torch or _tt()
         M, K, lda = _rows2(a, "a")
         N, kb_, ldb = _rows2(b, "b")
         if kb_ != K:
@@ -681,7 +702,7 @@ class Context:
     def fp8_linear_act(self, x, b, sb, y):
         """frx_fp8_linear_act: y = x w^T for f32 or bf16 x [M][K], quantised on
         the way, and FP8_TILES weights b [N][K], sb [ceil(N/128)][ceil(K/128)]."""
-        import torch
+        torch = _torch or _tt()
         M, K = x.shape
         N, kb_, ldb = _rows2(b, "b")
         if kb_ != K:
@@ -699,7 +720,7 @@ class Context:
         """frx_fp8_linear_grouped: rows offsets[e] to offsets[e + 1] of a [R][K]
         times expert e's codes b[e] [N][K], sb[e] [ceil(N/128)][ceil(K/128)]
         (stacked tensors, or lists of E)."""
-        import torch
+        torch = _torch or _tt()
         R, K, lda = _rows2(a, "a")
         E, kb = int(offsets.numel()) - 1, (K + 127) // 128
         N = int(y.shape[1]) if y.dim() == 2 else 0
@@ -708,14 +729,15 @@ class Context:
         bp, ldb = _per_expert(b, E, (N, K), torch.float8_e4m3fn, "b", rows=True)
         sp, _ = _per_expert(sb, E, ((N + 127) // 128, kb), torch.float32, "sb")
         _dense(y, (R, N), None, "y")
-        _check(lib().frx_fp8_linear_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(), bp, ldb, sp,
+        _check(lib().frx_fp8_linear_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
+                                            bp.buffer_info()[0], ldb, sp.buffer_info()[0],
                                             offsets.data_ptr(), E, y.data_ptr(), _dtype_code(y), R, K, N), self._h)
         return y
 
     def fp8_grad_weight_grouped(self, a, sa, b, sb, offsets, dw):
         """frx_fp8_grad_weight_grouped: dw[e] [N][K] = the sum over expert e's
         rows of dy (a [N][R], FP8_COLS) times x (b [K][R], FP8_COLS)."""
-        import torch
+        torch = _torch or _tt()
         N, R, lda = _rows2(a, "a")
         K, r_, ldb = _rows2(b, "b")
         if r_ != R:
@@ -728,7 +750,8 @@ class Context:
         _dense(sb, (K, rb), torch.float32, "sb")
         dp, _ = _per_expert(dw, E, (N, K), dw[0].dtype, "dw")
         _check(lib().frx_fp8_grad_weight_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
-                                                 b.data_ptr(), ldb, sb.data_ptr(), offsets.data_ptr(), E, dp,
+                                                 b.data_ptr(), ldb, sb.data_ptr(), offsets.data_ptr(), E,
+                                                 dp.buffer_info()[0],
                                                  _dtype_code(dw[0]), R, N, K), self._h)
         return dw
 
@@ -736,7 +759,7 @@ class Context:
     def moe_sort(self, topk_idx, rows: MoeRows):
         """frx_moe_sort: fills rows from topk_idx [T][top_k] int32 (an index
         outside [0, E) goes nowhere)."""
-        import torch
+        torch = _torch or _tt()
         _dense(topk_idx, (rows.T, rows.top_k), torch.int32, "topk_idx")
         _check(lib().frx_moe_sort(self._h, topk_idx.data_ptr(), rows._p), self._h)
         return rows
@@ -753,7 +776,7 @@ class Context:
     def moe_combine(self, ys, rows: MoeRows, w, y):
         """frx_moe_combine: y [T][H] = the sum of each token's rows of ys [R]
         [H], times w [T][top_k] f32 (None: every weight 1)."""
-        import torch
+        torch = _torch or _tt()
         H = int(y.shape[-1])
         _dense(ys, (rows.R, H), None, "ys")
         _dense(y, (rows.T, H), None, "y")
@@ -766,7 +789,7 @@ class Context:
     def moe_combine_backward(self, dy, ys, rows: MoeRows, w, dys, dw):
         """frx_moe_combine_backward: dys [R][H] and dw [T][top_k] f32 of
         moe_combine for dy [T][H]; ys and dw may both be None, w too."""
-        import torch
+        torch = _torch or _tt()
         H = int(dy.shape[-1])
         _dense(dy, (rows.T, H), None, "dy")
         _dense(dys, (rows.R, H), None, "dys")

@@ -98,6 +98,8 @@ struct frx_ctx {
   size_t spp_ws_bytes = 0;
   void *q8_ws = nullptr;  // 8-bit codes and scales of frx_fp8_linear_act's activations
   size_t q8_ws_bytes = 0;
+  void *sort_ws = nullptr;  // counts by chunk of frx_moe_sort
+  size_t sort_ws_bytes = 0;
   unsigned *sk_cnt = nullptr;  // its per-row-tile arrival counters (zero between launches)
   int gemv_split = FRX_GEMV_SPLIT_AUTO;
   unsigned *ffn_bar = nullptr;  // grid-barrier words of the one-launch FFN
@@ -202,6 +204,7 @@ void frx_destroy(frx_ctx *ctx) {
   if (ctx->xpl_ws) (void)hipFree(ctx->xpl_ws);
   if (ctx->spp_ws) (void)hipFree(ctx->spp_ws);
   if (ctx->q8_ws) (void)hipFree(ctx->q8_ws);
+  if (ctx->sort_ws) (void)hipFree(ctx->sort_ws);
   if (ctx->sk_cnt) (void)hipFree(ctx->sk_cnt);
   if (ctx->ffn_bar) (void)hipFree(ctx->ffn_bar);
   for (void *p : ctx->retired) (void)hipFree(p);
@@ -1691,7 +1694,14 @@ frx_status frx_moe_sort(frx_ctx *ctx, const uint32_t *topk_idx, const frx_moe_ro
   frx::RouteRows r;
   if (!topk_idx || !aligned_to(topk_idx, 4)) return fail(ctx, FRX_ERR_SHAPE, "topk_idx is null or unaligned");
   if ((st = check_rows(ctx, rows, &r)) != FRX_OK) return st;
-  const hipError_t e = frx::launch_route_sort(topk_idx, r, ctx->stream);
+  const size_t need = frx::route_sort_bytes(r);
+  int *hist = nullptr;
+  if (need && may_grow(ctx, ctx->sort_ws_bytes, need)) {
+    if ((st = ensure_buffer(ctx, &ctx->sort_ws, &ctx->sort_ws_bytes, need, "sort workspace allocation")) != FRX_OK)
+      return st;
+    hist = static_cast<int *>(ctx->sort_ws);
+  }
+  const hipError_t e = frx::launch_route_sort(topk_idx, r, hist, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "sort launch");
   return FRX_OK;
 }

@@ -376,7 +376,11 @@ struct RouteRows {
   int T, top_k, E, align, R;
   uint32_t *offsets, *row_of, *slot_of;
 };
-hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, hipStream_t stream);
+// Slots up to which one workgroup sorts; above, counts by chunk in `hist`
+// (route_sort_bytes) and a second launch.
+constexpr size_t ROUTE_ONE_WG = 4096;
+size_t route_sort_bytes(const RouteRows &r);
+hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, int *hist, hipStream_t stream);
 hipError_t launch_route_dispatch(const void *x, size_t row_bytes, const RouteRows &r, void *xs, hipStream_t stream);
 hipError_t launch_route_combine(const void *ys, int st_bf16, const RouteRows &r, const float *w, void *y, int yt_bf16,
                                 uint32_t H, hipStream_t stream);

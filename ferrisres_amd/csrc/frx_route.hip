@@ -15,54 +15,81 @@ namespace {
 constexpr int ROUTE_MAXE = 64;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
-// One workgroup: counts, then ranks chunk by chunk in slot order.
-__global__ __launch_bounds__(1024) void route_sort_kernel(const uint32_t *__restrict__ idx, RouteRows r) {
+constexpr int SORT_NT = 1024;  // slots of a chunk, one a thread
+
+// Counts of one chunk by expert, wave by wave, and each thread's rank among
+// the slots of its expert in its wave. e >= E: no expert. A wave finds the
+// lanes of equal expert with a ballot for each bit of the index.
+__device__ __forceinline__ int chunk_ranks(uint32_t e, int E, int (*wave_cnt)[ROUTE_MAXE]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  wave_cnt[wave][lane] = 0;
+  const bool in = e < (uint32_t)E;
+  unsigned long long same = __ballot(in);
+#pragma unroll
+  for (int b = 0; b < 6; b++) {
+    const unsigned long long m = __ballot((e >> b) & 1);
+    same &= (e >> b) & 1 ? m : ~m;
+  }
+  const int rank = __popcll(same & ((1ull << lane) - 1ull));
+  if (in && rank == 0) wave_cnt[wave][e] = __popcll(same);
+  return rank;
+}
+
+// Exclusive sum over the lanes of a wave.
+__device__ __forceinline__ int wave_before(int v) {
+  int x = v;
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if ((threadIdx.x & 63) >= o) x += y;
+  }
+  return x - v;
+}
+
+// One workgroup, chunk after chunk: counts first, then rows.
+__global__ __launch_bounds__(SORT_NT) void route_sort_kernel(const uint32_t *__restrict__ idx, RouteRows r) {
   __shared__ int wave_cnt[16][ROUTE_MAXE];
   __shared__ int base[ROUTE_MAXE];  // next row of each expert
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int A = r.T * r.top_k, E = r.E;
-  for (int i = tid; i < 16 * ROUTE_MAXE; i += 1024) wave_cnt[i / ROUTE_MAXE][i % ROUTE_MAXE] = 0;
-  for (int i = tid; i < r.R; i += 1024) r.slot_of[i] = kNone;
-  __syncthreads();
-  for (int a = tid; a < A; a += 1024) {
-    const uint32_t e = idx[a];
-    if (e < (uint32_t)E) atomicAdd(&wave_cnt[wave][e], 1);
+  if (tid < ROUTE_MAXE) base[tid] = 0;
+  for (int i = tid; i < r.R; i += SORT_NT) r.slot_of[i] = kNone;
+  uint32_t e = kNone;
+  int rank = 0;
+  for (int c0 = 0; c0 < A; c0 += SORT_NT) {
+    __syncthreads();
+    e = c0 + tid < A ? idx[c0 + tid] : kNone;
+    rank = chunk_ranks(e, E, wave_cnt);
+    __syncthreads();
+    if (tid < E) {
+      int s = 0;
+      for (int w = 0; w < 16; w++) s += wave_cnt[w][tid];
+      base[tid] += s;
+    }
   }
   __syncthreads();
   if (wave == 0) {
-    int c = 0;
-    if (lane < E)
-      for (int w = 0; w < 16; w++) c += wave_cnt[w][lane];
-    c = (c + r.align - 1) / r.align * r.align;
-    int x = c;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
-    base[lane] = x - c;
-    if (lane < E) r.offsets[lane] = (uint32_t)(x - c);
-    if (lane == E - 1) r.offsets[E] = (uint32_t)x;
+    const int c = lane < E ? (base[lane] + r.align - 1) & -r.align : 0;
+    const int at = wave_before(c);
+    base[lane] = at;
+    if (lane < E) r.offsets[lane] = (uint32_t)at;
+    if (lane == E - 1) r.offsets[E] = (uint32_t)(at + c);
   }
-  __syncthreads();  // also orders the cleared slot_of before the rows below
-  for (int c0 = 0; c0 < A; c0 += 1024) {
-    const int a = c0 + tid;
-    const uint32_t e = a < A ? idx[a] : kNone;
-    int rank = 0;
-    for (int ee = 0; ee < E; ee++) {
-      const unsigned long long m = __ballot(e == (uint32_t)ee);
-      if (lane == 0) wave_cnt[wave][ee] = __popcll(m);
-      if (e == (uint32_t)ee) rank = __popcll(m & ((1ull << lane) - 1ull));
+  for (int c0 = 0; c0 < A; c0 += SORT_NT) {
+    __syncthreads();  // (the first also orders the cleared slot_of before the rows below)
+    if (A > SORT_NT) {  // one chunk: its ranks are still there
+      e = c0 + tid < A ? idx[c0 + tid] : kNone;
+      rank = chunk_ranks(e, E, wave_cnt);
+      __syncthreads();
     }
-    __syncthreads();
-    if (a < A) {
+    if (c0 + tid < A) {
       uint32_t row = kNone;
       if (e < (uint32_t)E) {
         int before = base[e];
         for (int w = 0; w < wave; w++) before += wave_cnt[w][e];
         row = (uint32_t)(before + rank);
-        r.slot_of[row] = (uint32_t)a;
+        r.slot_of[row] = (uint32_t)(c0 + tid);
       }
-      r.row_of[a] = row;
+      r.row_of[c0 + tid] = row;
     }
     __syncthreads();
     if (tid < E) {
@@ -70,8 +97,77 @@ __global__ __launch_bounds__(1024) void route_sort_kernel(const uint32_t *__rest
       for (int w = 0; w < 16; w++) s += wave_cnt[w][tid];
       base[tid] += s;
     }
-    __syncthreads();
   }
+}
+
+// Many chunks, a workgroup each: hist[chunk][expert], then (a launch later)
+// every workgroup adds up the chunks before its own.
+__global__ __launch_bounds__(SORT_NT) void route_count_kernel(const uint32_t *__restrict__ idx, int A, int E,
+                                                              int *__restrict__ hist) {
+  __shared__ int wave_cnt[16][ROUTE_MAXE];
+  const int a = blockIdx.x * SORT_NT + threadIdx.x;
+  chunk_ranks(a < A ? idx[a] : kNone, E, wave_cnt);
+  __syncthreads();
+  if (threadIdx.x < ROUTE_MAXE) {
+    int s = 0;
+    for (int w = 0; w < 16; w++) s += wave_cnt[w][threadIdx.x];
+    hist[blockIdx.x * ROUTE_MAXE + threadIdx.x] = s;
+  }
+}
+
+__global__ __launch_bounds__(SORT_NT) void route_place_kernel(const uint32_t *__restrict__ idx, RouteRows r,
+                                                              const int *__restrict__ hist) {
+  __shared__ int wave_cnt[16][ROUTE_MAXE];
+  __shared__ int part[2][16][ROUTE_MAXE];  // counts of the chunks before this one; of all
+  __shared__ int first[ROUTE_MAXE], count[ROUTE_MAXE], end;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int A = r.T * r.top_k, E = r.E, G = gridDim.x, g = blockIdx.x;
+  const int a = g * SORT_NT + tid;
+  const uint32_t e = a < A ? idx[a] : kNone;
+  const int rank = chunk_ranks(e, E, wave_cnt);
+  int before = 0, all = 0;
+  for (int c = wave; c < G; c += 16) {
+    const int h = hist[c * ROUTE_MAXE + lane];
+    all += h;
+    before += c < g ? h : 0;
+  }
+  part[0][wave][lane] = before;
+  part[1][wave][lane] = all;
+  __syncthreads();
+  if (wave == 0) {
+    before = all = 0;
+    for (int w = 0; w < 16; w++) {
+      before += part[0][w][lane];
+      all += part[1][w][lane];
+    }
+    const int c = (all + r.align - 1) & -r.align;  // experts past E have none
+    const int at = wave_before(c);
+    first[lane] = at;
+    count[lane] = all;
+    if (lane == 63) end = at + c;
+    part[0][0][lane] = before;
+    if (g == 0) {
+      if (lane < E) r.offsets[lane] = (uint32_t)at;
+      if (lane == 63) r.offsets[E] = (uint32_t)(at + c);
+    }
+  }
+  __syncthreads();
+  if (a < A) {
+    uint32_t row = kNone;
+    if (e < (uint32_t)E) {
+      int at = first[e] + part[0][0][e];
+      for (int w = 0; w < wave; w++) at += wave_cnt[w][e];
+      row = (uint32_t)(at + rank);
+      r.slot_of[row] = (uint32_t)a;
+    }
+    r.row_of[a] = row;
+  }
+  // rows of no route: between the segments (a wave an expert), and from the end on
+  for (int x = g * 16 + wave; x < E; x += G * 16) {
+    const int z = x + 1 < E ? first[x + 1] : end;
+    for (int i = first[x] + count[x] + lane; i < z; i += 64) r.slot_of[i] = kNone;
+  }
+  for (int i = end + a; i < r.R; i += G * SORT_NT) r.slot_of[i] = kNone;
 }
 
 // One row per wave, W bytes per lane and load.
@@ -89,70 +185,152 @@ __global__ __launch_bounds__(256) void route_dispatch_kernel(const char *__restr
   for (size_t i = lane; i < row_bytes / sizeof(V); i += 64) dst[i] = slot >= A ? V{} : src[i];
 }
 
-__device__ __forceinline__ float ldf(const float *p, size_t i) { return p[i]; }
-__device__ __forceinline__ float ldf(const uint16_t *p, size_t i) { return bf16_to_f32(p[i]); }
-__device__ __forceinline__ void stf(float *p, size_t i, float v) { p[i] = v; }
-__device__ __forceinline__ void stf(uint16_t *p, size_t i, float v) { p[i] = (uint16_t)bf16_rne_nb(v); }
-
-#pragma clang fp contract(off)
-template <typename ST, typename YT>
-__global__ __launch_bounds__(256) void route_combine_kernel(const ST *__restrict__ ys, RouteRows r,
-                                                            const float *__restrict__ w, YT *__restrict__ y,
-                                                            uint32_t H) {
-  const size_t t = blockIdx.x;
-  for (uint32_t h = threadIdx.x; h < H; h += 256) {
-    float acc = 0.0f;
-    for (int j = 0; j < r.top_k; j++) {
-      const uint32_t row = r.row_of[t * r.top_k + j];
-      if (row >= (uint32_t)r.R) continue;
-      const float p = (w ? w[t * r.top_k + j] : 1.0f) * ldf(ys, (size_t)row * H + h);
-      acc = acc + p;
-    }
-    stf(y, t * H + h, acc);
+// Q consecutive values; the vector forms need 16-byte aligned rows (and Q
+// dividing them).
+__device__ __forceinline__ void ldq(const float *p, float (&v)[4]) {
+  const f32x4 a = *reinterpret_cast<const f32x4 *>(p);
+#pragma unroll
+  for (int i = 0; i < 4; i++) v[i] = a[i];
+}
+__device__ __forceinline__ void ldq(const float *p, float (&v)[8]) {
+  float a[4], b[4];
+  ldq(p, a);
+  ldq(p + 4, b);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[i] = a[i];
+    v[4 + i] = b[i];
   }
 }
-#pragma clang fp contract(on)
+__device__ __forceinline__ void ldq(const uint16_t *p, float (&v)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[2 * i] = __uint_as_float(a[i] << 16);
+    v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void ldq(const float *p, float (&v)[1]) { v[0] = *p; }
+__device__ __forceinline__ void ldq(const uint16_t *p, float (&v)[1]) { v[0] = bf16_to_f32(*p); }
+template <int Q>
+__device__ __forceinline__ void stq(float *p, const float (&v)[Q]) {
+  if constexpr (Q == 1) *p = v[0];
+  else
+#pragma unroll
+    for (int i = 0; i < Q; i += 4) *reinterpret_cast<f32x4 *>(p + i) = (f32x4){v[i], v[i + 1], v[i + 2], v[i + 3]};
+}
+template <int Q>
+__device__ __forceinline__ void stq(uint16_t *p, const float (&v)[Q]) {
+  uint32_t h[Q];
+#pragma unroll
+  for (int i = 0; i < Q; i++) h[i] = bf16_rne_nb(v[i]);
+  if constexpr (Q == 1) *p = (uint16_t)h[0];
+  else
+    *reinterpret_cast<u32x4 *>(p) = (u32x4){h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+}
 
-// A workgroup per token; then one per 4 rows for the rows of no route.
-template <typename DT, typename ST>
+#pragma clang fp contract(off)
+// Q columns of one token a thread; 1 << tb threads a token (256 and several
+// workgroups for long rows, several tokens a workgroup for short ones). The
+// rows of four routes are loaded before the first is added.
+template <typename ST, typename YT, int Q>
+__global__ __launch_bounds__(256) void route_combine_kernel(const ST *__restrict__ ys, RouteRows r,
+                                                            const float *__restrict__ w, YT *__restrict__ y,
+                                                            uint32_t H, int tb) {
+  constexpr int C = 4;
+  const size_t t = (size_t)blockIdx.x * (256 >> tb) + (threadIdx.x >> tb);
+  const uint32_t h = (blockIdx.y * 256 + (threadIdx.x & ((1 << tb) - 1))) * Q;
+  if (t >= (size_t)r.T || h >= H) return;
+  const uint32_t *row_of = r.row_of + t * r.top_k;
+  float acc[Q];
+#pragma unroll
+  for (int q = 0; q < Q; q++) acc[q] = 0.0f;
+  for (int j0 = 0; j0 < r.top_k; j0 += C) {
+    uint32_t row[C];
+    float g[C], v[C][Q];
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      row[c] = j0 + c < r.top_k ? row_of[j0 + c] : kNone;
+      g[c] = w && j0 + c < r.top_k ? w[t * r.top_k + j0 + c] : 1.0f;
+    }
+#pragma unroll
+    for (int c = 0; c < C; c++)
+      if (row[c] < (uint32_t)r.R) ldq(ys + (size_t)row[c] * H + h, v[c]);
+#pragma unroll
+    for (int c = 0; c < C; c++)
+      if (row[c] < (uint32_t)r.R)
+#pragma unroll
+        for (int q = 0; q < Q; q++) acc[q] = acc[q] + g[c] * v[c][q];
+  }
+  stq<Q>(y + t * H + h, acc);
+}
+
+// A wave a route: dy's row is read once for each of its token's routes, from
+// cache after the first (neighbouring waves). Then waves of 64 rows each look
+// for rows of no route.
+template <typename DT, typename ST, int Q>
 __global__ __launch_bounds__(256) void route_combine_backward_kernel(const DT *__restrict__ dy,
                                                                      const ST *__restrict__ ys, RouteRows r,
                                                                      const float *__restrict__ w,
                                                                      ST *__restrict__ dys, float *__restrict__ dw,
                                                                      uint32_t H) {
-  __shared__ float part[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (blockIdx.x >= (unsigned)r.T) {
-    const size_t row = (size_t)(blockIdx.x - r.T) * 4 + wave;
-    if (row >= r.R || row >= r.offsets[r.E] || r.slot_of[row] != kNone) return;
-    for (uint32_t h = lane; h < H; h += 64) stf(dys, row * H + h, 0.0f);
+  const int lane = threadIdx.x & 63;
+  const uint32_t A = (uint32_t)r.T * (uint32_t)r.top_k;
+  const uint32_t slot = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (slot >= A) {
+    const uint32_t r0 = (slot - A) * 64, end = min(r.offsets[r.E], (uint32_t)r.R);
+    unsigned long long none = __ballot(r0 + lane < end && r.slot_of[min(r0 + lane, (uint32_t)r.R - 1)] == kNone);
+    for (; none; none &= none - 1) {
+      const float z[Q] = {};
+      ST *d = dys + (size_t)(r0 + __ffsll(none) - 1) * H;
+      for (uint32_t h = lane * Q; h < H; h += 64 * Q) stq<Q>(d + h, z);
+    }
     return;
   }
-  const size_t t = blockIdx.x;
-  for (int j = 0; j < r.top_k; j++) {
-    const uint32_t row = r.row_of[t * r.top_k + j];
-    float dot = 0.0f;
-    if (row < (uint32_t)r.R) {
-      const float g = w ? w[t * r.top_k + j] : 1.0f;
-      for (uint32_t h = threadIdx.x; h < H; h += 256) {
-        const float d = ldf(dy, t * H + h);
-        stf(dys, (size_t)row * H + h, g * d);
-        if (ys) dot += d * ldf(ys, (size_t)row * H + h);
+  const uint32_t row = r.row_of[slot];
+  float dot = 0.0f;
+  if (row < (uint32_t)r.R) {
+    const float g = w ? w[slot] : 1.0f;
+    const DT *src = dy + (size_t)(slot / r.top_k) * H;
+    const ST *other = ys + (size_t)row * H;
+    ST *d = dys + (size_t)row * H;
+#pragma unroll 4
+    for (uint32_t h = lane * Q; h < H; h += 64 * Q) {
+      float a[Q], p[Q];
+      ldq(src + h, a);
+#pragma unroll
+      for (int q = 0; q < Q; q++) p[q] = g * a[q];
+      if (ys) {
+        float b[Q];
+        ldq(other + h, b);
+#pragma unroll
+        for (int q = 0; q < Q; q++) dot = dot + a[q] * b[q];
       }
+      stq<Q>(d + h, p);
     }
-    if (!dw) continue;
-    for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
-    if (lane == 0) part[wave] = dot;
-    __syncthreads();
-    if (threadIdx.x == 0) dw[t * r.top_k + j] = (part[0] + part[1]) + (part[2] + part[3]);
-    __syncthreads();
   }
+  if (!dw) return;
+  for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
+  if (lane == 0) dw[slot] = dot;
 }
+#pragma clang fp contract(on)
 
 }  // namespace
 
-hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, hipStream_t stream) {
-  hipLaunchKernelGGL(route_sort_kernel, dim3(1), dim3(1024), 0, stream, idx, r);
+size_t route_sort_bytes(const RouteRows &r) {
+  const size_t A = (size_t)r.T * r.top_k;
+  return A <= ROUTE_ONE_WG ? 0 : (A + SORT_NT - 1) / SORT_NT * ROUTE_MAXE * sizeof(int);
+}
+
+hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, int *hist, hipStream_t stream) {
+  if (!hist) {
+    hipLaunchKernelGGL(route_sort_kernel, dim3(1), dim3(SORT_NT), 0, stream, idx, r);
+    return hipGetLastError();
+  }
+  const int A = r.T * r.top_k;
+  const dim3 grid((A + SORT_NT - 1) / SORT_NT);
+  hipLaunchKernelGGL(route_count_kernel, grid, dim3(SORT_NT), 0, stream, idx, A, r.E, hist);
+  hipLaunchKernelGGL(route_place_kernel, grid, dim3(SORT_NT), 0, stream, idx, r, hist);
   return hipGetLastError();
 }
 
@@ -166,16 +344,35 @@ hipError_t launch_route_dispatch(const void *x, size_t row_bytes, const RouteRow
   return hipGetLastError();
 }
 
+// Whether rows of `bytes` from each of the pointers on are 16-byte aligned.
+static bool rows16(const void *a, const void *b, const void *c, size_t bytes) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) | bytes) &
+          15) == 0;
+}
+
+template <typename ST, typename YT, int Q>
+static hipError_t combine_go(const ST *ys, const RouteRows &r, const float *w, YT *y, uint32_t H, hipStream_t stream) {
+  const uint32_t need = (H + Q - 1) / Q;
+  int tb = 0;
+  while (tb < 8 && (1u << tb) < need) tb++;
+  const dim3 grid((unsigned)((r.T + (256 >> tb) - 1) / (256 >> tb)), (need + 255) / 256);
+  hipLaunchKernelGGL((route_combine_kernel<ST, YT, Q>), grid, dim3(256), 0, stream, ys, r, w, y, H, tb);
+  return hipGetLastError();
+}
+
+template <typename ST, typename YT>
+static hipError_t combine_q(const ST *ys, const RouteRows &r, const float *w, YT *y, uint32_t H, hipStream_t stream) {
+  // 16 bytes of the narrower type a thread
+  constexpr int Q = sizeof(ST) == 4 && sizeof(YT) == 4 ? 4 : 8;
+  if (rows16(ys, y, nullptr, (size_t)H * 2) && H % Q == 0) return combine_go<ST, YT, Q>(ys, r, w, y, H, stream);
+  return combine_go<ST, YT, 1>(ys, r, w, y, H, stream);
+}
+
 template <typename ST>
 static hipError_t combine_t(const ST *ys, const RouteRows &r, const float *w, void *y, int yt_bf16, uint32_t H,
                             hipStream_t stream) {
-  if (yt_bf16)
-    hipLaunchKernelGGL((route_combine_kernel<ST, uint16_t>), dim3(r.T), dim3(256), 0, stream, ys, r, w,
-                       static_cast<uint16_t *>(y), H);
-  else
-    hipLaunchKernelGGL((route_combine_kernel<ST, float>), dim3(r.T), dim3(256), 0, stream, ys, r, w,
-                       static_cast<float *>(y), H);
-  return hipGetLastError();
+  return yt_bf16 ? combine_q(ys, r, w, static_cast<uint16_t *>(y), H, stream)
+                 : combine_q(ys, r, w, static_cast<float *>(y), H, stream);
 }
 
 hipError_t launch_route_combine(const void *ys, int st_bf16, const RouteRows &r, const float *w, void *y, int yt_bf16,
@@ -187,9 +384,15 @@ hipError_t launch_route_combine(const void *ys, int st_bf16, const RouteRows &r,
 template <typename DT, typename ST>
 static hipError_t combine_backward_t(const void *dy, const void *ys, const RouteRows &r, const float *w, void *dys,
                                      float *dw, uint32_t H, hipStream_t stream) {
-  hipLaunchKernelGGL((route_combine_backward_kernel<DT, ST>), dim3((unsigned)(r.T + (r.R + 3) / 4)), dim3(256), 0,
-                     stream, static_cast<const DT *>(dy), static_cast<const ST *>(ys), r, w,
-                     static_cast<ST *>(dys), dw, H);
+  constexpr int Q = sizeof(DT) == 4 && sizeof(ST) == 4 ? 4 : 8;
+  const size_t waves = (size_t)r.T * r.top_k + (r.align > 1 ? ((size_t)r.R + 63) / 64 : 0);
+  const dim3 grid((unsigned)((waves + 3) / 4));
+  if (rows16(dy, ys, dys, (size_t)H * 2) && H % Q == 0)
+    hipLaunchKernelGGL((route_combine_backward_kernel<DT, ST, Q>), grid, dim3(256), 0, stream,
+                       static_cast<const DT *>(dy), static_cast<const ST *>(ys), r, w, static_cast<ST *>(dys), dw, H);
+  else
+    hipLaunchKernelGGL((route_combine_backward_kernel<DT, ST, 1>), grid, dim3(256), 0, stream,
+                       static_cast<const DT *>(dy), static_cast<const ST *>(ys), r, w, static_cast<ST *>(dys), dw, H);
   return hipGetLastError();
 }
 
