@@ -1572,7 +1572,7 @@ static frx_status check_fp8_side(frx_ctx *ctx, const void *b, const void *sb, co
 static frx_status fp8_run(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa, const uint8_t *b,
                           size_t ldb, const float *sb, uint32_t b_rows, void *y, frx_dtype yt, uint32_t M, uint32_t K,
                           uint32_t N) {
-  frx::Fp8Plan plan = frx::fp8_plan(M, K, N, ctx->cus);
+  frx::Fp8Plan plan = frx::fp8_plan(M, K, N, (int)b_rows, yt == FRX_BF16, ctx->cus);
   const size_t need = frx::fp8_part_bytes(M, N, plan);
   if (need && !may_grow(ctx, ctx->gk_ws_bytes, need)) {
     plan.S = 1;  // a first call under capture: whole K
@@ -1609,7 +1609,7 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
   if (!aligned_to(x, dtype_bytes(xt))) return fail(ctx, FRX_ERR_SHAPE, "x must be aligned to its elements");
   if ((st = check_fp8(ctx, b, K, FRX_FP8_E4M3, sb, ldb, yt, M, K, N)) != FRX_OK) return st;
   if ((st = check_fp8_side(ctx, b, sb, y, yt)) != FRX_OK) return st;
-  const frx::Fp8Plan plan = frx::fp8_plan(M, K, N, ctx->cus);
+  const frx::Fp8Plan plan = frx::fp8_plan(M, K, N, 128, yt == FRX_BF16, ctx->cus);
   if (plan.tile == frx::FP8_T_SKINNY && frx::fp8_act_fits(M, K)) {
     const hipError_t e = frx::launch_fp8_linear_act(x, xt == FRX_BF16, b, ldb, sb, y, yt == FRX_BF16, M, K, N, plan,
                                                     ctx->stream);

@@ -1,5 +1,8 @@
 // frx_fp8.hip — launches of the 8-bit floating-point linears (engine: frx_fp8.hpp).
+#include <cmath>
+
 #include "frx_fp8_skinny.hpp"
+#include "frx_fp8_ring.hpp"
 
 namespace frx {
 
@@ -40,16 +43,30 @@ __device__ __forceinline__ void fill_operands(Fp8Operands &o, const uint8_t *a, 
   o.K = (int)K;
 }
 
-template <int BM, int BN, int WM, int WN, bool E5M2, bool BR1, typename YT>
-__global__ __launch_bounds__(WM *WN * 64) void fp8_dense_kernel(const DenseArgs p) {
-  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, BR1, sizeof(YT) == 4>;
+// The tile of workgroup `bid` of mts x nts. Hardware deals workgroups out to the
+// 8 XCDs in turn; each XCD gets a contiguous run of tiles, ordered by groups of
+// GM tiles of tokens, within a group down the tokens first, so that the tiles
+// an XCD works on at a time share rows of both sides in its L2.
+template <int GM>
+__device__ __forceinline__ void xcd_tile(uint32_t bid, uint32_t mts, uint32_t nts, uint32_t &mt, uint32_t &nt) {
+  const uint32_t total = mts * nts, q = total / 8, r = total % 8, xcd = bid % 8, i = bid / 8;
+  const uint32_t lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + i;
+  const uint32_t group = lin / (GM * nts), rest = lin - group * (GM * nts);
+  const uint32_t gm = min((uint32_t)GM, mts - group * GM);
+  nt = rest / gm;
+  mt = group * GM + rest - nt * gm;
+}
+
+template <typename Tile, bool BR1, typename YT>
+__global__ __launch_bounds__(Tile::NT, 2) void fp8_dense_kernel(const DenseArgs p) {
   extern __shared__ __align__(16) uint32_t lds[];
-  const uint32_t mts = (p.M + BM - 1) / BM;
-  const uint32_t nt = blockIdx.x / mts, mt = blockIdx.x - nt * mts;
+  constexpr int BM = Tile::BM, BN = Tile::BN;
+  uint32_t mt, nt;
+  xcd_tile<8>(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, mt, nt);
   const uint32_t m0 = mt * BM, n0 = nt * BN;
   Fp8Operands o;
   fill_operands<BR1>(o, p.a, p.lda, p.sa, p.b, p.ldb, p.sb, m0, min((uint32_t)BM, p.M - m0), n0,
-                                   min((uint32_t)BN, p.N - n0), p.K);
+                     min((uint32_t)BN, p.N - n0), p.K);
   const int kbs = (int)((p.K + 127) >> 7);
   o.kb0 = p.part ? (int)blockIdx.z * p.per : 0;
   o.kb1 = p.part ? min(o.kb0 + p.per, kbs) : kbs;
@@ -107,7 +124,7 @@ __device__ __forceinline__ int expert_tile(const uint32_t *offsets, int E, uint3
 }
 
 template <int BM, int BN, int WM, int WN, bool E5M2, typename YT>
-__global__ __launch_bounds__(WM *WN * 64) void fp8_grouped_kernel(const GroupArgs p) {
+__global__ __launch_bounds__(WM *WN * 64, 2) void fp8_grouped_kernel(const GroupArgs p) {
   using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, false, sizeof(YT) == 4>;
   extern __shared__ __align__(16) uint32_t lds[];
   const uint32_t nts = (p.N + BN - 1) / BN;
@@ -161,7 +178,7 @@ struct GradArgs {
 };
 
 template <int BM, int BN, int WM, int WN, bool E5M2, typename YT>
-__global__ __launch_bounds__(WM *WN * 64) void fp8_grad_kernel(const GradArgs p) {
+__global__ __launch_bounds__(WM *WN * 64, 2) void fp8_grad_kernel(const GradArgs p) {
   using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, true, sizeof(YT) == 4>;
   extern __shared__ __align__(16) uint32_t lds[];
   const uint32_t mts = (p.N + BM - 1) / BM;
@@ -182,16 +199,29 @@ __global__ __launch_bounds__(WM *WN * 64) void fp8_grad_kernel(const GradArgs p)
   Tile::template store<YT>(acc, dw + at, p.K, o.a_rows, o.b_rows, quads<YT>(dw, p.K));
 }
 
-// y = the parts added in order.
+// y = the parts added in order, four values a thread (n of them, parts n apart).
 template <typename YT>
 __global__ __launch_bounds__(256) void fp8_join_kernel(const float *__restrict__ part, int S, size_t n,
                                                        YT *__restrict__ y) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
-  float v = part[i];
-  for (int s = 1; s < S; s++) v += part[(size_t)s * n + i];
-  if constexpr (sizeof(YT) == 4) y[i] = v;
-  else y[i] = (uint16_t)bf16_rne_nb(v);
+  if (((n & 3) | (reinterpret_cast<uintptr_t>(y) & (4 * sizeof(YT) - 1))) == 0) {
+    f32x4 v = *reinterpret_cast<const f32x4 *>(part + i);
+    for (int s = 1; s < S; s++) v += *reinterpret_cast<const f32x4 *>(part + (size_t)s * n + i);
+    if constexpr (sizeof(YT) == 4) {
+      *reinterpret_cast<f32x4 *>(y + i) = v;
+    } else {
+      *reinterpret_cast<u32x2 *>(y + i) = (u32x2){bf16_rne_nb(v[0]) | (bf16_rne_nb(v[1]) << 16),
+                                                 bf16_rne_nb(v[2]) | (bf16_rne_nb(v[3]) << 16)};
+    }
+    return;
+  }
+  for (size_t k = i; k < n && k < i + 4; k++) {
+    float v = part[k];
+    for (int s = 1; s < S; s++) v += part[(size_t)s * n + k];
+    if constexpr (sizeof(YT) == 4) y[k] = v;
+    else y[k] = (uint16_t)bf16_rne_nb(v);
+  }
 }
 
 template <typename K, typename A>
@@ -202,14 +232,23 @@ hipError_t go(K kernel, int lds, std::atomic<uint64_t> &done, dim3 grid, int nt,
   return hipGetLastError();
 }
 
-template <int BM, int BN, int WM, int WN, bool E5M2, bool BR1, typename YT>
+template <typename Tile, bool BR1, typename YT>
 hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, BR1, sizeof(YT) == 4>;
-  const size_t tiles = (size_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  const size_t tiles = (size_t)((p.M + Tile::BM - 1) / Tile::BM) * ((p.N + Tile::BN - 1) / Tile::BN);
   if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  return go(fp8_dense_kernel<BM, BN, WM, WN, E5M2, BR1, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, 1, S),
-            Tile::NT, stream, p);
+  return go(fp8_dense_kernel<Tile, BR1, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, 1, S), Tile::NT, stream, p);
+}
+
+template <bool E5M2, bool BR1, typename YT>
+hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
+  constexpr bool WIDE = sizeof(YT) == 4;
+  if (tile == FP8_T_RING4) return dense_go<Fp8Ring<4, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
+  if constexpr (!BR1)
+    if (tile == FP8_T_RING6) return dense_go<Fp8Ring<6, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
+  if constexpr (!BR1 && !WIDE)
+    if (tile == FP8_T_RING8) return dense_go<Fp8Ring<8, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
+  return dense_go<Fp8Tile<128, 128, 2, 2, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
 }
 
 template <int RT, bool E5M2, bool BR1, typename XT, typename YT>
@@ -236,11 +275,6 @@ template <typename YT>
 hipError_t skinny_any(int e5m2, int b_rows, int rt, const Fp8Skinny &p, hipStream_t stream) {
   if (b_rows == 1) return e5m2 ? skinny_go<true, true, uint8_t, YT>(rt, p, stream) : skinny_go<false, true, uint8_t, YT>(rt, p, stream);
   return e5m2 ? skinny_go<true, false, uint8_t, YT>(rt, p, stream) : skinny_go<false, false, uint8_t, YT>(rt, p, stream);
-}
-
-template <bool E5M2, bool BR1, typename YT>
-hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
-  return dense_go<128, 128, 2, 2, E5M2, BR1, YT>(p, S, stream);
 }
 
 // fn<E5M2, BR1 or none, YT>(args) for run-time choices of them.
@@ -272,7 +306,25 @@ hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
 
 }  // namespace
 
-Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
+// Tiles of many tokens: height x width, workgroups resident at once on a
+// compute unit, and what a step of 128 columns takes (ns, all of them resident;
+// 8192^3, 2048 x 4096 x 11008 and 4096^3). The 8-bit pipe in tiles of 256 x 256
+// is the fastest per product (2943 TFLOP/s at 8192^3; 192: 2545, 128: 2127, 128 x
+// 128 from LDS alone 1930), the smaller ones where it would leave units idle (us,
+// 256 / 192 / 128 / 128 x 128: 2048 x 4096 x 11008 105 / 88 / 110 / 126, 2048 x
+// 4096 x 4096 53 / 43 / 37 / 49, 4096^3 53 / 78 / 76 / 90). On the bf16 pipe widening
+// the operands bounds them all (2048 x 4096 x 11008: 168 / 183 / 166 us for 192 /
+// 128 / 128 x 128; 333 x 5120 x 13824 94 / 70 / 75).
+struct TileCost {
+  int tile, bm, bn, wgs, ns;
+};
+constexpr TileCost kNarrow[] = {{FP8_T_RING8, 256, 256, 1, 1460}, {FP8_T_RING6, 192, 256, 1, 1130},
+                                {FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
+constexpr TileCost kWide[] = {{FP8_T_RING6, 192, 256, 1, 2600}, {FP8_T_RING4, 128, 256, 1, 1800},
+                              {FP8_T_128, 128, 128, 2, 1750}};
+constexpr TileCost kWideRows[] = {{FP8_T_RING4, 128, 256, 1, 2200}, {FP8_T_128, 128, 128, 2, 2150}};
+
+Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, int cus) {
   if (M <= 16) {
     // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
     const uint32_t tiles = (N + 15) / 16;
@@ -287,7 +339,29 @@ Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
     }
     return {FP8_T_SKINNY, 1, best};
   }
-  return {FP8_T_128, 1, (int)((K + 127) / 128)};
+  const int steps = (int)((K + 127) / 128);
+  const TileCost *costs = yt_bf16 ? kNarrow : b_rows == 1 ? kWideRows : kWide;
+  const int count = yt_bf16 ? 4 : b_rows == 1 ? 2 : 3;
+  Fp8Plan plan = {FP8_T_128, 1, steps};
+  double least = 1e30;
+  for (int t = 0; t < count; t++) {
+    const TileCost &c = costs[t];
+    if (yt_bf16 && b_rows == 1 && c.tile != FP8_T_RING4 && c.tile != FP8_T_128) continue;  // not built
+    const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    // a K slice more: fewer steps, but every part is written and read (4 bytes a value at
+    // about 4 TB/s) and the parts joined by another launch (4 us)
+    for (int S = 1; S <= 8 && S <= steps; S++) {
+      const int per = (steps + S - 1) / S;
+      if ((S - 1) * per >= steps) continue;  // an empty slice
+      const double rounds = std::ceil(tiles * S / ((double)c.wgs * cus));
+      const double ns = rounds * per * c.ns + (S > 1 ? 4000.0 + (double)S * M * N * 8 / 4000 : 0.0);
+      if (ns < least) {
+        least = ns;
+        plan = {c.tile, S, per};
+      }
+    }
+  }
+  return plan;
 }
 
 size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p) { return p.S > 1 ? (size_t)p.S * M * N * 4 : 0; }
@@ -305,7 +379,7 @@ hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float
                                : dense_any<float>(e5m2, b_rows, plan.tile, p, plan.S, stream);
   if (e != hipSuccess || plan.S == 1) return e;
   const size_t n = (size_t)M * N;
-  const dim3 grid((unsigned)((n + 255) / 256));
+  const dim3 grid((unsigned)((n + 1023) / 1024));
   if (yt_bf16) hipLaunchKernelGGL(fp8_join_kernel<uint16_t>, grid, dim3(256), 0, stream, part, plan.S, n, (uint16_t *)y);
   else hipLaunchKernelGGL(fp8_join_kernel<float>, grid, dim3(256), 0, stream, part, plan.S, n, (float *)y);
   return hipGetLastError();

@@ -23,10 +23,10 @@
 // every wave issues the same number of loads per stage. 16-byte pieces are
 // XOR-swizzled by row on the source side, which spreads an operand read (16
 // rows at one piece) over all banks. Rows past the tile's valid rows are
-// clamped to the last one (their results are not stored); K's last step
-// clamps pieces past K into the row and clears them on the token side in LDS
-// (one side suffices: a clamped piece of the other side is of the same row,
-// so a NaN in it is in that row's sums anyway).
+// clamped to the last one (their results are not stored). K's last step reads
+// past K into the next row (nothing past the buffer's end, which is the last
+// row's K) and clears those pieces of both sides, so that no NaN there meets
+// a zero.
 #pragma once
 #include "frx_gemm2.hpp"
 #include "frx_internal.hpp"
@@ -97,10 +97,50 @@ struct Fp8Operands {
   int kb0, kb1;          // blocks of 128 to sum over
 };
 
+// Zeros in a stage's rows from column K on (k0: the stage's first column).
+__device__ __forceinline__ void fp8_clear_tail(uint32_t *rows, int n, int k0, int K, int nt) {
+  for (int i = threadIdx.x; i < n * 8; i += nt)
+    if (k0 + 16 * (i & 7) >= K)
+      *reinterpret_cast<u32x4 *>(rows + (i >> 3) * 32 + ((i & 7) ^ xswz(i >> 3)) * 4) = (u32x4){0, 0, 0, 0};
+}
+
+// The results of a lane, FN x FM fragments from (token m0, weight row n0) of the
+// tile on. y: the tile's first element, row stride ldy. vec: quads of y are
+// aligned to their size.
+template <int FN, int FM, typename YT>
+__device__ __forceinline__ void fp8_store(const f32x4 (&acc)[FN][FM], YT *y, size_t ldy, int m0, int n0, int m_rows,
+                                          int n_rows, bool vec) {
+#pragma unroll
+  for (int fm = 0; fm < FM; fm++) {
+    const int m = m0 + fm * 16;
+    if (m >= m_rows) continue;
+#pragma unroll
+    for (int fn = 0; fn < FN; fn++) {
+      const int n = n0 + fn * 16;
+      if (n >= n_rows) continue;
+      YT *d = y + (size_t)m * ldy + n;
+      const f32x4 v = acc[fn][fm];
+      if constexpr (sizeof(YT) == 4) {
+        if (vec && n + 4 <= n_rows) *reinterpret_cast<f32x4 *>(d) = v;
+        else
+          for (int e = 0; e < 4 && n + e < n_rows; e++) d[e] = v[e];
+      } else {
+        uint32_t h[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = bf16_rne_nb(v[e]);
+        if (vec && n + 4 <= n_rows) *reinterpret_cast<u32x2 *>(d) = (u32x2){h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
+        else
+          for (int e = 0; e < 4 && n + e < n_rows; e++) d[e] = (uint16_t)h[e];
+      }
+    }
+  }
+}
+
 // BM tokens x BN weight rows, WM x WN waves, BR1: a scale per weight row, WIDE:
 // the bf16 pipe.
-template <int BM, int BN, int WM, int WN, bool E5M2, bool BR1, bool WIDE>
+template <int BM_, int BN_, int WM, int WN, bool E5M2, bool BR1, bool WIDE>
 struct Fp8Tile {
+  static constexpr int BM = BM_, BN = BN_;
   using Pipe = Fp8Pipe<WIDE>;
   static constexpr int WAVES = WM * WN, NT = WAVES * 64;
   static constexpr int TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
@@ -121,29 +161,11 @@ struct Fp8Tile {
                                                __amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb,
                                                __amdgpu_buffer_rsrc_t rsa, __amdgpu_buffer_rsrc_t rsb, int kb,
                                                int wave) {
-    const int k0 = kb * 128;
-    const uint32_t lane = threadIdx.x & 63;
-    if (k0 + 128 <= o.K) {
+    const uint32_t k0 = 128u * (uint32_t)kb;
 #pragma unroll
-      for (int i = 0; i < LA; i++)
-        lds_load16(ra, stage + (wave * LA + i) * 256, f.a[i], (uint32_t)k0);
+    for (int i = 0; i < LA; i++) lds_load16(ra, stage + (wave * LA + i) * 256, f.a[i], k0);
 #pragma unroll
-      for (int i = 0; i < LB; i++)
-        lds_load16(rb, stage + BM * 32 + (wave * LB + i) * 256, f.b[i], (uint32_t)k0);
-    } else {
-      // the last, shorter step: pieces past K read the row's last piece
-      const uint32_t last = (uint32_t)(o.K - 16 - k0);
-#pragma unroll
-      for (int i = 0; i < LA; i++) {
-        const uint32_t c = 16 * ((lane & 7) ^ xswz((wave * LA + i) * 8 + (lane >> 3)));
-        lds_load16(ra, stage + (wave * LA + i) * 256, f.a[i] - c + min(c, last), (uint32_t)k0);
-      }
-#pragma unroll
-      for (int i = 0; i < LB; i++) {
-        const uint32_t c = 16 * ((lane & 7) ^ xswz((wave * LB + i) * 8 + (lane >> 3)));
-        lds_load16(rb, stage + BM * 32 + (wave * LB + i) * 256, f.b[i] - c + min(c, last), (uint32_t)k0);
-      }
-    }
+    for (int i = 0; i < LB; i++) lds_load16(rb, stage + BM * 32 + (wave * LB + i) * 256, f.b[i], k0);
 #pragma unroll
     for (int i = 0; i < SPW; i++) {
       const int s = wave * SPW + i;  // uniform
@@ -201,9 +223,7 @@ struct Fp8Tile {
       __syncthreads();  // for every wave, and the other stage's last reads are done
       if (kb + 1 < o.kb1) issue(lds + ((kb + 1 - o.kb0) & 1) * STAGE, o, f, ra, rb, rsa, rsb, kb + 1, wave);
       if (kb * 128 + 128 > o.K) {
-        for (int i = threadIdx.x; i < BM * 8; i += NT)
-          if (kb * 128 + 16 * (i & 7) >= o.K)
-            *reinterpret_cast<u32x4 *>(cur + (i >> 3) * 32 + ((i & 7) ^ xswz(i >> 3)) * 4) = (u32x4){0, 0, 0, 0};
+        fp8_clear_tail(cur, BM + BN, kb * 128, o.K, NT);
         __syncthreads();
       }
       const float *sc = reinterpret_cast<const float *>(cur + DATA);
@@ -215,51 +235,51 @@ struct Fp8Tile {
         if (BR1) sw[fn] = *reinterpret_cast<const f32x4 *>(sc + SIA * 64 + wn * TN + fn * 16 + 4 * g);
       }
       const float sblk = sc[SIA * 64 + wn * TN];
+      // one token fragment's products are issued between the multiply-adds of
+      // the one before, so that neither waits for the other; the next
+      // fragment's codes are on their way from LDS meanwhile
+      i32x8 xc = operand(cur, wm * TM + l16, g);
+      float sn = sc[wm * TM + l16], s[2] = {0.f, 0.f};
+      f32x4 p[2][FN];
 #pragma unroll
-      for (int fm = 0; fm < FM; fm++) {
-        const auto x = Pipe::template op<E5M2>(operand(cur, wm * TM + fm * 16 + l16, g));
-        float s = sc[wm * TM + fm * 16 + l16];
-        if (!BR1) s *= sblk;
+      for (int fm = 0; fm <= FM; fm++) {
+        typename Pipe::Op x;
+        if (fm < FM) {
+          x = Pipe::template op<E5M2>(xc);
+          s[fm & 1] = BR1 ? sn : sn * sblk;
+          if (fm + 1 < FM) {
+            xc = operand(cur, wm * TM + (fm + 1) * 16 + l16, g);
+            sn = sc[wm * TM + (fm + 1) * 16 + l16];
+          }
+        }
 #pragma unroll
         for (int fn = 0; fn < FN; fn++) {
-          const f32x4 p = Pipe::template mul<E5M2>(w[fn], x);
+          if (fm < FM) p[fm & 1][fn] = Pipe::template mul<E5M2>(w[fn], x);
+          if (fm > 0) {
+            const float q = s[(fm - 1) & 1];
 #pragma unroll
-          for (int e = 0; e < 4; e++) acc[fn][fm][e] += p[e] * (BR1 ? s * sw[fn][e] : s);
+            for (int e = 0; e < 4; e++) acc[fn][fm - 1][e] += p[(fm - 1) & 1][fn][e] * (BR1 ? q * sw[fn][e] : q);
+          }
         }
+        if (fm > 0 && fm < FM) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+          for (int fn = 0; fn < FN; fn++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, WIDE ? 4 : 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, BR1 ? 8 : 4, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 
-  // y: the tile's first element, row stride ldy. vec: 16 (f32) or 8 (bf16)
-  // byte aligned quads.
   template <typename YT>
-  __device__ static void store(const f32x4 (&acc)[FN][FM], YT *y, size_t ldy, int m_rows, int n_rows, bool vec) {
+  __device__ __forceinline__ static void store(const f32x4 (&acc)[FN][FM], YT *y, size_t ldy, int m_rows, int n_rows,
+                                               bool vec) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave % WM, wn = wave / WM, l16 = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int fm = 0; fm < FM; fm++) {
-      const int m = wm * TM + fm * 16 + l16;
-      if (m >= m_rows) continue;
-#pragma unroll
-      for (int fn = 0; fn < FN; fn++) {
-        const int n = wn * TN + fn * 16 + 4 * g;
-        if (n >= n_rows) continue;
-        YT *d = y + (size_t)m * ldy + n;
-        const f32x4 v = acc[fn][fm];
-        if constexpr (sizeof(YT) == 4) {
-          if (vec && n + 4 <= n_rows) *reinterpret_cast<f32x4 *>(d) = v;
-          else
-            for (int e = 0; e < 4 && n + e < n_rows; e++) d[e] = v[e];
-        } else {
-          uint32_t h[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) h[e] = bf16_rne_nb(v[e]);
-          if (vec && n + 4 <= n_rows) *reinterpret_cast<u32x2 *>(d) = (u32x2){h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
-          else
-            for (int e = 0; e < 4 && n + e < n_rows; e++) d[e] = (uint16_t)h[e];
-        }
-      }
-    }
+    fp8_store<FN, FM>(acc, y, ldy, (wave % WM) * TM + (lane & 15), (wave / WM) * TN + 4 * (lane >> 4), m_rows, n_rows,
+                      vec);
   }
 };
 

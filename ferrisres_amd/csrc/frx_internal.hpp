@@ -348,8 +348,8 @@ struct Fp8Plan {
   int tile;     // FP8_T_*
   int S, per;   // K slices, blocks of 128 in each (FP8_T_SKINNY: 1, 16-row tiles of a workgroup)
 };
-enum { FP8_T_256 = 0, FP8_T_128 = 1, FP8_T_64 = 2, FP8_T_32 = 3, FP8_T_SKINNY = 4 };
-Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int cus);
+enum { FP8_T_SKINNY = 0, FP8_T_128 = 1, FP8_T_RING8 = 2, FP8_T_RING6 = 3, FP8_T_RING4 = 4 };
+Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, int cus);
 size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p);
 hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
                              const float *sb, int b_rows, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
