@@ -1515,6 +1515,9 @@ static bool aligned_to(const void *p, size_t n) { return reinterpret_cast<uintpt
 static bool is_dtype(frx_dtype t) { return t == FRX_F32 || t == FRX_BF16; }
 static size_t dtype_bytes(frx_dtype t) { return t == FRX_BF16 ? 2 : 4; }
 constexpr uint32_t kMaxDim = 0x7FFFFF00u;
+// a launch holds less than 2^32 work-items: so many workgroups of 256, half as
+// many tiles of 512
+constexpr size_t kMaxWgs = ((size_t)1 << 24) - 1;
 // a tile of 256 rows is addressed by 32-bit offsets
 constexpr size_t kMaxCodeLd = (size_t)1 << 23;
 
@@ -1536,7 +1539,7 @@ frx_status frx_fp8_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t 
   if (!aligned_to(x, dtype_bytes(xt)) || !aligned_to(q, 16) || !aligned_to(scale, 4))
     return fail(ctx, FRX_ERR_SHAPE, "x and scale must be aligned to their elements, q to 16 bytes");
   const size_t kb = (K + 127) / 128, mb = (M + 127) / 128;
-  if ((blocks == FRX_FP8_ROWS ? ((size_t)M * kb + 15) / 16 : kb * mb) > 0x7FFFFFFFu)
+  if ((blocks == FRX_FP8_ROWS ? ((size_t)M * kb + 15) / 16 : kb * mb) > kMaxWgs)
     return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
   const hipError_t e = frx::launch_fp8_quantize(x, xt == FRX_BF16, M, K, ldx, (int)blocks, code == FRX_FP8_E5M2, q,
                                                 ldq, scale, ctx->stream);
@@ -1554,7 +1557,7 @@ static frx_status check_fp8(frx_ctx *ctx, const void *a, size_t lda, frx_fp8 at,
   if (K % 16 != 0) return fail(ctx, FRX_ERR_SHAPE, "%u columns of codes must be a multiple of 16", K);
   if (lda % 16 != 0 || ldb % 16 != 0 || lda < K || ldb < K || lda > kMaxCodeLd || ldb > kMaxCodeLd)
     return fail(ctx, FRX_ERR_SHAPE, "lda=%zu and ldb=%zu must be multiples of 16 from %u to 2^23", lda, ldb, K);
-  if (M > kMaxDim || N > kMaxDim || (size_t)((M + 31) / 32) * ((N + 63) / 64) > 0x3FFFFFFFu)
+  if (M > kMaxDim || N > kMaxDim || ((size_t)(M + 63) / 64 + frx::FP8_MAXE) * ((N + 127) / 128) > kMaxWgs)
     return fail(ctx, FRX_ERR_SHAPE, "M=%u N=%u too large", M, N);
   if (!aligned_to(a, 16) || !aligned_to(sa, 4))
     return fail(ctx, FRX_ERR_SHAPE, "codes must be 16-byte aligned, scales 4-byte");
@@ -1617,7 +1620,7 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
     return FRX_OK;
   }
   const size_t kb = (K + 127) / 128, codes = a256((size_t)M * K), need = codes + (size_t)M * kb * 4;
-  if (((size_t)M * kb + 15) / 16 > 0x7FFFFFFFu) return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
+  if (((size_t)M * kb + 15) / 16 > kMaxWgs) return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
   if (!may_grow(ctx, ctx->q8_ws_bytes, need))
     return fail(ctx, FRX_ERR_UNSUPPORTED, "the first call at this size allocates and cannot be captured into a graph");
   if ((st = ensure_buffer(ctx, &ctx->q8_ws, &ctx->q8_ws_bytes, need, "fp8 activation workspace allocation")) != FRX_OK)
@@ -1672,6 +1675,10 @@ size_t frx_moe_rows_capacity(uint32_t T, uint32_t top_k, uint32_t E, uint32_t al
   return (n + align - 1) / align * align;
 }
 
+// Rows and columns stay below this: a launch holds less than 2^32 work-items
+// and 65536 workgroups in y.
+constexpr uint32_t kMaxRows = 1u << 24;
+
 static frx_status check_rows(frx_ctx *ctx, const frx_moe_rows *r, frx::RouteRows *out) {
   if (!r || !r->offsets || !r->row_of || !r->slot_of) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
   if (r->T == 0) return fail(ctx, FRX_ERR_SHAPE, "no tokens");
@@ -1680,7 +1687,7 @@ static frx_status check_rows(frx_ctx *ctx, const frx_moe_rows *r, frx::RouteRows
   if (r->align == 0 || r->align > 128 || (r->align & (r->align - 1)))
     return fail(ctx, FRX_ERR_SHAPE, "align=%u must be a power of two up to 128", r->align);
   const size_t need = frx_moe_rows_capacity(r->T, r->top_k, r->E, r->align);
-  if (need > 0x3FFFFFFFu || r->R > 0x3FFFFFFFu) return fail(ctx, FRX_ERR_SHAPE, "T=%u R=%u too large", r->T, r->R);
+  if (need >= kMaxRows || r->R >= kMaxRows) return fail(ctx, FRX_ERR_SHAPE, "T=%u R=%u: 2^24 rows or more", r->T, r->R);
   if (r->R < need) return fail(ctx, FRX_ERR_SHAPE, "R=%u holds fewer than the %zu rows there may be", r->R, need);
   if (!aligned_to(r->offsets, 4) || !aligned_to(r->row_of, 4) || !aligned_to(r->slot_of, 4))
     return fail(ctx, FRX_ERR_SHAPE, "the index arrays must be 4-byte aligned");
@@ -1727,7 +1734,7 @@ frx_status frx_moe_combine(frx_ctx *ctx, const void *ys, frx_dtype st_, const fr
   frx::RouteRows r;
   if (!ys || !y) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
   if (!is_dtype(st_) || !is_dtype(yt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
-  if (H == 0 || H > (1u << 28)) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^28]", H);
+  if (H == 0 || H >= kMaxRows) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^24)", H);
   if (!aligned_to(ys, dtype_bytes(st_)) || !aligned_to(y, dtype_bytes(yt)) || !aligned_to(w, 4))
     return fail(ctx, FRX_ERR_SHAPE, "ys, y and w must be aligned to their elements");
   if ((st = check_rows(ctx, rows, &r)) != FRX_OK) return st;
@@ -1744,7 +1751,7 @@ frx_status frx_moe_combine_backward(frx_ctx *ctx, const void *dy, frx_dtype dt, 
   if (!dy || !dys) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
   if (!ys != !dw) return fail(ctx, FRX_ERR_SHAPE, "ys and dw come together");
   if (!is_dtype(dt) || !is_dtype(st_)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
-  if (H == 0 || H > (1u << 28)) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^28]", H);
+  if (H == 0 || H >= kMaxRows) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^24)", H);
   if (!aligned_to(dy, dtype_bytes(dt)) || !aligned_to(ys, dtype_bytes(st_)) || !aligned_to(dys, dtype_bytes(st_)) ||
       !aligned_to(w, 4) || !aligned_to(dw, 4))
     return fail(ctx, FRX_ERR_SHAPE, "dy, ys, dys, w and dw must be aligned to their elements");

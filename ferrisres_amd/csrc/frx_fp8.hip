@@ -51,10 +51,11 @@ template <int GM>
 __device__ __forceinline__ void xcd_tile(uint32_t bid, uint32_t mts, uint32_t nts, uint32_t &mt, uint32_t &nt) {
   const uint32_t total = mts * nts, q = total / 8, r = total % 8, xcd = bid % 8, i = bid / 8;
   const uint32_t lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + i;
-  const uint32_t group = lin / (GM * nts), rest = lin - group * (GM * nts);
-  const uint32_t gm = min((uint32_t)GM, mts - group * GM);
+  const uint32_t rows = min((uint32_t)GM, mts);  // (GM * nts may pass 32 bits)
+  const uint32_t group = lin / (rows * nts), rest = lin - group * (rows * nts);
+  const uint32_t gm = min(rows, mts - group * rows);
   nt = rest / gm;
-  mt = group * GM + rest - nt * gm;
+  mt = group * rows + rest - nt * gm;
 }
 
 template <typename Tile, bool BR1, typename YT>
@@ -123,25 +124,26 @@ __device__ __forceinline__ int expert_tile(const uint32_t *offsets, int E, uint3
   return e;
 }
 
-template <int BM, int BN, int WM, int WN, bool E5M2, typename YT>
-__global__ __launch_bounds__(WM *WN * 64, 2) void fp8_grouped_kernel(const GroupArgs p) {
-  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, false, sizeof(YT) == 4>;
+// mts: tiles of rows there may be. An XCD's run of tiles goes down the rows
+// first: the tiles of an expert's rows share its weights in that L2.
+template <typename Tile, typename YT>
+__global__ __launch_bounds__(Tile::NT, 2) void fp8_grouped_kernel(const GroupArgs p, uint32_t mts) {
   extern __shared__ __align__(16) uint32_t lds[];
-  const uint32_t nts = (p.N + BN - 1) / BN;
-  const uint32_t mt = blockIdx.x / nts, nt = blockIdx.x - mt * nts;
+  constexpr int BM = Tile::BM, BN = Tile::BN;
+  uint32_t mt, nt;
+  xcd_tile<0x40000000>(blockIdx.x, mts, (p.N + BN - 1) / BN, mt, nt);
   uint32_t m0, end;
   const int e = expert_tile<BM>(p.offsets, p.E, p.R, mt, m0, end);
   if (e < 0) return;
   const uint32_t n0 = nt * BN;
   Fp8Operands o;
   fill_operands<false>(o, p.a, p.lda, p.sa, p.b[e], p.ldb, p.sb[e], m0, min((uint32_t)BM, end - m0), n0,
-                                     min((uint32_t)BN, p.N - n0), p.K);
+                       min((uint32_t)BN, p.N - n0), p.K);
   o.kb0 = 0;
   o.kb1 = (int)((p.K + 127) >> 7);
   f32x4 acc[Tile::FN][Tile::FM];
   Tile::run(lds, o, acc);
-  const size_t at = (size_t)m0 * p.N + n0;
-  Tile::template store<YT>(acc, (YT *)p.y + at, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
+  Tile::template store<YT>(acc, (YT *)p.y + (size_t)m0 * p.N + n0, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
 }
 
 template <int RT, bool E5M2, bool BR1, typename XT, typename YT>
@@ -224,6 +226,9 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float *__restrict__
   }
 }
 
+// Workgroups of 512 in a launch: it holds less than 2^32 work-items.
+constexpr size_t FP8_MAX_TILES = (size_t)1 << 23;
+
 template <typename K, typename A>
 hipError_t go(K kernel, int lds, std::atomic<uint64_t> &done, dim3 grid, int nt, hipStream_t stream, const A &args) {
   const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), lds, done);
@@ -236,14 +241,15 @@ template <typename Tile, bool BR1, typename YT>
 hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const size_t tiles = (size_t)((p.M + Tile::BM - 1) / Tile::BM) * ((p.N + Tile::BN - 1) / Tile::BN);
-  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
   return go(fp8_dense_kernel<Tile, BR1, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, 1, S), Tile::NT, stream, p);
 }
 
 template <bool E5M2, bool BR1, typename YT>
 hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
   constexpr bool WIDE = sizeof(YT) == 4;
-  if (tile == FP8_T_RING4) return dense_go<Fp8Ring<4, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
+  if constexpr (!(BR1 && WIDE))
+    if (tile == FP8_T_RING4) return dense_go<Fp8Ring<4, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
   if constexpr (!BR1)
     if (tile == FP8_T_RING6) return dense_go<Fp8Ring<6, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
   if constexpr (!BR1 && !WIDE)
@@ -284,14 +290,41 @@ hipError_t dense_any(int e5m2, int b_rows, int tile, const DenseArgs &p, int S, 
   return e5m2 ? dense_tile<true, false, YT>(tile, p, S, stream) : dense_tile<false, false, YT>(tile, p, S, stream);
 }
 
-template <int BM, int BN, bool E5M2, typename YT>
+template <typename Tile, typename YT>
 hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  using Tile = Fp8Tile<BM, BN, 2, 2, E5M2, false, sizeof(YT) == 4>;
-  const size_t tiles = ((size_t)(p.R + BM - 1) / BM + p.E) * ((p.N + BN - 1) / BN);
-  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
-  return go(fp8_grouped_kernel<BM, BN, 2, 2, E5M2, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles), Tile::NT, stream,
-            p);
+  const size_t mts = (size_t)(p.R + Tile::BM - 1) / Tile::BM + p.E, tiles = mts * ((p.N + Tile::BN - 1) / Tile::BN);
+  if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(fp8_grouped_kernel<Tile, YT>), Tile::LDS_BYTES, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((fp8_grouped_kernel<Tile, YT>), dim3((unsigned)tiles), dim3(Tile::NT), Tile::LDS_BYTES, stream, p,
+                     (uint32_t)mts);
+  return hipGetLastError();
+}
+
+// The lengths of the groups are not known here, so the tile is chosen for equal
+// ones: R / E rows and half a tile of remainder each. steps * ns a round, a
+// round the tiles that a compute unit holds at once. Measured, us, 8 experts,
+// bf16, K -> N (64 x 128 / 128 x 256 / 256 x 256): 12 rows 2048 -> 5632
+// 21.4 / 21.7 / 26.1; 64 rows 33 / 25 / 30; 128 rows 42 / 45 / 34, 5632 -> 2048
+// 51 / 54 / 66; 256 rows 59 / 49 / 66; 384 rows 77 / 72 / 72; 1024 rows 173 / 143 / 143.
+double grouped_cost(const GroupArgs &p, uint32_t bm, uint32_t bn, double ns, double alone, int cus) {
+  const double rows = (double)p.R / p.E / bm + 0.5;
+  const double tiles = p.E * (rows < 1 ? 1 : rows) * ((p.N + bn - 1) / bn);
+  return std::max(alone, ns * std::ceil(tiles / cus));
+}
+
+template <bool E5M2, typename YT>
+hipError_t grouped_tile(const GroupArgs &p, int cus, hipStream_t stream) {
+  constexpr bool WIDE = sizeof(YT) == 4;
+  const double c64 = grouped_cost(p, 64, 128, WIDE ? 600 : 430, 1000, cus);
+  const double c128 = grouped_cost(p, 128, 256, WIDE ? 1800 : 1010, 0, cus);
+  if constexpr (!WIDE) {
+    if (grouped_cost(p, 256, 256, 1460, 0, cus) < std::min(c64, c128))
+      return grouped_go<Fp8Ring<8, E5M2, false, false>, YT>(p, stream);
+  }
+  return c128 < c64 ? grouped_go<Fp8Ring<4, E5M2, false, WIDE>, YT>(p, stream)
+                    : grouped_go<Fp8Tile<64, 128, 2, 2, E5M2, false, WIDE>, YT>(p, stream);
 }
 
 template <int BM, int BN, bool E5M2, typename YT>
@@ -299,7 +332,7 @@ hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   using Tile = Fp8Tile<BM, BN, 2, 2, E5M2, true, sizeof(YT) == 4>;
   const size_t tiles = (size_t)((p.N + BM - 1) / BM) * ((p.K + BN - 1) / BN);
-  if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
   return go(fp8_grad_kernel<BM, BN, 2, 2, E5M2, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, (unsigned)E),
             Tile::NT, stream, p);
 }
@@ -321,8 +354,11 @@ struct TileCost {
 constexpr TileCost kNarrow[] = {{FP8_T_RING8, 256, 256, 1, 1460}, {FP8_T_RING6, 192, 256, 1, 1130},
                                 {FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
 constexpr TileCost kWide[] = {{FP8_T_RING6, 192, 256, 1, 2600}, {FP8_T_RING4, 128, 256, 1, 1800},
-                              {FP8_T_128, 128, 128, 2, 1750}};
-constexpr TileCost kWideRows[] = {{FP8_T_RING4, 128, 256, 1, 2200}, {FP8_T_128, 128, 128, 2, 2150}};
+                              {FP8_T_128, 128, 128, 2, 1870}};
+// A scale per weight row (weight gradients): sixteen more multiplies a product,
+// taller tiles run out of registers; on the bf16 pipe 128 x 256 takes 2200.
+constexpr TileCost kNarrowRows[] = {{FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
+constexpr TileCost kWideRows[] = {{FP8_T_128, 128, 128, 2, 2150}};
 
 Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, int cus) {
   if (M <= 16) {
@@ -340,13 +376,12 @@ Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, in
     return {FP8_T_SKINNY, 1, best};
   }
   const int steps = (int)((K + 127) / 128);
-  const TileCost *costs = yt_bf16 ? kNarrow : b_rows == 1 ? kWideRows : kWide;
-  const int count = yt_bf16 ? 4 : b_rows == 1 ? 2 : 3;
+  const TileCost *costs = b_rows == 1 ? (yt_bf16 ? kNarrowRows : kWideRows) : yt_bf16 ? kNarrow : kWide;
+  const int count = b_rows == 1 ? (yt_bf16 ? 2 : 1) : yt_bf16 ? 4 : 3;
   Fp8Plan plan = {FP8_T_128, 1, steps};
   double least = 1e30;
   for (int t = 0; t < count; t++) {
     const TileCost &c = costs[t];
-    if (yt_bf16 && b_rows == 1 && c.tile != FP8_T_RING4 && c.tile != FP8_T_128) continue;  // not built
     const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
     // a K slice more: fewer steps, but every part is written and read (4 bytes a value at
     // about 4 TB/s) and the parts joined by another launch (4 us)
@@ -409,9 +444,10 @@ hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const floa
     p.b[e] = b[e];
     p.sb[e] = sb[e];
   }
-  if (R <= 8u * (uint32_t)E) {
-    const size_t tiles = ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16);
-    if (tiles > 0x7FFFFFFFu) return hipErrorInvalidValue;
+  // us, 8 experts, 16-row tiles / 64 x 128: 2 rows 5632 -> 2048 19.4 / 40.1, 2048 -> 5632 20.7 / 21.2,
+  // 1024^2 5.1 / 8.2; 8 rows 22.5 / 40.1, 24.2 / 21.3, 5.4 / 8.1
+  const size_t tiles = ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16);
+  if (R <= 8u * (uint32_t)E && tiles < FP8_MAX_TILES) {
     const dim3 grid((unsigned)tiles), block(FP8_SK_WAVES * 64);
     constexpr int lds = (int)fp8_skinny_red_bytes(1);
     if (yt_bf16) {
@@ -423,8 +459,8 @@ hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const floa
     }
     return hipGetLastError();
   }
-  if (yt_bf16) return e5m2 ? grouped_go<64, 128, true, uint16_t>(p, stream) : grouped_go<64, 128, false, uint16_t>(p, stream);
-  return e5m2 ? grouped_go<64, 128, true, float>(p, stream) : grouped_go<64, 128, false, float>(p, stream);
+  if (yt_bf16) return e5m2 ? grouped_tile<true, uint16_t>(p, cus, stream) : grouped_tile<false, uint16_t>(p, cus, stream);
+  return e5m2 ? grouped_tile<true, float>(p, cus, stream) : grouped_tile<false, float>(p, cus, stream);
 }
 
 hipError_t launch_fp8_grad_weight(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b,

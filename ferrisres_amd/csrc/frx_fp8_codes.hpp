@@ -25,6 +25,13 @@ __device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d
   }
 }
 
+// The first n of eight codes, zeros behind them.
+__device__ __forceinline__ u32x2 fp8_keep(u32x2 c, uint32_t n) {
+  c.x &= n >= 4 ? ~0u : (1u << (8 * n)) - 1;
+  c.y &= n >= 8 ? ~0u : n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1;
+  return c;
+}
+
 __device__ __forceinline__ float ld1(const float *p) { return *p; }
 __device__ __forceinline__ float ld1(const uint16_t *p) { return bf16_to_f32(*p); }
 

@@ -40,19 +40,17 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const XT *__restrict__ x,
   const float s = fp8_block_codes<E5M2>(v, c);
   if (k < ((K + 15) & ~15u)) {
     // a value past K has no code of its block, whatever its scale
-    if (k + 8 > K) {
-      const uint32_t n = k < K ? K - k : 0;
-      c.x &= n >= 4 ? ~0u : (1u << (8 * n)) - 1;
-      c.y &= n <= 4 ? 0u : (1u << (8 * (n - 4))) - 1;
-    }
-    *reinterpret_cast<u32x2 *>(q + (size_t)m * ldq + k) = c;
+    *reinterpret_cast<u32x2 *>(q + (size_t)m * ldq + k) = fp8_keep(c, k < K ? min(8u, K - k) : 0);
   }
   if ((threadIdx.x & 15) == 0) scale[blk] = s;
 }
 
-// A 128 x 128 tile of x per workgroup of 256: thread (wave w, lane l) holds
-// rows 32w .. 32w + 31 of columns 2l and 2l + 1. The codes go through LDS so
-// that whole 128-byte rows of q are written.
+// A 128 x 128 tile of x per workgroup of 256: thread (wave w, lane group h of
+// 16, lane c of it) holds rows 32w + 8h .. + 7 of columns 8c .. 8c + 7, read 16
+// bytes of bf16 (32 of f32) a row. Codes that keep x's order go straight to q
+// (128 bytes of a row from 16 lanes); transposed ones through LDS, a column's
+// 8 rows as 8 bytes, in chunks XOR-swizzled by column / 8 so that the 16 lanes
+// of a group hit different banks.
 //   COLS: a scale per column (its 128 rows), q transposed
 //   TILES, TILES_T: one scale
 template <typename XT, bool E5M2, int BLOCKS, bool VEC>
@@ -60,101 +58,94 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(const XT *__restrict__ x,
                                                        uint8_t *__restrict__ q, size_t ldq,
                                                        float *__restrict__ scale) {
   constexpr bool T = BLOCKS != FRXQ_TILES;
-  constexpr int PITCH = 128 + 16;  // bytes of a staged row
-  __shared__ __align__(16) uint8_t st[128 * PITCH];
+  __shared__ __align__(16) u32x2 st[T ? 128 * 16 : 1];
   __shared__ uint32_t red[4][128];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 4, c = lane & 15;
   const uint32_t kb = (K + 127) / 128, mb = (M + 127) / 128;
   const uint32_t mt = blockIdx.x / kb, kt = blockIdx.x - mt * kb;
-  const uint32_t k = kt * 128 + 2 * lane, m0 = mt * 128 + 32 * wave;
-  float v[32][2];
+  const uint32_t k = kt * 128 + 8 * c, m0 = mt * 128 + 32 * wave + 8 * h;
+  float v[8][8];
 #pragma unroll
-  for (int i = 0; i < 32; i++) {
-    const uint32_t m = m0 + i;
-    v[i][0] = v[i][1] = 0.0f;
-    if (m < M) {
-      const XT *src = x + (size_t)m * ldx + k;
-      if (VEC && k + 2 <= K) {
-        if constexpr (sizeof(XT) == 2) {
-          const uint32_t p = *reinterpret_cast<const uint32_t *>(src);
-          v[i][0] = __uint_as_float(p << 16);
-          v[i][1] = __uint_as_float(p & 0xFFFF0000u);
-        } else {
-          const float2 p = *reinterpret_cast<const float2 *>(src);
-          v[i][0] = p.x;
-          v[i][1] = p.y;
-        }
-      } else {
-        if (k < K) v[i][0] = ld1(src);
-        if (k + 1 < K) v[i][1] = ld1(src + 1);
-      }
+  for (int i = 0; i < 8; i++) {
+    const XT *src = x + (size_t)(m0 + i) * ldx + k;
+    if (m0 + i < M && VEC && k + 8 <= K) {
+      ld8v(src, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[i][j] = m0 + i < M && k + j < K ? ld1(src + j) : 0.0f;
     }
   }
-  uint32_t mx[2] = {0, 0};
+  uint32_t mx[8];
 #pragma unroll
-  for (int i = 0; i < 32; i++)
+  for (int j = 0; j < 8; j++) {
+    mx[j] = 0;
 #pragma unroll
-    for (int c = 0; c < 2; c++) mx[c] = max(mx[c], __float_as_uint(v[i][c]) & FP8_MAG);
+    for (int i = 0; i < 8; i++) mx[j] = max(mx[j], __float_as_uint(v[i][j]) & FP8_MAG);
+  }
+  float s[8], inv[8];
   if constexpr (BLOCKS == FRXQ_COLS) {
-    red[wave][2 * lane] = mx[0];
-    red[wave][2 * lane + 1] = mx[1];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      mx[j] = max(mx[j], (uint32_t)__shfl_xor((int)mx[j], 16));
+      mx[j] = max(mx[j], (uint32_t)__shfl_xor((int)mx[j], 32));
+      if (h == 0) red[wave][8 * c + j] = mx[j];
+    }
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < 2; c++)
+    for (int j = 0; j < 8; j++) {
+      s[j] = fp8_scale<E5M2>(max(max(red[0][8 * c + j], red[1][8 * c + j]), max(red[2][8 * c + j], red[3][8 * c + j])));
+      inv[j] = 1.0f / s[j];
+    }
+    if (threadIdx.x < 16)
 #pragma unroll
-      for (int w = 0; w < 4; w++) mx[c] = max(mx[c], red[w][2 * lane + c]);
+      for (int j = 0; j < 8; j++)
+        if (k + j < K) scale[(size_t)(k + j) * mb + mt] = s[j];
   } else {
-    uint32_t m = max(mx[0], mx[1]);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) m = max(m, mx[j]);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
     if (lane == 0) red[wave][0] = m;
     __syncthreads();
-    m = max(max(red[0][0], red[1][0]), max(red[2][0], red[3][0]));
-    mx[0] = mx[1] = m;
-  }
-  float s[2], inv[2];
+    s[0] = fp8_scale<E5M2>(max(max(red[0][0], red[1][0]), max(red[2][0], red[3][0])));
+    inv[0] = 1.0f / s[0];
 #pragma unroll
-  for (int c = 0; c < 2; c++) {
-    s[c] = fp8_scale<E5M2>(mx[c]);
-    inv[c] = 1.0f / s[c];
+    for (int j = 1; j < 8; j++) inv[j] = inv[0];
+    if (threadIdx.x == 0) scale[BLOCKS == FRXQ_TILES ? (size_t)mt * kb + kt : (size_t)kt * mb + mt] = s[0];
   }
-  if constexpr (BLOCKS == FRXQ_COLS) {
-    if (wave == 0) {
-      if (k < K) scale[(size_t)k * mb + mt] = s[0];
-      if (k + 1 < K) scale[(size_t)(k + 1) * mb + mt] = s[1];
+  // a place past M or K holds a zero, but a scale that is no number would make
+  // it a NaN: bytes of such places are cleared
+  if constexpr (!T) {
+    const uint32_t n = k < K ? min(8u, K - k) : 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (m0 + i >= M || k >= ((K + 15) & ~15u)) continue;
+      u32x2 w;
+      w.x = fp8_pack4<E5M2>(v[i][0] * inv[0], v[i][1] * inv[1], v[i][2] * inv[2], v[i][3] * inv[3]);
+      w.y = fp8_pack4<E5M2>(v[i][4] * inv[4], v[i][5] * inv[5], v[i][6] * inv[6], v[i][7] * inv[7]);
+      *reinterpret_cast<u32x2 *>(q + (size_t)(m0 + i) * ldq + k) = fp8_keep(w, n);
     }
-  } else if (threadIdx.x == 0) {
-    scale[BLOCKS == FRXQ_TILES ? (size_t)mt * kb + kt : (size_t)kt * mb + mt] = s[0];
-  }
-  // a place past M or K holds a zero, but a scale that is no number would make it a NaN
-  const uint32_t rows = m0 < M ? min(32u, M - m0) : 0;
-  if constexpr (T) {
-#pragma unroll
-    for (int c = 0; c < 2; c++)
-#pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        uint32_t w = fp8_pack4<E5M2>(v[i][c] * inv[c], v[i + 1][c] * inv[c], v[i + 2][c] * inv[c],
-                                     v[i + 3][c] * inv[c]);
-        if (rows < (uint32_t)i + 4) w &= rows <= (uint32_t)i ? 0u : (1u << (8 * (rows - i))) - 1;
-        *reinterpret_cast<uint32_t *>(st + (2 * lane + c) * PITCH + 32 * wave + i) = w;
-      }
   } else {
-    const uint32_t keep = k + 1 < K ? 0xFFFFu : k < K ? 0xFFu : 0u;
+    const uint32_t n = m0 < M ? min(8u, M - m0) : 0;
 #pragma unroll
-    for (int i = 0; i < 32; i++)
-      *reinterpret_cast<uint16_t *>(st + (32 * wave + i) * PITCH + 2 * lane) =
-          (uint16_t)(fp8_pack4<E5M2>(v[i][0] * inv[0], v[i][1] * inv[1], 0.f, 0.f) & keep);
-  }
-  __syncthreads();
-  // rows of q: 8 lanes of 16 bytes each
-  const uint32_t qrows = T ? K : M, qcols = ((T ? M : K) + 15) & ~15u;
-  const uint32_t r0 = (T ? kt : mt) * 128, c0 = (T ? mt : kt) * 128;
+    for (int j = 0; j < 8; j++) {
+      u32x2 w;
+      w.x = fp8_pack4<E5M2>(v[0][j] * inv[j], v[1][j] * inv[j], v[2][j] * inv[j], v[3][j] * inv[j]);
+      w.y = fp8_pack4<E5M2>(v[4][j] * inv[j], v[5][j] * inv[j], v[6][j] * inv[j], v[7][j] * inv[j]);
+      st[(8 * c + j) * 16 + ((4 * wave + h) ^ c)] = fp8_keep(w, n);
+    }
+    __syncthreads();
+    // rows of q: 8 lanes of 16 bytes (two chunks, exchanged where the swizzle is odd) each
+    const uint32_t r0 = kt * 128, c0 = mt * 128, qcols = (M + 15) & ~15u;
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const uint32_t r = (threadIdx.x >> 3) + 32 * i, c = (threadIdx.x & 7) * 16;
-    if (r0 + r < qrows && c0 + c < qcols)
-      *reinterpret_cast<u32x4 *>(q + (size_t)(r0 + r) * ldq + c0 + c) =
-          *reinterpret_cast<const u32x4 *>(st + r * PITCH + c);
+    for (int i = 0; i < 4; i++) {
+      const uint32_t r = (threadIdx.x >> 3) + 32 * i, p = threadIdx.x & 7, z = r >> 3;
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(&st[r * 16 + ((2 * p) ^ (z & ~1u))]);
+      if (r0 + r < K && c0 + 16 * p < qcols)
+        *reinterpret_cast<u32x4 *>(q + (size_t)(r0 + r) * ldq + c0 + 16 * p) =
+            z & 1 ? (u32x4){w.z, w.w, w.x, w.y} : w;
+    }
   }
 }
 
@@ -162,15 +153,14 @@ template <typename XT, bool E5M2>
 hipError_t quantize_t(const XT *x, uint32_t M, uint32_t K, size_t ldx, int blocks, uint8_t *q, size_t ldq,
                       float *scale, hipStream_t stream) {
   const uint32_t kb = (K + 127) / 128, mb = (M + 127) / 128;
+  const bool vec = ((reinterpret_cast<uintptr_t>(x) | (ldx * sizeof(XT))) & 15) == 0;
   if (blocks == FRXQ_ROWS) {
-    const bool vec = ((reinterpret_cast<uintptr_t>(x) | (ldx * sizeof(XT))) & 15) == 0;
     const size_t wgs = ((size_t)M * kb + 15) / 16;
     if (wgs > 0x7FFFFFFFu) return hipErrorInvalidValue;
     const auto fn = vec ? fp8_rows_kernel<XT, E5M2, true> : fp8_rows_kernel<XT, E5M2, false>;
     hipLaunchKernelGGL(fn, dim3((unsigned)wgs), dim3(256), 0, stream, x, M, K, ldx, kb, q, ldq, scale);
     return hipGetLastError();
   }
-  const bool vec = ((reinterpret_cast<uintptr_t>(x) | (ldx * sizeof(XT))) & (2 * sizeof(XT) - 1)) == 0;
   using Fn = void (*)(const XT *, uint32_t, uint32_t, size_t, uint8_t *, size_t, float *);
   Fn fn;
   if (blocks == FRXQ_COLS) fn = vec ? fp8_tile_kernel<XT, E5M2, FRXQ_COLS, true> : fp8_tile_kernel<XT, E5M2, FRXQ_COLS, false>;

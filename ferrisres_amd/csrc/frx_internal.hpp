@@ -378,7 +378,7 @@ struct RouteRows {
 };
 // Slots up to which one workgroup sorts; above, counts by chunk in `hist`
 // (route_sort_bytes) and a second launch.
-constexpr size_t ROUTE_ONE_WG = 4096;
+constexpr int ROUTE_ONE_WG = 4096;
 size_t route_sort_bytes(const RouteRows &r);
 hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, int *hist, hipStream_t stream);
 hipError_t launch_route_dispatch(const void *x, size_t row_bytes, const RouteRows &r, void *xs, hipStream_t stream);

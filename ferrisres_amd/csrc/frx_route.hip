@@ -15,7 +15,8 @@ namespace {
 constexpr int ROUTE_MAXE = 64;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
-constexpr int SORT_NT = 1024;  // slots of a chunk, one a thread
+constexpr int SORT_NT = 1024;     // slots of a chunk, one a thread
+constexpr int ROUTE_RUNS = 1024;  // runs of chunks: each reads the counts of all
 
 // Counts of one chunk by expert, wave by wave, and each thread's rank among
 // the slots of its expert in its wave. e >= E: no expert. A wave finds the
@@ -23,6 +24,7 @@ constexpr int SORT_NT = 1024;  // slots of a chunk, one a thread
 __device__ __forceinline__ int chunk_ranks(uint32_t e, int E, int (*wave_cnt)[ROUTE_MAXE]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   wave_cnt[wave][lane] = 0;
+  __builtin_amdgcn_wave_barrier();  // lanes of one wave: its LDS stores keep their order
   const bool in = e < (uint32_t)E;
   unsigned long long same = __ballot(in);
 #pragma unroll
@@ -100,31 +102,34 @@ __global__ __launch_bounds__(SORT_NT) void route_sort_kernel(const uint32_t *__r
   }
 }
 
-// Many chunks, a workgroup each: hist[chunk][expert], then (a launch later)
-// every workgroup adds up the chunks before its own.
-__global__ __launch_bounds__(SORT_NT) void route_count_kernel(const uint32_t *__restrict__ idx, int A, int E,
+// Many chunks: runs of `per` of them (1 up to ROUTE_RUNS chunks), a workgroup a
+// run. hist[run][expert], then (a launch later) every workgroup adds up the runs
+// before its own.
+__global__ __launch_bounds__(SORT_NT) void route_count_kernel(const uint32_t *__restrict__ idx, int A, int E, int per,
                                                               int *__restrict__ hist) {
   __shared__ int wave_cnt[16][ROUTE_MAXE];
-  const int a = blockIdx.x * SORT_NT + threadIdx.x;
-  chunk_ranks(a < A ? idx[a] : kNone, E, wave_cnt);
-  __syncthreads();
-  if (threadIdx.x < ROUTE_MAXE) {
-    int s = 0;
-    for (int w = 0; w < 16; w++) s += wave_cnt[w][threadIdx.x];
-    hist[blockIdx.x * ROUTE_MAXE + threadIdx.x] = s;
+  const int tid = threadIdx.x, first = blockIdx.x * per * SORT_NT;
+  int s = 0;
+  for (int a = first; a < A && a < first + per * SORT_NT; a += SORT_NT) {
+    if (a > first) __syncthreads();  // the counts before are added up
+    chunk_ranks(a + tid < A ? idx[a + tid] : kNone, E, wave_cnt);
+    __syncthreads();
+    if (tid < ROUTE_MAXE)
+      for (int w = 0; w < 16; w++) s += wave_cnt[w][tid];
   }
+  if (tid < ROUTE_MAXE) hist[blockIdx.x * ROUTE_MAXE + tid] = s;
 }
 
-__global__ __launch_bounds__(SORT_NT) void route_place_kernel(const uint32_t *__restrict__ idx, RouteRows r,
+__global__ __launch_bounds__(SORT_NT) void route_place_kernel(const uint32_t *__restrict__ idx, RouteRows r, int per,
                                                               const int *__restrict__ hist) {
   __shared__ int wave_cnt[16][ROUTE_MAXE];
-  __shared__ int part[2][16][ROUTE_MAXE];  // counts of the chunks before this one; of all
-  __shared__ int first[ROUTE_MAXE], count[ROUTE_MAXE], end;
+  __shared__ int part[2][16][ROUTE_MAXE];  // counts of the runs before this one; of all
+  __shared__ int first[ROUTE_MAXE], count[ROUTE_MAXE], base[ROUTE_MAXE], end;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int A = r.T * r.top_k, E = r.E, G = gridDim.x, g = blockIdx.x;
-  const int a = g * SORT_NT + tid;
-  const uint32_t e = a < A ? idx[a] : kNone;
-  const int rank = chunk_ranks(e, E, wave_cnt);
+  const int a0 = g * per * SORT_NT;
+  uint32_t e = a0 + tid < A ? idx[a0 + tid] : kNone;
+  int rank = chunk_ranks(e, E, wave_cnt);
   int before = 0, all = 0;
   for (int c = wave; c < G; c += 16) {
     const int h = hist[c * ROUTE_MAXE + lane];
@@ -144,30 +149,41 @@ __global__ __launch_bounds__(SORT_NT) void route_place_kernel(const uint32_t *__
     const int at = wave_before(c);
     first[lane] = at;
     count[lane] = all;
+    base[lane] = at + before;
     if (lane == 63) end = at + c;
-    part[0][0][lane] = before;
     if (g == 0) {
       if (lane < E) r.offsets[lane] = (uint32_t)at;
       if (lane == 63) r.offsets[E] = (uint32_t)(at + c);
     }
   }
   __syncthreads();
-  if (a < A) {
-    uint32_t row = kNone;
-    if (e < (uint32_t)E) {
-      int at = first[e] + part[0][0][e];
-      for (int w = 0; w < wave; w++) at += wave_cnt[w][e];
-      row = (uint32_t)(at + rank);
-      r.slot_of[row] = (uint32_t)a;
+  for (int a = a0;;) {
+    if (a + tid < A) {
+      uint32_t row = kNone;
+      if (e < (uint32_t)E) {
+        int at = base[e];
+        for (int w = 0; w < wave; w++) at += wave_cnt[w][e];
+        row = (uint32_t)(at + rank);
+        r.slot_of[row] = (uint32_t)(a + tid);
+      }
+      r.row_of[a + tid] = row;
     }
-    r.row_of[a] = row;
+    a += SORT_NT;
+    if (a >= A || a >= a0 + per * SORT_NT) break;
+    __syncthreads();
+    if (tid < ROUTE_MAXE)
+      for (int w = 0; w < 16; w++) base[tid] += wave_cnt[w][tid];
+    __syncthreads();
+    e = a + tid < A ? idx[a + tid] : kNone;
+    rank = chunk_ranks(e, E, wave_cnt);
+    __syncthreads();
   }
   // rows of no route: between the segments (a wave an expert), and from the end on
   for (int x = g * 16 + wave; x < E; x += G * 16) {
     const int z = x + 1 < E ? first[x + 1] : end;
     for (int i = first[x] + count[x] + lane; i < z; i += 64) r.slot_of[i] = kNone;
   }
-  for (int i = end + a; i < r.R; i += G * SORT_NT) r.slot_of[i] = kNone;
+  for (int i = end + g * SORT_NT + tid; i < r.R; i += G * SORT_NT) r.slot_of[i] = kNone;
 }
 
 // One row per wave, W bytes per lane and load.
@@ -266,8 +282,8 @@ __global__ __launch_bounds__(256) void route_combine_kernel(const ST *__restrict
 }
 
 // A wave a route: dy's row is read once for each of its token's routes, from
-// cache after the first (neighbouring waves). Then waves of 64 rows each look
-// for rows of no route.
+// cache after the first (neighbouring waves). Then (align > 1) a wave a row,
+// for those of no route.
 template <typename DT, typename ST, int Q>
 __global__ __launch_bounds__(256) void route_combine_backward_kernel(const DT *__restrict__ dy,
                                                                      const ST *__restrict__ ys, RouteRows r,
@@ -278,13 +294,10 @@ __global__ __launch_bounds__(256) void route_combine_backward_kernel(const DT *_
   const uint32_t A = (uint32_t)r.T * (uint32_t)r.top_k;
   const uint32_t slot = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (slot >= A) {
-    const uint32_t r0 = (slot - A) * 64, end = min(r.offsets[r.E], (uint32_t)r.R);
-    unsigned long long none = __ballot(r0 + lane < end && r.slot_of[min(r0 + lane, (uint32_t)r.R - 1)] == kNone);
-    for (; none; none &= none - 1) {
-      const float z[Q] = {};
-      ST *d = dys + (size_t)(r0 + __ffsll(none) - 1) * H;
-      for (uint32_t h = lane * Q; h < H; h += 64 * Q) stq<Q>(d + h, z);
-    }
+    const uint32_t row = slot - A;
+    if (row >= (uint32_t)r.R || row >= r.offsets[r.E] || r.slot_of[row] != kNone) return;
+    const float z[Q] = {};
+    for (uint32_t h = lane * Q; h < H; h += 64 * Q) stq<Q>(dys + (size_t)row * H + h, z);
     return;
   }
   const uint32_t row = r.row_of[slot];
@@ -317,9 +330,16 @@ __global__ __launch_bounds__(256) void route_combine_backward_kernel(const DT *_
 
 }  // namespace
 
+// Chunks of a run, and the runs there are.
+static int sort_runs(const RouteRows &r, int &per) {
+  const int chunks = (r.T * r.top_k + SORT_NT - 1) / SORT_NT;
+  per = (chunks + ROUTE_RUNS - 1) / ROUTE_RUNS;
+  return (chunks + per - 1) / per;
+}
+
 size_t route_sort_bytes(const RouteRows &r) {
-  const size_t A = (size_t)r.T * r.top_k;
-  return A <= ROUTE_ONE_WG ? 0 : (A + SORT_NT - 1) / SORT_NT * ROUTE_MAXE * sizeof(int);
+  int per;
+  return r.T * r.top_k <= ROUTE_ONE_WG ? 0 : sort_runs(r, per) * ROUTE_MAXE * sizeof(int);
 }
 
 hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, int *hist, hipStream_t stream) {
@@ -327,10 +347,10 @@ hipError_t launch_route_sort(const uint32_t *idx, const RouteRows &r, int *hist,
     hipLaunchKernelGGL(route_sort_kernel, dim3(1), dim3(SORT_NT), 0, stream, idx, r);
     return hipGetLastError();
   }
-  const int A = r.T * r.top_k;
-  const dim3 grid((A + SORT_NT - 1) / SORT_NT);
-  hipLaunchKernelGGL(route_count_kernel, grid, dim3(SORT_NT), 0, stream, idx, A, r.E, hist);
-  hipLaunchKernelGGL(route_place_kernel, grid, dim3(SORT_NT), 0, stream, idx, r, hist);
+  int per;
+  const dim3 grid(sort_runs(r, per));
+  hipLaunchKernelGGL(route_count_kernel, grid, dim3(SORT_NT), 0, stream, idx, r.T * r.top_k, r.E, per, hist);
+  hipLaunchKernelGGL(route_place_kernel, grid, dim3(SORT_NT), 0, stream, idx, r, per, hist);
   return hipGetLastError();
 }
 
@@ -385,7 +405,7 @@ template <typename DT, typename ST>
 static hipError_t combine_backward_t(const void *dy, const void *ys, const RouteRows &r, const float *w, void *dys,
                                      float *dw, uint32_t H, hipStream_t stream) {
   constexpr int Q = sizeof(DT) == 4 && sizeof(ST) == 4 ? 4 : 8;
-  const size_t waves = (size_t)r.T * r.top_k + (r.align > 1 ? ((size_t)r.R + 63) / 64 : 0);
+  const size_t waves = (size_t)r.T * r.top_k + (r.align > 1 ? r.R : 0);
   const dim3 grid((unsigned)((waves + 3) / 4));
   if (rows16(dy, ys, dys, (size_t)H * 2) && H % Q == 0)
     hipLaunchKernelGGL((route_combine_backward_kernel<DT, ST, Q>), grid, dim3(256), 0, stream,

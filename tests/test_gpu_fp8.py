@@ -487,3 +487,78 @@ def test_runs_are_repeatable(ctx, m, k, n):
     for y in ys:
         ctx.fp8_linear(a, sa, b, sb, y)
     assert all(torch.equal(ys[0], y) for y in ys[1:])
+
+
+@pytest.mark.parametrize("m,k,n", [(2000, 272, 6000), (2500, 272, 3600), (38400, 144, 100)])
+@pytest.mark.parametrize("code,b_rows,out", [(E5M2, 128, "bf16"), (E4M3, 128, "f32"), (E4M3, 1, "bf16")])
+def test_linear_over_many_tokens(ctx, m, k, n, code, b_rows, out):
+    """Enough tiles for the widest ones, and a tall narrow product."""
+    a, sa, av = operand(m + k, m, k, code)
+    b, sb, bv = operand(n + k + 1, n, k, E4M3, tiles=b_rows == 128)
+    y = torch.full((m, n), float("nan"), dtype=DT[out], device=DEV)
+    ctx.fp8_linear(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), y)
+    check(y, av @ bv.t(), av.abs() @ bv.abs().t(), k)
+
+
+@pytest.mark.parametrize("rows,code,out", [(1200, E4M3, "bf16"), (2400, E5M2, "bf16"), (2400, E4M3, "bf16"),
+                                           (1920, E5M2, "f32"), (1920, E4M3, "f32")])
+def test_grouped_over_many_rows(ctx, rows, code, out):
+    """Groups of many rows and of none or one, odd widths, rows behind the last group."""
+    k, n, E, behind = 272, 3001, 8, 7
+    sizes = [rows // 3, 0, rows // 8, 1, 129, rows // 6, 127]
+    sizes.append(rows - behind - sum(sizes))
+    off = np.concatenate([[0], np.cumsum(sizes)])
+    a, sa, av = operand(k + rows, rows, k, code)
+    ops = [operand(7 + e, n, k, E4M3, tiles=True) for e in range(E)]
+    y = torch.full((rows, n), 5.0, dtype=DT[out], device=DEV)
+    ctx.fp8_linear_grouped(a.to(DEV), sa.to(DEV), [o[0].to(DEV) for o in ops], [o[1].to(DEV) for o in ops],
+                           torch.tensor(off, dtype=torch.int32, device=DEV), y)
+    for e in range(E):
+        i, j = int(off[e]), int(off[e + 1])
+        if j > i:
+            check(y[i:j], av[i:j] @ ops[e][2].t(), av[i:j].abs() @ ops[e][2].abs().t(), k)
+    assert (y[int(off[-1]):] == 5.0).all()
+
+
+def test_split_product_first_under_capture(ctx):
+    """A product that would split K, captured by a context that never ran: it needs no workspace and keeps its
+    answer over replays; afterwards the same context allocates and splits."""
+    c = frx.Context(0)
+    side = torch.cuda.Stream()
+    c.set_stream(side)
+    m, k, n = 64, 5632, 640
+    a, sa, av = operand(1, m, k, E4M3)
+    b, sb, bv = operand(2, n, k, E4M3, tiles=True)
+    a, sa, b, sb = (t.to(DEV) for t in (a, sa, b, sb))
+    y = torch.zeros((m, n), device=DEV)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        c.fp8_linear(a, sa, b, sb, y)
+    for _ in range(3):
+        y.fill_(-1.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        check(y, av @ bv.t(), av.abs() @ bv.abs().t(), k)
+        y.fill_(-1.0)
+        torch.cuda.synchronize()
+        c.fp8_linear(a, sa, b, sb, y)
+        c.synchronize()
+        check(y, av @ bv.t(), av.abs() @ bv.abs().t(), k)
+    del g
+    c.close()
+
+
+def test_sizes_past_a_launch_are_refused(ctx):
+    """Shapes of more work-items than a launch holds, before anything is read."""
+    t = torch.zeros((64,), device=DEV)
+    p, L, h = t.data_ptr(), frx.lib(), ctx._h
+    shape = L.frx_fp8_linear(h, p, 16, 0, p, p, 16, p, 128, p, 0, 1, 24, 1)  # K of no multiple of 16: a shape error
+    assert shape != 0
+    assert L.frx_fp8_linear(h, p, 16, 0, p, p, 16, p, 128, p, 0, 1 << 30, 16, 1) == shape
+    assert L.frx_fp8_linear(h, p, 16, 0, p, p, 16, p, 128, p, 0, 1, 16, 1 << 30) == shape
+    assert L.frx_fp8_quantize(h, p, 0, 1 << 30, 16, 16, frx.FP8_ROWS, 0, p, 16, p) == shape
+    assert L.frx_fp8_linear_act(h, p, 0, p, 16, p, p, 0, 1 << 30, 16, 1) == shape
+    torch.cuda.synchronize()
+    assert not t.any()

@@ -4,6 +4,8 @@ training step of an expert layer through all of them.
 The sort is integers, the dispatch copies, dys one f32 product: compared bit for bit. A combination rounds each product
 and each of its top_k additions once, 2^-24 relative to the sum of the magnitudes, and then to its output type; a dot
 product over H terms any order of H additions and a rounding of each product."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -406,3 +408,42 @@ def test_refusals(ctx):
             call()
     with pytest.raises(TypeError):
         ctx.moe_combine(f(8, 8).half(), rows, None, f(4, 8))
+
+
+@pytest.mark.parametrize("T,top_k,E,align,how", [(700001, 2, 5, 128, "holes"), (1048577, 1, 64, 1, "any")])
+def test_sort_of_very_many(ctx, T, top_k, E, align, how):
+    """More chunks of slots than workgroups that count them."""
+    idx = routes(T + E, T, top_k, E, how)
+    rows = make(ctx, idx, E, align, extra=1000)
+    flat = np.where((idx >= 0) & (idx < E), idx, E).reshape(-1)
+    order = np.argsort(flat, kind="stable")
+    count = np.bincount(flat, minlength=E + 1)[:E]
+    off = np.concatenate([[0], np.cumsum(-(-count // align) * align)])
+    row_of, slot_of = np.full(T * top_k, -1, np.int64), np.full(rows.R, -1, np.int64)
+    at = 0
+    for e in range(E):
+        slots = order[at:at + count[e]]
+        at += count[e]
+        row_of[slots] = off[e] + np.arange(count[e])
+        slot_of[off[e]:off[e] + count[e]] = slots
+    assert np.array_equal(rows.offsets.cpu().numpy(), off)
+    assert np.array_equal(rows.row_of.cpu().numpy().reshape(-1), row_of)
+    assert np.array_equal(rows.slot_of.cpu().numpy(), slot_of)
+
+
+def test_sizes_past_a_launch_are_refused(ctx):
+    """Rows and columns of more than a launch holds, before anything is read."""
+    rows = frx.MoeRows.empty(4, 2, 3, 1, device=DEV)
+    t = torch.zeros((64,), device=DEV)
+    p, L, h = t.data_ptr(), frx.lib(), ctx._h
+    small = rows._c
+    shape = L.frx_moe_combine(h, p, 0, ctypes.byref(small), None, p, 0, 0)
+    assert shape != 0
+    assert L.frx_moe_combine(h, p, 0, ctypes.byref(small), None, p, 0, 1 << 24) == shape
+    assert L.frx_moe_combine_backward(h, p, 0, None, 0, ctypes.byref(small), None, p, None, 1 << 24) == shape
+    big = type(small).from_buffer_copy(small)
+    big.T, big.R = 1 << 23, 1 << 24
+    assert L.frx_moe_sort(h, p, ctypes.byref(big)) == shape
+    assert L.frx_moe_dispatch(h, p, 4, ctypes.byref(big), p) == shape
+    torch.cuda.synchronize()
+    assert not t.any()
