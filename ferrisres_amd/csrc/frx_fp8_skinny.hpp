@@ -104,7 +104,11 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
     wrow[r] = p.b + (size_t)min(n0 + 16 * r + l16, p.N - 1) * p.ldb;
     if (BR1) srow[r] = p.sb + (size_t)(n0 + 16 * r + 4 * g) * kbs;
   }
-  const float *sblk = p.sb + (size_t)(n0 >> 7) * kbs;  // uniform (BR1: unused)
+  // the row tiles' scales, uniform: three tiles may run over a block's end
+  constexpr int NB = BR1 ? 0 : 128 % (16 * RT) == 0 ? 1 : RT;
+  const float *sblk[RT];
+#pragma unroll
+  for (int r = 0; r < NB; r++) sblk[r] = p.sb + (size_t)(min(n0 + 16 * r, p.N - 1) >> 7) * kbs;
   f32x4 acc[RT];
 #pragma unroll
   for (int r = 0; r < RT; r++) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -136,14 +140,16 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
       if (kb * 128 + 16 * g >= K) xlo = (u32x4){0, 0, 0, 0};
       if (kb * 128 + 64 + 16 * g >= K) xhi = (u32x4){0, 0, 0, 0};
     }
-    if (!BR1) s *= sblk[kb];
+    float sw[RT];
+#pragma unroll
+    for (int r = 0; r < NB; r++) sw[r] = s * sblk[r][kb];
     const auto x = Pipe::template op<E5M2>(fp8_join(xlo, xhi));
 #pragma unroll
     for (int r = 0; r < RT; r++) {
       const f32x4 q = Pipe::template mul<E5M2>(Pipe::template op<false>(fp8_join(wlo[r], whi[r])), x);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        float f = s;
+        float f = BR1 ? s : sw[NB == RT ? r : 0];
         if (BR1) f *= n0 + 16 * r + 4 * g + e < p.N ? srow[r][(size_t)e * kbs + kb] : 0.f;
         acc[r][e] += q[e] * f;
       }

@@ -562,3 +562,22 @@ def test_sizes_past_a_launch_are_refused(ctx):
     assert L.frx_fp8_linear_act(h, p, 0, p, 16, p, p, 0, 1 << 30, 16, 1) == shape
     torch.cuda.synchronize()
     assert not t.any()
+
+
+@pytest.mark.parametrize("m,n", [(1, 4112), (4, 8208), (16, 11008), (3, 11000), (16, 15001)])
+@pytest.mark.parametrize("code,b_rows,out", [(E4M3, 128, "bf16"), (E5M2, 128, "f32"), (E4M3, 1, "f32")])
+def test_linear_of_few_tokens_over_many_rows(ctx, m, n, code, b_rows, out):
+    """Two to four row tiles a workgroup, with blocks of 128 rows that end inside one's run; the form that quantises."""
+    k = 272
+    a, sa, av = operand(m + n, m, k, code)
+    b, sb, bv = operand(n + k, n, k, E4M3, tiles=b_rows == 128)
+    y = torch.full((m, n), float("nan"), dtype=DT[out], device=DEV)
+    ctx.fp8_linear(a.to(DEV), sa.to(DEV), b.to(DEV), sb.to(DEV), y)
+    check(y, av @ bv.t(), av.abs() @ bv.abs().t(), k)
+    if b_rows == 128 and code == E4M3:
+        x = values(n, m, k, "bf16").to(DEV)
+        _, q, s, _ = quantize(ctx, x, frx.FP8_ROWS, E4M3)
+        ctx.fp8_linear(q, s, b.to(DEV), sb.to(DEV), y)
+        y2 = torch.full_like(y, float("nan"))
+        ctx.fp8_linear_act(x, b.to(DEV), sb.to(DEV), y2)
+        assert torch.equal(y, y2)
