@@ -83,10 +83,10 @@ __device__ __forceinline__ void fp8_skinny_quantize(const Fp8Skinny &p, uint8_t 
   }
 }
 
-template <int RT, bool E5M2, bool BR1, typename XT, typename YT>
+template <int RT, bool E5M2, bool BR1, bool WIDE, typename XT, typename YT>
 __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x4 *red) {
   constexpr bool CODES = sizeof(XT) == 1;
-  using Pipe = Fp8Pipe<sizeof(YT) == 4>;
+  using Pipe = Fp8Pipe<WIDE>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const int K = (int)p.K, kbs = (K + 127) >> 7;

@@ -581,3 +581,22 @@ def test_linear_of_few_tokens_over_many_rows(ctx, m, n, code, b_rows, out):
         y2 = torch.full_like(y, float("nan"))
         ctx.fp8_linear_act(x, b.to(DEV), sb.to(DEV), y2)
         assert torch.equal(y, y2)
+
+
+@pytest.mark.parametrize("sizes", [[3, 0, 5, 1], [64, 200, 0, 129], [700, 650, 800, 1]])
+def test_gradient_rows_are_rounded_once(ctx, sizes):
+    """E5M2 rows times the experts' weights: the bf16 result is the f32 one rounded, so that a token of one route gets
+    its gradient with no error but that rounding's."""
+    k, n = 528, 300
+    off = np.concatenate([[0], np.cumsum(sizes)])
+    a, sa, av = operand(3, int(off[-1]), k, E5M2)
+    ops = [operand(7 + e, n, k, E4M3, tiles=True) for e in range(len(sizes))]
+    b, sb = [o[0].to(DEV) for o in ops], [o[1].to(DEV) for o in ops]
+    y = [torch.empty((int(off[-1]), n), dtype=t, device=DEV) for t in (torch.float32, torch.bfloat16)]
+    for out in y:
+        ctx.fp8_linear_grouped(a.to(DEV), sa.to(DEV), b, sb, torch.tensor(off, dtype=torch.int32, device=DEV), out)
+    assert torch.equal(y[0].bfloat16(), y[1])
+    for e in range(len(sizes)):
+        i, j = int(off[e]), int(off[e + 1])
+        if j > i:
+            check(y[0][i:j], av[i:j] @ ops[e][2].t(), av[i:j].abs() @ ops[e][2].abs().t(), k)
