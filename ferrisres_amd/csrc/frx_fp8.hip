@@ -154,10 +154,10 @@ __global__ __launch_bounds__(Tile::NT, 2) void fp8_grouped_kernel(const GroupArg
   Tile::template store<YT>(acc, (YT *)p.y + (size_t)m0 * p.N + n0, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
 }
 
-template <int RT, bool E5M2, bool BR1, typename XT, typename YT>
+template <int RT, int TT, bool E5M2, bool BR1, typename XT, typename YT>
 __global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_kernel(const Fp8Skinny p) {
   extern __shared__ __align__(16) uint32_t lds[];
-  fp8_skinny<RT, E5M2, BR1, sizeof(YT) == 4, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
+  fp8_skinny<RT, TT, E5M2, BR1, sizeof(YT) == 4, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
 // Sorted rows in tiles of 16 (decode batches: a few rows of each expert).
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_grouped_kernel(c
   const uint32_t kbs = (p.K + 127) >> 7;
   const Fp8Skinny q = {p.a + (size_t)m0 * p.lda, p.sa + (size_t)m0 * kbs, p.b[e], p.sb[e],
                        static_cast<YT *>(p.y) + (size_t)m0 * p.N, p.lda, p.ldb, min(16u, end - m0), p.K, p.N, 0};
-  fp8_skinny<RT, E5M2, false, fp8_grouped_wide<E5M2, YT>, uint8_t, YT>(q, nt * 16 * RT, reinterpret_cast<f32x4 *>(lds));
+  fp8_skinny<RT, 1, E5M2, false, fp8_grouped_wide<E5M2, YT>, uint8_t, YT>(q, nt * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
 // Weight gradients: expert blockIdx.y sums over the blocks of its rows. Here
@@ -265,30 +265,39 @@ hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
   return dense_go<Fp8Tile<128, 128, 2, 2, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
 }
 
-template <int RT, bool E5M2, bool BR1, typename XT, typename YT>
+template <int RT, int TT, bool E5M2, bool BR1, typename XT, typename YT>
 hipError_t skinny_rt(const Fp8Skinny &p, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  constexpr int most = (int)fp8_skinny_red_bytes(RT) + (sizeof(XT) == 1 ? 0 : (int)FP8_ACT_MAX_BYTES);
-  const auto kernel = fp8_skinny_kernel<RT, E5M2, BR1, XT, YT>;
-  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), most, done);
+  constexpr size_t red = fp8_skinny_red_bytes(RT * TT);
+  const auto kernel = fp8_skinny_kernel<RT, TT, E5M2, BR1, XT, YT>;
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel),
+                                  (int)(red + (sizeof(XT) == 1 ? 0 : FP8_ACT_MAX_BYTES)), done);
   if (e != hipSuccess) return e;
-  const size_t lds = fp8_skinny_red_bytes(RT) + (sizeof(XT) == 1 ? 0 : fp8_skinny_act_bytes(p.M, p.K));
+  const size_t lds = red + (sizeof(XT) == 1 ? 0 : fp8_skinny_act_bytes(p.M, p.K));
   hipLaunchKernelGGL(kernel, dim3((p.N + 16 * RT - 1) / (16 * RT)), dim3(FP8_SK_WAVES * 64), lds, stream, p);
   return hipGetLastError();
 }
 
-template <bool E5M2, bool BR1, typename XT, typename YT>
+template <int TT, bool E5M2, bool BR1, typename XT, typename YT>
 hipError_t skinny_go(int rt, const Fp8Skinny &p, hipStream_t stream) {
-  if (rt == 4) return skinny_rt<4, E5M2, BR1, XT, YT>(p, stream);
-  if (rt == 3) return skinny_rt<3, E5M2, BR1, XT, YT>(p, stream);
-  if (rt == 2) return skinny_rt<2, E5M2, BR1, XT, YT>(p, stream);
-  return skinny_rt<1, E5M2, BR1, XT, YT>(p, stream);
+  if constexpr (TT <= 2) {
+    if (rt == 4) return skinny_rt<4, TT, E5M2, BR1, XT, YT>(p, stream);
+    if (rt == 3) return skinny_rt<3, TT, E5M2, BR1, XT, YT>(p, stream);
+  }
+  if (rt == 2) return skinny_rt<2, TT, E5M2, BR1, XT, YT>(p, stream);
+  return skinny_rt<1, TT, E5M2, BR1, XT, YT>(p, stream);
+}
+
+template <bool E5M2, bool BR1, typename YT>
+hipError_t skinny_tt(int rt, const Fp8Skinny &p, hipStream_t stream) {
+  if (p.M > 32) return skinny_go<4, E5M2, BR1, uint8_t, YT>(rt, p, stream);
+  return p.M > 16 ? skinny_go<2, E5M2, BR1, uint8_t, YT>(rt, p, stream) : skinny_go<1, E5M2, BR1, uint8_t, YT>(rt, p, stream);
 }
 
 template <typename YT>
 hipError_t skinny_any(int e5m2, int b_rows, int rt, const Fp8Skinny &p, hipStream_t stream) {
-  if (b_rows == 1) return e5m2 ? skinny_go<true, true, uint8_t, YT>(rt, p, stream) : skinny_go<false, true, uint8_t, YT>(rt, p, stream);
-  return e5m2 ? skinny_go<true, false, uint8_t, YT>(rt, p, stream) : skinny_go<false, false, uint8_t, YT>(rt, p, stream);
+  if (b_rows == 1) return e5m2 ? skinny_tt<true, true, YT>(rt, p, stream) : skinny_tt<false, true, YT>(rt, p, stream);
+  return e5m2 ? skinny_tt<true, false, YT>(rt, p, stream) : skinny_tt<false, false, YT>(rt, p, stream);
 }
 
 // fn<E5M2, BR1 or none, YT>(args) for run-time choices of them.
@@ -373,12 +382,18 @@ constexpr TileCost kNarrowRows[] = {{FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128
 constexpr TileCost kWideRows[] = {{FP8_T_128, 128, 128, 2, 2150}};
 
 Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, int cus) {
-  if (M <= 16) {
+  // Few tokens: no join, no tile of 128 mostly empty. Up to 32 always (us, against tiles of 128 x 256
+  // in K slices: 32 tokens, K x N 1024^2 4.1 / 9.6, 4096^2 10.2 / 14.7, 4096 x 11008 15.7 / 17.4, 11008 x 4096
+  // 20.9 / 20.1), up to 64 while two row tiles a workgroup cover N and the waves' slices of K are short, since
+  // every workgroup reads all tokens (64 tokens, 1024^2 5.7 / 10.8, 4096^2 14.5 / 17.5, 4096 x 8192 17.8 / 18.9,
+  // f32 2048 x 5632 10.9 / 19.7; 40 tokens f32 5120^2 20.7 / 21.0; 11008 x 4096 31.1 / 22.4).
+  const int steps = (int)((K + 127) / 128), most = M <= 32 ? 4 : 2;  // row tiles a workgroup
+  if (M <= 32 || (M <= 64 && N <= 32u * cus && steps <= 40)) {
     // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
     const uint32_t tiles = (N + 15) / 16;
     int best = 1;
     uint32_t least = ~0u;
-    for (int rt = 1; rt <= 4; rt++) {
+    for (int rt = 1; rt <= most; rt++) {
       const uint32_t wgs = (tiles + rt - 1) / rt, rounds = (wgs + cus - 1) / cus * rt;
       if (rounds <= least) {
         least = rounds;
@@ -387,7 +402,6 @@ Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, in
     }
     return {FP8_T_SKINNY, 1, best};
   }
-  const int steps = (int)((K + 127) / 128);
   const TileCost *costs = b_rows == 1 ? (yt_bf16 ? kNarrowRows : kWideRows) : yt_bf16 ? kNarrow : kWide;
   const int count = b_rows == 1 ? (yt_bf16 ? 2 : 1) : yt_bf16 ? 4 : 3;
   Fp8Plan plan = {FP8_T_128, 1, steps};
@@ -442,10 +456,10 @@ hipError_t launch_fp8_linear_act(const void *x, int xt_bf16, const uint8_t *b, s
   const int vec = ((reinterpret_cast<uintptr_t>(x) | (size_t)K * (xt_bf16 ? 2 : 4)) & 15) == 0;
   const Fp8Skinny p = {x, nullptr, b, sb, y, K, ldb, M, K, N, vec};
   if (xt_bf16)
-    return yt_bf16 ? skinny_go<false, false, uint16_t, uint16_t>(plan.per, p, stream)
-                   : skinny_go<false, false, uint16_t, float>(plan.per, p, stream);
-  return yt_bf16 ? skinny_go<false, false, float, uint16_t>(plan.per, p, stream)
-                 : skinny_go<false, false, float, float>(plan.per, p, stream);
+    return yt_bf16 ? skinny_go<1, false, false, uint16_t, uint16_t>(plan.per, p, stream)
+                   : skinny_go<1, false, false, uint16_t, float>(plan.per, p, stream);
+  return yt_bf16 ? skinny_go<1, false, false, float, uint16_t>(plan.per, p, stream)
+                 : skinny_go<1, false, false, float, float>(plan.per, p, stream);
 }
 
 hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *const *b,

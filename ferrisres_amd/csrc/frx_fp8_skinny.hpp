@@ -1,4 +1,4 @@
-// frx_fp8_skinny.hpp — the 8-bit product for up to 16 tokens.
+// frx_fp8_skinny.hpp — the 8-bit product for up to 32 tokens.
 //
 // Bound by the weights' bytes: each is read once, straight into registers (a
 // lane of an MFMA operand holds 32 codes of one row: two 16-byte loads, 64
@@ -35,7 +35,7 @@ struct Fp8Skinny {
   void *y;         // of the first token
   size_t lda;      // elements of a
   size_t ldb;
-  uint32_t M, K, N;  // M: 1 to 16
+  uint32_t M, K, N;  // M: 1 to 16 * TT
   int vec;         // activations: rows 16-byte aligned
 };
 
@@ -43,7 +43,7 @@ constexpr int FP8_SK_WAVES = 8;
 
 // Dynamic LDS of a workgroup: the slices' sums; behind them the codes and
 // scales that it makes of activations.
-__host__ __device__ constexpr size_t fp8_skinny_red_bytes(int rt) { return (size_t)FP8_SK_WAVES * rt * 64 * 16; }
+__host__ __device__ constexpr size_t fp8_skinny_red_bytes(int tiles) { return (size_t)FP8_SK_WAVES * tiles * 64 * 16; }
 __host__ __device__ constexpr size_t fp8_skinny_act_bytes(uint32_t M, uint32_t K) {
   return (size_t)M * K + (size_t)M * ((K + 127) >> 7) * 4;
 }
@@ -83,7 +83,7 @@ __device__ __forceinline__ void fp8_skinny_quantize(const Fp8Skinny &p, uint8_t 
   }
 }
 
-template <int RT, bool E5M2, bool BR1, bool WIDE, typename XT, typename YT>
+template <int RT, int TT, bool E5M2, bool BR1, bool WIDE, typename XT, typename YT>
 __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x4 *red) {
   constexpr bool CODES = sizeof(XT) == 1;
   using Pipe = Fp8Pipe<WIDE>;
@@ -92,11 +92,16 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
   const int K = (int)p.K, kbs = (K + 127) >> 7;
   const int per = (kbs + FP8_SK_WAVES - 1) / FP8_SK_WAVES;
   const int kb0 = wave * per, kb1 = min(kb0 + per, kbs);
-  const uint32_t tok = min((uint32_t)l16, p.M - 1);
-  uint8_t *codes = reinterpret_cast<uint8_t *>(red) + fp8_skinny_red_bytes(RT);
+  uint8_t *codes = reinterpret_cast<uint8_t *>(red) + fp8_skinny_red_bytes(RT * TT);
   float *scales = reinterpret_cast<float *>(codes + (size_t)p.M * K);
-  const uint8_t *xrow = CODES ? static_cast<const uint8_t *>(p.a) + (size_t)tok * p.lda : codes + (size_t)tok * K;
-  const float *sx = (CODES ? p.sa : scales) + (size_t)tok * kbs;
+  const uint8_t *xrow[TT];
+  const float *sx[TT];
+#pragma unroll
+  for (int t = 0; t < TT; t++) {
+    const uint32_t tok = min((uint32_t)(16 * t + l16), p.M - 1);
+    xrow[t] = CODES ? static_cast<const uint8_t *>(p.a) + (size_t)tok * p.lda : codes + (size_t)tok * K;
+    sx[t] = (CODES ? p.sa : scales) + (size_t)tok * kbs;
+  }
   const uint8_t *wrow[RT];
   const float *srow[RT];
 #pragma unroll
@@ -109,9 +114,11 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
   const float *sblk[RT];
 #pragma unroll
   for (int r = 0; r < NB; r++) sblk[r] = p.sb + (size_t)(min(n0 + 16 * r, p.N - 1) >> 7) * kbs;
-  f32x4 acc[RT];
+  f32x4 acc[RT][TT];
 #pragma unroll
-  for (int r = 0; r < RT; r++) acc[r] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < RT; r++)
+#pragma unroll
+    for (int t = 0; t < TT; t++) acc[r][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   u32x4 wlo[RT], whi[RT];
   if constexpr (!CODES) {
     // a wave without blocks loads the last one's weights and drops them
@@ -120,53 +127,63 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
     fp8_skinny_quantize<XT>(p, codes, scales);
     __syncthreads();
   }
-  float s4 = 0.f;  // scales of four blocks: lane (token, g) has the g-th's
+  float s4[TT] = {};  // scales of four blocks: lane (token, g) has the g-th's
   for (int kb = kb0; kb < kb1; kb++) {
     if (CODES || kb > kb0) {
 #pragma unroll
       for (int r = 0; r < RT; r++) fp8_row_load(wrow[r], kb * 128, K, g, wlo[r], whi[r]);
     }
-    u32x4 xlo, xhi;
-    fp8_row_load(xrow, kb * 128, K, g, xlo, xhi);
-    float s;
-    if constexpr (CODES) {
-      const int j = (kb - kb0) & 3;
-      if (j == 0) s4 = sx[min(kb + g, kb1 - 1)];
-      s = __shfl(s4, 16 * j + l16);
-    } else {
-      s = sx[kb];
-    }
-    if (kb * 128 + 128 > K) {  // pieces past K: zeros on the token side
-      if (kb * 128 + 16 * g >= K) xlo = (u32x4){0, 0, 0, 0};
-      if (kb * 128 + 64 + 16 * g >= K) xhi = (u32x4){0, 0, 0, 0};
-    }
-    float sw[RT];
+    typename Pipe::Op x[TT];
+    float s[TT];
 #pragma unroll
-    for (int r = 0; r < NB; r++) sw[r] = s * sblk[r][kb];
-    const auto x = Pipe::template op<E5M2>(fp8_join(xlo, xhi));
+    for (int t = 0; t < TT; t++) {
+      u32x4 xlo, xhi;
+      fp8_row_load(xrow[t], kb * 128, K, g, xlo, xhi);
+      if constexpr (CODES) {
+        const int j = (kb - kb0) & 3;
+        if (j == 0) s4[t] = sx[t][min(kb + g, kb1 - 1)];
+        s[t] = __shfl(s4[t], 16 * j + l16);
+      } else {
+        s[t] = sx[t][kb];
+      }
+      if (kb * 128 + 128 > K) {  // pieces past K: zeros on the token side
+        if (kb * 128 + 16 * g >= K) xlo = (u32x4){0, 0, 0, 0};
+        if (kb * 128 + 64 + 16 * g >= K) xhi = (u32x4){0, 0, 0, 0};
+      }
+      x[t] = Pipe::template op<E5M2>(fp8_join(xlo, xhi));
+    }
+    float sb[RT];
+#pragma unroll
+    for (int r = 0; r < NB; r++) sb[r] = sblk[r][kb];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
-      const f32x4 q = Pipe::template mul<E5M2>(Pipe::template op<false>(fp8_join(wlo[r], whi[r])), x);
+      const auto w = Pipe::template op<false>(fp8_join(wlo[r], whi[r]));
+      float sw[4];
+      if (BR1)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float f = BR1 ? s : sw[NB == RT ? r : 0];
-        if (BR1) f *= n0 + 16 * r + 4 * g + e < p.N ? srow[r][(size_t)e * kbs + kb] : 0.f;
-        acc[r][e] += q[e] * f;
+        for (int e = 0; e < 4; e++) sw[e] = n0 + 16 * r + 4 * g + e < p.N ? srow[r][(size_t)e * kbs + kb] : 0.f;
+#pragma unroll
+      for (int t = 0; t < TT; t++) {
+        const f32x4 q = Pipe::template mul<E5M2>(w, x[t]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[r][t][e] += q[e] * (s[t] * (BR1 ? sw[e] : sb[NB == RT ? r : 0]));
       }
     }
   }
   // the slices, in order
 #pragma unroll
-  for (int r = 0; r < RT; r++) red[(wave * RT + r) * 64 + lane] = acc[r];
+  for (int r = 0; r < RT; r++)
+#pragma unroll
+    for (int t = 0; t < TT; t++) red[(wave * RT * TT + r * TT + t) * 64 + lane] = acc[r][t];
   __syncthreads();
-  static_assert(RT <= FP8_SK_WAVES, "a wave each for the row tiles");
-  if (wave >= RT) return;
+  static_assert(RT * TT <= FP8_SK_WAVES, "a wave each for the tiles");
+  if (wave >= RT * TT) return;
   f32x4 v = red[wave * 64 + lane];
 #pragma unroll
-  for (int w = 1; w < FP8_SK_WAVES; w++) v += red[(w * RT + wave) * 64 + lane];
-  const uint32_t n = n0 + 16 * wave + 4 * g;
-  if ((uint32_t)l16 >= p.M || n >= p.N) return;
-  YT *d = static_cast<YT *>(p.y) + (size_t)l16 * p.N + n;
+  for (int w = 1; w < FP8_SK_WAVES; w++) v += red[(w * RT * TT + wave) * 64 + lane];
+  const uint32_t n = n0 + 16 * (wave / TT) + 4 * g, m = 16 * (wave % TT) + l16;
+  if (m >= p.M || n >= p.N) return;
+  YT *d = static_cast<YT *>(p.y) + (size_t)m * p.N + n;
   const bool vec = ((reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(YT) - 1)) | (p.N & 3)) == 0;
   if constexpr (sizeof(YT) == 4) {
     if (vec) *reinterpret_cast<f32x4 *>(d) = v;
