@@ -339,6 +339,8 @@ def _per_expert(ts, E, shape, dtype, name, rows=False):
     """(array.array of E device addresses, row stride) of a stacked tensor [E, ...]
     or a list of E tensors; rows: 2-D with unit column stride, all of one row
     stride, else contiguous."""
+    if E < 1:
+        raise _shape_err("offsets [E + 1] must be of at least one expert")
     if len(ts) != E:
         raise _shape_err(f"{name} holds {len(ts)} experts, expected {E}")
     if hasattr(ts, "dim"):  # stacked
@@ -692,7 +694,7 @@ class Context:
             raise TypeError(f"b must be float8_e4m3fn, got {b.dtype}")
         kb = (K + 127) // 128
         _dense(sa, (M, kb), torch.float32, "sa")
-        b_rows = 1 if sb.shape[0] == N else 128
+        b_rows = 1 if len(sb) == N else 128
         _dense(sb, (N if b_rows == 1 else (N + 127) // 128, kb), torch.float32, "sb")
         _dense(y, (M, N), None, "y")
         _check(lib().frx_fp8_linear(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(), b.data_ptr(), ldb,
@@ -703,7 +705,7 @@ class Context:
         """frx_fp8_linear_act: y = x w^T for f32 or bf16 x [M][K], quantised on
         the way, and FP8_TILES weights b [N][K], sb [ceil(N/128)][ceil(K/128)]."""
         torch = _torch or _tt()
-        M, K = x.shape
+        M, K, _ = _rows2(x, "x")
         N, kb_, ldb = _rows2(b, "b")
         if kb_ != K:
             raise _shape_err(f"b has {kb_} columns, x {K}")
@@ -748,7 +750,8 @@ class Context:
         _dense(offsets, (E + 1,), torch.int32, "offsets")
         _dense(sa, (N, rb), torch.float32, "sa")
         _dense(sb, (K, rb), torch.float32, "sb")
-        dp, _ = _per_expert(dw, E, (N, K), dw[0].dtype, "dw")
+        dt = dw[0].dtype if len(dw) else None
+        dp, _ = _per_expert(dw, E, (N, K), dt, "dw")
         _check(lib().frx_fp8_grad_weight_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
                                                  b.data_ptr(), ldb, sb.data_ptr(), offsets.data_ptr(), E,
                                                  dp.buffer_info()[0],
@@ -769,7 +772,7 @@ class Context:
         rows of any type whose bytes are a multiple of 4."""
         _dense(x, (rows.T, *x.shape[1:]), None, "x")
         _dense(xs, (rows.R, *x.shape[1:]), x.dtype, "xs")
-        _check(lib().frx_moe_dispatch(self._h, x.data_ptr(), x.numel() // rows.T * x.element_size(), rows._p,
+        _check(lib().frx_moe_dispatch(self._h, x.data_ptr(), x.numel() // max(rows.T, 1) * x.element_size(), rows._p,
                                       xs.data_ptr()), self._h)
         return xs
 

@@ -120,3 +120,19 @@ def test_binding_checks_experts_and_rows(ctx):
     refuses(frx.FrxError, lambda: ctx.moe_combine_backward(torch.zeros((4, 8)), None, rows, None,
                                                            torch.zeros((rows.R, 8)), torch.zeros((4, 2))))
     refuses(frx.FrxError, lambda: frx.MoeRows(3, 1, i32(3), i32(4, 2), i32(9)))
+
+
+def test_binding_checks_nothing_to_do(ctx):
+    """No experts, no tokens, a vector in a matrix' place."""
+    i32 = lambda *d: torch.zeros(d, dtype=torch.int32)  # noqa: E731
+    a, sa, y = torch.zeros((12, 256)).to(E4M3), torch.zeros((12, 2)), torch.zeros((12, 40))
+    for b, sb in ((torch.zeros((0, 40, 256)).to(E4M3), torch.zeros((0, 1, 2))), ([], [])):
+        refuses(frx.FrxError, lambda: ctx.fp8_linear_grouped(a, sa, b, sb, i32(1), y))
+    dy = torch.zeros((40, 16)).to(E5M2)
+    for off, dw in ((i32(1), []), (i32(1), torch.zeros((0, 40, 12))), (i32(0), [])):
+        refuses(frx.FrxError, lambda: ctx.fp8_grad_weight_grouped(dy, torch.zeros((40, 1)), a[:, :16],
+                                                                  torch.zeros((12, 1)), off, dw))
+    b, sb = torch.zeros((40, 256)).to(E4M3), torch.zeros((1, 2))
+    refuses(frx.FrxError, lambda: ctx.fp8_linear_act(torch.zeros(256), b, sb, y))
+    rows = frx.MoeRows.empty(0, 2, 3, 4, device="cpu")
+    reaches_the_library(lambda: ctx.moe_dispatch(torch.zeros((0, 8)), rows, torch.zeros((rows.R, 8))))
