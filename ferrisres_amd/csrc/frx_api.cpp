@@ -1675,9 +1675,8 @@ size_t frx_moe_rows_capacity(uint32_t T, uint32_t top_k, uint32_t E, uint32_t al
   return (n + align - 1) / align * align;
 }
 
-// Rows and columns stay below this: a launch holds less than 2^32 work-items
-// and 65536 workgroups in y.
-constexpr uint32_t kMaxRows = 1u << 24;
+// A launch holds less than 2^32 work-items and 65536 workgroups in y.
+constexpr uint32_t kMaxRows = 1u << 24, kMaxCols = 65535u * 256;
 
 static frx_status check_rows(frx_ctx *ctx, const frx_moe_rows *r, frx::RouteRows *out) {
   if (!r || !r->offsets || !r->row_of || !r->slot_of) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
@@ -1734,7 +1733,7 @@ frx_status frx_moe_combine(frx_ctx *ctx, const void *ys, frx_dtype st_, const fr
   frx::RouteRows r;
   if (!ys || !y) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
   if (!is_dtype(st_) || !is_dtype(yt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
-  if (H == 0 || H >= kMaxRows) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^24)", H);
+  if (H == 0 || H > kMaxCols) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, %u]", H, kMaxCols);
   if (!aligned_to(ys, dtype_bytes(st_)) || !aligned_to(y, dtype_bytes(yt)) || !aligned_to(w, 4))
     return fail(ctx, FRX_ERR_SHAPE, "ys, y and w must be aligned to their elements");
   if ((st = check_rows(ctx, rows, &r)) != FRX_OK) return st;
@@ -1751,7 +1750,7 @@ frx_status frx_moe_combine_backward(frx_ctx *ctx, const void *dy, frx_dtype dt, 
   if (!dy || !dys) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
   if (!ys != !dw) return fail(ctx, FRX_ERR_SHAPE, "ys and dw come together");
   if (!is_dtype(dt) || !is_dtype(st_)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
-  if (H == 0 || H >= kMaxRows) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, 2^24)", H);
+  if (H == 0 || H > kMaxCols) return fail(ctx, FRX_ERR_SHAPE, "H=%u must be in [1, %u]", H, kMaxCols);
   if (!aligned_to(dy, dtype_bytes(dt)) || !aligned_to(ys, dtype_bytes(st_)) || !aligned_to(dys, dtype_bytes(st_)) ||
       !aligned_to(w, 4) || !aligned_to(dw, 4))
     return fail(ctx, FRX_ERR_SHAPE, "dy, ys, dys, w and dw must be aligned to their elements");

@@ -92,14 +92,6 @@ struct GroupArgs {
   const float *sb[FP8_MAXE];
 };
 
-// The pipe of the experts' products: gradients' (E5M2) rows sum in fp32 whatever
-// the output, since the one row of a token with one route is handed on as it
-// is. It costs little where the weights' bytes bound (16 experts of 64 rows,
-// 5632 -> 2048: 62.5 us on the 8-bit pipe, 64.5 on the bf16 one; 8 of 1024, 2048 ->
-// 5632: 143, 218).
-template <bool E5M2, typename YT>
-constexpr bool fp8_grouped_wide = E5M2 || sizeof(YT) == 4;
-
 // Expert e's rows [first, end), kept inside the R rows there are.
 __device__ __forceinline__ void expert_rows(const uint32_t *offsets, int e, uint32_t R, uint32_t &first,
                                             uint32_t &end) {
@@ -172,7 +164,7 @@ __global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_grouped_kernel(c
   const uint32_t kbs = (p.K + 127) >> 7;
   const Fp8Skinny q = {p.a + (size_t)m0 * p.lda, p.sa + (size_t)m0 * kbs, p.b[e], p.sb[e],
                        static_cast<YT *>(p.y) + (size_t)m0 * p.N, p.lda, p.ldb, min(16u, end - m0), p.K, p.N, 0};
-  fp8_skinny<RT, 1, E5M2, false, fp8_grouped_wide<E5M2, YT>, uint8_t, YT>(q, nt * 16 * RT, reinterpret_cast<f32x4 *>(lds));
+  fp8_skinny<RT, 1, E5M2, false, true, uint8_t, YT>(q, nt * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
 // Weight gradients: expert blockIdx.y sums over the blocks of its rows. Here
@@ -319,33 +311,37 @@ hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// The 8-bit pipe. The lengths of the groups are not known here, so the tile is
-// chosen for equal ones: R / E rows and half a tile of remainder each, a step's
-// ns times the tiles of the fullest compute unit (64 x 128: several resident).
-// Measured, us, 8 experts, K -> N (64 x 128 / 128 x 256 / 256 x 256): 12 rows 2048 ->
-// 5632 21.4 / 21.7 / 26.1; 64 rows 33 / 25 / 30; 128 rows 42 / 45 / 34, 5632 -> 2048
-// 51 / 54 / 66; 256 rows 59 / 49 / 66; 384 rows 77 / 72 / 72; 1024 rows 173 / 143 / 143.
-// 16 experts of 64 rows, 184 MB of weights: 54 / 52 / 63.
-double grouped_cost(const GroupArgs &p, uint32_t bm, uint32_t bn, double ns, double alone, int cus) {
-  const double rows = (double)p.R / p.E / bm + 0.5;
-  const double tiles = p.E * (rows < 1 ? 1 : rows) * ((p.N + bn - 1) / bn);
-  return std::max(alone, ns * std::ceil(tiles / cus));
+// The pipe and the tile of the experts' products. Rows of experts are handed on
+// (a token of one route gets its row as it is), so they sum exact products in
+// fp32 where the weights' bytes bound and that costs little: on the bf16 pipe, in
+// tiles of 64 x 128. From 256 rows an expert on (R / E: the groups' lengths are
+// not known here) the products bound, and bf16 rows of e4m3 codes take the 8-bit
+// pipe in tiles of 128 or 256 x 256, priced for groups of equal length with half a
+// tile of remainder. Gradients' rows (e5m2) and f32 outputs stay on the bf16 pipe.
+// us, K -> N, bf16 64 x 128 / 8-bit 64 x 128 / 128 x 256 / 256 x 256:
+//   8 experts   128 rows 2048 -> 5632    44 /  42 /  45 /  33
+//               256 rows 2048 -> 5632     - /  59 /  49 /  66
+//               384 rows 2048 -> 5632    92 /  77 /  72 /  72
+//              1024 rows 2048 -> 5632   218 / 173 / 143 / 143
+//   16 experts   64 rows 5632 -> 2048    62 /  61 /  55 /  61
+//                64 rows 2048 -> 5632     - /  54 /  52 /  63
+//   16 experts of 64 rows padded to 128, 5632 -> 2048    64 / 62 / 61 / 67
+// Other tiles of the bf16 pipe (128 x 128 / 128 x 256): 8 x 128 rows 53 / 66, 8 x 1024
+// 205 / 205, 16 x 64 padded to 128 87 / 77: widening bounds every tile alike.
+double grouped_cost(const GroupArgs &p, uint32_t bm, uint32_t bn, double ns, int cus) {
+  const double tiles = p.E * ((double)p.R / p.E / bm + 0.5) * ((p.N + bn - 1) / bn);
+  return ns * std::ceil(tiles / cus);
 }
 
-// The bf16 pipe takes 64 x 128 throughout: widening bounds every tile alike.
-// us, 8 experts, E5M2 (64 x 128 / 128 x 128 / 128 x 256): 128 rows 2048 -> 5632
-// 44 / 53 / 66; 256 rows 5632 -> 2048 75 / 82 / 77; 1024 rows 2048 -> 5632
-// 218 / 205 / 205. 16 experts of 64 rows padded to 128, 5632 -> 2048: 64 / 87 / 77.
 template <bool E5M2, typename YT>
 hipError_t grouped_tile(const GroupArgs &p, int cus, hipStream_t stream) {
-  constexpr bool WIDE = fp8_grouped_wide<E5M2, YT>;
-  if constexpr (!WIDE) {
-    const double c64 = grouped_cost(p, 64, 128, 430, 1000, cus), c128 = grouped_cost(p, 128, 256, 1010, 0, cus);
-    if (grouped_cost(p, 256, 256, 1460, 0, cus) < std::min(c64, c128))
-      return grouped_go<Fp8Ring<8, E5M2, false, false>, YT>(p, stream);
-    if (c128 < c64) return grouped_go<Fp8Ring<4, E5M2, false, false>, YT>(p, stream);
+  if constexpr (!E5M2 && sizeof(YT) == 2) {
+    if (p.R >= 256u * (uint32_t)p.E)
+      return grouped_cost(p, 256, 256, 1460, cus) < grouped_cost(p, 128, 256, 1010, cus)
+                 ? grouped_go<Fp8Ring<8, E5M2, false, false>, YT>(p, stream)
+                 : grouped_go<Fp8Ring<4, E5M2, false, false>, YT>(p, stream);
   }
-  return grouped_go<Fp8Tile<64, 128, 2, 2, E5M2, false, WIDE>, YT>(p, stream);
+  return grouped_go<Fp8Tile<64, 128, 2, 2, E5M2, false, true>, YT>(p, stream);
 }
 
 template <int BM, int BN, bool E5M2, typename YT>

@@ -318,8 +318,9 @@ typedef enum frx_fp8_blocks {
  * 57344; code = the product x * f32(1 / scale) rounded to nearest even. Each
  * of these is one f32 rounding, so codes and scales are reproducible bit for
  * bit. amax is the largest magnitude of the block; a NaN or an infinity in
- * a block becomes its scale (and NaN codes), so that it reaches every product
- * it belongs to. A block at an edge has fewer values.
+ * a block becomes its scale (under an infinite one finite values become zeros),
+ * so that every product it belongs to is a NaN. A block at an edge has fewer
+ * values.
  * ldq: bytes between rows of q, a multiple of 16 and at least the row length
  * (K; COLS and TILES_T: M) rounded up to 16; the codes from there to that
  * multiple are written as zeros, which is how a row length of any size enters
@@ -339,12 +340,17 @@ frx_status frx_fp8_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t 
  *     dw = dy^T x:  a = dy COLS,   b = x COLS      (sums over the tokens, rounded
  *                                  up to 16: the quantiser's zero codes)
  * Sums in fp32: a block's 128 products on the matrix pipe, then the blocks in
- * order, each times its two scales; one rounding to yt at the end. Requires
- * K % 16 == 0, lda and ldb multiples of 16 and >= K, a and b 16-byte aligned,
- * M, N >= 1; y aligned to its element. Few rows, or few tiles, split K over
- * workgroups: fp32 parts in a context workspace (allocated on the first call
- * at a larger size; a call under graph capture that would have to allocate
- * runs unsplit), added in order. */
+ * order, each times its two scales; one rounding to yt at the end. For an f32 y
+ * the products are exact and added in fp32. For a bf16 y the 8-bit pipe adds
+ * them, which cuts the products of each group of 8 to 2^-13 of the largest
+ * one's power of two: less than 2^-10 of the sum of the magnitudes, 1.5e-5 of
+ * the result on normally distributed values, before the 2^-9 of bf16.
+ * Requires K % 16 == 0, lda and ldb multiples of 16, >= K and <= 2^23, a and b
+ * 16-byte aligned, M, N >= 1, (M / 64 + 65) * ceil(N / 128) < 2^24; y aligned to
+ * its element. Where there are few tiles, K is split over workgroups: fp32 parts
+ * in a context workspace (allocated on the first call at a larger size; a call
+ * under graph capture that would have to allocate runs unsplit), added in
+ * order. */
 frx_status frx_fp8_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
                           const uint8_t *b, size_t ldb, const float *sb, uint32_t b_rows, void *y,
                           frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
@@ -353,7 +359,8 @@ frx_status frx_fp8_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at
  * (ROWS, e4m3) and frx_fp8_linear (b_rows = 128) in one call, with the two
  * calls' result bit for bit. Up to 4 tokens (of 16000 columns together) it
  * is one launch, the codes in LDS; above, they lie in a context workspace (which
- * must be there before a graph capture: FRX_ERR_UNSUPPORTED otherwise). */
+ * must be there before a graph capture: FRX_ERR_UNSUPPORTED otherwise). K % 16
+ * == 0 and K <= 2^23 for x's codes too. */
 frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
                               const float *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
 
@@ -362,7 +369,9 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
  *   a [R][lda], sa [R][ceil(K / 128)]; b[e] [N][ldb] e4m3, sb[e] [ceil(N / 128)]
  *   [ceil(K / 128)] (host arrays of E device pointers); offsets [E + 1] u32 on
  *   the device, ascending; y [R][N]. Rows from offsets[E] on are neither read
- *   nor written. 1 <= E <= 64; otherwise as frx_fp8_linear. No allocation. */
+ *   nor written. 1 <= E <= 64; otherwise as frx_fp8_linear, except that a bf16 y
+ *   too is the fp32 sum of exact products, rounded once, for e5m2 rows
+ *   (gradients) and for R < 256 E. No allocation. */
 frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
                                   const uint8_t *const *b, size_t ldb, const float *const *sb,
                                   const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R,
@@ -390,7 +399,7 @@ frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t ld
 typedef struct frx_moe_rows {
   uint32_t T, top_k, E; /* 1 <= top_k <= 64, 1 <= E <= 64 */
   uint32_t align;       /* 1 to 128, a power of two */
-  uint32_t R;           /* rows there is room for: at least frx_moe_rows_capacity */
+  uint32_t R;           /* rows there is room for: at least frx_moe_rows_capacity, below 2^24 */
   uint32_t *offsets;    /* [E + 1] first row of each expert; offsets[E]: the end */
   uint32_t *row_of;     /* [T][top_k] row of each route; 0xFFFFFFFF: it goes nowhere */
   uint32_t *slot_of;    /* [R] slot of each row; 0xFFFFFFFF: a row of no route (between
@@ -418,7 +427,7 @@ frx_status frx_moe_dispatch(frx_ctx *ctx, const void *x, size_t row_bytes, const
 /* y[t] = sum_j w[t][j] * ys[row_of[t][j]], in the order of j from 0, each product and
  * addition one f32 rounding, one rounding to yt at the end; a route that goes
  * nowhere adds nothing (whatever its weight), a token without routes gets zeros. ys [R][H]
- * st, y [T][H] yt, w [T][top_k] f32 or NULL (every weight 1). H >= 1. */
+ * st, y [T][H] yt, w [T][top_k] f32 or NULL (every weight 1). 1 <= H <= 65535 * 256. */
 frx_status frx_moe_combine(frx_ctx *ctx, const void *ys, frx_dtype st, const frx_moe_rows *rows,
                            const float *w, void *y, frx_dtype yt, uint32_t H);
 

@@ -600,3 +600,35 @@ def test_gradient_rows_are_rounded_once(ctx, sizes):
         i, j = int(off[e]), int(off[e + 1])
         if j > i:
             check(y[0][i:j], av[i:j] @ ops[e][2].t(), av[i:j].abs() @ ops[e][2].abs().t(), k)
+
+
+@pytest.mark.parametrize("sizes,n", [([300, 260], 515), ([0, 900, 1], 132)])
+def test_grouped_of_long_groups(ctx, sizes, n):
+    """256 rows an expert and more: the 8-bit pipe."""
+    k, behind = 400, 5
+    off = np.concatenate([[0], np.cumsum(sizes)])
+    rows = int(off[-1]) + behind
+    a, sa, av = operand(5, rows, k, E4M3)
+    ops = [operand(7 + e, n, k, E4M3, tiles=True) for e in range(len(sizes))]
+    y = torch.full((rows, n), 5.0, dtype=torch.bfloat16, device=DEV)
+    ctx.fp8_linear_grouped(a.to(DEV), sa.to(DEV), [o[0].to(DEV) for o in ops], [o[1].to(DEV) for o in ops],
+                           torch.tensor(off, dtype=torch.int32, device=DEV), y)
+    for e in range(len(sizes)):
+        i, j = int(off[e]), int(off[e + 1])
+        if j > i:
+            check(y[i:j], av[i:j] @ ops[e][2].t(), av[i:j].abs() @ ops[e][2].abs().t(), k)
+    assert (y[-behind:] == 5.0).all()
+
+
+def test_few_rows_of_experts_are_rounded_once(ctx):
+    """Up to 256 rows an expert the bf16 result of e4m3 rows is the f32 one rounded."""
+    k, n, E = 528, 300, 4
+    for rows in (5, 200, 1000):
+        off = torch.tensor([0, rows // 4, rows // 4, rows - 1, rows], dtype=torch.int32, device=DEV)
+        a, sa, _ = operand(3, rows, k, E4M3)
+        ops = [operand(7 + e, n, k, E4M3, tiles=True) for e in range(E)]
+        y = [torch.empty((rows, n), dtype=t, device=DEV) for t in (torch.float32, torch.bfloat16)]
+        for out in y:
+            ctx.fp8_linear_grouped(a.to(DEV), sa.to(DEV), [o[0].to(DEV) for o in ops], [o[1].to(DEV) for o in ops],
+                                   off, out)
+        assert torch.equal(y[0].bfloat16(), y[1])
