@@ -358,13 +358,15 @@ hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
 
 // Tiles of many tokens: height x width, workgroups resident at once on a
 // compute unit, and what a step of 128 columns takes (ns, all of them resident;
-// 8192^3, 2048 x 4096 x 11008 and 4096^3). The 8-bit pipe in tiles of 256 x 256
-// is the fastest per product (2943 TFLOP/s at 8192^3; 192: 2545, 128: 2127, 128 x
-// 128 from LDS alone 1930), the smaller ones where it would leave units idle (us,
-// 256 / 192 / 128 / 128 x 128: 2048 x 4096 x 11008 105 / 88 / 110 / 126, 2048 x
-// 4096 x 4096 53 / 43 / 37 / 49, 4096^3 53 / 78 / 76 / 90). On the bf16 pipe widening
-// the operands bounds them all (2048 x 4096 x 11008: 168 / 183 / 166 us for 192 /
-// 128 / 128 x 128; 333 x 5120 x 13824 94 / 70 / 75).
+// 8192^3, 2048 x 4096 x 11008 and 4096^3). On the 8-bit pipe a taller tile costs
+// less per product, and a smaller one pays where the taller would leave units
+// idle (us, 256 / 192 / 128 / 128 x 128: 8192^3 374 / 432 / 517 / 570, 2048 x 4096 x
+// 11008 105 / 88 / 110 / 126, 2048 x 4096 x 4096 53 / 43 / 37 / 49, 4096^3 53 / 78 / 76 /
+// 90). Long products run into the card's power: 8192^3 takes 350 us on zeros
+// (3140 TFLOP/s) and 460 on normal values; a library's product with one scale for
+// all takes 257 and 348. On the bf16 pipe widening the operands bounds them all
+// (2048 x 4096 x 11008: 168 / 183 / 166 us for 192 / 128 / 128 x 128; 333 x 5120 x
+// 13824 94 / 70 / 75).
 struct TileCost {
   int tile, bm, bn, wgs, ns;
 };

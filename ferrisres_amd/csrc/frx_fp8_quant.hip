@@ -9,7 +9,10 @@
 // infinity and infinity above every number, so either becomes the scale.
 //
 // Bound by memory: 2 or 4 bytes in and 1 out per value, about 4 VALU ops per
-// value (mask, max, multiply, half a conversion).
+// value (mask, max, multiply, half a conversion). us: rows of 2048 x 5632 bf16
+// 8.8 (3.9 TB/s; a large copy moves 4.7), columns of 1999 x 11008 bf16 22.7 (2.9 TB/s),
+// tiles of 4096 x 11008 f32 46.8 (4.8 TB/s), their codes transposed right after,
+// from the cache, 34.3.
 #include "frx_fp8_codes.hpp"
 #include "frx_internal.hpp"
 

@@ -1,10 +1,13 @@
 // frx_fp8_ring.hpp — the 8-bit product for many tokens, software-pipelined.
 //
 // A tile of 32 * FM tokens x 256 weight rows on 8 waves of 16 * FM x 64, two to a
-// SIMD, over two LDS stages (three up to 128 tokens), one block of 128 columns each. Large tiles: what
-// a compute unit reads per product halves from 128 x 128 to 256 x 256, and so
-// does the rate at which the L2's latency has to be covered. Step t issues
-// block t's products, and between them
+// SIMD, over two LDS stages (three at 128 tokens), one block of 128 columns
+// each. Large tiles: what a compute unit reads per product halves from 128 x 128
+// to 256 x 256, and so does the rate at which the L2's latency has to be
+// covered. Bound by issue: 4 multiply-adds beside each product, the DMA's and
+// the operands' instructions (8192^3 in 256 x 256 tiles 374 us, without any DMA
+// 306), and by power (frx_fp8.hip). Step t issues block t's products, and
+// between them
 //  - the multiply-adds of the token fragment before (the last one's of block
 //    t - 1 behind the first products of block t), so that no product waits for
 //    another's result;
@@ -14,7 +17,9 @@
 // weights in registers, so the DMA of a later block's weights (t + 2 with two
 // stages) goes into their place. Before the last one block t + 1 has landed
 // (each wave has waited for its own loads) and block t's tokens are read, so
-// the later block's follow: two bursts, each at least a step ahead of its use.
+// the later block's follow: each at least a step ahead of its use, spread over
+// the products (in two bursts 2048 x 4096 x 11008 took 104 us, spread 88; in one
+// 134).
 #pragma once
 #include "frx_fp8.hpp"
 
@@ -35,7 +40,7 @@ struct Fp8Ring {
   static constexpr int FM = FM_, FN = 4, WM = 2, WN = 4, WAVES = WM * WN, NT = WAVES * 64;
   static constexpr int TM = FM * 16, TN = FN * 16, BM = WM * TM, BN = WN * TN;
   static constexpr int LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;  // 1 KB load instructions of a wave and stage
-  static_assert(BM % (8 * WAVES) == 0 && FM % 2 == 0, "loads split evenly; products alternate between two sets");
+  static_assert(FM >= 4 && FM % 2 == 0, "loads split evenly; products alternate between two sets; loads between barriers");
   static constexpr int SIA = (BM + 63) / 64, SIB = BR1 ? BN / 64 : 1;  // scale load instructions
   static constexpr int SPW = (SIA + SIB + WAVES - 1) / WAVES;
   static constexpr int DATA = (BM + BN) * 32;  // dwords
@@ -181,17 +186,16 @@ struct Fp8Ring {
             __builtin_amdgcn_sched_barrier(0);
           }
           if (end) {
-            // in flight behind block kb + 1: whole blocks up to kb + NS, and of that one the
-            // weights (which FM == 2 issues below)
-            wait_all_but<(NS - 2) * LOADS + (FM == 2 ? 0 : LB)>();
+            // in flight behind block kb + 1: whole blocks up to kb + NS, and of that one the weights
+            wait_all_but<(NS - 2) * LOADS + LB>();
             barrier_nofence();
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < EARLY; i++) load(i, cur, c, kb + NS);
           }
           // the weights' loads, a part to each fragment between the barriers
-          constexpr int SPAN = FM > 2 ? FM - 2 : 1, PER = (LB + SPAN - 1) / SPAN;
-          if (FM == 2 ? fm == 1 : fm >= 1 && !end) {
+          constexpr int PER = (LB + FM - 3) / (FM - 2);
+          if (fm >= 1 && !end) {
             const int first = (fm - 1) * PER;
 #pragma unroll
             for (int i = first; i < first + PER && i < LB; i++) load(LA + i, cur, c, kb + NS);

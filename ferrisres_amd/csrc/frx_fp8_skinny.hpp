@@ -1,4 +1,4 @@
-// frx_fp8_skinny.hpp — the 8-bit product for up to 32 tokens.
+// frx_fp8_skinny.hpp — the 8-bit product for up to 64 tokens.
 //
 // Bound by the weights' bytes: each is read once, straight into registers (a
 // lane of an MFMA operand holds 32 codes of one row: two 16-byte loads, 64
@@ -14,8 +14,9 @@
 // tiles as leave each compute unit one workgroup (fp8_plan). us, 1 / 16 tokens,
 // graph replays over cold weights: 2048 x 2048 3.9 / 4.9, 4096 x 4096 6.6 / 8.1,
 // 11008 x 4096 12.1 / 13.5 (3.7 / 3.3 TB/s; a large copy moves 4.7), 13824 x 5120
-// 20.4 at 16. Loads of 2 or 4 blocks ahead of the products were slower (16
-// tokens of 11008 x 4096 14.6 / 14.8), as were 4 or 16 waves.
+// 18.2 at 16. Loads of 2 or 4 blocks ahead of the products were slower (16
+// tokens of 11008 x 4096 14.6 / 14.8), as were 4 or 16 waves. Above 16 tokens a
+// wave holds two or four token tiles (TT) against the same weights.
 //
 // XT uint8_t: a's codes with scales. Else up to FP8_ACT_MAX_M f32 or bf16
 // tokens, whose codes and scales the workgroup makes in LDS while its first

@@ -4,7 +4,10 @@
 // start at multiples of `align`.
 // dispatch: xs[row] = x[token of row].   combine: y[t] = sum_j w[t][j] ys[row_of[t][j]].
 // combine_backward: dys[row] = w[slot] dy[token], dw[t][j] = <dy[t], ys[row_of[t][j]]>.
-// All but the sort are bound by memory.
+// All but the sort are bound by memory. us, 8192 tokens of 4096 bf16 columns, two
+// routes each: dispatch 38.6 (201 MB, 5.2 TB/s with tokens read once from HBM),
+// combine 49 (4.1 TB/s), combine_backward 57 (336 MB, 5.9 TB/s), sort 10 (two
+// launches); 33 tokens of four routes 2.4 to 4.3 each.
 #include "frx_device.hpp"
 #include "frx_internal.hpp"
 
