@@ -316,7 +316,7 @@ def _fp8_code(t) -> int:
 def _rows2(t, name):
     """(rows, columns, row stride in elements) of a 2-D tensor with unit
     column stride."""
-    if len(t.shape) != 2:
+    if t.dim() != 2:
         raise _shape_err(f"{name} must be 2-D, got shape {tuple(t.shape)}")
     m, n = t.shape
     ld, col = t.stride()
@@ -341,21 +341,21 @@ def _per_expert(ts, E, shape, dtype, name, rows=False):
     stride, else contiguous."""
     if E < 1:
         raise _shape_err("offsets [E + 1] must be of at least one expert")
-    if len(ts) != E:
-        raise _shape_err(f"{name} holds {len(ts)} experts, expected {E}")
     if hasattr(ts, "dim"):  # stacked
-        if ts.dtype != dtype:
+        if ts.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {ts.dtype}")
-        if tuple(ts.shape[1:]) != tuple(shape):
+        m, n = shape
+        if ts.shape != (E, m, n):
             raise _shape_err(f"{name} has shape {tuple(ts.shape)}, expected {(E, *shape)}")
         step, ld, col = ts.stride()
-        m, n = shape
         if (n > 1 and col != 1) or (m > 1 and ld < n) or (not rows and m > 1 and ld != n):
             raise _shape_err(f"{name} must have {'unit column stride' if rows else 'contiguous experts'}, got strides "
                              f"{ts.stride()}")
         base, step = ts.data_ptr(), step * ts.element_size()
         at = array.array("Q", range(base, base + E * step, step) if step else [base] * E)
         return at, ld if m > 1 else max(ld, n)
+    if len(ts) != E:
+        raise _shape_err(f"{name} holds {len(ts)} experts, expected {E}")
     ld = None
     for t in ts:
         if t.dtype != dtype:
