@@ -146,9 +146,17 @@ __global__ __launch_bounds__(Tile::NT, 2) void fp8_grouped_kernel(const GroupArg
   Tile::template store<YT>(acc, (YT *)p.y + (size_t)m0 * p.N + n0, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
 }
 
+// blockIdx.y: the group of 16 * TT tokens.
 template <int RT, int TT, bool E5M2, bool BR1, typename XT, typename YT>
-__global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_kernel(const Fp8Skinny p) {
+__global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_kernel(Fp8Skinny p) {
   extern __shared__ __align__(16) uint32_t lds[];
+  if constexpr (TT == 4) {
+    const uint32_t m0 = blockIdx.y * 64;
+    p.a = static_cast<const XT *>(p.a) + m0 * p.lda;
+    p.sa += (size_t)m0 * ((p.K + 127) >> 7);
+    p.y = static_cast<YT *>(p.y) + (size_t)m0 * p.N;
+    p.M = min(64u, p.M - m0);
+  }
   fp8_skinny<RT, TT, E5M2, BR1, sizeof(YT) == 4, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
@@ -266,7 +274,8 @@ hipError_t skinny_rt(const Fp8Skinny &p, hipStream_t stream) {
                                   (int)(red + (sizeof(XT) == 1 ? 0 : FP8_ACT_MAX_BYTES)), done);
   if (e != hipSuccess) return e;
   const size_t lds = red + (sizeof(XT) == 1 ? 0 : fp8_skinny_act_bytes(p.M, p.K));
-  hipLaunchKernelGGL(kernel, dim3((p.N + 16 * RT - 1) / (16 * RT)), dim3(FP8_SK_WAVES * 64), lds, stream, p);
+  hipLaunchKernelGGL(kernel, dim3((p.N + 16 * RT - 1) / (16 * RT), (p.M + 16 * TT - 1) / (16 * TT)),
+                     dim3(FP8_SK_WAVES * 64), lds, stream, p);
   return hipGetLastError();
 }
 
@@ -384,9 +393,13 @@ Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, in
   // in K slices: 32 tokens, K x N 1024^2 4.1 / 9.6, 4096^2 10.2 / 14.7, 4096 x 11008 15.7 / 17.4, 11008 x 4096
   // 20.9 / 20.1), up to 64 while two row tiles a workgroup cover N and the waves' slices of K are short, since
   // every workgroup reads all tokens (64 tokens, 1024^2 5.7 / 10.8, 4096^2 14.5 / 17.5, 4096 x 8192 17.8 / 18.9,
-  // f32 2048 x 5632 10.9 / 19.7; 40 tokens f32 5120^2 20.7 / 21.0; 11008 x 4096 31.1 / 22.4).
+  // f32 2048 x 5632 10.9 / 19.7; 40 tokens f32 5120^2 20.7 / 21.0; 11008 x 4096 31.1 / 22.4), more in groups of 64
+  // while two rounds of workgroups hold them and K is short for that (128 tokens, 2048^2 8.5 / 14.6, 4096 x 2048 12.9 /
+  // 17.5, 2048 x 4096 13.8 / 16.6; 256 tokens, 2048^2 13.7 / 16.9, f32 2048 x 1024 8.6 / 18.2; 512 tokens, 1024^2
+  // 9.3 / 13.3; but 128 tokens 4096^2 23.0 / 22.6, 256 tokens 5120 x 2048 28.8 / 21.1).
   const int steps = (int)((K + 127) / 128), most = M <= 32 ? 4 : 2;  // row tiles a workgroup
-  if (M <= 32 || (M <= 64 && N <= 32u * cus && steps <= 40)) {
+  const size_t rounds64 = ((size_t)((M + 63) / 64) * ((N + 15) / 16) + cus - 1) / cus;
+  if (M <= 32 || (M <= 64 && N <= 32u * cus && steps <= 40) || (rounds64 <= 2 && rounds64 * steps <= 40)) {
     // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
     const uint32_t tiles = (N + 15) / 16;
     int best = 1;

@@ -1,4 +1,4 @@
-// frx_fp8_skinny.hpp — the 8-bit product for up to 64 tokens.
+// frx_fp8_skinny.hpp — the 8-bit product for up to 64 tokens, or a few groups of 64.
 //
 // Bound by the weights' bytes: each is read once, straight into registers (a
 // lane of an MFMA operand holds 32 codes of one row: two 16-byte loads, 64

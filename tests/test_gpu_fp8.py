@@ -632,3 +632,18 @@ def test_few_rows_of_experts_are_rounded_once(ctx):
             ctx.fp8_linear_grouped(a.to(DEV), sa.to(DEV), [o[0].to(DEV) for o in ops], [o[1].to(DEV) for o in ops],
                                    off, out)
         assert torch.equal(y[0].bfloat16(), y[1])
+
+
+@pytest.mark.parametrize("m,k,n", [(65, 272, 100), (128, 2048, 516), (200, 400, 1000), (511, 1024, 130), (130, 5120, 33)])
+@pytest.mark.parametrize("code,b_rows,out", [(E4M3, 128, "bf16"), (E5M2, 128, "f32"), (E4M3, 1, "f32")])
+def test_linear_in_groups_of_64_tokens(ctx, m, k, n, code, b_rows, out):
+    """Several groups over few rows, the last one not full; codes and an output inside larger buffers."""
+    a, sa, av = operand(m + k, m, k, code)
+    b, sb, bv = operand(n + k + 1, n, k, E4M3, tiles=b_rows == 128)
+    wide = torch.full((m, k + 32), 0x7F, dtype=torch.uint8, device=DEV).view(code)
+    wide[:, :k].copy_(a.to(DEV))
+    buf = torch.full((m * n + 8,), 3.0, dtype=DT[out], device=DEV)
+    y = buf[3:3 + m * n].view(m, n)
+    ctx.fp8_linear(wide[:, :k], sa.to(DEV), b.to(DEV), sb.to(DEV), y)
+    check(y, av @ bv.t(), av.abs() @ bv.abs().t(), k)
+    assert (buf[:3] == 3.0).all() and (buf[3 + m * n:] == 3.0).all()
