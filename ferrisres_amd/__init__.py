@@ -26,6 +26,7 @@ MOE_TERNARY_MOE_LAYER, MOE_CPU_MOE_LAYER = 0, 1
 QUANT_ABSMEAN, QUANT_STE = 0, 1
 FP8_E4M3, FP8_E5M2 = 0, 1
 FP8_ROWS, FP8_COLS, FP8_TILES, FP8_TILES_T = 0, 1, 2, 3
+FP8_SUMS_F32, FP8_SUMS_PIPE = 0, 1
 
 _STATUS = {
     0: "Ok", 1: "Gpu", 2: "Shape", 3: "Device", 4: "Shader", 5: "OOM", 6: "Unsupported",
@@ -118,6 +119,7 @@ _SIGS = {
     "frx_moe_dispatch": (_int, [_vp, _vp, _sz, _vp, _vp]),
     "frx_moe_combine": (_int, [_vp, _vp, _int, _vp, _vp, _vp, _int, _u32]),
     "frx_moe_combine_backward": (_int, [_vp, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _u32]),
+    "frx_set_fp8_sums": (_int, [_vp, _int]),
     "frx_set_gemv_split": (_int, [_vp, _int]),
     "frx_workspace_stats": (_int, [_vp, ctypes.POINTER(_sz), ctypes.POINTER(_sz), ctypes.POINTER(_u32)]),
     "frx_release_retired": (_int, [_vp]),
@@ -757,6 +759,11 @@ class Context:
                                                  dp.buffer_info()[0],
                                                  _dtype_code(dw[0]), R, N, K), self._h)
         return dw
+
+    def set_fp8_sums(self, mode: int):
+        """frx_set_fp8_sums: FP8_SUMS_F32 (default: every sum in fp32) or
+        FP8_SUMS_PIPE (bf16 outputs on the 8-bit pipe where it is faster)."""
+        _check(lib().frx_set_fp8_sums(self._h, mode), self._h)
 
     # Tokens sorted by expert, and back.
     def moe_sort(self, topk_idx, rows: MoeRows):

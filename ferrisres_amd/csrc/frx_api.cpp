@@ -102,6 +102,7 @@ struct frx_ctx {
   size_t sort_ws_bytes = 0;
   unsigned *sk_cnt = nullptr;  // its per-row-tile arrival counters (zero between launches)
   int gemv_split = FRX_GEMV_SPLIT_AUTO;
+  int fp8_sums = FRX_FP8_SUMS_F32;
   unsigned *ffn_bar = nullptr;  // grid-barrier words of the one-launch FFN
   int ffn_mode = FRX_FFN_AUTO;
   int moe_routing = FRX_MOE_TERNARY_MOE_LAYER;
@@ -273,6 +274,15 @@ frx_status frx_set_gemv_split(frx_ctx *ctx, frx_gemv_split mode) {
   if (mode != FRX_GEMV_SPLIT_AUTO && mode != FRX_GEMV_SPLIT_ALWAYS && mode != FRX_GEMV_SPLIT_NEVER)
     return fail(ctx, FRX_ERR_UNSUPPORTED, "unknown split mode %d", (int)mode);
   ctx->gemv_split = mode;
+  return FRX_OK;
+}
+
+frx_status frx_set_fp8_sums(frx_ctx *ctx, frx_fp8_sums mode) {
+  if (!ctx) return FRX_ERR_DEVICE;
+  ctx->err[0] = 0;
+  if (mode != FRX_FP8_SUMS_F32 && mode != FRX_FP8_SUMS_PIPE)
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "unknown sums %d", (int)mode);
+  ctx->fp8_sums = mode;
   return FRX_OK;
 }
 
@@ -1572,10 +1582,14 @@ static frx_status check_fp8_side(frx_ctx *ctx, const void *b, const void *sb, co
   return FRX_OK;
 }
 
+// Whether the 8-bit pipe may add up outputs of this type.
+static bool fp8_pipe8(const frx_ctx *ctx, frx_dtype yt) { return yt == FRX_BF16 && ctx->fp8_sums == FRX_FP8_SUMS_PIPE; }
+
 static frx_status fp8_run(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa, const uint8_t *b,
                           size_t ldb, const float *sb, uint32_t b_rows, void *y, frx_dtype yt, uint32_t M, uint32_t K,
                           uint32_t N) {
-  frx::Fp8Plan plan = frx::fp8_plan(M, K, N, (int)b_rows, yt == FRX_BF16, ctx->cus);
+  const bool pipe8 = fp8_pipe8(ctx, yt);
+  frx::Fp8Plan plan = frx::fp8_plan(M, K, N, (int)b_rows, pipe8, ctx->cus);
   const size_t need = frx::fp8_part_bytes(M, N, plan);
   if (need && !may_grow(ctx, ctx->gk_ws_bytes, need)) {
     plan.S = 1;  // a first call under capture: whole K
@@ -1585,8 +1599,8 @@ static frx_status fp8_run(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at
     if (st != FRX_OK) return st;
   }
   const hipError_t e = frx::launch_fp8_linear(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, (int)b_rows, y,
-                                              yt == FRX_BF16, M, K, N, plan, reinterpret_cast<float *>(ctx->gk_ws),
-                                              ctx->stream);
+                                              yt == FRX_BF16, pipe8, M, K, N, plan,
+                                              reinterpret_cast<float *>(ctx->gk_ws), ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "fp8 linear launch");
   return FRX_OK;
 }
@@ -1612,7 +1626,7 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
   if (!aligned_to(x, dtype_bytes(xt))) return fail(ctx, FRX_ERR_SHAPE, "x must be aligned to its elements");
   if ((st = check_fp8(ctx, b, K, FRX_FP8_E4M3, sb, ldb, yt, M, K, N)) != FRX_OK) return st;
   if ((st = check_fp8_side(ctx, b, sb, y, yt)) != FRX_OK) return st;
-  const frx::Fp8Plan plan = frx::fp8_plan(M, K, N, 128, yt == FRX_BF16, ctx->cus);
+  const frx::Fp8Plan plan = frx::fp8_plan(M, K, N, 128, fp8_pipe8(ctx, yt), ctx->cus);
   if (plan.tile == frx::FP8_T_SKINNY && frx::fp8_act_fits(M, K)) {
     const hipError_t e = frx::launch_fp8_linear_act(x, xt == FRX_BF16, b, ldb, sb, y, yt == FRX_BF16, M, K, N, plan,
                                                     ctx->stream);
@@ -1645,7 +1659,7 @@ frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, fr
     if ((st = check_fp8_side(ctx, b[e], sb[e], y, yt)) != FRX_OK) return st;
   if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
   const hipError_t e = frx::launch_fp8_grouped(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, offsets, (int)E, y,
-                                               yt == FRX_BF16, R, K, N, ctx->cus, ctx->stream);
+                                               yt == FRX_BF16, fp8_pipe8(ctx, yt), R, K, N, ctx->cus, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "fp8 grouped linear launch");
   return FRX_OK;
 }
@@ -1662,7 +1676,7 @@ frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t ld
     if ((st = check_fp8_side(ctx, b, sb, dw[e], yt)) != FRX_OK) return st;
   if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
   const hipError_t e = frx::launch_fp8_grad_weight(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, offsets, (int)E, dw,
-                                                   yt == FRX_BF16, R, N, K, ctx->stream);
+                                                   yt == FRX_BF16, fp8_pipe8(ctx, yt), R, N, K, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "fp8 weight gradient launch");
   return FRX_OK;
 }

@@ -157,7 +157,7 @@ __global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_kernel(Fp8Skinny
     p.y = static_cast<YT *>(p.y) + (size_t)m0 * p.N;
     p.M = min(64u, p.M - m0);
   }
-  fp8_skinny<RT, TT, E5M2, BR1, sizeof(YT) == 4, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
+  fp8_skinny<RT, TT, E5M2, BR1, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
 // Sorted rows in tiles of 16 (decode batches: a few rows of each expert).
@@ -172,7 +172,7 @@ __global__ __launch_bounds__(FP8_SK_WAVES * 64) void fp8_skinny_grouped_kernel(c
   const uint32_t kbs = (p.K + 127) >> 7;
   const Fp8Skinny q = {p.a + (size_t)m0 * p.lda, p.sa + (size_t)m0 * kbs, p.b[e], p.sb[e],
                        static_cast<YT *>(p.y) + (size_t)m0 * p.N, p.lda, p.ldb, min(16u, end - m0), p.K, p.N, 0};
-  fp8_skinny<RT, 1, E5M2, false, true, uint8_t, YT>(q, nt * 16 * RT, reinterpret_cast<f32x4 *>(lds));
+  fp8_skinny<RT, 1, E5M2, false, uint8_t, YT>(q, nt * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
 // Weight gradients: expert blockIdx.y sums over the blocks of its rows. Here
@@ -187,9 +187,9 @@ struct GradArgs {
   void *dw[FP8_MAXE];
 };
 
-template <int BM, int BN, int WM, int WN, bool E5M2, typename YT>
-__global__ __launch_bounds__(WM *WN * 64, 2) void fp8_grad_kernel(const GradArgs p) {
-  using Tile = Fp8Tile<BM, BN, WM, WN, E5M2, true, sizeof(YT) == 4>;
+template <typename Tile, typename YT>
+__global__ __launch_bounds__(Tile::NT, 2) void fp8_grad_kernel(const GradArgs p) {
+  constexpr int BM = Tile::BM, BN = Tile::BN;
   extern __shared__ __align__(16) uint32_t lds[];
   const uint32_t mts = (p.N + BM - 1) / BM;
   const uint32_t nt = blockIdx.x / mts, mt = blockIdx.x - nt * mts;
@@ -253,9 +253,8 @@ hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
   return go(fp8_dense_kernel<Tile, BR1, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, 1, S), Tile::NT, stream, p);
 }
 
-template <bool E5M2, bool BR1, typename YT>
+template <bool E5M2, bool BR1, bool WIDE, typename YT>
 hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
-  constexpr bool WIDE = sizeof(YT) == 4;
   if constexpr (!(BR1 && WIDE))
     if (tile == FP8_T_RING4) return dense_go<Fp8Ring<4, E5M2, BR1, WIDE>, BR1, YT>(p, S, stream);
   if constexpr (!BR1)
@@ -301,11 +300,11 @@ hipError_t skinny_any(int e5m2, int b_rows, int rt, const Fp8Skinny &p, hipStrea
   return e5m2 ? skinny_tt<true, false, YT>(rt, p, stream) : skinny_tt<false, false, YT>(rt, p, stream);
 }
 
-// fn<E5M2, BR1 or none, YT>(args) for run-time choices of them.
-template <typename YT>
+template <bool WIDE, typename YT>
 hipError_t dense_any(int e5m2, int b_rows, int tile, const DenseArgs &p, int S, hipStream_t stream) {
-  if (b_rows == 1) return e5m2 ? dense_tile<true, true, YT>(tile, p, S, stream) : dense_tile<false, true, YT>(tile, p, S, stream);
-  return e5m2 ? dense_tile<true, false, YT>(tile, p, S, stream) : dense_tile<false, false, YT>(tile, p, S, stream);
+  if (b_rows == 1)
+    return e5m2 ? dense_tile<true, true, WIDE, YT>(tile, p, S, stream) : dense_tile<false, true, WIDE, YT>(tile, p, S, stream);
+  return e5m2 ? dense_tile<true, false, WIDE, YT>(tile, p, S, stream) : dense_tile<false, false, WIDE, YT>(tile, p, S, stream);
 }
 
 template <typename Tile, typename YT>
@@ -320,14 +319,12 @@ hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// The pipe and the tile of the experts' products. Rows of experts are handed on
-// (a token of one route gets its row as it is), so they sum exact products in
-// fp32 where the weights' bytes bound and that costs little: on the bf16 pipe, in
-// tiles of 64 x 128. From 256 rows an expert on (R / E: the groups' lengths are
-// not known here) the products bound, and bf16 rows of e4m3 codes take the 8-bit
-// pipe in tiles of 128 or 256 x 256, priced for groups of equal length with half a
-// tile of remainder. Gradients' rows (e5m2) and f32 outputs stay on the bf16 pipe.
-// us, K -> N, bf16 64 x 128 / 8-bit 64 x 128 / 128 x 256 / 256 x 256:
+// The tile of the experts' products. On the bf16 pipe 64 x 128: widening bounds every tile
+// alike. bf16 rows of e4m3 codes that the caller lets the 8-bit pipe sum go there from 256
+// rows an expert on (R / E: the groups' lengths are not known here), where the products
+// bound, in tiles of 128 or 256 x 256, priced for groups of equal length with half a tile
+// of remainder; below, the weights' bytes bound and it would gain little. us, K -> N, bf16
+// pipe 64 x 128 / 8-bit 64 x 128 / 128 x 256 / 256 x 256:
 //   8 experts   128 rows 2048 -> 5632    44 /  42 /  45 /  33
 //               256 rows 2048 -> 5632     - /  59 /  49 /  66
 //               384 rows 2048 -> 5632    92 /  77 /  72 /  72
@@ -336,16 +333,16 @@ hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
 //                64 rows 2048 -> 5632     - /  54 /  52 /  63
 //   16 experts of 64 rows padded to 128, 5632 -> 2048    64 / 62 / 61 / 67
 // Other tiles of the bf16 pipe (128 x 128 / 128 x 256): 8 x 128 rows 53 / 66, 8 x 1024
-// 205 / 205, 16 x 64 padded to 128 87 / 77: widening bounds every tile alike.
+// 205 / 205, 16 x 64 padded to 128 87 / 77.
 double grouped_cost(const GroupArgs &p, uint32_t bm, uint32_t bn, double ns, int cus) {
   const double tiles = p.E * ((double)p.R / p.E / bm + 0.5) * ((p.N + bn - 1) / bn);
   return ns * std::ceil(tiles / cus);
 }
 
 template <bool E5M2, typename YT>
-hipError_t grouped_tile(const GroupArgs &p, int cus, hipStream_t stream) {
+hipError_t grouped_tile(const GroupArgs &p, int pipe8, int cus, hipStream_t stream) {
   if constexpr (!E5M2 && sizeof(YT) == 2) {
-    if (p.R >= 256u * (uint32_t)p.E)
+    if (pipe8 && p.R >= 256u * (uint32_t)p.E)
       return grouped_cost(p, 256, 256, 1460, cus) < grouped_cost(p, 128, 256, 1010, cus)
                  ? grouped_go<Fp8Ring<8, E5M2, false, false>, YT>(p, stream)
                  : grouped_go<Fp8Ring<4, E5M2, false, false>, YT>(p, stream);
@@ -353,14 +350,13 @@ hipError_t grouped_tile(const GroupArgs &p, int cus, hipStream_t stream) {
   return grouped_go<Fp8Tile<64, 128, 2, 2, E5M2, false, true>, YT>(p, stream);
 }
 
-template <int BM, int BN, bool E5M2, typename YT>
+template <bool E5M2, bool WIDE, typename YT>
 hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
-  using Tile = Fp8Tile<BM, BN, 2, 2, E5M2, true, sizeof(YT) == 4>;
-  const size_t tiles = (size_t)((p.N + BM - 1) / BM) * ((p.K + BN - 1) / BN);
+  using Tile = Fp8Tile<128, 128, 2, 2, E5M2, true, WIDE>;
+  const size_t tiles = (size_t)((p.N + Tile::BM - 1) / Tile::BM) * ((p.K + Tile::BN - 1) / Tile::BN);
   if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
-  return go(fp8_grad_kernel<BM, BN, 2, 2, E5M2, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, (unsigned)E),
-            Tile::NT, stream, p);
+  return go(fp8_grad_kernel<Tile, YT>, Tile::LDS_BYTES, done, dim3((unsigned)tiles, (unsigned)E), Tile::NT, stream, p);
 }
 
 }  // namespace
@@ -388,7 +384,7 @@ constexpr TileCost kWide[] = {{FP8_T_RING6, 192, 256, 1, 2600}, {FP8_T_RING4, 12
 constexpr TileCost kNarrowRows[] = {{FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
 constexpr TileCost kWideRows[] = {{FP8_T_128, 128, 128, 2, 2150}};
 
-Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, int cus) {
+Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int pipe8, int cus) {
   // Few tokens: no join, no tile of 128 mostly empty. Up to 32 always (us, against tiles of 128 x 256
   // in K slices: 32 tokens, K x N 1024^2 4.1 / 9.6, 4096^2 10.2 / 14.7, 4096 x 11008 15.7 / 17.4, 11008 x 4096
   // 20.9 / 20.1), up to 64 while two row tiles a workgroup cover N and the waves' slices of K are short, since
@@ -413,8 +409,8 @@ Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, in
     }
     return {FP8_T_SKINNY, 1, best};
   }
-  const TileCost *costs = b_rows == 1 ? (yt_bf16 ? kNarrowRows : kWideRows) : yt_bf16 ? kNarrow : kWide;
-  const int count = b_rows == 1 ? (yt_bf16 ? 2 : 1) : yt_bf16 ? 4 : 3;
+  const TileCost *costs = b_rows == 1 ? (pipe8 ? kNarrowRows : kWideRows) : pipe8 ? kNarrow : kWide;
+  const int count = b_rows == 1 ? (pipe8 ? 2 : 1) : pipe8 ? 4 : 3;
   Fp8Plan plan = {FP8_T_128, 1, steps};
   double least = 1e30;
   for (int t = 0; t < count; t++) {
@@ -439,16 +435,17 @@ Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, in
 size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p) { return p.S > 1 ? (size_t)p.S * M * N * 4 : 0; }
 
 hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
-                             const float *sb, int b_rows, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
-                             const Fp8Plan &plan, float *part, hipStream_t stream) {
+                             const float *sb, int b_rows, void *y, int yt_bf16, int pipe8, uint32_t M, uint32_t K,
+                             uint32_t N, const Fp8Plan &plan, float *part, hipStream_t stream) {
   if (plan.tile == FP8_T_SKINNY) {
     const Fp8Skinny p = {a, sa, b, sb, y, lda, ldb, M, K, N, 0};
     return yt_bf16 ? skinny_any<uint16_t>(e5m2, b_rows, plan.per, p, stream)
                    : skinny_any<float>(e5m2, b_rows, plan.per, p, stream);
   }
   const DenseArgs p = {a, b, sa, sb, y, plan.S > 1 ? part : nullptr, lda, ldb, M, K, N, plan.per};
-  const hipError_t e = yt_bf16 ? dense_any<uint16_t>(e5m2, b_rows, plan.tile, p, plan.S, stream)
-                               : dense_any<float>(e5m2, b_rows, plan.tile, p, plan.S, stream);
+  const hipError_t e = !yt_bf16 ? dense_any<true, float>(e5m2, b_rows, plan.tile, p, plan.S, stream)
+                       : pipe8  ? dense_any<false, uint16_t>(e5m2, b_rows, plan.tile, p, plan.S, stream)
+                                : dense_any<true, uint16_t>(e5m2, b_rows, plan.tile, p, plan.S, stream);
   if (e != hipSuccess || plan.S == 1) return e;
   const size_t n = (size_t)M * N;
   const dim3 grid((unsigned)((n + 1023) / 1024));
@@ -475,7 +472,7 @@ hipError_t launch_fp8_linear_act(const void *x, int xt_bf16, const uint8_t *b, s
 
 hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *const *b,
                               size_t ldb, const float *const *sb, const uint32_t *offsets, int E, void *y,
-                              int yt_bf16, uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream) {
+                              int yt_bf16, int pipe8, uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream) {
   GroupArgs p = {a, sa, y, offsets, lda, ldb, R, K, N, E, {}, {}};
   for (int e = 0; e < E; e++) {
     p.b[e] = b[e];
@@ -496,17 +493,19 @@ hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const floa
     }
     return hipGetLastError();
   }
-  if (yt_bf16) return e5m2 ? grouped_tile<true, uint16_t>(p, cus, stream) : grouped_tile<false, uint16_t>(p, cus, stream);
-  return e5m2 ? grouped_tile<true, float>(p, cus, stream) : grouped_tile<false, float>(p, cus, stream);
+  if (yt_bf16)
+    return e5m2 ? grouped_tile<true, uint16_t>(p, pipe8, cus, stream) : grouped_tile<false, uint16_t>(p, pipe8, cus, stream);
+  return e5m2 ? grouped_tile<true, float>(p, pipe8, cus, stream) : grouped_tile<false, float>(p, pipe8, cus, stream);
 }
 
 hipError_t launch_fp8_grad_weight(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b,
                                   size_t ldb, const float *sb, const uint32_t *offsets, int E, void *const *dw,
-                                  int yt_bf16, uint32_t R, uint32_t N, uint32_t K, hipStream_t stream) {
+                                  int yt_bf16, int pipe8, uint32_t R, uint32_t N, uint32_t K, hipStream_t stream) {
   GradArgs p = {a, b, sa, sb, offsets, lda, ldb, R, N, K, {}};
   for (int e = 0; e < E; e++) p.dw[e] = dw[e];
-  if (yt_bf16) return e5m2 ? grad_go<128, 128, true, uint16_t>(p, E, stream) : grad_go<128, 128, false, uint16_t>(p, E, stream);
-  return e5m2 ? grad_go<128, 128, true, float>(p, E, stream) : grad_go<128, 128, false, float>(p, E, stream);
+  if (!yt_bf16) return e5m2 ? grad_go<true, true, float>(p, E, stream) : grad_go<false, true, float>(p, E, stream);
+  if (pipe8) return e5m2 ? grad_go<true, false, uint16_t>(p, E, stream) : grad_go<false, false, uint16_t>(p, E, stream);
+  return e5m2 ? grad_go<true, true, uint16_t>(p, E, stream) : grad_go<false, true, uint16_t>(p, E, stream);
 }
 
 }  // namespace frx

@@ -7,16 +7,17 @@
 // then holds four consecutive n of one token, so a block's scale is one number
 // per lane and token fragment (b_rows = 128).
 //
-// Two pipes, chosen by the output's type:
-//  - bf16 outputs: v_mfma_f32_16x16x128_f8f6f4, which covers exactly one block
-//    (4356 TFLOP/s in a loop of nothing else). It adds groups of 8 products
-//    cut to 14 bits below the group's largest power of two (measured: beside a
-//    product of 2^8 one of 2^-5 is kept and one of 2^-6 is dropped; across
-//    groups the sum is fp32): at most 2^-10 of a group's magnitudes, 1.5e-5 of
-//    the result on normal values, against the 2^-9 of the bf16 rounding.
-//  - f32 outputs, which would show that, and most experts' rows (frx_fp8.hip): the codes widened to bf16 (exact, one
-//    conversion per two codes) into four v_mfma_f32_16x16x32_bf16, whose
-//    products are exact and whose sums are fp32, at half the rate.
+// Two pipes:
+//  - bf16 (WIDE), for every output unless the caller asks otherwise: the codes widened to
+//    bf16 (exact, one conversion per two codes) into four v_mfma_f32_16x16x32_bf16,
+//    whose products are exact and whose sums are fp32.
+//  - 8-bit, for bf16 outputs under FRX_FP8_SUMS_PIPE: v_mfma_f32_16x16x128_f8f6f4, which
+//    covers exactly one block at twice the rate (4356 TFLOP/s in a loop of nothing else).
+//    It adds groups of 8 products cut to multiples of 2^-13 of the group's largest power
+//    of two (measured: beside a product of 2^8 one of 2^-5 is kept and one of 2^-6 is
+//    dropped; across groups the sum is fp32): at most 2^-10 of a group's magnitudes,
+//    1.5e-5 of the result on normal values, which turns the bf16 rounding of 1 in 130
+//    values. So it is a choice of the caller's.
 //
 // Data movement. Rows of 128 bytes go global -> LDS with 16-byte LDS DMA
 // (buffer_load ... lds), the scales of the step with 4-byte DMA behind them, so

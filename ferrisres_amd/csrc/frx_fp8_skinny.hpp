@@ -84,10 +84,12 @@ __device__ __forceinline__ void fp8_skinny_quantize(const Fp8Skinny &p, uint8_t 
   }
 }
 
-template <int RT, int TT, bool E5M2, bool BR1, bool WIDE, typename XT, typename YT>
+// On the bf16 pipe whatever the output: the 8-bit one would save 3% (bf16 y, 64 tokens of
+// 4096 x 4096 14.5 us against 15.0).
+template <int RT, int TT, bool E5M2, bool BR1, typename XT, typename YT>
 __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x4 *red) {
   constexpr bool CODES = sizeof(XT) == 1;
-  using Pipe = Fp8Pipe<WIDE>;
+  using Pipe = Fp8Pipe<true>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const int K = (int)p.K, kbs = (K + 127) >> 7;

@@ -349,11 +349,12 @@ struct Fp8Plan {
   int S, per;   // K slices, blocks of 128 in each (FP8_T_SKINNY: 1, 16-row tiles of a workgroup)
 };
 enum { FP8_T_SKINNY = 0, FP8_T_128 = 1, FP8_T_RING8 = 2, FP8_T_RING6 = 3, FP8_T_RING4 = 4 };
-Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int yt_bf16, int cus);
+// pipe8: the 8-bit pipe may sum (bf16 outputs under FRX_FP8_SUMS_PIPE), here and below
+Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int pipe8, int cus);
 size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p);
 hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
-                             const float *sb, int b_rows, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
-                             const Fp8Plan &plan, float *part, hipStream_t stream);
+                             const float *sb, int b_rows, void *y, int yt_bf16, int pipe8, uint32_t M, uint32_t K,
+                             uint32_t N, const Fp8Plan &plan, float *part, hipStream_t stream);
 // x f32 or bf16 [M][K], quantised on the way (FP8_T_SKINNY plans whose
 // activations fit: fp8_act_fits). Every workgroup makes the codes for itself,
 // which pays while they are few (11008 x 4096, us, one launch / quantiser and
@@ -366,10 +367,11 @@ hipError_t launch_fp8_linear_act(const void *x, int xt_bf16, const uint8_t *b, s
                                  hipStream_t stream);
 hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *const *b,
                               size_t ldb, const float *const *sb, const uint32_t *offsets, int E, void *y,
-                              int yt_bf16, uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream);
+                              int yt_bf16, int pipe8, uint32_t R, uint32_t K, uint32_t N, int cus,
+                              hipStream_t stream);
 hipError_t launch_fp8_grad_weight(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b,
                                   size_t ldb, const float *sb, const uint32_t *offsets, int E, void *const *dw,
-                                  int yt_bf16, uint32_t R, uint32_t N, uint32_t K, hipStream_t stream);
+                                  int yt_bf16, int pipe8, uint32_t R, uint32_t N, uint32_t K, hipStream_t stream);
 
 // ---- tokens sorted by expert, and back (frx_route.hip) -----------------------
 struct RouteRows {

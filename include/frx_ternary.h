@@ -313,6 +313,22 @@ typedef enum frx_fp8_blocks {
   FRX_FP8_BLOCKS_RANGE_ = 0x7fffffff
 } frx_fp8_blocks;
 
+/* How the products below add up a bf16 y (an f32 y always goes by FRX_FP8_SUMS_F32). */
+typedef enum frx_fp8_sums {
+  FRX_FP8_SUMS_F32 = 0,  /* exact products added in fp32, one rounding to bf16 at the end (default) */
+  FRX_FP8_SUMS_PIPE = 1, /* where it is faster, on the matrix pipe for 8-bit operands, which cuts the
+                            products of each group of 8 to 2^-13 of the largest one's power of two: less
+                            than 2^-10 of the sum of the magnitudes, 1.5e-5 of the result on normally
+                            distributed values, before the 2^-9 of bf16 */
+  FRX_FP8_SUMS_RANGE_ = 0x7fffffff
+} frx_fp8_sums;
+
+/* Selects the sums of every 8-bit linear that the context runs from here on (a
+ * captured graph keeps those that it was captured with). The pipe is used above a
+ * few tokens (up to 1.9 times as fast: 2048 tokens of 4096 x 11008 88 us against
+ * 167), and by frx_fp8_linear_grouped for e4m3 rows where R >= 256 E. */
+frx_status frx_set_fp8_sums(frx_ctx *ctx, frx_fp8_sums mode);
+
 /* Codes and scales of x [M][K] (f32 or bf16, row stride ldx >= K elements).
  * For each block: scale = max(amax * f32(1 / top), 2^-126), top = 448 or
  * 57344; code = the product x * f32(1 / scale) rounded to nearest even. Each
@@ -339,12 +355,9 @@ frx_status frx_fp8_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t 
  *     dx = dy w:    a = dy ROWS,   b = w TILES_T   (M x N times N x K)
  *     dw = dy^T x:  a = dy COLS,   b = x COLS      (sums over the tokens, rounded
  *                                  up to 16: the quantiser's zero codes)
- * Sums in fp32: a block's 128 products on the matrix pipe, then the blocks in
- * order, each times its two scales; one rounding to yt at the end. For an f32 y
- * the products are exact and added in fp32. For a bf16 y the 8-bit pipe adds
- * them, which cuts the products of each group of 8 to 2^-13 of the largest
- * one's power of two: less than 2^-10 of the sum of the magnitudes, 1.5e-5 of
- * the result on normally distributed values, before the 2^-9 of bf16.
+ * Sums in fp32: a block's 128 products, which are exact, on the matrix pipe, then
+ * the blocks in order, each times its two scales; one rounding to yt at the end
+ * (frx_set_fp8_sums selects fewer bits for a bf16 y).
  * Requires K % 16 == 0, lda and ldb multiples of 16, >= K and <= 2^23, a and b
  * 16-byte aligned, M, N >= 1, (M / 64 + 65) * ceil(N / 128) < 2^24; y aligned to
  * its element. Where there are few tiles, K is split over workgroups: fp32 parts
@@ -369,9 +382,7 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
  *   a [R][lda], sa [R][ceil(K / 128)]; b[e] [N][ldb] e4m3, sb[e] [ceil(N / 128)]
  *   [ceil(K / 128)] (host arrays of E device pointers); offsets [E + 1] u32 on
  *   the device, ascending; y [R][N]. Rows from offsets[E] on are neither read
- *   nor written. 1 <= E <= 64; otherwise as frx_fp8_linear, except that a bf16 y
- *   too is the fp32 sum of exact products, rounded once, for e5m2 rows
- *   (gradients) and for R < 256 E. No allocation. */
+ *   nor written. 1 <= E <= 64; otherwise as frx_fp8_linear. No allocation. */
 frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
                                   const uint8_t *const *b, size_t ldb, const float *const *sb,
                                   const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R,
