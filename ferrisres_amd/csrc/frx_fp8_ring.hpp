@@ -135,7 +135,10 @@ struct Fp8Ring {
     };
     const auto add = [&](f32x4 &a, const f32x4 &p, float s, const f32x4 &sw) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) a[e] += p[e] * (BR1 ? s * sw[e] : s);
+      for (int e = 0; e < 4; e++) {
+        if (BR1) a[e] += p[e] * s * sw[e];
+        else a[e] += p[e] * s;
+      }
     };
     const int full = min(o.kb1, o.K >> 7);  // whole blocks; at most one more behind them
     if (o.kb0 < full) {
@@ -153,16 +156,18 @@ struct Fp8Ring {
       typename Pipe::Op w[FN];
       i32x8 xc;  // the next token fragment
       f32x4 p[2][FN], sw[FN] = {};
-      float sn, sb = 0.f, s[2] = {0.f, 0.f};
+      float sn, s[2] = {0.f, 0.f};
+      Fp8Block sb;
 #pragma unroll
       for (int fn = 0; fn < FN; fn++) {
         w[fn] = Pipe::template op<false>(op(lds, wo + fn * 512));
         p[1][fn] = (f32x4){0.f, 0.f, 0.f, 0.f};
         if (BR1) sw[fn] = *reinterpret_cast<const f32x4 *>(lds + bo + fn * 16);
       }
-      if (!BR1) sb = reinterpret_cast<const float *>(lds)[bo];
+      if (!BR1) sb = Fp8Block(reinterpret_cast<const float *>(lds)[bo]);
       xc = op(lds, xo);
       sn = reinterpret_cast<const float *>(lds)[so];
+      Fp8Factor xf = fp8_factor<WIDE, BR1>(sn, sb);
       int at = 0;  // dwords to the stage of block kb
       for (int kb = o.kb0; kb < full; kb++) {
         uint32_t *cur = lds + at;
@@ -171,7 +176,7 @@ struct Fp8Ring {
         uint32_t *nxt = lds + at;
         uint32_t *prv = nxt;  // the stage of block kb - 1 (and of kb - 1 + NS)
         if (NS == 3) prv = lds + (at == 2 * STAGE ? 0 : at + STAGE);
-        float sbn = sb;
+        float sbn = 0.f;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int fm = 0; fm < FM; fm++) {
@@ -200,8 +205,8 @@ struct Fp8Ring {
 #pragma unroll
             for (int i = first; i < first + PER && i < LB; i++) load(LA + i, cur, c, kb + NS);
           }
-          const auto x = Pipe::template op<E5M2>(xc);
-          s[fm & 1] = BR1 ? sn : sn * sb;
+          const auto x = Pipe::template op<E5M2>(xc, xf.f);
+          s[fm & 1] = xf.s;
           // the next fragment's operand
           const uint32_t *st = end ? nxt : cur;
           xc = op(st, xo + (fm + 1) % FM * 512);
@@ -217,6 +222,8 @@ struct Fp8Ring {
             if (end) w[fn] = Pipe::template op<false>(WIDE ? wr[fn] : op(nxt, wo + fn * 512));
             if (CARRY || fm > 0) add(acc[fn][(fm + FM - 1) % FM], p[(fm + 1) & 1][fn], s[(fm + 1) & 1], sw[fn]);
           }
+          if (end && !BR1) sb = Fp8Block(sbn);
+          xf = fp8_factor<WIDE, BR1>(sn, sb);
           // a product; the operand reads behind the first; its multiply-adds
 #pragma unroll
           for (int fn = 0; fn < FN; fn++) {
@@ -240,7 +247,6 @@ struct Fp8Ring {
             }
           }
         }
-        sb = sbn;
       }
       if (CARRY)
 #pragma unroll
@@ -259,12 +265,12 @@ struct Fp8Ring {
       const float *sc = reinterpret_cast<const float *>(lds);
 #pragma unroll
       for (int fm = 0; fm < FM; fm++) {
-        const auto x = Pipe::template op<E5M2>(op(lds, xo + fm * 512));
-        const float s = BR1 ? sc[so + fm * 16] : sc[so + fm * 16] * sc[bo];
+        const Fp8Factor xf = fp8_factor<WIDE, BR1>(sc[so + fm * 16], Fp8Block(BR1 ? 0.f : sc[bo]));
+        const auto x = Pipe::template op<E5M2>(op(lds, xo + fm * 512), xf.f);
 #pragma unroll
         for (int fn = 0; fn < FN; fn++) {
           const f32x4 sw = BR1 ? *reinterpret_cast<const f32x4 *>(lds + bo + fn * 16) : (f32x4){0.f, 0.f, 0.f, 0.f};
-          add(acc[fn][fm], Pipe::template mul<E5M2>(Pipe::template op<false>(op(lds, wo + fn * 512)), x), s, sw);
+          add(acc[fn][fm], Pipe::template mul<E5M2>(Pipe::template op<false>(op(lds, wo + fn * 512)), x), xf.s, sw);
         }
       }
     }

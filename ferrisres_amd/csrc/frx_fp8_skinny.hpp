@@ -136,6 +136,9 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
 #pragma unroll
       for (int r = 0; r < RT; r++) fp8_row_load(wrow[r], kb * 128, K, g, wlo[r], whi[r]);
     }
+    Fp8Block sb[RT];
+#pragma unroll
+    for (int r = 0; r < NB; r++) sb[r] = Fp8Block(sblk[r][kb]);
     typename Pipe::Op x[TT];
     float s[TT];
 #pragma unroll
@@ -153,11 +156,14 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
         if (kb * 128 + 16 * g >= K) xlo = (u32x4){0, 0, 0, 0};
         if (kb * 128 + 64 + 16 * g >= K) xhi = (u32x4){0, 0, 0, 0};
       }
-      x[t] = Pipe::template op<E5M2>(fp8_join(xlo, xhi));
+      float f = 1.0f;
+      if (NB == 1) {
+        const Fp8Factor xf = fp8_factor<true, BR1>(s[t], sb[0]);
+        s[t] = xf.s;
+        f = xf.f;
+      }
+      x[t] = Pipe::template op<E5M2>(fp8_join(xlo, xhi), f);
     }
-    float sb[RT];
-#pragma unroll
-    for (int r = 0; r < NB; r++) sb[r] = sblk[r][kb];
 #pragma unroll
     for (int r = 0; r < RT; r++) {
       const auto w = Pipe::template op<false>(fp8_join(wlo[r], whi[r]));
@@ -168,8 +174,17 @@ __device__ __forceinline__ void fp8_skinny(const Fp8Skinny &p, uint32_t n0, f32x
 #pragma unroll
       for (int t = 0; t < TT; t++) {
         const f32x4 q = Pipe::template mul<E5M2>(w, x[t]);
+        if constexpr (BR1) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[r][t][e] += q[e] * (s[t] * (BR1 ? sw[e] : sb[NB == RT ? r : 0]));
+          for (int e = 0; e < 4; e++) acc[r][t][e] += q[e] * s[t] * sw[e];
+        } else if constexpr (NB == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[r][t][e] += q[e] * s[t];
+        } else {  // blocks of their own: the factor's power of two goes to the product
+          const Fp8Factor xf = fp8_factor<true, BR1>(s[t], sb[r]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[r][t][e] += q[e] * xf.f * xf.s;
+        }
       }
     }
   }

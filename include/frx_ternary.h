@@ -319,7 +319,8 @@ typedef enum frx_fp8_sums {
   FRX_FP8_SUMS_PIPE = 1, /* where it is faster, on the matrix pipe for 8-bit operands, which cuts the
                             products of each group of 8 to 2^-13 of the largest one's power of two: less
                             than 2^-10 of the sum of the magnitudes, 1.5e-5 of the result on normally
-                            distributed values, before the 2^-9 of bf16 */
+                            distributed values, before the 2^-9 of bf16. The two scales of a block are
+                            multiplied in f32 first, which loses bits of products below 2^-126 */
   FRX_FP8_SUMS_RANGE_ = 0x7fffffff
 } frx_fp8_sums;
 
@@ -357,7 +358,10 @@ frx_status frx_fp8_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t 
  *                                  up to 16: the quantiser's zero codes)
  * Sums in fp32: a block's 128 products, which are exact, on the matrix pipe, then
  * the blocks in order, each times its two scales; one rounding to yt at the end
- * (frx_set_fp8_sums selects fewer bits for a bf16 y).
+ * (frx_set_fp8_sums selects fewer bits for a bf16 y). The product of the two
+ * scales may be smaller than any f32 number (gradients of 1e-30 and less). With
+ * b_rows = 1 a block's product is multiplied by sa first, which holds for values of
+ * a up to 5e33.
  * Requires K % 16 == 0, lda and ldb multiples of 16, >= K and <= 2^23, a and b
  * 16-byte aligned, M, N >= 1, (M / 64 + 65) * ceil(N / 128) < 2^24; y aligned to
  * its element. Where there are few tiles, K is split over workgroups: fp32 parts
