@@ -337,10 +337,11 @@ def _dense(t, shape, dtype, name):
         raise _shape_err(f"{name} must be contiguous")
 
 
-def _per_expert(ts, E, shape, dtype, name, rows=False):
+def _per_expert(ts, E, shape, dtype, name, rows=False, out=False):
     """(array.array of E device addresses, row stride) of a stacked tensor [E, ...]
     or a list of E tensors; rows: 2-D with unit column stride, all of one row
-    stride, else contiguous."""
+    stride, else contiguous. out: written to, so the experts lie apart (the library
+    looks at a list's addresses itself)."""
     if E < 1:
         raise _shape_err("offsets [E + 1] must be of at least one expert")
     if hasattr(ts, "dim"):  # stacked
@@ -353,6 +354,8 @@ def _per_expert(ts, E, shape, dtype, name, rows=False):
         if (n > 1 and col != 1) or (m > 1 and ld < n) or (not rows and m > 1 and ld != n):
             raise _shape_err(f"{name} must have {'unit column stride' if rows else 'contiguous experts'}, got strides "
                              f"{ts.stride()}")
+        if out and E > 1 and step < m * n:
+            raise _shape_err(f"{name}: the experts overlap, got strides {ts.stride()}")
         base, step = ts.data_ptr(), step * ts.element_size()
         at = array.array("Q", range(base, base + E * step, step) if step else [base] * E)
         return at, ld if m > 1 else max(ld, n)
@@ -753,7 +756,7 @@ class Context:
         _dense(sa, (N, rb), torch.float32, "sa")
         _dense(sb, (K, rb), torch.float32, "sb")
         dt = dw[0].dtype if len(dw) else None
-        dp, _ = _per_expert(dw, E, (N, K), dt, "dw")
+        dp, _ = _per_expert(dw, E, (N, K), dt, "dw", out=True)
         _check(lib().frx_fp8_grad_weight_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
                                                  b.data_ptr(), ldb, sb.data_ptr(), offsets.data_ptr(), E,
                                                  dp.buffer_info()[0],

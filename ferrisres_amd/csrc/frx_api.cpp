@@ -16,6 +16,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <mutex>
 #include <vector>
 
@@ -1674,6 +1675,12 @@ frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t ld
   if ((st = check_fp8(ctx, a, lda, at, sa, ldb, yt, N, R, K)) != FRX_OK) return st;
   for (uint32_t e = 0; e < E; e++)
     if ((st = check_fp8_side(ctx, b, sb, dw[e], yt)) != FRX_OK) return st;
+  // two experts' workgroups must not write one place
+  uintptr_t to[frx::FP8_MAXE];
+  for (uint32_t e = 0; e < E; e++) to[e] = reinterpret_cast<uintptr_t>(dw[e]);
+  std::sort(to, to + E);
+  for (uint32_t e = 1; e < E; e++)
+    if (to[e] - to[e - 1] < (size_t)N * K * dtype_bytes(yt)) return fail(ctx, FRX_ERR_SHAPE, "two experts' dw overlap");
   if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
   const hipError_t e = frx::launch_fp8_grad_weight(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, offsets, (int)E, dw,
                                                    yt == FRX_BF16, fp8_pipe8(ctx, yt), R, N, K, ctx->stream);

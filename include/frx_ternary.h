@@ -398,7 +398,7 @@ frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, fr
  *   a [N][lda] codes of type at (dy), sa [N][ceil(R / 128)]; b [K][ldb] e4m3
  *   codes (x), sb [K][ceil(R / 128)]; offsets [E + 1] as above, multiples of 128
  *   (a sort with align = 128); dw[e] [N][K] yt (host array of E device
- *   pointers; zeros for an expert without rows). R % 16 == 0, 1 <= E <= 64. No
+ *   pointers, of matrices that do not overlap; zeros for an expert without rows). R % 16 == 0, 1 <= E <= 64. No
  *   allocation. */
 frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at,
                                        const float *sa, const uint8_t *b, size_t ldb, const float *sb,
