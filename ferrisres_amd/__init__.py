@@ -315,6 +315,11 @@ def _fp8_code(t) -> int:
     raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2, got {t.dtype}")
 
 
+def _one_row(n):
+    """The row stride that stands for a single row's, which no address goes by: one that the library takes."""
+    return (n + 15) // 16 * 16
+
+
 def _rows2(t, name):
     """(rows, columns, row stride in elements) of a 2-D tensor with unit
     column stride."""
@@ -324,7 +329,7 @@ def _rows2(t, name):
     ld, col = t.stride()
     if n > 1 and col != 1:
         raise _shape_err(f"{name} must have unit column stride, got strides {t.stride()}")
-    return m, n, ld if m > 1 else max(ld, n)
+    return m, n, ld if m > 1 else _one_row(n)
 
 
 def _dense(t, shape, dtype, name):
@@ -358,7 +363,7 @@ def _per_expert(ts, E, shape, dtype, name, rows=False, out=False):
             raise _shape_err(f"{name}: the experts overlap, got strides {ts.stride()}")
         base, step = ts.data_ptr(), step * ts.element_size()
         at = array.array("Q", range(base, base + E * step, step) if step else [base] * E)
-        return at, ld if m > 1 else max(ld, n)
+        return at, ld if m > 1 else _one_row(n)
     if len(ts) != E:
         raise _shape_err(f"{name} holds {len(ts)} experts, expected {E}")
     ld = None

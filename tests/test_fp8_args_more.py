@@ -34,3 +34,21 @@ def test_shared_weights_are_read(ctx):  # noqa: F811
     off = torch.zeros((4,), dtype=torch.int32)
     reaches_the_library(lambda: ctx.fp8_linear_grouped(a, sa, b.expand(3, 40, 256), sb.expand(3, 1, 2), off, y))
     reaches_the_library(lambda: ctx.fp8_linear_grouped(a, sa, [b] * 3, [sb] * 3, off, y))
+
+
+@pytest.mark.parametrize("n", [16, 48, 256])
+def test_a_single_row_has_any_stride(ctx, n):  # noqa: F811
+    """The stride of a matrix of one row leads nowhere: whatever it is, the library gets one that it takes (a multiple
+    of 16 that holds the row, up to 2^23), and rows of different strides may be one list's."""
+    buf = torch.zeros((64 + n,)).to(E4M3)
+    one = [buf.as_strided((1, n), (stride, 1)) for stride in (0, 1, n, n + 5, n + 16, 1 << 24)]
+    for t in one:
+        assert frx._rows2(t, "a")[:2] == (1, n)
+        ld = frx._rows2(t, "a")[2]
+        assert ld % 16 == 0 and n <= ld <= 1 << 23
+    at, ld = frx._per_expert(one, len(one), (1, n), E4M3, "b", rows=True)
+    assert ld % 16 == 0 and n <= ld <= 1 << 23 and len(at) == len(one)
+    at, ld = frx._per_expert(buf.as_strided((3, 1, n), (16, 1000003, 1)), 3, (1, n), E4M3, "b", rows=True)
+    assert ld % 16 == 0 and n <= ld <= 1 << 23 and at[1] - at[0] == 16
+    for rows in (2, 3):  # more rows: the stride as it is
+        assert frx._rows2(buf.as_strided((rows, n), (5, 1)), "a")[2] == 5

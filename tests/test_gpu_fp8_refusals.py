@@ -35,3 +35,30 @@ def test_gradients_of_experts_lie_apart(ctx):
     ctx.fp8_grad_weight_grouped(a, sa, b, sb, off, [at(2 * N * K), at(0), at(N * K)])
     torch.cuda.synchronize()
     assert not buf[:E * N * K].any() and (buf[E * N * K:] == 7.0).all()
+
+
+def test_a_single_row_has_any_stride(ctx):
+    """One token (one weight row) out of a matrix whose rows are of no multiple of 16 apart, in every operand."""
+    k = 272
+    g = torch.Generator().manual_seed(1)
+    wide = torch.randn((3, k + 5), generator=g).to(DEV)
+    x = wide[1:2, :k]
+    q, s = torch.zeros((1, k), dtype=E4M3, device=DEV), torch.zeros((1, 3), device=DEV)
+    ctx.fp8_quantize(x, frx.FP8_ROWS, q, s)
+    raw = torch.zeros((2 * 1000003 + k,), dtype=torch.uint8, device=DEV).view(E4M3)
+    q2 = raw.as_strided((1, k), (1000003, 1))  # the codes at its start, of an odd row stride
+    s2 = torch.zeros_like(s)
+    ctx.fp8_quantize(x, frx.FP8_ROWS, q2, s2)
+    assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(s, s2)
+    w = torch.randn((24, k), generator=g).to(DEV)
+    b, sb = torch.zeros((24, k), dtype=E4M3, device=DEV), torch.zeros((1, 3), device=DEV)
+    ctx.fp8_quantize(w, frx.FP8_TILES, b, sb)
+    y, y2 = torch.zeros((1, 24), device=DEV), torch.zeros((1, 24), device=DEV)
+    ctx.fp8_linear(q, s, b, sb, y)
+    ctx.fp8_linear(q2, s, b, sb, y2)
+    assert torch.equal(y, y2) and y.abs().min() > 0
+    t, t2 = torch.zeros((24, 1), device=DEV), torch.zeros((24, 1), device=DEV)
+    ctx.fp8_quantize(w, frx.FP8_ROWS, b, rows := torch.zeros((24, 3), device=DEV))
+    ctx.fp8_linear(b, rows, q, s, t)  # the row as the one weight row
+    ctx.fp8_linear(b, rows, q2, s, t2)
+    assert torch.equal(t, t2) and t.abs().min() > 0
