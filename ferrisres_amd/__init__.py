@@ -704,7 +704,7 @@ class Context:
             raise TypeError(f"b must be float8_e4m3fn, got {b.dtype}")
         kb = (K + 127) // 128
         _dense(sa, (M, kb), torch.float32, "sa")
-        b_rows = 1 if len(sb) == N else 128
+        b_rows = 128 if len(sb) == (N + 127) // 128 else 1  # (one weight row: either, as fp8_linear_act)
         _dense(sb, (N if b_rows == 1 else (N + 127) // 128, kb), torch.float32, "sb")
         _dense(y, (M, N), None, "y")
         _check(lib().frx_fp8_linear(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(), b.data_ptr(), ldb,
