@@ -315,6 +315,13 @@ def _fp8_code(t) -> int:
     raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2, got {t.dtype}")
 
 
+def _here(d, *ts):
+    """The tensors (None among them) are on device d, the context's: an address of any other memory would fault there."""
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise FrxError(3, f"a tensor is on {t.device}, the context on cuda:{d}")
+
+
 def _one_row(n):
     """The row stride that stands for a single row's, which no address goes by: one that the library takes."""
     return (n + 15) // 16 * 16
@@ -342,16 +349,18 @@ def _dense(t, shape, dtype, name):
         raise _shape_err(f"{name} must be contiguous")
 
 
-def _per_expert(ts, E, shape, dtype, name, rows=False, out=False):
+def _per_expert(ts, E, shape, dtype, name, rows=False, out=False, dev=-1):
     """(array.array of E device addresses, row stride) of a stacked tensor [E, ...]
     or a list of E tensors; rows: 2-D with unit column stride, all of one row
-    stride, else contiguous. out: written to, so the experts lie apart (the library
+    stride, else contiguous; dev: their device. out: written to, so the experts lie apart (the library
     looks at a list's addresses itself)."""
     if E < 1:
         raise _shape_err("offsets [E + 1] must be of at least one expert")
     if hasattr(ts, "dim"):  # stacked
         if ts.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {ts.dtype}")
+        if ts.get_device() != dev:
+            _here(dev, ts)
         m, n = shape
         if ts.shape != (E, m, n):
             raise _shape_err(f"{name} has shape {tuple(ts.shape)}, expected {(E, *shape)}")
@@ -379,6 +388,7 @@ def _per_expert(ts, E, shape, dtype, name, rows=False, out=False):
             ld = stride
         else:
             _dense(t, shape, dtype, name)
+    _here(dev, *ts)
     return array.array("Q", [t.data_ptr() for t in ts]), ld
 
 
@@ -396,6 +406,8 @@ class MoeRows:
         _dense(offsets, (self.E + 1,), torch.int32, "offsets")
         _dense(row_of, (self.T, self.top_k), torch.int32, "row_of")
         _dense(slot_of, (self.R,), torch.int32, "slot_of")
+        if not offsets.device == row_of.device == slot_of.device:
+            raise FrxError(3, f"the index tensors are on {offsets.device}, {row_of.device} and {slot_of.device}")
         self.offsets, self.row_of, self.slot_of = offsets, row_of, slot_of
         self._c = _MoeRowsC(self.T, self.top_k, self.E, self.align, self.R, offsets.data_ptr(), row_of.data_ptr(),
                             slot_of.data_ptr())
@@ -433,10 +445,12 @@ class DeviceBuffer:
 class Context:
     """Owns an frx_ctx bound to one device and (optionally) a torch stream."""
 
+    _dev = -1  # the device's index, as torch counts them (-1: host memory)
+
     def __init__(self, device: int = 0, stream=None):
         h = _vp()
         _check(lib().frx_create(device, ctypes.byref(h)))
-        self._h = h
+        self._h, self._dev = h, device
         if stream is not None:
             self.set_stream(stream)
 
@@ -687,6 +701,8 @@ class Context:
             raise _shape_err(f"q has shape {tuple(q.shape)}, expected {(r, (c + 15) // 16 * 16)}")
         sr = (r + 127) // 128 if blocks in (FP8_TILES, FP8_TILES_T) else r
         _dense(scale, (sr, (c + 127) // 128), torch.float32, "scale")
+        if not x.get_device() == q.get_device() == scale.get_device() == self._dev:
+            _here(self._dev, x, q, scale)
         _check(lib().frx_fp8_quantize(self._h, x.data_ptr(), _dtype_code(x), M, K, ldx, blocks, _fp8_code(q),
                                       q.data_ptr(), ldq, scale.data_ptr()), self._h)
         return q, scale
@@ -707,6 +723,8 @@ class Context:
         b_rows = 128 if len(sb) == (N + 127) // 128 else 1  # (one weight row: either, as fp8_linear_act)
         _dense(sb, (N if b_rows == 1 else (N + 127) // 128, kb), torch.float32, "sb")
         _dense(y, (M, N), None, "y")
+        if not a.get_device() == sa.get_device() == b.get_device() == sb.get_device() == y.get_device() == self._dev:
+            _here(self._dev, a, sa, b, sb, y)
         _check(lib().frx_fp8_linear(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(), b.data_ptr(), ldb,
                                     sb.data_ptr(), b_rows, y.data_ptr(), _dtype_code(y), M, K, N), self._h)
         return y
@@ -724,6 +742,8 @@ class Context:
         _dense(x, (M, K), None, "x")
         _dense(sb, ((N + 127) // 128, (K + 127) // 128), torch.float32, "sb")
         _dense(y, (M, N), None, "y")
+        if not x.get_device() == b.get_device() == sb.get_device() == y.get_device() == self._dev:
+            _here(self._dev, x, b, sb, y)
         _check(lib().frx_fp8_linear_act(self._h, x.data_ptr(), _dtype_code(x), b.data_ptr(), ldb, sb.data_ptr(),
                                         y.data_ptr(), _dtype_code(y), M, K, N), self._h)
         return y
@@ -738,9 +758,11 @@ class Context:
         N = int(y.shape[1]) if y.dim() == 2 else 0
         _dense(offsets, (E + 1,), torch.int32, "offsets")
         _dense(sa, (R, kb), torch.float32, "sa")
-        bp, ldb = _per_expert(b, E, (N, K), torch.float8_e4m3fn, "b", rows=True)
-        sp, _ = _per_expert(sb, E, ((N + 127) // 128, kb), torch.float32, "sb")
+        bp, ldb = _per_expert(b, E, (N, K), torch.float8_e4m3fn, "b", rows=True, dev=self._dev)
+        sp, _ = _per_expert(sb, E, ((N + 127) // 128, kb), torch.float32, "sb", dev=self._dev)
         _dense(y, (R, N), None, "y")
+        if not a.get_device() == sa.get_device() == offsets.get_device() == y.get_device() == self._dev:
+            _here(self._dev, a, sa, offsets, y)
         _check(lib().frx_fp8_linear_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
                                             bp.buffer_info()[0], ldb, sp.buffer_info()[0],
                                             offsets.data_ptr(), E, y.data_ptr(), _dtype_code(y), R, K, N), self._h)
@@ -761,7 +783,8 @@ class Context:
         _dense(sa, (N, rb), torch.float32, "sa")
         _dense(sb, (K, rb), torch.float32, "sb")
         dt = dw[0].dtype if len(dw) else None
-        dp, _ = _per_expert(dw, E, (N, K), dt, "dw", out=True)
+        dp, _ = _per_expert(dw, E, (N, K), dt, "dw", out=True, dev=self._dev)
+        _here(self._dev, a, sa, b, sb, offsets)
         _check(lib().frx_fp8_grad_weight_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
                                                  b.data_ptr(), ldb, sb.data_ptr(), offsets.data_ptr(), E,
                                                  dp.buffer_info()[0],
@@ -779,6 +802,8 @@ class Context:
         outside [0, E) goes nowhere)."""
         torch = _torch or _tt()
         _dense(topk_idx, (rows.T, rows.top_k), torch.int32, "topk_idx")
+        if not topk_idx.get_device() == rows.slot_of.get_device() == self._dev:
+            _here(self._dev, topk_idx, rows.slot_of)
         _check(lib().frx_moe_sort(self._h, topk_idx.data_ptr(), rows._p), self._h)
         return rows
 
@@ -787,6 +812,8 @@ class Context:
         rows of any type whose bytes are a multiple of 4."""
         _dense(x, (rows.T, *x.shape[1:]), None, "x")
         _dense(xs, (rows.R, *x.shape[1:]), x.dtype, "xs")
+        if not x.get_device() == rows.slot_of.get_device() == xs.get_device() == self._dev:
+            _here(self._dev, x, rows.slot_of, xs)
         _check(lib().frx_moe_dispatch(self._h, x.data_ptr(), x.numel() // max(rows.T, 1) * x.element_size(), rows._p,
                                       xs.data_ptr()), self._h)
         return xs
@@ -800,6 +827,7 @@ class Context:
         _dense(y, (rows.T, H), None, "y")
         if w is not None:
             _dense(w, (rows.T, rows.top_k), torch.float32, "w")
+        _here(self._dev, ys, rows.slot_of, w, y)
         _check(lib().frx_moe_combine(self._h, ys.data_ptr(), _dtype_code(ys), rows._p, w if w is None else w.data_ptr(),
                                      y.data_ptr(), _dtype_code(y), H), self._h)
         return y
@@ -818,6 +846,7 @@ class Context:
             _dense(dw, (rows.T, rows.top_k), torch.float32, "dw")
         if w is not None:
             _dense(w, (rows.T, rows.top_k), torch.float32, "w")
+        _here(self._dev, dy, ys, rows.slot_of, w, dys, dw)
         ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
         _check(lib().frx_moe_combine_backward(self._h, dy.data_ptr(), _dtype_code(dy), ptr(ys), _dtype_code(dys),
                                               rows._p, ptr(w), dys.data_ptr(), ptr(dw), H), self._h)

@@ -52,3 +52,34 @@ def test_a_single_row_has_any_stride(ctx, n):  # noqa: F811
     assert ld % 16 == 0 and n <= ld <= 1 << 23 and at[1] - at[0] == 16
     for rows in (2, 3):  # more rows: the stride as it is
         assert frx._rows2(buf.as_strided((rows, n), (5, 1)), "a")[2] == 5
+
+
+def test_tensors_of_another_device_are_refused(ctx):  # noqa: F811
+    """Host tensors (or another card's) before a context of cuda:0: a device error of the binding's own, in place of
+    an address that means nothing there."""
+    i32 = lambda *d: torch.zeros(d, dtype=torch.int32)  # noqa: E731
+    ctx._dev = 0
+
+    def refused(call):
+        with pytest.raises(frx.FrxError, match="the context on cuda:0") as e:
+            call()
+        assert e.value.kind == "Device"
+    a, sa = torch.zeros((4, 256)).to(E4M3), torch.zeros((4, 2))
+    b, sb, y = torch.zeros((40, 256)).to(E4M3), torch.zeros((1, 2)), torch.zeros((4, 40))
+    refused(lambda: ctx.fp8_quantize(torch.zeros((4, 256)), frx.FP8_ROWS, a, sa))
+    refused(lambda: ctx.fp8_linear(a, sa, b, sb, y))
+    refused(lambda: ctx.fp8_linear_act(torch.zeros((4, 256)), b, sb, y))
+    refused(lambda: ctx.fp8_linear_grouped(a, sa, b[None], sb[None], i32(2), y))
+    refused(lambda: ctx.fp8_linear_grouped(a, sa, [b], [sb], i32(2), y))
+    refused(lambda: ctx.fp8_grad_weight_grouped(*grad_args(2), torch.zeros((2, 40, 24))))
+    refused(lambda: ctx.fp8_grad_weight_grouped(*grad_args(1), [torch.zeros((40, 24))]))
+    rows = frx.MoeRows.empty(4, 2, 3, 1, device="cpu")
+    x, xs = torch.zeros((4, 8)), torch.zeros((rows.R, 8))
+    refused(lambda: ctx.moe_sort(i32(4, 2), rows))
+    refused(lambda: ctx.moe_dispatch(x, rows, xs))
+    refused(lambda: ctx.moe_combine(xs, rows, None, x))
+    refused(lambda: ctx.moe_combine(xs, rows, torch.zeros((4, 2)), x))
+    refused(lambda: ctx.moe_combine_backward(x, xs, rows, None, xs.clone(), torch.zeros((4, 2))))
+    meta = torch.zeros((4, 2), dtype=torch.int32, device="meta")
+    with pytest.raises(frx.FrxError, match="index tensors"):
+        frx.MoeRows(3, 1, i32(4), meta, i32(8))
