@@ -1,6 +1,4 @@
 // frx_fp8.hip — launches of the 8-bit floating-point linears (engine: frx_fp8.hpp).
-#include <cmath>
-
 #include "frx_fp8_skinny.hpp"
 #include "frx_fp8_ring.hpp"
 
@@ -234,9 +232,6 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float *__restrict__
   }
 }
 
-// Workgroups of 512 in a launch: it holds less than 2^32 work-items.
-constexpr size_t FP8_MAX_TILES = (size_t)1 << 23;
-
 template <typename K, typename A>
 hipError_t go(K kernel, int lds, std::atomic<uint64_t> &done, dim3 grid, int nt, hipStream_t stream, const A &args) {
   const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), lds, done);
@@ -319,33 +314,16 @@ hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// The tile of the experts' products. On the bf16 pipe 64 x 128: widening bounds every tile
-// alike. bf16 rows of e4m3 codes that the caller lets the 8-bit pipe sum go there from 256
-// rows an expert on (R / E: the groups' lengths are not known here), where the products
-// bound, in tiles of 128 or 256 x 256, priced for groups of equal length with half a tile
-// of remainder; below, the weights' bytes bound and it would gain little. us, K -> N, bf16
-// pipe 64 x 128 / 8-bit 64 x 128 / 128 x 256 / 256 x 256:
-//   8 experts   128 rows 2048 -> 5632    44 /  42 /  45 /  33
-//               256 rows 2048 -> 5632     - /  59 /  49 /  66
-//               384 rows 2048 -> 5632    92 /  77 /  72 /  72
-//              1024 rows 2048 -> 5632   218 / 173 / 143 / 143
-//   16 experts   64 rows 5632 -> 2048    62 /  61 /  55 /  61
-//                64 rows 2048 -> 5632     - /  54 /  52 /  63
-//   16 experts of 64 rows padded to 128, 5632 -> 2048    64 / 62 / 61 / 67
-// Other tiles of the bf16 pipe (128 x 128 / 128 x 256): 8 x 128 rows 53 / 66, 8 x 1024
-// 205 / 205, 16 x 64 padded to 128 87 / 77.
-double grouped_cost(const GroupArgs &p, uint32_t bm, uint32_t bn, double ns, int cus) {
-  const double tiles = p.E * ((double)p.R / p.E / bm + 0.5) * ((p.N + bn - 1) / bn);
-  return ns * std::ceil(tiles / cus);
-}
-
 template <bool E5M2, typename YT>
-hipError_t grouped_tile(const GroupArgs &p, int pipe8, int cus, hipStream_t stream) {
+hipError_t grouped_any(const GroupArgs &p, int tile, hipStream_t stream) {
+  if (tile == FP8_T_SKINNY) {
+    const dim3 grid((unsigned)(((p.R + 15) / 16 + p.E) * ((p.N + 15) / 16))), block(FP8_SK_WAVES * 64);
+    hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, E5M2, YT>), grid, block, (int)fp8_skinny_red_bytes(1), stream, p);
+    return hipGetLastError();
+  }
   if constexpr (!E5M2 && sizeof(YT) == 2) {
-    if (pipe8 && p.R >= 256u * (uint32_t)p.E)
-      return grouped_cost(p, 256, 256, 1460, cus) < grouped_cost(p, 128, 256, 1010, cus)
-                 ? grouped_go<Fp8Ring<8, E5M2, false, false>, YT>(p, stream)
-                 : grouped_go<Fp8Ring<4, E5M2, false, false>, YT>(p, stream);
+    if (tile == FP8_T_RING8) return grouped_go<Fp8Ring<8, E5M2, false, false>, YT>(p, stream);
+    if (tile == FP8_T_RING4) return grouped_go<Fp8Ring<4, E5M2, false, false>, YT>(p, stream);
   }
   return grouped_go<Fp8Tile<64, 128, 2, 2, E5M2, false, true>, YT>(p, stream);
 }
@@ -360,77 +338,6 @@ hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
 }
 
 }  // namespace
-
-// Tiles of many tokens: height x width, workgroups resident at once on a
-// compute unit, and what a step of 128 columns takes (ns, all of them resident;
-// 8192^3, 2048 x 4096 x 11008 and 4096^3). On the 8-bit pipe a taller tile costs
-// less per product, and a smaller one pays where the taller would leave units
-// idle (us, 256 / 192 / 128 / 128 x 128: 8192^3 374 / 432 / 517 / 570, 2048 x 4096 x
-// 11008 105 / 88 / 110 / 126, 2048 x 4096 x 4096 53 / 43 / 37 / 49, 4096^3 53 / 78 / 76 /
-// 90). Long products run into the card's power: 8192^3 takes 350 us on zeros
-// (3140 TFLOP/s) and 460 on normal values; a library's product with one scale for
-// all takes 257 and 348. On the bf16 pipe widening the operands bounds them all
-// (2048 x 4096 x 11008: 168 / 183 / 166 us for 192 / 128 / 128 x 128; 333 x 5120 x
-// 13824 94 / 70 / 75).
-struct TileCost {
-  int tile, bm, bn, wgs, ns;
-};
-constexpr TileCost kNarrow[] = {{FP8_T_RING8, 256, 256, 1, 1460}, {FP8_T_RING6, 192, 256, 1, 1130},
-                                {FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
-constexpr TileCost kWide[] = {{FP8_T_RING6, 192, 256, 1, 2600}, {FP8_T_RING4, 128, 256, 1, 1800},
-                              {FP8_T_128, 128, 128, 2, 1870}};
-// A scale per weight row (weight gradients): sixteen more multiplies a product,
-// taller tiles run out of registers; on the bf16 pipe 128 x 256 takes 2200.
-constexpr TileCost kNarrowRows[] = {{FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
-constexpr TileCost kWideRows[] = {{FP8_T_128, 128, 128, 2, 2150}};
-
-Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int pipe8, int cus) {
-  // Few tokens: no join, no tile of 128 mostly empty. Up to 32 always (us, against tiles of 128 x 256
-  // in K slices: 32 tokens, K x N 1024^2 4.1 / 9.6, 4096^2 10.2 / 14.7, 4096 x 11008 15.7 / 17.4, 11008 x 4096
-  // 20.9 / 20.1), up to 64 while two row tiles a workgroup cover N and the waves' slices of K are short, since
-  // every workgroup reads all tokens (64 tokens, 1024^2 5.7 / 10.8, 4096^2 14.5 / 17.5, 4096 x 8192 17.8 / 18.9,
-  // f32 2048 x 5632 10.9 / 19.7; 40 tokens f32 5120^2 20.7 / 21.0; 11008 x 4096 31.1 / 22.4), more in groups of 64
-  // while two rounds of workgroups hold them and K is short for that (128 tokens, 2048^2 8.5 / 14.6, 4096 x 2048 12.9 /
-  // 17.5, 2048 x 4096 13.8 / 16.6; 256 tokens, 2048^2 13.7 / 16.9, f32 2048 x 1024 8.6 / 18.2; 512 tokens, 1024^2
-  // 9.3 / 13.3; but 128 tokens 4096^2 23.0 / 22.6, 256 tokens 5120 x 2048 28.8 / 21.1).
-  const int steps = (int)((K + 127) / 128), most = M <= 32 ? 4 : 2;  // row tiles a workgroup
-  const size_t rounds64 = ((size_t)((M + 63) / 64) * ((N + 15) / 16) + cus - 1) / cus;
-  if (M <= 32 || (M <= 64 && N <= 32u * cus && steps <= 40) || (rounds64 <= 2 && rounds64 * steps <= 40)) {
-    // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
-    const uint32_t tiles = (N + 15) / 16;
-    int best = 1;
-    uint32_t least = ~0u;
-    for (int rt = 1; rt <= most; rt++) {
-      const uint32_t wgs = (tiles + rt - 1) / rt, rounds = (wgs + cus - 1) / cus * rt;
-      if (rounds <= least) {
-        least = rounds;
-        best = rt;
-      }
-    }
-    return {FP8_T_SKINNY, 1, best};
-  }
-  const TileCost *costs = b_rows == 1 ? (pipe8 ? kNarrowRows : kWideRows) : pipe8 ? kNarrow : kWide;
-  const int count = b_rows == 1 ? (pipe8 ? 2 : 1) : pipe8 ? 4 : 3;
-  Fp8Plan plan = {FP8_T_128, 1, steps};
-  double least = 1e30;
-  for (int t = 0; t < count; t++) {
-    const TileCost &c = costs[t];
-    const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
-    // a K slice more: fewer steps, but every part is written and read (4 bytes a value at
-    // about 4 TB/s) and the parts joined by another launch (4 us)
-    for (int S = 1; S <= 8 && S <= steps; S++) {
-      const int per = (steps + S - 1) / S;
-      if ((S - 1) * per >= steps) continue;  // an empty slice
-      const double rounds = std::ceil(tiles * S / ((double)c.wgs * cus));
-      const double ns = rounds * per * c.ns + (S > 1 ? 4000.0 + (double)S * M * N * 8 / 4000 : 0.0);
-      if (ns < least) {
-        least = ns;
-        plan = {c.tile, S, per};
-      }
-    }
-  }
-  return plan;
-}
 
 size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p) { return p.S > 1 ? (size_t)p.S * M * N * 4 : 0; }
 
@@ -478,24 +385,9 @@ hipError_t launch_fp8_grouped(const uint8_t *a, size_t lda, int e5m2, const floa
     p.b[e] = b[e];
     p.sb[e] = sb[e];
   }
-  // us, 8 experts, 16-row tiles / 64 x 128: 2 rows 5632 -> 2048 19.4 / 40.1, 2048 -> 5632 20.7 / 21.2,
-  // 1024^2 5.1 / 8.2; 8 rows 22.5 / 40.1, 24.2 / 21.3, 5.4 / 8.1
-  const size_t tiles = ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16);
-  if (R <= 8u * (uint32_t)E && tiles < FP8_MAX_TILES) {
-    const dim3 grid((unsigned)tiles), block(FP8_SK_WAVES * 64);
-    constexpr int lds = (int)fp8_skinny_red_bytes(1);
-    if (yt_bf16) {
-      if (e5m2) hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, true, uint16_t>), grid, block, lds, stream, p);
-      else hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, false, uint16_t>), grid, block, lds, stream, p);
-    } else {
-      if (e5m2) hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, true, float>), grid, block, lds, stream, p);
-      else hipLaunchKernelGGL((fp8_skinny_grouped_kernel<1, false, float>), grid, block, lds, stream, p);
-    }
-    return hipGetLastError();
-  }
-  if (yt_bf16)
-    return e5m2 ? grouped_tile<true, uint16_t>(p, pipe8, cus, stream) : grouped_tile<false, uint16_t>(p, pipe8, cus, stream);
-  return e5m2 ? grouped_tile<true, float>(p, pipe8, cus, stream) : grouped_tile<false, float>(p, pipe8, cus, stream);
+  const int tile = fp8_grouped_tile(R, N, (uint32_t)E, pipe8 && !e5m2, cus);
+  if (yt_bf16) return e5m2 ? grouped_any<true, uint16_t>(p, tile, stream) : grouped_any<false, uint16_t>(p, tile, stream);
+  return e5m2 ? grouped_any<true, float>(p, tile, stream) : grouped_any<false, float>(p, tile, stream);
 }
 
 hipError_t launch_fp8_grad_weight(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b,

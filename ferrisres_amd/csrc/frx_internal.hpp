@@ -342,15 +342,9 @@ enum { FRXQ_ROWS = 0, FRXQ_COLS = 1, FRXQ_TILES = 2, FRXQ_TILES_T = 3 };  // frx
 // blocks: frx_fp8_blocks; e5m2: 0 e4m3, 1 e5m2
 hipError_t launch_fp8_quantize(const void *x, int xt_bf16, uint32_t M, uint32_t K, size_t ldx, int blocks, int e5m2,
                                uint8_t *q, size_t ldq, float *scale, hipStream_t stream);
-// y = a b^T with block scales (frx_fp8_linear). S > 1: K in S slices of `per`
-// blocks of 128, fp32 parts [S][M][N] in part, added in order.
-struct Fp8Plan {
-  int tile;     // FP8_T_*
-  int S, per;   // K slices, blocks of 128 in each (FP8_T_SKINNY: 1, 16-row tiles of a workgroup)
-};
-enum { FP8_T_SKINNY = 0, FP8_T_128 = 1, FP8_T_RING8 = 2, FP8_T_RING6 = 3, FP8_T_RING4 = 4 };
-// pipe8: the 8-bit pipe may sum (bf16 outputs under FRX_FP8_SUMS_PIPE), here and below
-Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int pipe8, int cus);
+// y = a b^T with block scales (frx_fp8_linear), as fp8_plan says. S > 1: K in S slices of
+// `per` blocks of 128, fp32 parts [S][M][N] in part, added in order. pipe8: the 8-bit pipe
+// may sum (bf16 outputs under FRX_FP8_SUMS_PIPE), here and below.
 size_t fp8_part_bytes(uint32_t M, uint32_t N, const Fp8Plan &p);
 hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float *sa, const uint8_t *b, size_t ldb,
                              const float *sb, int b_rows, void *y, int yt_bf16, int pipe8, uint32_t M, uint32_t K,

@@ -1,8 +1,11 @@
-// frx_policy.hpp — host-side rules: the sizes of the context workspaces and
-// the kernels of the decode FFN, kept free of HIP so that a CPU build can check
-// them.
+// frx_policy.hpp — host-side rules: the sizes of the context workspaces, the
+// kernels of the decode FFN and those of the 8-bit linears, kept free of HIP so
+// that a CPU build can check them.
 #pragma once
 #include <stddef.h>
+#include <stdint.h>
+
+#include <cmath>
 
 namespace frx {
 
@@ -110,6 +113,117 @@ constexpr bool group_fewer_rounds(int count, const int *n, int K, int planes, in
     apart += staged_rounds((n[i] + 15) / 16, tmax, cus);
   }
   return staged_rounds(tiles, tmax, cus) < apart;
+}
+
+// ---- the 8-bit floating-point linears --------------------------------------------
+
+enum { FP8_T_SKINNY = 0, FP8_T_128 = 1, FP8_T_RING8 = 2, FP8_T_RING6 = 3, FP8_T_RING4 = 4, FP8_T_64 = 5 };
+struct Fp8Plan {
+  int tile;     // FP8_T_*
+  int S, per;   // K slices, blocks of 128 in each (FP8_T_SKINNY: 1, 16-row tiles of a workgroup)
+};
+
+// Tiles of many tokens: height x width, workgroups resident at once on a
+// compute unit, and what a step of 128 columns takes (ns, all of them resident;
+// 8192^3, 2048 x 4096 x 11008 and 4096^3). On the 8-bit pipe a taller tile costs
+// less per product, and a smaller one pays where the taller would leave units
+// idle (us, 256 / 192 / 128 / 128 x 128: 8192^3 374 / 432 / 517 / 570, 2048 x 4096 x
+// 11008 105 / 88 / 110 / 126, 2048 x 4096 x 4096 53 / 43 / 37 / 49, 4096^3 53 / 78 / 76 /
+// 90). Long products run into the card's power: 8192^3 takes 350 us on zeros
+// (3140 TFLOP/s) and 460 on normal values; a library's product with one scale for
+// all takes 257 and 348. On the bf16 pipe widening the operands bounds them all
+// (2048 x 4096 x 11008: 168 / 183 / 166 us for 192 / 128 / 128 x 128; 333 x 5120 x
+// 13824 94 / 70 / 75).
+struct Fp8TileCost {
+  int tile, bm, bn, wgs, ns;
+};
+constexpr Fp8TileCost kFp8Narrow[] = {{FP8_T_RING8, 256, 256, 1, 1460}, {FP8_T_RING6, 192, 256, 1, 1130},
+                                {FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
+constexpr Fp8TileCost kFp8Wide[] = {{FP8_T_RING6, 192, 256, 1, 2600}, {FP8_T_RING4, 128, 256, 1, 1800},
+                              {FP8_T_128, 128, 128, 2, 1870}};
+// A scale per weight row (weight gradients): sixteen more multiplies a product,
+// taller tiles run out of registers; on the bf16 pipe 128 x 256 takes 2200.
+constexpr Fp8TileCost kFp8NarrowRows[] = {{FP8_T_RING4, 128, 256, 1, 1010}, {FP8_T_128, 128, 128, 2, 1110}};
+constexpr Fp8TileCost kFp8WideRows[] = {{FP8_T_128, 128, 128, 2, 2150}};
+
+// pipe8: the 8-bit pipe may sum (bf16 outputs under FRX_FP8_SUMS_PIPE), here and below.
+inline Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int pipe8, int cus) {
+  // Few tokens: no join, no tile of 128 mostly empty. Up to 32 always (us, against tiles of 128 x 256
+  // in K slices: 32 tokens, K x N 1024^2 4.1 / 9.6, 4096^2 10.2 / 14.7, 4096 x 11008 15.7 / 17.4, 11008 x 4096
+  // 20.9 / 20.1), up to 64 while two row tiles a workgroup cover N and the waves' slices of K are short, since
+  // every workgroup reads all tokens (64 tokens, 1024^2 5.7 / 10.8, 4096^2 14.5 / 17.5, 4096 x 8192 17.8 / 18.9,
+  // f32 2048 x 5632 10.9 / 19.7; 40 tokens f32 5120^2 20.7 / 21.0; 11008 x 4096 31.1 / 22.4), more in groups of 64
+  // while two rounds of workgroups hold them and K is short for that (128 tokens, 2048^2 8.5 / 14.6, 4096 x 2048 12.9 /
+  // 17.5, 2048 x 4096 13.8 / 16.6; 256 tokens, 2048^2 13.7 / 16.9, f32 2048 x 1024 8.6 / 18.2; 512 tokens, 1024^2
+  // 9.3 / 13.3; but 128 tokens 4096^2 23.0 / 22.6, 256 tokens 5120 x 2048 28.8 / 21.1).
+  const int steps = (int)((K + 127) / 128), most = M <= 32 ? 4 : 2;  // row tiles a workgroup
+  const size_t rounds64 = ((size_t)((M + 63) / 64) * ((N + 15) / 16) + cus - 1) / cus;
+  if (M <= 32 || (M <= 64 && N <= 32u * cus && steps <= 40) || (rounds64 <= 2 && rounds64 * steps <= 40)) {
+    // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
+    const uint32_t tiles = (N + 15) / 16;
+    int best = 1;
+    uint32_t least = ~0u;
+    for (int rt = 1; rt <= most; rt++) {
+      const uint32_t wgs = (tiles + rt - 1) / rt, rounds = (wgs + cus - 1) / cus * rt;
+      if (rounds <= least) {
+        least = rounds;
+        best = rt;
+      }
+    }
+    return {FP8_T_SKINNY, 1, best};
+  }
+  const Fp8TileCost *costs = b_rows == 1 ? (pipe8 ? kFp8NarrowRows : kFp8WideRows) : pipe8 ? kFp8Narrow : kFp8Wide;
+  const int count = b_rows == 1 ? (pipe8 ? 2 : 1) : pipe8 ? 4 : 3;
+  Fp8Plan plan = {FP8_T_128, 1, steps};
+  double least = 1e30;
+  for (int t = 0; t < count; t++) {
+    const Fp8TileCost &c = costs[t];
+    const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    // a K slice more: fewer steps, but every part is written and read (4 bytes a value at
+    // about 4 TB/s) and the parts joined by another launch (4 us)
+    for (int S = 1; S <= 8 && S <= steps; S++) {
+      const int per = (steps + S - 1) / S;
+      if ((S - 1) * per >= steps) continue;  // an empty slice
+      const double rounds = std::ceil(tiles * S / ((double)c.wgs * cus));
+      const double ns = rounds * per * c.ns + (S > 1 ? 4000.0 + (double)S * M * N * 8 / 4000 : 0.0);
+      if (ns < least) {
+        least = ns;
+        plan = {c.tile, S, per};
+      }
+    }
+  }
+  return plan;
+}
+
+// The tile of the experts' products. On the bf16 pipe 64 x 128: widening bounds every tile
+// alike. bf16 rows of e4m3 codes that the caller lets the 8-bit pipe sum go there from 256
+// rows an expert on (R / E: the groups' lengths are not known here), where the products
+// bound, in tiles of 128 or 256 x 256, priced for groups of equal length with half a tile
+// of remainder; below, the weights' bytes bound and it would gain little. us, K -> N, bf16
+// pipe 64 x 128 / 8-bit 64 x 128 / 128 x 256 / 256 x 256:
+//   8 experts   128 rows 2048 -> 5632    44 /  42 /  45 /  33
+//               256 rows 2048 -> 5632     - /  59 /  49 /  66
+//               384 rows 2048 -> 5632    92 /  77 /  72 /  72
+//              1024 rows 2048 -> 5632   218 / 173 / 143 / 143
+//   16 experts   64 rows 5632 -> 2048    62 /  61 /  55 /  61
+//                64 rows 2048 -> 5632     - /  54 /  52 /  63
+//   16 experts of 64 rows padded to 128, 5632 -> 2048    64 / 62 / 61 / 67
+// Other tiles of the bf16 pipe (128 x 128 / 128 x 256): 8 x 128 rows 53 / 66, 8 x 1024
+// 205 / 205, 16 x 64 padded to 128 87 / 77.
+inline double fp8_grouped_cost(uint32_t R, uint32_t N, uint32_t E, uint32_t bm, uint32_t bn, double ns, int cus) {
+  const double tiles = E * ((double)R / E / bm + 0.5) * ((N + bn - 1) / bn);
+  return ns * std::ceil(tiles / cus);
+}
+
+// Experts' rows: tiles of 16 where R / E is small (us, 8 experts, 16-row tiles / 64 x 128: 2
+// rows 5632 -> 2048 19.4 / 40.1, 2048 -> 5632 20.7 / 21.2, 1024^2 5.1 / 8.2; 8 rows 22.5 / 40.1,
+// 24.2 / 21.3, 5.4 / 8.1) and the launch holds its workgroups of 512 (less than 2^32
+// work-items).
+inline int fp8_grouped_tile(uint32_t R, uint32_t N, uint32_t E, int pipe8, int cus) {
+  if (R <= 8 * E && ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16) < (size_t)1 << 23) return FP8_T_SKINNY;
+  if (!pipe8 || R < 256 * E) return FP8_T_64;
+  return fp8_grouped_cost(R, N, E, 256, 256, 1460, cus) < fp8_grouped_cost(R, N, E, 128, 256, 1010, cus) ? FP8_T_RING8
+                                                                                                        : FP8_T_RING4;
 }
 
 }  // namespace frx
