@@ -304,7 +304,10 @@ __global__ __launch_bounds__(256) void route_combine_backward_kernel(const DT *_
     return;
   }
   const uint32_t row = r.row_of[slot];
-  float dot = 0.0f;
+  // a lane's sum goes by 8 products at a time, fused: 8 + H / 512 roundings instead of H / 32
+  constexpr uint32_t EVERY = Q < 8 ? 8 / Q : 1;
+  float dot = 0.0f, part = 0.0f;
+  uint32_t n = 0;
   if (row < (uint32_t)r.R) {
     const float g = w ? w[slot] : 1.0f;
     const DT *src = dy + (size_t)(slot / r.top_k) * H;
@@ -320,12 +323,17 @@ __global__ __launch_bounds__(256) void route_combine_backward_kernel(const DT *_
         float b[Q];
         ldq(other + h, b);
 #pragma unroll
-        for (int q = 0; q < Q; q++) dot = dot + a[q] * b[q];
+        for (int q = 0; q < Q; q++) part = __builtin_fmaf(a[q], b[q], part);
+        if (++n % EVERY == 0) {
+          dot = dot + part;
+          part = 0.0f;
+        }
       }
       stq<Q>(d + h, p);
     }
   }
   if (!dw) return;
+  dot = dot + part;
   for (int o = 32; o; o >>= 1) dot += __shfl_xor(dot, o);
   if (lane == 0) dw[slot] = dot;
 }

@@ -450,7 +450,8 @@ frx_status frx_moe_combine(frx_ctx *ctx, const void *ys, frx_dtype st, const frx
  *   dys[row_of[t][j]] = w[t][j] * dy[t]  ([R][H] st; rows of no route as in
  *                                         frx_moe_dispatch)
  *   dw[t][j] = sum_h dy[t][h] * ys[row_of[t][j]][h]  ([T][top_k] f32, 0 for a
- *                                         route that goes nowhere)
+ *                                         route that goes nowhere; at most 16 + H / 512
+ *                                         f32 roundings of a term's way into the sum)
  * ys and dw may both be NULL (no gradient of the weights), w may be NULL
  * (every weight 1). */
 frx_status frx_moe_combine_backward(frx_ctx *ctx, const void *dy, frx_dtype dt, const void *ys,
