@@ -751,7 +751,8 @@ class Context:
     def fp8_linear_grouped(self, a, sa, b, sb, offsets, y):
         """frx_fp8_linear_grouped: rows offsets[e] to offsets[e + 1] of a [R][K]
         times expert e's codes b[e] [N][K], sb[e] [ceil(N/128)][ceil(K/128)]
-        (stacked tensors, or lists of E)."""
+        (stacked tensors, or lists of E). The kernel goes by R: rows past those in
+        use cost time, so views of a, sa and y that end near them are faster."""
         torch = _torch or _tt()
         R, K, lda = _rows2(a, "a")
         E, kb = int(offsets.numel()) - 1, (K + 127) // 128

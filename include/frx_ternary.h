@@ -374,10 +374,10 @@ frx_status frx_fp8_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at
 
 /* y = x w^T for activations x [M][K] (f32 or bf16, contiguous): frx_fp8_quantize
  * (ROWS, e4m3) and frx_fp8_linear (b_rows = 128) in one call, with the two
- * calls' result bit for bit. Up to 4 tokens (of 16000 columns together) it
- * is one launch, the codes in LDS; above, they lie in a context workspace (which
- * must be there before a graph capture: FRX_ERR_UNSUPPORTED otherwise). K % 16
- * == 0 and K <= 2^23 for x's codes too. */
+ * calls' result bit for bit. Where M <= 4 and M * K + 4 * M * ceil(K / 128) <= 65536
+ * (4 tokens of up to 15872 columns) it is one launch, the codes in LDS; else they
+ * lie in a context workspace (which must be there before a graph capture:
+ * FRX_ERR_UNSUPPORTED otherwise). K % 16 == 0 and K <= 2^23 for x's codes too. */
 frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
                               const float *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
 
@@ -386,7 +386,13 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
  *   a [R][lda], sa [R][ceil(K / 128)]; b[e] [N][ldb] e4m3, sb[e] [ceil(N / 128)]
  *   [ceil(K / 128)] (host arrays of E device pointers); offsets [E + 1] u32 on
  *   the device, ascending; y [R][N]. Rows from offsets[E] on are neither read
- *   nor written. 1 <= E <= 64; otherwise as frx_fp8_linear. No allocation. */
+ *   nor written. 1 <= E <= 64; otherwise as frx_fp8_linear. No allocation.
+ * The groups' lengths lie on the device, so R stands for them: R <= 8 E takes the
+ * kernel for a few rows of each, and the grid is R's. A caller that knows a bound
+ * on the rows in use passes that as R, not the room there is (frx_moe_rows_capacity
+ * counts up to align - 1 rows more an expert; 8 tokens of 2 routes over 16 experts are 16
+ * rows with align = 1 and have room for 2048 with align = 128). The sums do not
+ * depend on it (FRX_FP8_SUMS_F32). */
 frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
                                   const uint8_t *const *b, size_t ldb, const float *const *sb,
                                   const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R,

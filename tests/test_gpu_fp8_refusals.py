@@ -62,3 +62,33 @@ def test_a_single_row_has_any_stride(ctx):
     ctx.fp8_linear(b, rows, q, s, t)  # the row as the one weight row
     ctx.fp8_linear(b, rows, q2, s, t2)
     assert torch.equal(t, t2) and t.abs().min() > 0
+
+
+@pytest.mark.parametrize("m,k,one_launch", [(4, 15872, True), (4, 15888, False), (3, 16384, True), (1, 63488, True),
+                                            (1, 63536, True), (1, 63552, False), (5, 256, False), (4, 256, True)])
+def test_which_calls_need_no_workspace(ctx, m, k, one_launch):
+    """frx_fp8_linear_act on a fresh context under capture: one launch where M <= 4 and M K + 4 M ceil(K / 128) <=
+    65536, as the header says, a refusal otherwise."""
+    assert one_launch == (m <= 4 and m * k + 4 * m * -(-k // 128) <= 65536)
+    side = torch.cuda.Stream()
+    ctx.set_stream(side)
+    x, y = torch.ones((m, k), device=DEV), torch.zeros((m, 16), device=DEV)
+    b, sb = torch.ones((16, k), device=DEV).to(E4M3), torch.ones((1, -(-k // 128)), device=DEV)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        y.add_(0.0)
+        if one_launch:
+            ctx.fp8_linear_act(x, b, sb, y)
+        else:
+            with pytest.raises(frx.FrxError, match="captured") as e:
+                ctx.fp8_linear_act(x, b, sb, y)
+            assert e.value.kind == "Unsupported"
+    for _ in range(2):
+        y.zero_()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        # ones against ones: a code of 448 and a scale of f32(1 / 448) give 1 up to two roundings, summed exactly enough
+        assert ((y - (k if one_launch else 0)).abs() <= k * 2.0 ** -20).all()
+    del g
