@@ -4,9 +4,11 @@
 // SIMD, over two LDS stages (three at 128 tokens), one block of 128 columns
 // each. Large tiles: what a compute unit reads per product halves from 128 x 128
 // to 256 x 256, and so does the rate at which the L2's latency has to be
-// covered. Bound by issue: 4 multiply-adds beside each product, the DMA's and
-// the operands' instructions (8192^3 in 256 x 256 tiles 374 us, without any DMA
-// 306), and by power (frx_fp8.hip). Step t issues block t's products, and
+// covered. On the 8-bit pipe bound by issue: 4 multiply-adds beside each product,
+// the DMA's and the operands' instructions (8192^3 in 256 x 256 tiles 374 us,
+// without any DMA 306), and by power (fp8_plan). On the bf16 pipe the widening of
+// the operands comes on top: a token fragment's 16 conversions for its 4 products in
+// every wave (8192^3 in 192 x 256 tiles 931). Step t issues block t's products, and
 // between them
 //  - the multiply-adds of the token fragment before (the last one's of block
 //    t - 1 behind the first products of block t), so that no product waits for
@@ -18,8 +20,8 @@
 // stages) goes into their place. Before the last one block t + 1 has landed
 // (each wave has waited for its own loads) and block t's tokens are read, so
 // the later block's follow: each at least a step ahead of its use, spread over
-// the products (in two bursts 2048 x 4096 x 11008 took 104 us, spread 88; in one
-// 134).
+// the products (8-bit pipe: in two bursts 2048 x 4096 x 11008 took 104 us, spread 88;
+// in one 134).
 #pragma once
 #include "frx_fp8.hpp"
 

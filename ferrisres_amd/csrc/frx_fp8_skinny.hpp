@@ -12,9 +12,9 @@
 // 4096 columns 17.1 us against 12.5 when every lane reads one token's), so
 // the scales of four blocks are one load, and a workgroup takes as many row
 // tiles as leave each compute unit one workgroup (fp8_plan). us, 1 / 16 tokens,
-// graph replays over cold weights: 2048 x 2048 3.9 / 4.9, 4096 x 4096 6.6 / 8.1,
-// 11008 x 4096 12.1 / 13.5 (3.7 / 3.3 TB/s; a large copy moves 4.7), 13824 x 5120
-// 18.2 at 16. Loads of 2 or 4 blocks ahead of the products were slower (16
+// graph replays over cold weights: 2048 x 2048 4.2 / 4.9, 4096 x 4096 7.2 / 7.6,
+// 11008 x 4096 11.7 / 12.5 (3.8 / 3.6 TB/s; a large copy moves 4.7), 13824 x 5120
+// 18.9 at 16. Loads of 2 or 4 blocks ahead of the products were slower (16
 // tokens of 11008 x 4096 14.6 / 14.8), as were 4 or 16 waves. Above 16 tokens a
 // wave holds two or four token tiles (TT) against the same weights.
 //

@@ -351,8 +351,9 @@ hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float
                              uint32_t N, const Fp8Plan &plan, float *part, hipStream_t stream);
 // x f32 or bf16 [M][K], quantised on the way (FP8_T_SKINNY plans whose
 // activations fit: fp8_act_fits). Every workgroup makes the codes for itself,
-// which pays while they are few (11008 x 4096, us, one launch / quantiser and
-// product: 1 token 13.1 / 14.8, 4 tokens 14.2 / 14.3).
+// which pays while they are few (us, one launch / quantiser and product: 2048 x
+// 2048, 1 token 4.8 / 6.3, 4 tokens 5.4 / 6.5; 4096 x 4096, 4 tokens 9.4 / 9.6; 11008 x
+// 4096, 1 token 13.1 / 14.1, 2 tokens 13.7 / 14.3, 4 tokens 14.9 / 14.4).
 constexpr uint32_t FP8_ACT_MAX_M = 4;
 constexpr size_t FP8_ACT_MAX_BYTES = 64 << 10;
 bool fp8_act_fits(uint32_t M, uint32_t K);

@@ -132,8 +132,8 @@ struct Fp8Plan {
 // 90). Long products run into the card's power: 8192^3 takes 350 us on zeros
 // (3140 TFLOP/s) and 460 on normal values; a library's product with one scale for
 // all takes 257 and 348. On the bf16 pipe widening the operands bounds them all
-// (2048 x 4096 x 11008: 168 / 183 / 166 us for 192 / 128 / 128 x 128; 333 x 5120 x
-// 13824 94 / 70 / 75).
+// (8192^3 931 / 952 / 998 us for 192 / 128 / 128 x 128, 2048 x 4096 x 11008 158 / 175 /
+// 174, 2048 x 4096 x 4096 80 / 61 / 63, 4096^3 158 / 119 / 119).
 struct Fp8TileCost {
   int tile, bm, bn, wgs, ns;
 };
@@ -148,14 +148,16 @@ constexpr Fp8TileCost kFp8WideRows[] = {{FP8_T_128, 128, 128, 2, 2150}};
 
 // pipe8: the 8-bit pipe may sum (bf16 outputs under FRX_FP8_SUMS_PIPE), here and below.
 inline Fp8Plan fp8_plan(uint32_t M, uint32_t K, uint32_t N, int b_rows, int pipe8, int cus) {
-  // Few tokens: no join, no tile of 128 mostly empty. Up to 32 always (us, against tiles of 128 x 256
-  // in K slices: 32 tokens, K x N 1024^2 4.1 / 9.6, 4096^2 10.2 / 14.7, 4096 x 11008 15.7 / 17.4, 11008 x 4096
-  // 20.9 / 20.1), up to 64 while two row tiles a workgroup cover N and the waves' slices of K are short, since
-  // every workgroup reads all tokens (64 tokens, 1024^2 5.7 / 10.8, 4096^2 14.5 / 17.5, 4096 x 8192 17.8 / 18.9,
-  // f32 2048 x 5632 10.9 / 19.7; 40 tokens f32 5120^2 20.7 / 21.0; 11008 x 4096 31.1 / 22.4), more in groups of 64
-  // while two rounds of workgroups hold them and K is short for that (128 tokens, 2048^2 8.5 / 14.6, 4096 x 2048 12.9 /
-  // 17.5, 2048 x 4096 13.8 / 16.6; 256 tokens, 2048^2 13.7 / 16.9, f32 2048 x 1024 8.6 / 18.2; 512 tokens, 1024^2
-  // 9.3 / 13.3; but 128 tokens 4096^2 23.0 / 22.6, 256 tokens 5120 x 2048 28.8 / 21.1).
+  // Few tokens: no join, no tile of 128 mostly empty. Up to 32 always (us, against the tiles, which split K here, on
+  // the bf16 pipe / on the 8-bit one: 32 tokens, K x N 1024^2 4.3 / 10.5 / 9.6, 4096^2 10.4 / 17.6 / 14.7, 4096 x 11008
+  // 16.5 / 22.4 / 17.4, 11008 x 4096 22.2 / 27.9 / 20.1), up to 64 while two row tiles a workgroup cover N and the waves'
+  // slices of K are short, since every workgroup reads all tokens (64 tokens, 1024^2 5.9 / 11.9 / 10.8, 4096^2 14.9 /
+  // 21.1 / 17.5, 4096 x 8192 18.7 / 22.7 / 18.9, f32 2048 x 5632 11.0 / 19.5; 40 tokens f32 5120^2 20.5 / 21.4; but 64 tokens
+  // 8192 x 4096 26.2 / 24.7, 11008 x 4096 33.1 / 29.9 / 22.4), more in groups of 64 while two rounds of workgroups hold
+  // them and K is short for that (128 tokens, 2048^2 8.6 / 18.6 / 14.6, 4096 x 2048 13.3 / 21.2 / 17.5, 2048 x 4096 14.1 /
+  // 21.0 / 16.6; 256 tokens, 2048^2 14.0 / 20.2 / 16.9, f32 2048 x 1024 8.6 / 18.4; 512 tokens, 1024^2 9.4 / 17.9 / 13.3; but
+  // 128 tokens 4096^2 23.2 / 24.9 / 22.6, 256 tokens 5120 x 2048 28.9 / 26.1 / 21.1). The 8-bit pipe's tiles set the lines;
+  // beside the bf16 pipe's they could lie at 52 blocks of a slice (6656 x 4096 21.8 / 23.9) and 64 of a round.
   const int steps = (int)((K + 127) / 128), most = M <= 32 ? 4 : 2;  // row tiles a workgroup
   const size_t rounds64 = ((size_t)((M + 63) / 64) * ((N + 15) / 16) + cus - 1) / cus;
   if (M <= 32 || (M <= 64 && N <= 32u * cus && steps <= 40) || (rounds64 <= 2 && rounds64 * steps <= 40)) {
