@@ -148,3 +148,26 @@ def test_small_gradients_end_to_end(ctx, size):
     av = q.cpu().double() * s.cpu().double().repeat_interleave(128, 1)[:, :n]
     bv = wq.cpu().double() * ws.cpu().double().repeat_interleave(128, 1).repeat_interleave(128, 0)[:k, :wq.shape[1]]
     check_small(y, av @ bv[:, :n].t(), av.abs() @ bv[:, :n].abs().t(), n)
+
+
+@pytest.mark.parametrize("n", [16, 4112])  # groups of 64 tokens; tiles
+@pytest.mark.parametrize("code", [E4M3, E5M2])
+@pytest.mark.parametrize("b_rows", [128, 1])
+@pytest.mark.parametrize("sa,sb", [(1.0, 1.0), (2.0 ** -100, 2.0 ** -10), (2.0 ** -90, 2.0 ** -20), (2.0 ** 100, 2.0 ** -110),
+                                   (2.0 ** -30, 2.0 ** -71)])
+def test_every_code_exactly(ctx, n, code, b_rows, sa, sb):
+    """One code a token, against ones: y is the code's value times the scales, exactly, whatever side of a line they
+    lie on; a NaN stays one and an infinity too."""
+    k = 144
+    a = torch.zeros((256, k), dtype=torch.uint8)
+    a[:, 130] = torch.arange(256)  # in the part of a block at the end
+    b = torch.zeros((n, k), dtype=torch.uint8)
+    b[:, 130] = torch.ones(1).to(E4M3).view(torch.uint8)
+    y = torch.full((256, n), 5.0, device=DEV)
+    ctx.fp8_linear(a.to(DEV).view(code), torch.full((256, 2), sa, device=DEV), b.to(DEV).view(E4M3),
+                   torch.full((n if b_rows == 1 else up(n, 128) // 128, 2), sb, device=DEV), y)
+    want = torch.arange(256, dtype=torch.uint8).view(code).double() * sa * sb
+    y = y.cpu().double()
+    assert torch.equal(torch.isnan(y), torch.isnan(want)[:, None].expand(256, n))
+    keep = ~torch.isnan(want)
+    assert torch.equal(y[keep], want[keep][:, None].expand(int(keep.sum()), n))
