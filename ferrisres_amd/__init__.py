@@ -316,10 +316,11 @@ def _fp8_code(t) -> int:
 
 
 def _here(d, *ts):
-    """The tensors (None among them) are on device d, the context's: an address of any other memory would fault there."""
+    """The tensors (None among them) and the sorted rows are on device d, the context's: an address of any other memory
+    would fault there."""
     for t in ts:
-        if t is not None and t.get_device() != d:
-            raise FrxError(3, f"a tensor is on {t.device}, the context on cuda:{d}")
+        if t is not None and (t._dev if isinstance(t, MoeRows) else t.get_device()) != d:
+            raise FrxError(3, f"a tensor is on {getattr(t, 'slot_of', t).device}, the context on cuda:{d}")
 
 
 def _one_row(n):
@@ -330,9 +331,10 @@ def _one_row(n):
 def _rows2(t, name):
     """(rows, columns, row stride in elements) of a 2-D tensor with unit
     column stride."""
-    if t.dim() != 2:
-        raise _shape_err(f"{name} must be 2-D, got shape {tuple(t.shape)}")
-    m, n = t.shape
+    shape = t.shape
+    if len(shape) != 2:
+        raise _shape_err(f"{name} must be 2-D, got shape {tuple(shape)}")
+    m, n = shape
     ld, col = t.stride()
     if n > 1 and col != 1:
         raise _shape_err(f"{name} must have unit column stride, got strides {t.stride()}")
@@ -408,7 +410,7 @@ class MoeRows:
         _dense(slot_of, (self.R,), torch.int32, "slot_of")
         if not offsets.device == row_of.device == slot_of.device:
             raise FrxError(3, f"the index tensors are on {offsets.device}, {row_of.device} and {slot_of.device}")
-        self.offsets, self.row_of, self.slot_of = offsets, row_of, slot_of
+        self.offsets, self.row_of, self.slot_of, self._dev = offsets, row_of, slot_of, slot_of.get_device()
         self._c = _MoeRowsC(self.T, self.top_k, self.E, self.align, self.R, offsets.data_ptr(), row_of.data_ptr(),
                             slot_of.data_ptr())
         self._p = ctypes.addressof(self._c)
@@ -694,10 +696,9 @@ class Context:
         up to a multiple of 16, any row stride that is one too."""
         torch = _torch or _tt()
         M, K, ldx = _rows2(x, "x")
-        turned = blocks in (FP8_COLS, FP8_TILES_T)
-        r, c = (K, M) if turned else (M, K)
+        r, c = (K, M) if blocks in (FP8_COLS, FP8_TILES_T) else (M, K)
         qr, qc, ldq = _rows2(q, "q")
-        if (qr, qc) != (r, (c + 15) // 16 * 16):
+        if qr != r or qc != (c + 15) // 16 * 16:
             raise _shape_err(f"q has shape {tuple(q.shape)}, expected {(r, (c + 15) // 16 * 16)}")
         sr = (r + 127) // 128 if blocks in (FP8_TILES, FP8_TILES_T) else r
         _dense(scale, (sr, (c + 127) // 128), torch.float32, "scale")
@@ -739,7 +740,8 @@ class Context:
             raise _shape_err(f"b has {kb_} columns, x {K}")
         if b.dtype != torch.float8_e4m3fn:
             raise TypeError(f"b must be float8_e4m3fn, got {b.dtype}")
-        _dense(x, (M, K), None, "x")
+        if not x.is_contiguous():
+            raise _shape_err("x must be contiguous")
         _dense(sb, ((N + 127) // 128, (K + 127) // 128), torch.float32, "sb")
         _dense(y, (M, N), None, "y")
         if not x.get_device() == b.get_device() == sb.get_device() == y.get_device() == self._dev:
@@ -756,12 +758,14 @@ class Context:
         torch = _torch or _tt()
         R, K, lda = _rows2(a, "a")
         E, kb = int(offsets.numel()) - 1, (K + 127) // 128
-        N = int(y.shape[1]) if y.dim() == 2 else 0
+        shape = y.shape
+        N = shape[1] if len(shape) == 2 else 0
         _dense(offsets, (E + 1,), torch.int32, "offsets")
         _dense(sa, (R, kb), torch.float32, "sa")
         bp, ldb = _per_expert(b, E, (N, K), torch.float8_e4m3fn, "b", rows=True, dev=self._dev)
         sp, _ = _per_expert(sb, E, ((N + 127) // 128, kb), torch.float32, "sb", dev=self._dev)
-        _dense(y, (R, N), None, "y")
+        if shape != (R, N) or not y.is_contiguous():
+            _dense(y, (R, N), None, "y")
         if not a.get_device() == sa.get_device() == offsets.get_device() == y.get_device() == self._dev:
             _here(self._dev, a, sa, offsets, y)
         _check(lib().frx_fp8_linear_grouped(self._h, a.data_ptr(), lda, _fp8_code(a), sa.data_ptr(),
@@ -801,20 +805,22 @@ class Context:
     def moe_sort(self, topk_idx, rows: MoeRows):
         """frx_moe_sort: fills rows from topk_idx [T][top_k] int32 (an index
         outside [0, E) goes nowhere)."""
-        torch = _torch or _tt()
-        _dense(topk_idx, (rows.T, rows.top_k), torch.int32, "topk_idx")
-        if not topk_idx.get_device() == rows.slot_of.get_device() == self._dev:
-            _here(self._dev, topk_idx, rows.slot_of)
+        _dense(topk_idx, (rows.T, rows.top_k), (_torch or _tt()).int32, "topk_idx")
+        if not topk_idx.get_device() == rows._dev == self._dev:
+            _here(self._dev, topk_idx, rows)
         _check(lib().frx_moe_sort(self._h, topk_idx.data_ptr(), rows._p), self._h)
         return rows
 
     def moe_dispatch(self, x, rows: MoeRows, xs):
         """frx_moe_dispatch: xs [R][...] = each row's token of x [T][...], for
         rows of any type whose bytes are a multiple of 4."""
-        _dense(x, (rows.T, *x.shape[1:]), None, "x")
-        _dense(xs, (rows.R, *x.shape[1:]), x.dtype, "xs")
-        if not x.get_device() == rows.slot_of.get_device() == xs.get_device() == self._dev:
-            _here(self._dev, x, rows.slot_of, xs)
+        shape = x.shape
+        row = shape[1:]
+        if shape != (rows.T, *row) or not x.is_contiguous():
+            _dense(x, (rows.T, *row), None, "x")
+        _dense(xs, (rows.R, *row), x.dtype, "xs")
+        if not x.get_device() == xs.get_device() == rows._dev == self._dev:
+            _here(self._dev, x, rows, xs)
         _check(lib().frx_moe_dispatch(self._h, x.data_ptr(), x.numel() // max(rows.T, 1) * x.element_size(), rows._p,
                                       xs.data_ptr()), self._h)
         return xs
@@ -823,12 +829,17 @@ class Context:
         """frx_moe_combine: y [T][H] = the sum of each token's rows of ys [R]
         [H], times w [T][top_k] f32 (None: every weight 1)."""
         torch = _torch or _tt()
-        H = int(y.shape[-1])
+        shape = y.shape
+        H = shape[-1]
         _dense(ys, (rows.R, H), None, "ys")
-        _dense(y, (rows.T, H), None, "y")
+        if shape != (rows.T, H) or not y.is_contiguous():
+            _dense(y, (rows.T, H), None, "y")
+        at = self._dev
         if w is not None:
             _dense(w, (rows.T, rows.top_k), torch.float32, "w")
-        _here(self._dev, ys, rows.slot_of, w, y)
+            at = w.get_device()
+        if not ys.get_device() == y.get_device() == rows._dev == at == self._dev:
+            _here(self._dev, ys, rows, w, y)
         _check(lib().frx_moe_combine(self._h, ys.data_ptr(), _dtype_code(ys), rows._p, w if w is None else w.data_ptr(),
                                      y.data_ptr(), _dtype_code(y), H), self._h)
         return y
@@ -837,20 +848,30 @@ class Context:
         """frx_moe_combine_backward: dys [R][H] and dw [T][top_k] f32 of
         moe_combine for dy [T][H]; ys and dw may both be None, w too."""
         torch = _torch or _tt()
-        H = int(dy.shape[-1])
-        _dense(dy, (rows.T, H), None, "dy")
+        shape = dy.shape
+        H = shape[-1]
+        if shape != (rows.T, H) or not dy.is_contiguous():
+            _dense(dy, (rows.T, H), None, "dy")
         _dense(dys, (rows.R, H), None, "dys")
         if (ys is None) != (dw is None):
             raise _shape_err("ys and dw come together")
+        dev = at = self._dev
+        p_ys = p_dw = p_w = None
         if ys is not None:
             _dense(ys, (rows.R, H), dys.dtype, "ys")
             _dense(dw, (rows.T, rows.top_k), torch.float32, "dw")
+            p_ys, p_dw = ys.data_ptr(), dw.data_ptr()
+            if not ys.get_device() == dw.get_device() == dev:
+                at = None
         if w is not None:
             _dense(w, (rows.T, rows.top_k), torch.float32, "w")
-        _here(self._dev, dy, ys, rows.slot_of, w, dys, dw)
-        ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-        _check(lib().frx_moe_combine_backward(self._h, dy.data_ptr(), _dtype_code(dy), ptr(ys), _dtype_code(dys),
-                                              rows._p, ptr(w), dys.data_ptr(), ptr(dw), H), self._h)
+            p_w = w.data_ptr()
+            if w.get_device() != dev:
+                at = None
+        if not dy.get_device() == dys.get_device() == rows._dev == at == dev:
+            _here(self._dev, dy, ys, rows, w, dys, dw)
+        _check(lib().frx_moe_combine_backward(self._h, dy.data_ptr(), _dtype_code(dy), p_ys, _dtype_code(dys),
+                                              rows._p, p_w, dys.data_ptr(), p_dw, H), self._h)
         return dys, dw
 
     def set_gemv_split(self, mode: int):

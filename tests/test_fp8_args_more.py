@@ -83,3 +83,26 @@ def test_tensors_of_another_device_are_refused(ctx):  # noqa: F811
     meta = torch.zeros((4, 2), dtype=torch.int32, device="meta")
     with pytest.raises(frx.FrxError, match="index tensors"):
         frx.MoeRows(3, 1, i32(4), meta, i32(8))
+
+
+def test_routing_shapes_are_checked(ctx):  # noqa: F811
+    """What the quick checks of the routing calls let through has the right shape and is contiguous; the rest is told
+    apart as before."""
+    rows = frx.MoeRows.empty(4, 2, 3, 1, device="cpu")
+    f = lambda *d: torch.zeros(d)  # noqa: E731
+    x, xs, w = f(4, 8), f(rows.R, 8), f(4, 2)
+    for call in (lambda: ctx.moe_dispatch(x, rows, xs), lambda: ctx.moe_dispatch(f(4, 2, 4), rows, f(rows.R, 2, 4)),
+                 lambda: ctx.moe_dispatch(f(4), rows, f(rows.R)), lambda: ctx.moe_combine(xs, rows, w, x),
+                 lambda: ctx.moe_combine_backward(x, xs, rows, w, xs.clone(), w.clone())):
+        reaches_the_library(call)
+    wide = f(4, 16)[:, ::2]
+    for call in (lambda: ctx.moe_dispatch(f(), rows, xs), lambda: ctx.moe_dispatch(f(5, 8), rows, xs),
+                 lambda: ctx.moe_dispatch(wide, rows, xs), lambda: ctx.moe_dispatch(x, rows, f(rows.R, 9)),
+                 lambda: ctx.moe_combine(xs, rows, w, f(5, 8)), lambda: ctx.moe_combine(xs, rows, w, wide),
+                 lambda: ctx.moe_combine(f(rows.R + 1, 8), rows, w, x), lambda: ctx.moe_combine(xs, rows, w, f(1, 4, 8)),
+                 lambda: ctx.moe_combine_backward(f(5, 8), xs, rows, w, xs.clone(), w.clone()),
+                 lambda: ctx.moe_combine_backward(wide, xs, rows, w, xs.clone(), w.clone()),
+                 lambda: ctx.moe_combine_backward(x, xs, rows, f(4, 3), xs.clone(), w.clone()),
+                 lambda: ctx.fp8_linear_grouped(f(12, 16).to(E4M3), f(12, 1), f(3, 40, 16).to(E4M3), f(3, 1, 1),
+                                                torch.zeros(4, dtype=torch.int32), f(12, 80)[:, ::2])):
+        refuses(frx.FrxError, call)
