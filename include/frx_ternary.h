@@ -326,8 +326,8 @@ typedef enum frx_fp8_sums {
 
 /* Selects the sums of every 8-bit linear that the context runs from here on (a
  * captured graph keeps those that it was captured with). The pipe is used above a
- * few tokens (up to 1.9 times as fast: 2048 tokens of 4096 x 11008 88 us against
- * 167), and by frx_fp8_linear_grouped for e4m3 rows where R >= 256 E. */
+ * few tokens (2048 tokens of 4096 x 11008 100 us against 158), and by
+ * frx_fp8_linear_grouped for e4m3 rows where R >= 256 E. */
 frx_status frx_set_fp8_sums(frx_ctx *ctx, frx_fp8_sums mode);
 
 /* Codes and scales of x [M][K] (f32 or bf16, row stride ldx >= K elements).
@@ -391,8 +391,8 @@ frx_status frx_fp8_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const u
  * kernel for a few rows of each, and the grid is R's. A caller that knows a bound
  * on the rows in use passes that as R, not the room there is (frx_moe_rows_capacity
  * counts up to align - 1 rows more an expert; 8 tokens of 2 routes over 16 experts are 16
- * rows with align = 1 and have room for 2048 with align = 128). The sums do not
- * depend on it (FRX_FP8_SUMS_F32). */
+ * rows with align = 1 and have room for 2048 with align = 128). Under
+ * FRX_FP8_SUMS_F32 it changes the order of a sum at the most. */
 frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
                                   const uint8_t *const *b, size_t ldb, const float *const *sb,
                                   const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R,
