@@ -170,7 +170,7 @@ def _plain_codes(x):
     v = b * ((254 - byte) << 23).view(torch.float32)[..., None]
     m = v.abs()
     code = (m > 0.25).to(torch.uint8) + (m >= 0.75) + (m > 1.25) + (m >= 1.75) + (m > 2.5) + (m >= 3.5) + (m > 5)
-    code = code + 8 * torch.signbit(v)
+    code = code + 8 * torch.signbit(v).to(torch.uint8)
     q = code[..., 0::2] + 16 * code[..., 1::2]
     return q.flatten(-2)[..., :_up(k, 32) // 2].contiguous(), byte.to(torch.uint8)
 
