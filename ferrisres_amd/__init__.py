@@ -27,6 +27,7 @@ QUANT_ABSMEAN, QUANT_STE = 0, 1
 FP8_E4M3, FP8_E5M2 = 0, 1
 FP8_ROWS, FP8_COLS, FP8_TILES, FP8_TILES_T = 0, 1, 2, 3
 FP8_SUMS_F32, FP8_SUMS_PIPE = 0, 1
+FP4_ROWS, FP4_COLS = 0, 1
 
 _STATUS = {
     0: "Ok", 1: "Gpu", 2: "Shape", 3: "Device", 4: "Shader", 5: "OOM", 6: "Unsupported",
@@ -114,6 +115,13 @@ _SIGS = {
                                       _u32]),
     "frx_fp8_grad_weight_grouped": (_int, [_vp, _vp, _sz, _int, _vp, _vp, _sz, _vp, _vp, _u32, _vp, _int, _u32, _u32,
                                            _u32]),
+    "frx_fp4_quantize": (_int, [_vp, _vp, _int, _u32, _u32, _sz, _int, _vp, _sz, _vp]),
+    "frx_fp4_dequantize": (_int, [_vp, _vp, _sz, _vp, _u32, _u32, _vp, _int, _sz]),
+    "frx_fp4_linear": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _int, _u32, _u32, _u32]),
+    "frx_fp4_linear_act": (_int, [_vp, _vp, _int, _vp, _sz, _vp, _vp, _int, _u32, _u32, _u32]),
+    "frx_fp4_linear_grouped": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _u32, _vp, _int, _u32, _u32, _u32]),
+    "frx_fp4_moe_ffn": (_int, [_vp, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
+                               _int, _vp, _int, _vp, _vp]),
     "frx_moe_rows_capacity": (_sz, [_u32, _u32, _u32, _u32]),
     "frx_moe_sort": (_int, [_vp, _vp, _vp]),
     "frx_moe_dispatch": (_int, [_vp, _vp, _sz, _vp, _vp]),
@@ -315,6 +323,22 @@ def _fp8_code(t) -> int:
     raise TypeError(f"codes must be float8_e4m3fn or float8_e5m2, got {t.dtype}")
 
 
+def _fp4_codes(t, name):
+    """(rows, bytes, row stride in bytes) of packed 4-bit codes."""
+    torch = _torch or _tt()
+    if t.dtype is not torch.uint8 and t.dtype is not torch.float4_e2m1fn_x2:
+        raise TypeError(f"{name} must be uint8 or float4_e2m1fn_x2, two codes to an element, got {t.dtype}")
+    return _rows2(t, name)
+
+
+def _fp4_scales(t, rows, k, name):
+    """The scales of `rows` rows of k codes: contiguous bytes, whole dwords a row."""
+    torch = _torch or _tt()
+    if t.dtype is not torch.uint8 and t.dtype is not torch.float8_e8m0fnu:
+        raise TypeError(f"{name} must be uint8 or float8_e8m0fnu, got {t.dtype}")
+    _dense(t, (rows, (k + 127) // 128 * 4), None, name)
+
+
 def _here(d, *ts):
     """The tensors (None among them) and the sorted rows are on device d, the context's: an address of any other memory
     would fault there."""
@@ -392,6 +416,15 @@ def _per_expert(ts, E, shape, dtype, name, rows=False, out=False, dev=-1):
             _dense(t, shape, dtype, name)
     _here(dev, *ts)
     return array.array("Q", [t.data_ptr() for t in ts]), ld
+
+
+def _fp4_experts(ts, E, shape, name, dev, rows=False, scales=False):
+    """_per_expert for codes, or scales, of either of their dtypes."""
+    torch = _torch or _tt()
+    dt = ts.dtype if hasattr(ts, "dtype") else ts[0].dtype if len(ts) else torch.uint8
+    if dt is not torch.uint8 and dt is not (torch.float8_e8m0fnu if scales else torch.float4_e2m1fn_x2):
+        raise TypeError(f"{name} must be uint8 or {'float8_e8m0fnu' if scales else 'float4_e2m1fn_x2'}, got {dt}")
+    return _per_expert(ts, E, shape, dt, name, rows=rows, dev=dev)
 
 
 class MoeRows:
@@ -795,6 +828,145 @@ class Context:
                                                  dp.buffer_info()[0],
                                                  _dtype_code(dw[0]), R, N, K), self._h)
         return dw
+
+    # 4-bit floating-point linears; codes are uint8 or float4_e2m1fn_x2 tensors of half
+    # the columns, scales uint8 or float8_e8m0fnu.
+    def fp4_quantize(self, x, blocks: int, q, scale):
+        """frx_fp4_quantize: codes and scales of x [M][K] (f32 or bf16, any row
+        stride) in blocks FP4_ROWS or FP4_COLS. q [M][K/2] (COLS: [K][M/2]) with
+        the codes of a row rounded up to a multiple of 32, any row stride that is
+        a multiple of 16 bytes; scale [M][4*ceil(K/128)] (COLS: K and M)."""
+        M, K, ldx = _rows2(x, "x")
+        r, c = (K, M) if blocks == FP4_COLS else (M, K)
+        qr, qc, ldq = _fp4_codes(q, "q")
+        if qr != r or qc != (c + 31) // 32 * 16:
+            raise _shape_err(f"q has shape {tuple(q.shape)}, expected {(r, (c + 31) // 32 * 16)}")
+        _fp4_scales(scale, r, c, "scale")
+        if not x.get_device() == q.get_device() == scale.get_device() == self._dev:
+            _here(self._dev, x, q, scale)
+        _check(lib().frx_fp4_quantize(self._h, x.data_ptr(), _dtype_code(x), M, K, ldx, blocks, q.data_ptr(), ldq,
+                                      scale.data_ptr()), self._h)
+        return q, scale
+
+    def fp4_dequantize(self, q, scale, y):
+        """frx_fp4_dequantize: the values y [M][K] (f32 or bf16, any row stride) of
+        codes q [M][K/2] in blocks FP4_ROWS, K rounded up to a multiple of 32 in q."""
+        M, K, ldy = _rows2(y, "y")
+        qr, qc, ldq = _fp4_codes(q, "q")
+        if qr != M or qc != (K + 31) // 32 * 16:
+            raise _shape_err(f"q has shape {tuple(q.shape)}, expected {(M, (K + 31) // 32 * 16)}")
+        _fp4_scales(scale, M, K, "scale")
+        if not q.get_device() == scale.get_device() == y.get_device() == self._dev:
+            _here(self._dev, q, scale, y)
+        _check(lib().frx_fp4_dequantize(self._h, q.data_ptr(), ldq, scale.data_ptr(), M, K, y.data_ptr(),
+                                        _dtype_code(y), ldy), self._h)
+        return y
+
+    def fp4_linear(self, a, sa, b, sb, y):
+        """frx_fp4_linear: y [M][N] = a b^T. a [M][K/2], sa [M][4*ceil(K/128)]; b
+        [N][K/2], sb [N][4*ceil(K/128)]."""
+        M, kh, lda = _fp4_codes(a, "a")
+        N, kb_, ldb = _fp4_codes(b, "b")
+        if kb_ != kh:
+            raise _shape_err(f"b has {kb_} bytes a row, a {kh}")
+        _fp4_scales(sa, M, 2 * kh, "sa")
+        _fp4_scales(sb, N, 2 * kh, "sb")
+        _dense(y, (M, N), None, "y")
+        if not a.get_device() == sa.get_device() == b.get_device() == sb.get_device() == y.get_device() == self._dev:
+            _here(self._dev, a, sa, b, sb, y)
+        _check(lib().frx_fp4_linear(self._h, a.data_ptr(), lda, sa.data_ptr(), b.data_ptr(), ldb, sb.data_ptr(),
+                                    y.data_ptr(), _dtype_code(y), M, 2 * kh, N), self._h)
+        return y
+
+    def fp4_linear_act(self, x, b, sb, y):
+        """frx_fp4_linear_act: y = x w^T for f32 or bf16 x [M][K], quantised on the
+        way, and weights b [N][K/2], sb [N][4*ceil(K/128)]."""
+        M, K, _ = _rows2(x, "x")
+        N, kb_, ldb = _fp4_codes(b, "b")
+        if 2 * kb_ != K:
+            raise _shape_err(f"b has {2 * kb_} columns, x {K}")
+        if not x.is_contiguous():
+            raise _shape_err("x must be contiguous")
+        _fp4_scales(sb, N, K, "sb")
+        _dense(y, (M, N), None, "y")
+        if not x.get_device() == b.get_device() == sb.get_device() == y.get_device() == self._dev:
+            _here(self._dev, x, b, sb, y)
+        _check(lib().frx_fp4_linear_act(self._h, x.data_ptr(), _dtype_code(x), b.data_ptr(), ldb, sb.data_ptr(),
+                                        y.data_ptr(), _dtype_code(y), M, K, N), self._h)
+        return y
+
+    def fp4_linear_grouped(self, a, sa, b, sb, offsets, y):
+        """frx_fp4_linear_grouped: rows offsets[e] to offsets[e + 1] of a [R][K/2]
+        times expert e's codes b[e] [N][K/2], sb[e] [N][4*ceil(K/128)] (stacked
+        tensors, or lists of E). The kernel goes by R: rows past those in use cost
+        time, so views of a, sa and y that end near them are faster."""
+        torch = _torch or _tt()
+        R, kh, lda = _fp4_codes(a, "a")
+        E, sk = int(offsets.numel()) - 1, (kh + 63) // 64 * 4
+        shape = y.shape
+        N = shape[1] if len(shape) == 2 else 0
+        _dense(offsets, (E + 1,), torch.int32, "offsets")
+        _fp4_scales(sa, R, 2 * kh, "sa")
+        bp, ldb = _fp4_experts(b, E, (N, kh), "b", self._dev, rows=True)
+        sp, _ = _fp4_experts(sb, E, (N, sk), "sb", self._dev, scales=True)
+        if shape != (R, N) or not y.is_contiguous():
+            _dense(y, (R, N), None, "y")
+        if not a.get_device() == sa.get_device() == offsets.get_device() == y.get_device() == self._dev:
+            _here(self._dev, a, sa, offsets, y)
+        _check(lib().frx_fp4_linear_grouped(self._h, a.data_ptr(), lda, sa.data_ptr(), bp.buffer_info()[0], ldb,
+                                            sp.buffer_info()[0], offsets.data_ptr(), E, y.data_ptr(), _dtype_code(y),
+                                            R, 2 * kh, N), self._h)
+        return y
+
+    def fp4_moe_ffn(self, x, router, w_gate, s_gate, w_up, s_up, w_down, s_down, y, topk_idx=None, topk_w=None,
+                    top_k=None, act: int = ACT_SILU):
+        """frx_fp4_moe_ffn: an expert layer for up to 64 tokens x [T][H] (f32 or
+        bf16) over weights in FP4_ROWS: w_gate, w_up [E][I][H/2], s_gate, s_up
+        [E][I][4*ceil(H/128)], w_down [E][H][I/2], s_down [E][H][4*ceil(I/128)]
+        (stacked tensors, or lists of E). router [E][H], or None: topk_idx
+        [T][top_k] int32 (an index outside [0, E) goes nowhere) and topk_w
+        [T][top_k] f32 are the routes; with a router they receive them. top_k: the
+        width of topk_idx where that is given."""
+        torch = _torch or _tt()
+        T, H, _ = _rows2(x, "x")
+        if not x.is_contiguous():
+            raise _shape_err("x must be contiguous")
+        E = len(w_gate)
+        if E < 1:
+            raise _shape_err("there must be at least one expert")
+        I = w_gate[0].shape[0] if w_gate[0].dim() == 2 else 0
+        routes = topk_idx if topk_idx is not None else topk_w
+        if routes is not None:
+            if routes.dim() != 2 or (top_k is not None and routes.shape[1] != top_k):
+                raise _shape_err(f"routes have shape {tuple(routes.shape)}, expected {(T, top_k)}")
+            top_k = routes.shape[1]
+        elif top_k is None:
+            raise _shape_err("top_k is not given")
+        if topk_idx is not None:
+            _dense(topk_idx, (T, top_k), torch.int32, "topk_idx")
+        if topk_w is not None:
+            _dense(topk_w, (T, top_k), torch.float32, "topk_w")
+        if router is None:
+            if topk_idx is None or topk_w is None:
+                raise _shape_err("without a router topk_idx and topk_w must be given")
+        else:
+            _dense(router, (E, H), None, "router")
+        _dense(y, (T, H), None, "y")
+        dev, sk, si = self._dev, (H + 127) // 128 * 4, (I + 127) // 128 * 4
+        hh, ih = (H + 1) // 2, (I + 1) // 2
+        keep = [_fp4_experts(w_gate, E, (I, hh), "w_gate", dev)[0],
+                _fp4_experts(s_gate, E, (I, sk), "s_gate", dev, scales=True)[0],
+                _fp4_experts(w_up, E, (I, hh), "w_up", dev)[0],
+                _fp4_experts(s_up, E, (I, sk), "s_up", dev, scales=True)[0],
+                _fp4_experts(w_down, E, (H, ih), "w_down", dev)[0],
+                _fp4_experts(s_down, E, (H, si), "s_down", dev, scales=True)[0]]
+        _here(dev, x, router, y, topk_idx, topk_w)
+        _check(lib().frx_fp4_moe_ffn(
+            self._h, x.data_ptr(), _dtype_code(x), router if router is None else router.data_ptr(),
+            0 if router is None else _dtype_code(router), *(k.buffer_info()[0] for k in keep), T, H, I, E, top_k, act,
+            y.data_ptr(), _dtype_code(y), topk_idx if topk_idx is None else topk_idx.data_ptr(),
+            topk_w if topk_w is None else topk_w.data_ptr()), self._h)
+        return y
 
     def set_fp8_sums(self, mode: int):
         """frx_set_fp8_sums: FP8_SUMS_F32 (default: every sum in fp32) or

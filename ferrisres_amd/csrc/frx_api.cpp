@@ -99,6 +99,10 @@ struct frx_ctx {
   size_t spp_ws_bytes = 0;
   void *q8_ws = nullptr;  // 8-bit codes and scales of frx_fp8_linear_act's activations
   size_t q8_ws_bytes = 0;
+  void *q4_ws = nullptr;  // 4-bit codes and scales of frx_fp4_linear_act's activations
+  size_t q4_ws_bytes = 0;
+  void *few_ws = nullptr;  // frx_fp4_moe_ffn's intermediate, and routes that the caller does not take
+  size_t few_ws_bytes = 0;
   void *sort_ws = nullptr;  // counts by chunk of frx_moe_sort
   size_t sort_ws_bytes = 0;
   unsigned *sk_cnt = nullptr;  // its per-row-tile arrival counters (zero between launches)
@@ -206,6 +210,8 @@ void frx_destroy(frx_ctx *ctx) {
   if (ctx->xpl_ws) (void)hipFree(ctx->xpl_ws);
   if (ctx->spp_ws) (void)hipFree(ctx->spp_ws);
   if (ctx->q8_ws) (void)hipFree(ctx->q8_ws);
+  if (ctx->q4_ws) (void)hipFree(ctx->q4_ws);
+  if (ctx->few_ws) (void)hipFree(ctx->few_ws);
   if (ctx->sort_ws) (void)hipFree(ctx->sort_ws);
   if (ctx->sk_cnt) (void)hipFree(ctx->sk_cnt);
   if (ctx->ffn_bar) (void)hipFree(ctx->ffn_bar);
@@ -1685,6 +1691,212 @@ frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t ld
   const hipError_t e = frx::launch_fp8_grad_weight(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, offsets, (int)E, dw,
                                                    yt == FRX_BF16, fp8_pipe8(ctx, yt), R, N, K, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "fp8 weight gradient launch");
+  return FRX_OK;
+}
+
+// ---- 4-bit floating-point linears -------------------------------------------------
+
+// a tile of 256 rows is addressed by 32-bit offsets
+constexpr size_t kMaxFp4Ld = (size_t)1 << 22;
+
+frx_status frx_fp4_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t M, uint32_t K, size_t ldx,
+                            frx_fp4_blocks blocks, uint8_t *q, size_t ldq, uint8_t *scale) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (!x || !q || !scale) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (M == 0 || K == 0) return fail(ctx, FRX_ERR_SHAPE, "empty shape M=%u K=%u", M, K);
+  if (!is_dtype(xt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (blocks != FRX_FP4_ROWS && blocks != FRX_FP4_COLS)
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "unknown blocks %d", (int)blocks);
+  if (M > kMaxDim || K > kMaxDim) return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u too large", M, K);
+  if (ldx < K) return fail(ctx, FRX_ERR_SHAPE, "ldx=%zu is less than K=%u", ldx, K);
+  const uint32_t len = blocks == FRX_FP4_COLS ? M : K;
+  if (ldq % 16 != 0 || ldq < ((size_t)len + 31) / 32 * 16)
+    return fail(ctx, FRX_ERR_SHAPE, "ldq=%zu must be a multiple of 16 that holds %u codes", ldq, len);
+  if (!aligned_to(x, dtype_bytes(xt)) || !aligned_to(q, 16) || !aligned_to(scale, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "x must be aligned to its elements, q to 16 bytes, scale to 4");
+  const size_t kb = (K + 127) / 128, mb = (M + 127) / 128;
+  if ((blocks == FRX_FP4_ROWS ? ((size_t)M * kb + 15) / 16 : kb * mb) > kMaxWgs)
+    return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
+  const hipError_t e = frx::launch_fp4_quantize(x, xt == FRX_BF16, M, K, ldx, blocks == FRX_FP4_COLS, q, ldq, scale,
+                                                ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp4 quantise launch");
+  return FRX_OK;
+}
+
+frx_status frx_fp4_dequantize(frx_ctx *ctx, const uint8_t *q, size_t ldq, const uint8_t *scale, uint32_t M, uint32_t K,
+                              void *y, frx_dtype yt, size_t ldy) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (!q || !scale || !y) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (M == 0 || K == 0) return fail(ctx, FRX_ERR_SHAPE, "empty shape M=%u K=%u", M, K);
+  if (!is_dtype(yt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (M > kMaxDim || K > kMaxDim || ((size_t)M * (((size_t)K + 7) / 8) + 255) / 256 > kMaxWgs)
+    return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u too large", M, K);
+  if (ldq % 16 != 0 || ldq < ((size_t)K + 31) / 32 * 16)
+    return fail(ctx, FRX_ERR_SHAPE, "ldq=%zu must be a multiple of 16 that holds %u codes", ldq, K);
+  if (ldy < K) return fail(ctx, FRX_ERR_SHAPE, "ldy=%zu is less than K=%u", ldy, K);
+  if (!aligned_to(q, 16) || !aligned_to(scale, 4) || !aligned_to(y, dtype_bytes(yt)))
+    return fail(ctx, FRX_ERR_SHAPE, "q must be aligned to 16 bytes, scale to 4, y to its elements");
+  const hipError_t e = frx::launch_fp4_dequantize(q, ldq, scale, M, K, y, yt == FRX_BF16, ldy, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp4 dequantise launch");
+  return FRX_OK;
+}
+
+// What the products ask of their operands: rows of a and of b, K columns.
+static frx_status check_fp4(frx_ctx *ctx, const void *a, size_t lda, const void *sa, size_t ldb, frx_dtype yt,
+                            uint32_t M, uint32_t K, uint32_t N) {
+  if (!a || !sa) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (M == 0 || K == 0 || N == 0) return fail(ctx, FRX_ERR_SHAPE, "empty shape M=%u K=%u N=%u", M, K, N);
+  if (!is_dtype(yt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (K % 32 != 0) return fail(ctx, FRX_ERR_SHAPE, "%u columns of codes must be a multiple of 32", K);
+  if (lda % 16 != 0 || ldb % 16 != 0 || lda < K / 2 || ldb < K / 2 || lda > kMaxFp4Ld || ldb > kMaxFp4Ld)
+    return fail(ctx, FRX_ERR_SHAPE, "lda=%zu and ldb=%zu must be multiples of 16 from %u to 2^22", lda, ldb, K / 2);
+  if (M > kMaxDim || N > kMaxDim || ((size_t)(M + 63) / 64 + frx::FP8_MAXE) * (((size_t)N + 127) / 128) > kMaxWgs ||
+      ((size_t)N + 15) / 16 >= ((size_t)1 << 23))
+    return fail(ctx, FRX_ERR_SHAPE, "M=%u N=%u too large", M, N);
+  if (!aligned_to(a, 16) || !aligned_to(sa, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "codes must be 16-byte aligned, scales 4-byte");
+  return FRX_OK;
+}
+
+// b and y of one product.
+static frx_status check_fp4_side(frx_ctx *ctx, const void *b, const void *sb, const void *y, frx_dtype yt) {
+  if (!b || !sb || !y) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (!aligned_to(b, 16) || !aligned_to(sb, 4) || !aligned_to(y, dtype_bytes(yt)))
+    return fail(ctx, FRX_ERR_SHAPE, "codes must be 16-byte aligned, scales 4-byte, y to its elements");
+  return FRX_OK;
+}
+
+static frx_status fp4_run(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
+                          const uint8_t *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N) {
+  frx::Fp4Plan plan = frx::fp4_plan(M, K, N, ctx->cus);
+  const size_t need = plan.S > 1 ? (size_t)plan.S * M * N * 4 : 0;
+  if (need && !may_grow(ctx, ctx->gk_ws_bytes, need)) {
+    plan.S = 1;  // a first call under capture: whole K
+    plan.per = (int)((K + 255) / 256);
+  } else if (need) {
+    const frx_status st = ensure_buffer(ctx, &ctx->gk_ws, &ctx->gk_ws_bytes, need, "fp4 split workspace allocation");
+    if (st != FRX_OK) return st;
+  }
+  const hipError_t e = frx::launch_fp4_linear(a, lda, sa, b, ldb, sb, y, yt == FRX_BF16, M, K, N, plan,
+                                              reinterpret_cast<float *>(ctx->gk_ws), ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp4 linear launch");
+  return FRX_OK;
+}
+
+frx_status frx_fp4_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
+                          const uint8_t *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if ((st = check_fp4(ctx, a, lda, sa, ldb, yt, M, K, N)) != FRX_OK) return st;
+  if ((st = check_fp4_side(ctx, b, sb, y, yt)) != FRX_OK) return st;
+  return fp4_run(ctx, a, lda, sa, b, ldb, sb, y, yt, M, K, N);
+}
+
+frx_status frx_fp4_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
+                              const uint8_t *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  // x takes the codes' place in the checks; its own alignment is its element's
+  if (!x) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (!is_dtype(xt)) return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (!aligned_to(x, dtype_bytes(xt))) return fail(ctx, FRX_ERR_SHAPE, "x must be aligned to its elements");
+  if ((st = check_fp4(ctx, b, K % 32 == 0 ? K / 2 : 16, sb, ldb, yt, M, K, N)) != FRX_OK) return st;
+  if ((st = check_fp4_side(ctx, b, sb, y, yt)) != FRX_OK) return st;
+  const frx::Fp4Plan plan = frx::fp4_plan(M, K, N, ctx->cus);
+  if (plan.tile == frx::FP4_T_SKINNY && frx::fp4_act_fits(M, K)) {
+    const hipError_t e = frx::launch_fp4_linear_act(x, xt == FRX_BF16, b, ldb, sb, y, yt == FRX_BF16, M, K, N, plan,
+                                                    ctx->stream);
+    if (e != hipSuccess) return hip_fail(ctx, e, "fp4 linear launch");
+    return FRX_OK;
+  }
+  const size_t kb = (K + 127) / 128, codes = a256((size_t)M * (K / 2)), need = codes + (size_t)M * kb * 4;
+  if (((size_t)M * kb + 15) / 16 > kMaxWgs) return fail(ctx, FRX_ERR_SHAPE, "M=%u K=%u: too many blocks", M, K);
+  if (!may_grow(ctx, ctx->q4_ws_bytes, need))
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "the first call at this size allocates and cannot be captured into a graph");
+  if ((st = ensure_buffer(ctx, &ctx->q4_ws, &ctx->q4_ws_bytes, need, "fp4 activation workspace allocation")) != FRX_OK)
+    return st;
+  uint8_t *q = static_cast<uint8_t *>(ctx->q4_ws), *sa = q + codes;
+  const hipError_t e = frx::launch_fp4_quantize(x, xt == FRX_BF16, M, K, K, 0, q, K / 2, sa, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp4 quantise launch");
+  return fp4_run(ctx, q, K / 2, sa, b, ldb, sb, y, yt, M, K, N);
+}
+
+frx_status frx_fp4_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint8_t *sa,
+                                  const uint8_t *const *b, size_t ldb, const uint8_t *const *sb,
+                                  const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R, uint32_t K,
+                                  uint32_t N) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (E == 0 || E > (uint32_t)frx::FP8_MAXE) return fail(ctx, FRX_ERR_SHAPE, "E=%u must be in [1, %d]", E, frx::FP8_MAXE);
+  if (!b || !sb || !offsets) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if ((st = check_fp4(ctx, a, lda, sa, ldb, yt, R, K, N)) != FRX_OK) return st;
+  for (uint32_t e = 0; e < E; e++)
+    if ((st = check_fp4_side(ctx, b[e], sb[e], y, yt)) != FRX_OK) return st;
+  if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
+  const hipError_t e = frx::launch_fp4_grouped(a, lda, sa, b, ldb, sb, offsets, (int)E, y, yt == FRX_BF16, R, K, N,
+                                               ctx->cus, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp4 grouped linear launch");
+  return FRX_OK;
+}
+
+frx_status frx_fp4_moe_ffn(frx_ctx *ctx, const void *x, frx_dtype xt, const void *router, frx_dtype rt,
+                           const uint8_t *const *w_gate, const uint8_t *const *s_gate, const uint8_t *const *w_up,
+                           const uint8_t *const *s_up, const uint8_t *const *w_down, const uint8_t *const *s_down,
+                           uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32_t top_k, frx_activation act, void *y,
+                           frx_dtype yt, uint32_t *topk_idx, float *topk_w) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (!x || !y || !w_gate || !s_gate || !w_up || !s_up || !w_down || !s_down)
+    return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if (!router && (!topk_idx || !topk_w)) return fail(ctx, FRX_ERR_SHAPE, "without a router the routes must be given");
+  if (!is_dtype(xt) || !is_dtype(yt) || (router && !is_dtype(rt)))
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "dtype must be FRX_F32 or FRX_BF16");
+  if (act != FRX_ACT_SILU && act != FRX_ACT_GELU_TANH) return fail(ctx, FRX_ERR_UNSUPPORTED, "activation %d", (int)act);
+  if (T == 0 || H == 0 || I == 0) return fail(ctx, FRX_ERR_SHAPE, "empty shape T=%u H=%u I=%u", T, H, I);
+  if (T > frx::FP4_MOE_MAX_T)
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "T=%u: for more than %u tokens sort them (frx_moe_sort) and use "
+                "frx_fp4_linear_grouped", T, frx::FP4_MOE_MAX_T);
+  if (H % 32 != 0 || I % 32 != 0 || H / 2 > kMaxFp4Ld || I / 2 > kMaxFp4Ld)
+    return fail(ctx, FRX_ERR_SHAPE, "H=%u and I=%u must be multiples of 32 up to 2^23", H, I);
+  if (E == 0 || E > (uint32_t)frx::FP8_MAXE || top_k == 0 || top_k > 64 || (router && top_k > E))
+    return fail(ctx, FRX_ERR_SHAPE, "E=%u top_k=%u must be in [1, 64], a router's top_k at most E", E, top_k);
+  if (!aligned_to(x, dtype_bytes(xt)) || !aligned_to(y, dtype_bytes(yt)) ||
+      (router && !aligned_to(router, dtype_bytes(rt))) || !aligned_to(topk_idx, 4) || !aligned_to(topk_w, 4))
+    return fail(ctx, FRX_ERR_SHAPE, "x, y, router, topk_idx and topk_w must be aligned to their elements");
+  frx::Fp4Moe p = {};
+  const uint8_t *const *w[6] = {w_gate, s_gate, w_up, s_up, w_down, s_down};
+  for (uint32_t e = 0; e < E; e++)
+    for (int k = 0; k < 3; k++) {
+      if ((st = check_fp4_side(ctx, w[2 * k][e], w[2 * k + 1][e], y, yt)) != FRX_OK) return st;
+      p.w[k][e] = w[2 * k][e];
+      p.s[k][e] = w[2 * k + 1][e];
+    }
+  const size_t h = a256(frx::fp4_moe_bytes(T, I, top_k, yt == FRX_BF16)), routes = a256((size_t)T * top_k * 4);
+  const size_t need = h + (router ? 2 * routes : 0);
+  if (!may_grow(ctx, ctx->few_ws_bytes, need))
+    return fail(ctx, FRX_ERR_UNSUPPORTED, "the first call at this size allocates and cannot be captured into a graph");
+  if ((st = ensure_buffer(ctx, &ctx->few_ws, &ctx->few_ws_bytes, need, "expert layer workspace allocation")) != FRX_OK)
+    return st;
+  uint8_t *ws = static_cast<uint8_t *>(ctx->few_ws);
+  p.x = x;
+  p.router = router;
+  p.y = y;
+  p.h = reinterpret_cast<uint16_t *>(ws);
+  p.idx = topk_idx ? topk_idx : reinterpret_cast<uint32_t *>(ws + h);
+  p.wts = topk_w ? topk_w : reinterpret_cast<float *>(ws + h + routes);
+  p.T = T;
+  p.H = H;
+  p.I = I;
+  p.E = E;
+  p.top_k = top_k;
+  p.xt_bf16 = xt == FRX_BF16;
+  p.rt_bf16 = rt == FRX_BF16;
+  p.yt_bf16 = yt == FRX_BF16;
+  p.act = (int)act;
+  const hipError_t e = frx::launch_fp4_moe(p, ctx->cus, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "expert layer launch");
   return FRX_OK;
 }
 

@@ -1,6 +1,7 @@
 // frx_fp8.hip — launches of the 8-bit floating-point linears (engine: frx_fp8.hpp).
 #include "frx_fp8_skinny.hpp"
 #include "frx_fp8_ring.hpp"
+#include "frx_tiles.hpp"
 
 namespace frx {
 
@@ -16,12 +17,6 @@ struct DenseArgs {
   uint32_t M, K, N;
   int per;  // per: blocks of 128 in a slice
 };
-
-// Whether rows of n elements from y on are whole aligned quads.
-template <typename YT>
-__device__ __forceinline__ bool quads(const void *y, uint32_t n) {
-  return ((reinterpret_cast<uintptr_t>(y) & (4 * sizeof(YT) - 1)) | (n & 3)) == 0;
-}
 
 template <bool BR1>
 __device__ __forceinline__ void fill_operands(Fp8Operands &o, const uint8_t *a, size_t lda, const float *sa,
@@ -39,21 +34,6 @@ __device__ __forceinline__ void fill_operands(Fp8Operands &o, const uint8_t *a, 
   o.b_rows = (int)nr;
   o.b_first = (int)(n0 & 127);
   o.K = (int)K;
-}
-
-// The tile of workgroup `bid` of mts x nts. Hardware deals workgroups out to the
-// 8 XCDs in turn; each XCD gets a contiguous run of tiles, ordered by groups of
-// GM tiles of tokens, within a group down the tokens first, so that the tiles
-// an XCD works on at a time share rows of both sides in its L2.
-template <int GM>
-__device__ __forceinline__ void xcd_tile(uint32_t bid, uint32_t mts, uint32_t nts, uint32_t &mt, uint32_t &nt) {
-  const uint32_t total = mts * nts, q = total / 8, r = total % 8, xcd = bid % 8, i = bid / 8;
-  const uint32_t lin = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + i;
-  const uint32_t rows = min((uint32_t)GM, mts);  // (GM * nts may pass 32 bits)
-  const uint32_t group = lin / (rows * nts), rest = lin - group * (rows * nts);
-  const uint32_t gm = min(rows, mts - group * rows);
-  nt = rest / gm;
-  mt = group * rows + rest - nt * gm;
 }
 
 template <typename Tile, bool BR1, typename YT>
@@ -89,38 +69,6 @@ struct GroupArgs {
   const uint8_t *b[FP8_MAXE];
   const float *sb[FP8_MAXE];
 };
-
-// Expert e's rows [first, end), kept inside the R rows there are.
-__device__ __forceinline__ void expert_rows(const uint32_t *offsets, int e, uint32_t R, uint32_t &first,
-                                            uint32_t &end) {
-  first = min(offsets[e], R);
-  end = max(min(offsets[e + 1], R), first);
-}
-
-// The expert of tile mt when every expert's rows are cut into tiles of BM, and
-// the tile's first row and its expert's last + 1; -1 past the last tile.
-// Lane e counts expert e's tiles; the expert is the first whose running count
-// passes mt.
-template <int BM>
-__device__ __forceinline__ int expert_tile(const uint32_t *offsets, int E, uint32_t R, uint32_t mt, uint32_t &m0,
-                                           uint32_t &end) {
-  const int lane = threadIdx.x & 63;
-  uint32_t first = 0, last = 0;
-  if (lane < E) expert_rows(offsets, lane, R, first, last);
-  const uint32_t tiles = (last - first + BM - 1) / BM;
-  uint32_t incl = tiles;
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint32_t v = (uint32_t)__shfl_up((int)incl, s);
-    if (lane >= s) incl += v;
-  }
-  const unsigned long long past = __ballot(lane < E && incl > mt);
-  if (past == 0) return -1;
-  const int e = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
-  const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(incl - tiles), e);
-  m0 = (uint32_t)__builtin_amdgcn_readlane((int)first, e) + (mt - before) * BM;
-  end = (uint32_t)__builtin_amdgcn_readlane((int)last, e);
-  return e;
-}
 
 // mts: tiles of rows there may be. An XCD's run of tiles goes down the rows
 // first: the tiles of an expert's rows share its weights in that L2.
@@ -205,31 +153,6 @@ __global__ __launch_bounds__(Tile::NT, 2) void fp8_grad_kernel(const GradArgs p)
   const size_t at = (size_t)m0 * p.K + n0;
   YT *dw = static_cast<YT *>(p.dw[e]);
   Tile::template store<YT>(acc, dw + at, p.K, o.a_rows, o.b_rows, quads<YT>(dw, p.K));
-}
-
-// y = the parts added in order, four values a thread (n of them, parts n apart).
-template <typename YT>
-__global__ __launch_bounds__(256) void fp8_join_kernel(const float *__restrict__ part, int S, size_t n,
-                                                       YT *__restrict__ y) {
-  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  if (((n & 3) | (reinterpret_cast<uintptr_t>(y) & (4 * sizeof(YT) - 1))) == 0) {
-    f32x4 v = *reinterpret_cast<const f32x4 *>(part + i);
-    for (int s = 1; s < S; s++) v += *reinterpret_cast<const f32x4 *>(part + (size_t)s * n + i);
-    if constexpr (sizeof(YT) == 4) {
-      *reinterpret_cast<f32x4 *>(y + i) = v;
-    } else {
-      *reinterpret_cast<u32x2 *>(y + i) = (u32x2){bf16_rne_nb(v[0]) | (bf16_rne_nb(v[1]) << 16),
-                                                 bf16_rne_nb(v[2]) | (bf16_rne_nb(v[3]) << 16)};
-    }
-    return;
-  }
-  for (size_t k = i; k < n && k < i + 4; k++) {
-    float v = part[k];
-    for (int s = 1; s < S; s++) v += part[(size_t)s * n + k];
-    if constexpr (sizeof(YT) == 4) y[k] = v;
-    else y[k] = (uint16_t)bf16_rne_nb(v);
-  }
 }
 
 template <typename K, typename A>
@@ -356,8 +279,8 @@ hipError_t launch_fp8_linear(const uint8_t *a, size_t lda, int e5m2, const float
   if (e != hipSuccess || plan.S == 1) return e;
   const size_t n = (size_t)M * N;
   const dim3 grid((unsigned)((n + 1023) / 1024));
-  if (yt_bf16) hipLaunchKernelGGL(fp8_join_kernel<uint16_t>, grid, dim3(256), 0, stream, part, plan.S, n, (uint16_t *)y);
-  else hipLaunchKernelGGL(fp8_join_kernel<float>, grid, dim3(256), 0, stream, part, plan.S, n, (float *)y);
+  if (yt_bf16) hipLaunchKernelGGL(join_parts_kernel<uint16_t>, grid, dim3(256), 0, stream, part, plan.S, n, (uint16_t *)y);
+  else hipLaunchKernelGGL(join_parts_kernel<float>, grid, dim3(256), 0, stream, part, plan.S, n, (float *)y);
   return hipGetLastError();
 }
 

@@ -368,6 +368,45 @@ hipError_t launch_fp8_grad_weight(const uint8_t *a, size_t lda, int e5m2, const 
                                   size_t ldb, const float *sb, const uint32_t *offsets, int E, void *const *dw,
                                   int yt_bf16, int pipe8, uint32_t R, uint32_t N, uint32_t K, hipStream_t stream);
 
+// ---- 4-bit floating-point linears (frx_fp4.hip, frx_fp4_quant.hip) ----------
+// cols: blocks of 32 rows, codes transposed (FRX_FP4_COLS)
+hipError_t launch_fp4_quantize(const void *x, int xt_bf16, uint32_t M, uint32_t K, size_t ldx, int cols, uint8_t *q,
+                               size_t ldq, uint8_t *scale, hipStream_t stream);
+hipError_t launch_fp4_dequantize(const uint8_t *q, size_t ldq, const uint8_t *scale, uint32_t M, uint32_t K, void *y,
+                                 int yt_bf16, size_t ldy, hipStream_t stream);
+// y = a b^T, as fp4_plan says. S > 1: K in S slices of `per` steps of 256 columns, fp32 parts
+// [S][M][N] in part, added in order.
+hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
+                             const uint8_t *sb, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
+                             const Fp4Plan &plan, float *part, hipStream_t stream);
+// x f32 or bf16 [M][K], quantised on the way by every workgroup for itself
+// (FP4_T_SKINNY plans whose activations fit: fp4_act_fits).
+constexpr uint32_t FP4_ACT_MAX_M = 4;
+constexpr size_t FP4_ACT_MAX_BYTES = 64 << 10;
+bool fp4_act_fits(uint32_t M, uint32_t K);
+hipError_t launch_fp4_linear_act(const void *x, int xt_bf16, const uint8_t *b, size_t ldb, const uint8_t *sb, void *y,
+                                 int yt_bf16, uint32_t M, uint32_t K, uint32_t N, const Fp4Plan &plan,
+                                 hipStream_t stream);
+hipError_t launch_fp4_grouped(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *const *b, size_t ldb,
+                              const uint8_t *const *sb, const uint32_t *offsets, int E, void *y, int yt_bf16,
+                              uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream);
+
+// ---- experts in 4 bits for a few tokens (frx_fp4_moe.hip) --------------------
+constexpr uint32_t FP4_MOE_MAX_T = 64;
+struct Fp4Moe {
+  const void *x, *router;  // router: null, the routes are given
+  void *y;
+  uint32_t *idx;           // [T][top_k]
+  float *wts;              // [T][top_k]
+  uint16_t *h;             // [T * top_k][planes][I] act(g) * u * weight as bf16 planes, zeros nowhere
+  uint32_t T, H, I, E, top_k;
+  int xt_bf16, rt_bf16, yt_bf16, act;
+  const uint8_t *w[3][FP8_MAXE], *s[3][FP8_MAXE];  // gate, up, down
+};
+constexpr int fp4_moe_planes(int yt_bf16) { return yt_bf16 ? 2 : 3; }
+size_t fp4_moe_bytes(uint32_t T, uint32_t I, uint32_t top_k, int yt_bf16);
+hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream);
+
 // ---- tokens sorted by expert, and back (frx_route.hip) -----------------------
 struct RouteRows {
   int T, top_k, E, align, R;

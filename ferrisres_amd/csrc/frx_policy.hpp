@@ -228,4 +228,38 @@ inline int fp8_grouped_tile(uint32_t R, uint32_t N, uint32_t E, int pipe8, int c
                                                                                                         : FP8_T_RING4;
 }
 
+// ---- the 4-bit floating-point linears --------------------------------------------
+
+enum { FP4_T_SKINNY = 0, FP4_T_128 = 1, FP4_T_64 = 2 };
+struct Fp4Plan {
+  int tile;    // FP4_T_*
+  int S, per;  // K slices, steps of 256 columns in each (FP4_T_SKINNY: 1, 16-row tiles of a workgroup)
+};
+
+inline Fp4Plan fp4_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
+  if (M <= 64) {
+    // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
+    const uint32_t tiles = (N + 15) / 16;
+    const int most = M <= 32 ? 4 : 2;
+    int best = 1;
+    uint32_t least = ~0u;
+    for (int rt = 1; rt <= most; rt++) {
+      const uint32_t wgs = (tiles + rt - 1) / rt, rounds = (wgs + cus - 1) / cus * rt;
+      if (rounds <= least) {
+        least = rounds;
+        best = rt;
+      }
+    }
+    return {FP4_T_SKINNY, 1, best};
+  }
+  return {FP4_T_128, 1, (int)((K + 255) / 256)};
+}
+
+// Experts' rows: tiles of 16 where R / E is small.
+inline int fp4_grouped_tile(uint32_t R, uint32_t N, uint32_t E, int cus) {
+  (void)cus;
+  if (R <= 8 * E && ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16) < (size_t)1 << 23) return FP4_T_SKINNY;
+  return FP4_T_64;
+}
+
 }  // namespace frx

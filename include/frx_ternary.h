@@ -411,6 +411,113 @@ frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t ld
                                        const uint32_t *offsets, uint32_t E, void *const *dw, frx_dtype yt,
                                        uint32_t R, uint32_t N, uint32_t K);
 
+/* ---- 4-bit floating-point linear, a power of two for each block of 32 ----------
+ * No counterpart in the reference. Half the bytes of the 8-bit linears above
+ * and the matrix pipe's fastest operands, for layers that keep more than a
+ * ternary weight but need not keep 8 bits. Codes are OCP e2m1 (0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6 and their negatives), two to a byte, the first in its low half; every
+ * 32 of them along the axis that a product sums over share a byte b that stands
+ * for 2^(b - 127) (OCP e8m0; 255: a NaN). A row's scales lie behind one another,
+ * rounded up to a multiple of 4 bytes: sk = 4 * ceil(K / 128) bytes a row. */
+typedef enum frx_fp4_blocks {
+  FRX_FP4_ROWS = 0, /* 1 x 32:  q [M][ldq], scale [M][4 * ceil(K / 128)] */
+  FRX_FP4_COLS = 1, /* 32 x 1, transposed: q [K][ldq], scale [K][4 * ceil(M / 128)] */
+  FRX_FP4_BLOCKS_RANGE_ = 0x7fffffff
+} frx_fp4_blocks;
+
+/* Codes and scales of x [M][K] (f32 or bf16, row stride ldx >= K elements). For
+ * each block: b = max(e, 2) - 2, e the biased f32 exponent of the largest
+ * magnitude (of a bf16 x the same; 0 for zeros and denormals); code = x *
+ * 2^(127 - b), which is exact, rounded to nearest even, 6 above 6. An infinity
+ * or a NaN in a block makes its b 255 and its codes zeros, so that every product
+ * that it belongs to is a NaN. A block at an edge has fewer values.
+ * ldq: bytes between rows of q, a multiple of 16 that holds the row's codes
+ * (K; COLS: M) rounded up to whole blocks; the codes of the last block past the
+ * row's end are zeros, which is how a row length of any size enters
+ * frx_fp4_linear, and so are the scales up to the multiple of 4. Bytes past
+ * them are left as they were. q 16-byte aligned, scale 4-byte, x to its
+ * elements. M, K >= 1. Stream-ordered, no allocation. */
+frx_status frx_fp4_quantize(frx_ctx *ctx, const void *x, frx_dtype xt, uint32_t M, uint32_t K, size_t ldx,
+                            frx_fp4_blocks blocks, uint8_t *q, size_t ldq, uint8_t *scale);
+
+/* The values y [M][K] (f32 or bf16, row stride ldy >= K elements) that codes and
+ * scales in the layout of FRX_FP4_ROWS stand for: code * 2^(b - 127), exact in
+ * either type (an infinity where it passes the type's largest number). Any
+ * K >= 1; otherwise as frx_fp4_quantize. */
+frx_status frx_fp4_dequantize(frx_ctx *ctx, const uint8_t *q, size_t ldq, const uint8_t *scale, uint32_t M, uint32_t K,
+                              void *y, frx_dtype yt, size_t ldy);
+
+/* y[m][n] = sum_b 2^(sa[m][b] + sb[n][b] - 254) * sum_{k in block b} a[m][k] * b[n][k]
+ *   a [M][lda bytes], sa [M][sk]; b [N][ldb bytes], sb [N][sk]; y [M][N] yt. The
+ *   three products of a layer:
+ *     y  = x w^T:   a = x ROWS,    b = w ROWS
+ *     dx = dy w:    a = dy ROWS,   b = w COLS  (M x N times N x K)
+ *     dw = dy^T x:  a = dy COLS,   b = x COLS  (sums over the tokens, rounded up to
+ *                                  32: the quantiser's zero codes)
+ * A block's sum is exact; blocks are added in fp32, one rounding to yt at the end.
+ * What the scales' bytes past ceil(K / 32) hold does not matter.
+ * Requires K % 32 == 0, lda and ldb multiples of 16, >= K / 2 and <= 2^22, a and b
+ * 16-byte aligned, scales 4-byte, M, N >= 1, N < 2^27, (M / 64 + 65) * ceil(N / 128) <
+ * 2^24; y aligned to its element. Where there are few tiles, K is split over
+ * workgroups: fp32 parts in a context workspace (allocated on the first call at a
+ * larger size; a call under graph capture that would have to allocate runs
+ * unsplit), added in order. */
+frx_status frx_fp4_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
+                          const uint8_t *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
+
+/* y = x w^T for activations x [M][K] (f32 or bf16, contiguous): frx_fp4_quantize
+ * (ROWS) and frx_fp4_linear in one call, with the two calls' result bit for bit.
+ * Where M <= 4 and M * (K / 2 + 4 * ceil(K / 128)) <= 65536 it is one launch, the
+ * codes in LDS; else they lie in a context workspace (which must be there before a
+ * graph capture: FRX_ERR_UNSUPPORTED otherwise). K % 32 == 0. */
+frx_status frx_fp4_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
+                              const uint8_t *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
+
+/* The product over rows sorted by expert (frx_moe_sort): row r of a, of expert
+ * e where offsets[e] <= r < offsets[e + 1], times the codes b[e].
+ *   a [R][lda], sa [R][sk]; b[e] [N][ldb], sb[e] [N][sk] (host arrays of E device
+ *   pointers); offsets [E + 1] u32 on the device, ascending; y [R][N]. Rows from
+ *   offsets[E] on are neither read nor written. 1 <= E <= 64; otherwise as
+ *   frx_fp4_linear. No allocation. frx_moe_dispatch moves codes (rows of
+ *   ceil(K / 32) * 16 bytes) and scales (rows of sk bytes) alike.
+ * The groups' lengths lie on the device, so R stands for them: a caller that
+ * knows a bound on the rows in use passes that as R, not the room there is. */
+frx_status frx_fp4_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint8_t *sa,
+                                  const uint8_t *const *b, size_t ldb, const uint8_t *const *sb,
+                                  const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R, uint32_t K,
+                                  uint32_t N);
+
+/* An expert layer for a few tokens, whose experts' weights are codes and scales in
+ * the layout of FRX_FP4_ROWS:
+ *   y[t] = sum_j topk_w[t][j] * down_e(act(gate_e x_t) * up_e x_t),  e = topk_idx[t][j]
+ *   x [T][H] xt; w_gate[e], w_up[e] [I][H / 2], s_gate[e], s_up[e] [I][4 * ceil(H / 128)];
+ *   w_down[e] [H][I / 2], s_down[e] [H][4 * ceil(I / 128)] (contiguous; host arrays of E
+ *   device pointers); y [T][H] yt; act: FRX_ACT_SILU or FRX_ACT_GELU_TANH.
+ * The activations stay as they are, neither x nor the intermediate becomes codes:
+ * products with the weights' values are exact, sums are fp32; the intermediate, times
+ * its route's weight, is kept to 2^-17 of itself for a bf16 y and whole for an f32
+ * one. (frx_fp4_linear_grouped quantises, for many tokens, where the products bound.)
+ * Routes:
+ *   router [E][H] rt: the top_k experts of the largest logits x router^T (fp32 sums),
+ *     ties to the lowest index, a NaN below every number, in that order; weights are the
+ *     softmax over the chosen logits. topk_idx [T][top_k] and topk_w [T][top_k] f32
+ *     receive them (either may be NULL). top_k <= E.
+ *   router NULL: topk_idx and topk_w are read. An index >= E goes nowhere (a padding
+ *     token, a dropped route); a token without routes gets zeros; an index may occur
+ *     twice in a token.
+ * A token of x with an infinity or a NaN gives values of its own that are not finite,
+ * and no other token's.
+ * 1 <= T <= 64 (FRX_ERR_UNSUPPORTED above), H % 32 == 0, I % 32 == 0, up to 2^23,
+ * 1 <= E <= 64, 1 <= top_k <= 64; codes 16-byte aligned, scales 4-byte, the others to
+ * their elements. Works in a context workspace (allocated on the first call at a larger
+ * size, which must not be under graph capture: FRX_ERR_UNSUPPORTED). Calls and graphs
+ * of one context that run at the same time share it and must be serialised. */
+frx_status frx_fp4_moe_ffn(frx_ctx *ctx, const void *x, frx_dtype xt, const void *router, frx_dtype rt,
+                           const uint8_t *const *w_gate, const uint8_t *const *s_gate, const uint8_t *const *w_up,
+                           const uint8_t *const *s_up, const uint8_t *const *w_down, const uint8_t *const *s_down,
+                           uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32_t top_k, frx_activation act, void *y,
+                           frx_dtype yt, uint32_t *topk_idx, float *topk_w);
+
 /* ---- tokens sorted by expert, and back ----------------------------------------
  * What frx_moe_ternary_ffn does inside around its ternary experts, for callers
  * with experts of another kind, and its gradients. A route is a pair (token t,
