@@ -1873,8 +1873,9 @@ frx_status frx_fp4_moe_ffn(frx_ctx *ctx, const void *x, frx_dtype xt, const void
       p.w[k][e] = w[2 * k][e];
       p.s[k][e] = w[2 * k + 1][e];
     }
-  const size_t h = a256(frx::fp4_moe_bytes(T, I, top_k, yt == FRX_BF16)), routes = a256((size_t)T * top_k * 4);
-  const size_t need = h + (router ? 2 * routes : 0);
+  const size_t h = a256(frx::fp4_moe_h_bytes(T, I, top_k, yt == FRX_BF16));
+  const size_t part = a256(frx::fp4_moe_part_bytes(T, H, I, E, top_k, yt == FRX_BF16));
+  const size_t routes = a256((size_t)T * top_k * 4), need = h + part + (router ? 2 * routes : 0);
   if (!may_grow(ctx, ctx->few_ws_bytes, need))
     return fail(ctx, FRX_ERR_UNSUPPORTED, "the first call at this size allocates and cannot be captured into a graph");
   if ((st = ensure_buffer(ctx, &ctx->few_ws, &ctx->few_ws_bytes, need, "expert layer workspace allocation")) != FRX_OK)
@@ -1884,8 +1885,9 @@ frx_status frx_fp4_moe_ffn(frx_ctx *ctx, const void *x, frx_dtype xt, const void
   p.router = router;
   p.y = y;
   p.h = reinterpret_cast<uint16_t *>(ws);
-  p.idx = topk_idx ? topk_idx : reinterpret_cast<uint32_t *>(ws + h);
-  p.wts = topk_w ? topk_w : reinterpret_cast<float *>(ws + h + routes);
+  p.part = reinterpret_cast<float *>(ws + h);
+  p.idx = topk_idx ? topk_idx : reinterpret_cast<uint32_t *>(ws + h + part);
+  p.wts = topk_w ? topk_w : reinterpret_cast<float *>(ws + h + part + routes);
   p.T = T;
   p.H = H;
   p.I = I;

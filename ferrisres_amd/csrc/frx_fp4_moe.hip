@@ -8,13 +8,19 @@
 // an f32 x as three bf16 planes that add up to it exactly; sums in fp32.
 //
 //   route     the router's logits, top-k and softmax, where the caller has none
-//   gate, up  a workgroup per 16 inner columns of an expert: the expert's tokens are
-//             gathered 16 at a time; h times the route's weight as bf16 planes, a row for
-//             each route
-//   down      a workgroup per 16 outputs adds up all experts: tokens are the matrix
-//             instruction's columns and an expert's column is its route's row of h, or
-//             zeros for a token that it does not serve. So no sum leaves the workgroup and
-//             no atomics decide an order.
+//   gate, up  h = act(g) * u times the route's weight, as bf16 planes, a row for each route
+//   down      a row of f32 sums for each route (and slice of I)
+//   combine   the routes of each token, in order
+//
+// gate_up and down run one workgroup of 8 waves on each compute unit, which takes an even
+// share of the row tiles of an expert in use (of a group of its tokens, where they are many: then
+// its weights are read again), one tile of 16 weight rows after the other. The
+// waves split K. A wave's slice of the expert's tokens stays in registers as long as the
+// expert does not change: columns of the matrix instruction are (token, plane) pairs, the
+// expert's tokens gathered. So a tile costs its weights' bytes, the widening, four matrix
+// instructions for 128 columns, and one exchange of the waves' sums through LDS. The weights
+// of the next tiles are on their way meanwhile, by LDS DMA into a ring that each wave has for
+// itself (held in registers they were waited for at every turn of the loop).
 #include "frx_fp4_codes.hpp"
 #include "frx_fp8.hpp"
 #include "frx_internal.hpp"
@@ -23,102 +29,276 @@ namespace frx {
 
 namespace {
 
-constexpr int WAVES = 8;
+constexpr int WAVES = 8, NT = WAVES * 64;
 
 // ---- routes ------------------------------------------------------------------------
 
-// Eight values from p on. vec: 16-byte aligned.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8]) {
-  if (vec) {
-    ld8v(p, v);
-  } else {
+constexpr int MOST_SLOTS = FP4_MOE_MAX_T * 64;
+constexpr int KEPT_SLOTS = 512;
+// Tokens up to which every workgroup of gate_up routes for itself.
+constexpr int FUSED_T = 4;
+
+// Unaligned 16 bytes (a tensor may begin at any element).
+typedef u32x4 __attribute__((aligned(2))) u32x4_u;
+
+struct FewArgs {
+  const void *x, *router;
+  uint32_t *idx;
+  float *wts;
+  uint16_t *h;  // [slot][planes][I]
+  float *part;  // [slice][slot][H]
+  uint32_t T, K, N;  // columns of a weight row, rows
+  int E, top_k, planes, act, rt_bf16, route, slices, per;  // slices of K, steps of 128 in each (down)
+  const uint8_t *w[2][FP8_MAXE], *s[2][FP8_MAXE];          // gate, up; or down
+};
+
+struct Shared {
+  const uint8_t *w[2][FP8_MAXE], *s[2][FP8_MAXE];
+  float logit[FUSED_T][64];
+  uint8_t expert[MOST_SLOTS];  // of each slot; 255: none
+  int count[FP8_MAXE];         // the expert's routes
+  float wts[KEPT_SLOTS];       // of each slot, where there are few
+  float share[64];             // of the expert at hand: its tokens' weights, added where a token names it twice,
+  uint16_t slot[64];           // their slots,
+  uint8_t token[64];           // and which they are
+};
+
+// Eight values from p on.
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4_u *>(p), b = *reinterpret_cast<const u32x4_u *>(p + 4);
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = ld1(p + i);
+  for (int i = 0; i < 4; i++) {
+    v[i] = __uint_as_float(a[i]);
+    v[4 + i] = __uint_as_float(b[i]);
+  }
+}
+__device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4_u *>(p);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[2 * i] = __uint_as_float(a[i] << 16);
+    v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
   }
 }
 
-// A workgroup of 4 waves per token. The experts of the largest logits, ties to the lowest
-// index, a NaN below every number; weights exp(l - l_max) over their sum.
-template <typename XT, typename RT>
-__global__ __launch_bounds__(256) void fp4_route_kernel(const XT *__restrict__ x, const RT *__restrict__ router,
-                                                        uint32_t H, int E, int top_k, uint32_t *__restrict__ idx,
-                                                        float *__restrict__ wts, int xvec, int rvec) {
-  __shared__ float logit[64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const XT *row = x + (size_t)blockIdx.x * H;
-  for (int e = wave; e < E; e += 4) {
-    float s = 0.f;
+// Logits of up to TM tokens from x on: a wave for each expert.
+template <int TM, typename XT, typename RT>
+__device__ __forceinline__ void router_logits(const XT *x, const RT *router, int T, uint32_t H, int E,
+                                              float (*logit)[64]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int e = wave; e < E; e += WAVES) {
+    float s[TM] = {};
+#pragma unroll 4
     for (uint32_t k = lane * 8; k < H; k += 512) {
-      float a[8], b[8];
-      load8(row + k, xvec, a);
-      load8(router + (size_t)e * H + k, rvec, b);
+      float r[8];
+      load8(router + (size_t)e * H + k, r);
 #pragma unroll
-      for (int i = 0; i < 8; i++) s = __builtin_fmaf(a[i], b[i], s);
+      for (int t = 0; t < TM; t++) {
+        float v[8];
+        load8(x + (size_t)min(t, T - 1) * H + k, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) s[t] = __builtin_fmaf(v[i], r[i], s[t]);
+      }
     }
 #pragma unroll
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-    if (lane == 0) logit[e] = s;
+    for (int t = 0; t < TM; t++) {
+#pragma unroll
+      for (int o = 32; o; o >>= 1) s[t] += __shfl_xor(s[t], o);
+      if (lane == 0 && t < T) logit[t][e] = s[t];
+    }
   }
-  __syncthreads();
-  if (wave) return;
+}
+
+// A wave: the experts of the largest logits, ties to the lowest index, a NaN below every
+// number; weights exp(l - l_max) over their sum. Lane e returns its expert's place among
+// them (top_k and more: none) and weight.
+__device__ __forceinline__ int top_experts(const float *logit, int E, int top_k, float &weight) {
+  const int lane = threadIdx.x & 63;
   const float mine = lane < E ? logit[lane] + 0.0f : 0.f;  // -0 orders as 0
   const uint32_t bits = __float_as_uint(mine);
-  uint64_t key = mine != mine ? 0 : bits >> 31 ? ~bits : bits | 0x80000000u;
-  key = lane < E ? ((key + 1) << 6) | (63 - lane) : 0;
-  float top = 0.f, sum = 0.f, w = 0.f;
-  int place = -1;
-  for (int j = 0; j < top_k; j++) {
-    uint64_t best = key;
+  const uint32_t key = mine != mine ? 0 : bits >> 31 ? ~bits : bits | 0x80000000u;
+  int rank = 0;  // experts ahead of this one
+  for (int i = 0; i < E; i++) {
+    const uint32_t other = (uint32_t)__builtin_amdgcn_readlane((int)key, i);
+    rank += other > key || (other == key && i < lane);
+  }
+  if (lane >= E) rank = 64;
+  const int first = __ffsll((unsigned long long)__ballot(rank == 0)) - 1;
+  const float top = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)bits, first));
+  float w = rank < top_k ? expf(mine - top) : 0.f, sum = w;
 #pragma unroll
-    for (int o = 32; o; o >>= 1) best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, o));
-    const int e = 63 - (int)(best & 63);
-    const float l = __shfl(mine, e);
-    if (j == 0) top = l;
-    const float p = expf(l - top);
-    sum += p;
-    if (lane == e) {
-      key = 0;
-      w = p;
-      place = j;
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  weight = w / sum;
+  return rank;
+}
+
+// A workgroup per token.
+template <typename XT, typename RT>
+__global__ __launch_bounds__(NT) void fp4_route_kernel(const XT *__restrict__ x, const RT *__restrict__ router,
+                                                       uint32_t H, int E, int top_k, uint32_t *__restrict__ idx,
+                                                       float *__restrict__ wts) {
+  __shared__ float logit[1][64];
+  const size_t t = blockIdx.x;
+  router_logits<1>(x + t * H, router, 1, H, E, logit);
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  float w;
+  const int place = top_experts(logit[0], E, top_k, w);
+  if (place < top_k) {
+    idx[t * top_k + place] = threadIdx.x;
+    wts[t * top_k + place] = w;
+  }
+}
+
+// Fills the experts' addresses and the routes. ROUTE: by
+// the router where the launch says so, workgroup 0 writing the routes for the launches behind.
+template <typename XT, bool ROUTE>
+__device__ __forceinline__ void read_routes(const FewArgs &p, Shared &sh) {
+  const int slots = (int)p.T * p.top_k, lane = threadIdx.x & 63;
+  if (threadIdx.x < 2 * FP8_MAXE) {  // (addressed by lane: one wait, beside the routes')
+    const int k = threadIdx.x >> 6;
+    sh.w[k][lane] = p.w[k][lane];
+    sh.s[k][lane] = p.s[k][lane];
+  }
+  if (threadIdx.x < FP8_MAXE) sh.count[threadIdx.x] = 0;
+  __syncthreads();
+  if (ROUTE && p.route) {
+    const XT *x = static_cast<const XT *>(p.x);
+    if (p.T == 1) {
+      if (p.rt_bf16) router_logits<1>(x, static_cast<const uint16_t *>(p.router), 1, p.K, p.E, sh.logit);
+      else router_logits<1>(x, static_cast<const float *>(p.router), 1, p.K, p.E, sh.logit);
+    } else {
+      if (p.rt_bf16) router_logits<FUSED_T>(x, static_cast<const uint16_t *>(p.router), (int)p.T, p.K, p.E, sh.logit);
+      else router_logits<FUSED_T>(x, static_cast<const float *>(p.router), (int)p.T, p.K, p.E, sh.logit);
+    }
+    __syncthreads();
+    const int t = threadIdx.x >> 6;
+    if (t < (int)p.T) {
+      float w;
+      const int place = top_experts(sh.logit[t], p.E, p.top_k, w), s = t * p.top_k + place;
+      if (place < p.top_k) {
+        sh.expert[s] = lane;
+        atomicAdd(&sh.count[lane], 1);
+        sh.wts[s] = w;
+        if (blockIdx.x == 0) {
+          p.idx[s] = lane;
+          p.wts[s] = w;
+        }
+      }
+    }
+  } else {
+    for (int s = threadIdx.x; s < slots; s += NT) {
+      const uint32_t e = p.idx[s];
+      if (s < KEPT_SLOTS) sh.wts[s] = p.wts[s];
+      sh.expert[s] = e < (uint32_t)p.E ? e : 255;
+      if (e < (uint32_t)p.E) atomicAdd(&sh.count[e], 1);
     }
   }
-  if (place >= 0) {
-    idx[(size_t)blockIdx.x * top_k + place] = lane;
-    wts[(size_t)blockIdx.x * top_k + place] = w / sum;
-  }
+  __syncthreads();
 }
 
-// The experts that any route goes to, as bits; every thread of the workgroup gets them.
-__device__ __forceinline__ uint64_t active_experts(const uint32_t *idx, int slots, int E, uint32_t (&word)[2]) {
-  if (threadIdx.x < 2) word[threadIdx.x] = 0;
-  __syncthreads();
-  for (int s = threadIdx.x; s < slots; s += blockDim.x) {
-    const uint32_t e = idx[s];
-    if (e < (uint32_t)E) atomicOr(&word[e >> 5], 1u << (e & 31));
+// The experts in use, each as often as `tokens` of its routes at a time take: lane e has
+// expert e's.
+struct Groups {
+  uint64_t active;
+  int groups, upto, total;
+  __device__ __forceinline__ Groups(const Shared &sh, int E, int tokens) {
+    const int lane = threadIdx.x & 63, n = lane < E ? sh.count[lane] : 0;
+    active = __ballot(n > 0);
+    groups = upto = n > 0;
+    if (__ballot(n > tokens) == 0) {
+      total = __popcll(active);
+    } else {
+      groups = 0;
+      for (int left = n; left > 0; left -= tokens) groups++;
+      upto = groups;
+      for (int s = 1; s < 64; s <<= 1) {
+        const int v = __shfl_up(upto, s);
+        if (lane >= s) upto += v;
+      }
+      total = __builtin_amdgcn_readlane(upto, 63);
+    }
   }
-  __syncthreads();
-  return word[0] | ((uint64_t)word[1] << 32);
+  // Group u's expert, and which of that expert's groups it is.
+  __device__ __forceinline__ int find(int u, int &which) const {
+    which = 0;
+    if (total == __popcll(active)) {  // one of each
+      uint64_t m = active;
+      for (int i = 0; i < u; i++) m &= m - 1;
+      return __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)m) - 1);
+    }
+    const int e = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(upto > u)) - 1);
+    which = u - __builtin_amdgcn_readlane(upto - groups, e);
+    return e;
+  }
+};
+
+// a / b for numbers below 2^22.
+__device__ __forceinline__ int div22(int a, int b) {
+  const int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));  // one off at most
+  const int r = a - q * b;
+  return r < 0 ? q - 1 : r >= b ? q + 1 : q;
 }
 
-// The a-th set bit's place.
-__device__ __forceinline__ int nth_bit(uint64_t m, int a) {
-  for (int i = 0; i < a; i++) m &= m - 1;
-  return __ffsll((unsigned long long)m) - 1;
+// Which of `units` (an expert, or a slice of one, with `tiles` row tiles) this workgroup works on, and
+// on which tiles: units share the workgroups evenly, so that one belongs to no two of them; where
+// there are more units than workgroups, whole units in turn.
+struct Share {
+  int unit, step, first, last;
+  __device__ __forceinline__ Share(int units, int tiles) {
+    const int b = blockIdx.x, G = gridDim.x;
+    if (units == 0) {  // nothing is routed
+      unit = first = last = 0;
+      step = 1;
+    } else if (units <= G) {
+      unit = div22(b * units + units - 1, G);  // of b in [u G / units, (u + 1) G / units)
+      const int lo = div22(unit * G, units), n = div22((unit + 1) * G, units) - lo, i = b - lo;
+      const int q = div22(tiles, n), r = tiles - q * n;
+      first = q * i + min(i, r);
+      last = first + q + (i < r);
+      step = units;
+    } else {
+      unit = b;
+      step = G;
+      first = 0;
+      last = tiles;
+    }
+  }
+};
+
+// Expert e's tokens into slot[] (and share[] where WEIGHTS): the first slot of each that
+// names it. Every wave finds them; wave 0 writes. Returns their number. The caller puts
+// barriers before (nobody reads the lists any more) and behind.
+template <bool WEIGHTS>
+__device__ __forceinline__ int list_tokens(const FewArgs &p, Shared &sh, int e) {
+  const int lane = threadIdx.x & 63;
+  const auto weight = [&](int s) { return s < KEPT_SLOTS ? sh.wts[s] : p.wts[s]; };
+  int first = -1;
+  float w = 0.f;
+  if (lane < (int)p.T)
+    for (int j = 0; j < p.top_k; j++)
+      if (sh.expert[lane * p.top_k + j] == e) {
+        if (first < 0) first = lane * p.top_k + j;
+        if (WEIGHTS && threadIdx.x < 64) w += weight(lane * p.top_k + j);
+      }
+  const uint64_t mine = __ballot(first >= 0);
+  if (threadIdx.x < 64 && first >= 0) {
+    const int at = __popcll(mine & ((1ull << lane) - 1));
+    sh.slot[at] = (uint16_t)first;
+    sh.token[at] = (uint8_t)lane;
+    if (WEIGHTS) sh.share[at] = w;
+  }
+  return __popcll(mine);
 }
 
 // ---- operands ----------------------------------------------------------------------
 
-// The 32 codes of a lane times 2^(b - 127) as bf16, 8 to an operand.
-__device__ __forceinline__ void widen(const u32x4 &c, uint32_t b, u32x4 (&w)[4]) {
-  const float s = fp4_power(b);
-#pragma unroll
-  for (int q = 0; q < 4; q++) {
-    w[q].x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], s, 0));
-    w[q].y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], s, 1));
-    w[q].z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], s, 2));
-    w[q].w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c[q], s, 3));
-  }
+// Eight codes times 2^(b - 127) as bf16; s = fp4_power(b).
+__device__ __forceinline__ u32x4 widen8(uint32_t c, float s) {
+  return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
 }
 
 // A value as bf16 planes of which each holds the next 8 bits: three add up to it.
@@ -127,233 +307,361 @@ __device__ __forceinline__ float cut8(float v, uint32_t &plane) {
   return v - __uint_as_float(plane);
 }
 
-// Eight activations as P operands.
-template <typename XT, int P>
-__device__ __forceinline__ void act8(const XT *p, bool vec, u32x4 (&o)[P]) {
-  if constexpr (sizeof(XT) == 2) {
-    if (vec) {
-      o[0] = *reinterpret_cast<const u32x4 *>(p);
-    } else {
+// Plane `plane` of eight activations.
+__device__ __forceinline__ u32x4 act8(const uint16_t *p, int) { return *reinterpret_cast<const u32x4_u *>(p); }
+__device__ __forceinline__ u32x4 act8(const float *p, int plane) {
+  float v[8];
+  load8(p, v);
+  uint32_t h[8];
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[0][i] = p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+  for (int i = 0; i < 8; i++) {
+    float left = v[i];
+    for (int j = 0; j < 2; j++) {
+      uint32_t u;
+      const float next = cut8(left, u);
+      left = j < plane ? next : left;
     }
-  } else {
-    float v[8];
-    load8(p, vec, v);
+    h[i] = __float_as_uint(left);
+  }
+  u32x4 o;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float a = v[2 * i], b = v[2 * i + 1];
+  for (int i = 0; i < 4; i++) o[i] = (h[2 * i] >> 16) | (h[2 * i + 1] & 0xFFFF0000u);
+  return o;
+}
+
+// An address that is the same in every lane.
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+  const uint64_t v = reinterpret_cast<uintptr_t>(p);
+  return reinterpret_cast<const uint8_t *>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                                           (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// What a wave reads of a tile of 16 rows, STEPS of 128 columns from step kb on: lane (row l16,
+// group g) block 4 kb + g of its row, 16 bytes at lane * 16 in LDS, and the scales of 4 blocks
+// as a dword, lane (row, step). Blocks from `blocks` on repeat the last one; they count under
+// the scale 2^-127 and meet zeros of x.
+template <int STEPS>
+struct Place {
+  static constexpr int DWORDS = STEPS * 256 + (STEPS + 3) / 4 * 64, LOADS = STEPS + (STEPS + 3) / 4;
+  uint32_t c[STEPS], s[(STEPS + 3) / 4];
+  int inside;  // of the lane's blocks so many are the row's
+  __device__ __forceinline__ void set(int K, int kb, int blocks, int l16, int g) {
+    const int kbs = (K + 127) >> 7;
 #pragma unroll
-      for (int j = 0; j < P; j++) {
-        uint32_t u, w;
-        a = cut8(a, u);
-        b = cut8(b, w);
-        o[j][i] = (u >> 16) | w;
-      }
+    for (int i = 0; i < STEPS; i++) c[i] = (uint32_t)(l16 * (K / 2) + 16 * min((kb + i) * 4 + g, blocks - 1));
+#pragma unroll
+    for (int i = 0; i < (STEPS + 3) / 4; i++) s[i] = (uint32_t)(l16 * kbs + min(kb + 4 * i + g, kbs - 1)) * 4;
+    inside = max(0, (blocks - kb * 4 - g + 3) >> 2);
+  }
+  // codes, scales: of the tile's first row
+  __device__ __forceinline__ void load(uint32_t *to, const uint8_t *codes, const uint8_t *scales, int K) const {
+    const __amdgpu_buffer_rsrc_t rc = buffer_rsrc(codes, 16u * (uint32_t)(K / 2)), rs = buffer_rsrc(scales, 16u * fp4_scale_bytes(K));
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) lds_load16(rc, to + i * 256, c[i], 0);
+#pragma unroll
+    for (int i = 0; i < (STEPS + 3) / 4; i++) lds_load4(rs, to + STEPS * 256 + i * 64, s[i], 0);
+  }
+};
+
+// from: a wave's piece of a tile, loaded as above; inside: of the lane's blocks so many count.
+template <int STEPS, int CT>
+__device__ __forceinline__ void multiply(f32x4 (&acc)[CT], const uint32_t *from, const u32x4 (&x)[STEPS][4][CT],
+                                         int inside, int cols) {
+  const int lane = threadIdx.x & 63;
+  const uint8_t *scales = reinterpret_cast<const uint8_t *>(from + STEPS * 256) + (lane & 15) * 4 + (lane >> 4);
+#pragma unroll
+  for (int i = 0; i < STEPS; i++) {
+    const u32x4 c = *reinterpret_cast<const u32x4 *>(from + i * 256 + lane * 4);
+    const float s = fp4_power(i < inside ? scales[i * 64] : 0);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const u32x4 v = widen8(c[q], s);
+#pragma unroll
+      for (int t = 0; t < CT; t++)
+        if (CT == 1 || 16 * t < cols) acc[t] = mfma16(v, x[i][q][t], acc[t]);
     }
   }
+}
+
+__device__ __forceinline__ float activate(float g, int act) {
+  if (act == 0) return g / (1.0f + expf(-g));
+  return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
 }
 
 // ---- gate and up -------------------------------------------------------------------
 
-template <int ACT>
-__device__ __forceinline__ float activate(float g) {
-  if constexpr (ACT == 0) {
-    return g / (1.0f + expf(-g));
-  } else {
-    return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
-  }
+// A barrier that waits for this wave's LDS accesses alone: __syncthreads() would wait for the
+// weights on their way too.
+__device__ __forceinline__ void barrier_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
-struct FewArgs {
-  const void *x;
-  const uint32_t *idx;
-  const float *wts;
-  uint16_t *h;
-  void *y;
-  uint32_t T, H, I;
-  int E, top_k, vec;
-  const uint8_t *w[2][FP8_MAXE], *s[2][FP8_MAXE];  // gate, up; or down
-};
+// The waves' sums in LDS, floats: 16 x 16 of a column tile as 4 groups of 4 rows, 80 apart, [column]
+// [row of 4] in each: a group's banks are 16 from the next one's.
+constexpr int RED = 320;
+__device__ __forceinline__ void put_sums(float *red, const f32x4 &v) {
+  const int lane = threadIdx.x & 63;
+  *reinterpret_cast<f32x4 *>(red + (lane >> 4) * 80 + (lane & 15) * 4) = v;
+}
+// Sum of a token's planes over the waves, STRIDE apart, for row r of the tile, in order.
+template <int P, int STRIDE>
+__device__ __forceinline__ float waves_sum(const float *red, int token, int r) {
+  float v = 0.f;
+#pragma unroll
+  for (int j = 0; j < P; j++) {
+    const int col = token * P + j;
+    const float *at = red + (col >> 4) * RED + (r >> 2) * 80 + (col & 15) * 4 + (r & 3);
+#pragma unroll 8
+    for (int w = 0; w < WAVES; w++) v += at[w * STRIDE];
+  }
+  return v;
+}
 
-// P: planes of x; HP: planes of h.
-template <typename XT, int HP, int ACT>
-__global__ __launch_bounds__(WAVES * 64) void fp4_gate_up_kernel(const FewArgs p) {
-  constexpr int P = sizeof(XT) == 2 ? 1 : 3;
-  __shared__ uint32_t word[2];
-  __shared__ uint32_t tok[64], slot[64];
-  __shared__ float share[64];
-  __shared__ f32x4 red[WAVES][2][64];
-  const uint64_t active = active_experts(p.idx, (int)p.T * p.top_k, p.E, word);
-  if ((int)blockIdx.y >= __popcll(active)) return;
-  const int e = __builtin_amdgcn_readfirstlane(nth_bit(active, blockIdx.y));
+// CT column tiles of 16 (token, plane) pairs at a time; D pieces of weights (a tile of gate, the
+// same of up, the next tile of gate ...) on their way; RB buffers for the waves' sums, with one
+// a second barrier guards it. CHUNKED: K is longer than the waves hold and goes by chunks, x
+// loaded anew for each.
+template <typename XT, int STEPS, int CT, int D, int RB, bool CHUNKED>
+__global__ __launch_bounds__(NT) void fp4_gate_up_kernel(const FewArgs p) {
+  constexpr int P = sizeof(XT) == 2 ? 1 : 3, TOKENS = 16 * CT / P, DW = Place<STEPS>::DWORDS;
+  extern __shared__ __align__(16) uint32_t lds[];
+  __shared__ Shared sh;
+  read_routes<XT, true>(p, sh);
+  const Groups groups(sh, p.E, TOKENS);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  // the expert's tokens, a route taken twice as one of both weights
-  int first = -1;
-  float w = 0.f;
-  if (lane < (int)p.T)
-    for (int j = 0; j < p.top_k; j++)
-      if (p.idx[lane * p.top_k + j] == (uint32_t)e) {
-        if (first < 0) first = j;
-        w += p.wts[lane * p.top_k + j];
-      }
-  const uint64_t mine = __ballot(first >= 0);
-  const int n = __popcll(mine);
-  if (wave == 0 && first >= 0) {
-    const int at = __popcll(mine & ((1ull << lane) - 1));
-    tok[at] = lane;
-    slot[at] = lane * p.top_k + first;
-    share[at] = w;
-  }
-  __syncthreads();
-  const int K = (int)p.H, kbs = (K + 127) >> 7, per = (kbs + WAVES - 1) / WAVES;
-  const int kb0 = min(wave * per, kbs), kb1 = min(kb0 + per, kbs);
-  const uint32_t n0 = blockIdx.x * 16;
-  const size_t row = min(n0 + l16, p.I - 1);
-  const uint8_t *wg = p.w[0][e] + row * (K / 2), *wu = p.w[1][e] + row * (K / 2);
-  const uint8_t *sg = p.s[0][e] + row * (4 * kbs), *su = p.s[1][e] + row * (4 * kbs);
-  for (int c0 = 0; c0 < n; c0 += 16) {
-    const XT *x = static_cast<const XT *>(p.x) + (size_t)tok[min(c0 + l16, n - 1)] * K;
-    f32x4 ag = {0.f, 0.f, 0.f, 0.f}, au = ag;
-    for (int kb = kb0; kb < kb1; kb++) {
-      const int blk = min(kb * 4 + g, K / 32 - 1);
-      const bool inside = kb * 4 + g < K / 32;
-      const u32x4 cg = *reinterpret_cast<const u32x4 *>(wg + 16 * blk), cu = *reinterpret_cast<const u32x4 *>(wu + 16 * blk);
-      u32x4 vg[4], vu[4];
-      widen(cg, inside ? sg[blk] : 0, vg);
-      widen(cu, inside ? su[blk] : 0, vu);
+  const int K = (int)p.K, blocks = K / 32, kbs = (K + 127) >> 7, tiles = (int)p.N / 16;
+  const int chunks = CHUNKED ? (kbs + WAVES * STEPS - 1) / (WAVES * STEPS) : 1;
+  const Share share(groups.total, tiles);
+  const int t0 = share.first, count = share.last - t0;
+  Place<STEPS> place;
+  place.set(K, wave * STEPS, blocks, l16, g);
+  uint32_t *ring = lds + wave * (D * DW);
+  float *reds = reinterpret_cast<float *>(lds + WAVES * D * DW);
+  int phase = 0;
+  if (count == 0) return;
+  for (int u = share.unit; u < groups.total; u += share.step) {
+    int which;
+    const int e = groups.find(u, which);
+    const uint8_t *wg = uniform(sh.w[0][e]), *wu = uniform(sh.w[1][e]), *sg = uniform(sh.s[0][e]), *su = uniform(sh.s[1][e]);
+    const int pieces = 2 * count * chunks;
+    // piece j: matrix j % 2, step j / 2 (past the last one it is loaded again: the waits go by the number of loads)
+    const auto load_w = [&](int j, int d) {
+      j = j < pieces ? j : pieces - 2 + (j & 1);
+      const int i = CHUNKED ? (j >> 1) / chunks : j >> 1;
+      if (CHUNKED) place.set(K, ((j >> 1) - i * chunks) * WAVES * STEPS + wave * STEPS, blocks, l16, g);
+      const size_t c = (size_t)(t0 + i) * 16 * (K / 2), s = (size_t)(t0 + i) * 16 * (4 * kbs);
+      place.load(ring + d * DW, (j & 1 ? wu : wg) + c, (j & 1 ? su : sg) + s, K);
+    };
+    // the first pieces, then x, which arrives behind them, then the others
+    constexpr int EARLY = CHUNKED ? D : 2;
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
-        u32x4 v[P];
-        act8<XT, P>(x + 32 * blk + 8 * q, p.vec, v);
+    for (int d = 0; d < EARLY; d++) load_w(d, d);
+    barrier_lds();
+    const int n = list_tokens<true>(p, sh, e);
+    barrier_lds();
+    const int c0 = which * TOKENS, cols = min(n - c0, TOKENS) * P;
+    if (cols > 0) {  // (a token may name an expert twice)
+      u32x4 x[STEPS][4][CT];
+      int inside = 0;
+      const auto load_x = [&](int kb0) {
 #pragma unroll
-        for (int j = 0; j < P; j++) {
-          if (!inside) v[j] = (u32x4){0, 0, 0, 0};
-          ag = mfma16(vg[q], v[j], ag);
-          au = mfma16(vu[q], v[j], au);
-        }
-      }
-    }
-    red[wave][0][lane] = ag;
-    red[wave][1][lane] = au;
-    __syncthreads();
-    if (wave == 0) {
+        for (int t = 0; t < CT; t++) {
+          const int col = 16 * t + l16, tok = sh.token[c0 + min(col, cols - 1) / P];
+          const XT *from = static_cast<const XT *>(p.x);
 #pragma unroll
-      for (int i = 1; i < WAVES; i++) {
-        ag += red[i][0][lane];
-        au += red[i][1][lane];
-      }
-      const uint32_t i0 = n0 + 4 * g;
-      if (c0 + l16 < n && i0 < p.I) {  // I % 32 == 0: whole quads
-        const float sh = share[c0 + l16];
-        uint32_t plane[HP][4];
+          for (int i = 0; i < STEPS; i++) {
+            const int b = (kb0 + i) * 4 + g;
+            const bool use = b < blocks && col < cols;
+            const uint32_t o = (uint32_t)tok * K + 32 * min(b, blocks - 1);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float v = activate<ACT>(ag[i]) * au[i] * sh;
-          if constexpr (HP == 2) {
-            plane[0][i] = bf16_rne_nb(v);
-            plane[1][i] = bf16_rne_nb(v - __uint_as_float(plane[0][i] << 16));
-          } else {
-#pragma unroll
-            for (int j = 0; j < HP; j++) {
-              uint32_t u;
-              v = cut8(v, u);
-              plane[j][i] = u >> 16;
+            for (int q = 0; q < 4; q++) {
+              x[i][q][t] = act8(from + (o + 8 * q), col % P);
+              if (!use) x[i][q][t] = (u32x4){0, 0, 0, 0};
             }
+            if (sizeof(XT) == 4 && (CT * STEPS > 4) && (i & 1)) __builtin_amdgcn_sched_barrier(0);  // (two values a register: not all at once)
           }
         }
-        uint16_t *d = p.h + (size_t)slot[c0 + l16] * HP * p.I + i0;
+        inside = max(0, (blocks - kb0 * 4 - g + 3) >> 2);
+      };
+      if (!CHUNKED) {
+        __builtin_amdgcn_sched_barrier(0);
+        load_x(wave * STEPS);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < HP; j++)
-          *reinterpret_cast<u32x2 *>(d + (size_t)j * p.I) =
-              (u32x2){plane[j][0] | (plane[j][1] << 16), plane[j][2] | (plane[j][3] << 16)};
+        for (int d = EARLY; d < D; d++) load_w(d, d);
+      }
+      f32x4 acc[2][CT];
+      int chunk = 0, tile = t0, d = 0;
+      for (int j = 0; j < pieces; j += 2) {
+        if (CHUNKED) load_x(chunk * WAVES * STEPS + wave * STEPS);
+        if (!CHUNKED || chunk == 0)
+#pragma unroll
+          for (int t = 0; t < CT; t++) acc[0][t] = acc[1][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          wait_vmcnt<(D - 1) * Place<STEPS>::LOADS>();
+          __builtin_amdgcn_sched_barrier(0);
+          multiply<STEPS, CT>(acc[m], ring + d * DW, x, inside, cols);
+          __builtin_amdgcn_sched_barrier(0);
+          load_w(j + m + D, d);
+          d = d + 1 == D ? 0 : d + 1;
+        }
+        if (CHUNKED && ++chunk < chunks) continue;
+        chunk = 0;
+        constexpr int MAT = CT * RED + 32, WAVE = 2 * MAT;  // [wave][matrix][column tile]
+        float *red = reds + phase * (WAVES * WAVE);
+        if (RB == 2) phase ^= 1;
+        else barrier_lds();
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int t = 0; t < CT; t++)
+            if (16 * t < cols) put_sums(red + wave * WAVE + m * MAT + t * RED, acc[m][t]);
+        barrier_lds();
+        // a thread an inner column (of 16), matrix and token
+        const int r = threadIdx.x & 15, m = (threadIdx.x >> 4) & 1;
+        for (int token = threadIdx.x >> 5; token * P < cols; token += NT / 32) {
+          const float sum = waves_sum<P, WAVE>(red + m * MAT, token, r);
+          const float other = __shfl_xor(sum, 16);
+          if (m) continue;
+          const float v = activate(sum, p.act) * other * sh.share[c0 + token];
+          uint16_t *to = p.h + (size_t)sh.slot[c0 + token] * p.planes * p.N + (uint32_t)tile * 16 + r;
+          if (p.planes == 2) {
+            const uint32_t hi = bf16_rne_nb(v);
+            to[0] = (uint16_t)hi;
+            to[p.N] = (uint16_t)bf16_rne_nb(v - __uint_as_float(hi << 16));
+          } else {
+            uint32_t u;
+            float left = cut8(v, u);
+            to[0] = (uint16_t)(u >> 16);
+            left = cut8(left, u);
+            to[p.N] = (uint16_t)(u >> 16);
+            (void)cut8(left, u);
+            to[2 * (size_t)p.N] = (uint16_t)(u >> 16);
+          }
+        }
+        tile++;
       }
     }
-    __syncthreads();
+    wait_vmcnt<0>();  // nothing is in flight into the ring any more
   }
 }
 
 // ---- down --------------------------------------------------------------------------
 
-// TT: tiles of 16 tokens.
-template <int TT, int HP, typename YT>
-__global__ __launch_bounds__(WAVES * 64) void fp4_down_kernel(const FewArgs p) {
-  __shared__ uint32_t word[2];
-  __shared__ int16_t table[64 * 64];  // [active expert][token]: the route's slot; -1: none
-  __shared__ f32x4 red[WAVES][TT][64];
-  const int slots = (int)p.T * p.top_k;
-  const uint64_t active = active_experts(p.idx, slots, p.E, word);
-  const int experts = __popcll(active);
-  for (int i = threadIdx.x; i < experts * (int)p.T; i += blockDim.x) table[i] = -1;
-  __syncthreads();
-  for (int s = threadIdx.x; s < slots; s += blockDim.x) {
-    const uint32_t e = p.idx[s];
-    if (e >= (uint32_t)p.E) continue;
-    const int t = s / p.top_k;
-    bool first = true;
-    for (int k = t * p.top_k; k < s; k++) first &= p.idx[k] != e;
-    if (first) table[__popcll(active & ((1ull << e) - 1)) * p.T + t] = (int16_t)s;
-  }
-  __syncthreads();
+// A unit is a group of an expert's tokens and a slice of K; P planes of h; D tiles' weights on their way.
+template <int P, int STEPS, int CT, int D>
+__global__ __launch_bounds__(NT) void fp4_down_kernel(const FewArgs p) {
+  constexpr int TOKENS = 16 * CT / P;
+  extern __shared__ __align__(16) uint32_t lds[];
+  __shared__ Shared sh;
+  read_routes<uint16_t, false>(p, sh);
+  const Groups groups(sh, p.E, TOKENS);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int K = (int)p.I, kbs = (K + 127) >> 7, units = experts * kbs, per = (units + WAVES - 1) / WAVES;
-  const int u0 = min(wave * per, units), u1 = min(u0 + per, units);
-  const uint32_t n0 = blockIdx.x * 16;
-  const size_t row = min(n0 + l16, p.H - 1);
-  f32x4 acc[TT];
+  const int K = (int)p.K, blocks = K / 32, kbs = (K + 127) >> 7, tiles = (int)p.N / 16;
+  const int units = groups.total * p.slices, slots = (int)p.T * p.top_k;
+  const Share share(units, tiles);
+  const int t0 = share.first, count = share.last - t0;
+  constexpr int DW = Place<STEPS>::DWORDS;
+  uint32_t *ring = lds + wave * (D * DW);
+  float *reds = reinterpret_cast<float *>(lds + WAVES * D * DW);
+  int phase = 0;
+  if (count == 0) return;
+  for (int u = share.unit; u < units; u += share.step) {
+    const int group = div22(u, p.slices), slice = u - group * p.slices;
+    int which;
+    const int e = groups.find(group, which);
+    const uint8_t *wd = uniform(sh.w[0][e]), *sd = uniform(sh.s[0][e]);
+    const int kb = slice * p.per + wave * STEPS;
+    const int stop = min((slice + 1) * p.per * 4, blocks);  // the slice's blocks
+    Place<STEPS> place;
+    place.set(K, kb, stop, l16, g);
+    const auto load_w = [&](int j, int d) {
+      const size_t row = (size_t)(t0 + min(j, count - 1)) * 16;
+      place.load(ring + d * DW, wd + row * (K / 2), sd + row * (4 * kbs), K);
+    };
+    load_w(0, 0);
+    barrier_lds();
+    const int n = list_tokens<false>(p, sh, e);
+    barrier_lds();
+    const int c0 = which * TOKENS, cols = min(n - c0, TOKENS) * P;
+    if (cols > 0) {
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 x[STEPS][4][CT];
 #pragma unroll
-  for (int t = 0; t < TT; t++) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  for (int u = u0; u < u1;) {
-    const int a = u / kbs, stop = min(u1, (a + 1) * kbs);
-    const int e = __builtin_amdgcn_readfirstlane(nth_bit(active, a));
-    int slot[TT];
-    f32x4 part[TT];  // of this expert: a token that it does not serve drops it, whatever the weights are
+      for (int t = 0; t < CT; t++) {
+        const int col = 16 * t + l16, cc = min(col, cols - 1);
+        const uint16_t *row = p.h + ((size_t)sh.slot[c0 + cc / P] * P + cc % P) * K;
 #pragma unroll
-    for (int t = 0; t < TT; t++) {
-      const int tok = 16 * t + l16;
-      slot[t] = tok < (int)p.T ? table[a * p.T + tok] : -1;
-      part[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
-    for (; u < stop; u++) {
-      const int kb = u - a * kbs;
-      const int blk = min(kb * 4 + g, K / 32 - 1);
-      const bool inside = kb * 4 + g < K / 32;
-      u32x4 w[4];
-      widen(*reinterpret_cast<const u32x4 *>(p.w[0][e] + row * (K / 2) + 16 * blk),
-            inside ? p.s[0][e][row * (4 * kbs) + blk] : 0, w);
+        for (int i = 0; i < STEPS; i++) {
+          const int b = (kb + i) * 4 + g;
 #pragma unroll
-      for (int t = 0; t < TT; t++) {
-        if (__ballot(slot[t] >= 0) == 0) continue;
-        const bool here = slot[t] >= 0 && inside;
-        const uint16_t *h = p.h + (size_t)max(slot[t], 0) * HP * p.I + 32 * blk;
+          for (int q = 0; q < 4; q++)
+            x[i][q][t] = *reinterpret_cast<const u32x4 *>(row + 32 * min(b, stop - 1) + 8 * q);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < HP; j++)
+      for (int d = 1; d < D; d++) load_w(d, d);
+      wait_vmcnt<(D - 1) * Place<STEPS>::LOADS>();
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            u32x4 v = {0, 0, 0, 0};
-            if (here) v = *reinterpret_cast<const u32x4 *>(h + (size_t)j * p.I + 8 * q);
-            part[t] = mfma16(w[q], v, part[t]);
-          }
+      for (int t = 0; t < CT; t++)
+#pragma unroll
+        for (int i = 0; i < STEPS; i++)
+          if ((kb + i) * 4 + g >= stop || 16 * t + l16 >= cols)
+#pragma unroll
+            for (int q = 0; q < 4; q++) x[i][q][t] = (u32x4){0, 0, 0, 0};
+      int d = 0;
+      for (int j = 0; j < count; j++) {
+        f32x4 acc[CT];
+#pragma unroll
+        for (int t = 0; t < CT; t++) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        wait_vmcnt<(D - 1) * Place<STEPS>::LOADS>();
+        __builtin_amdgcn_sched_barrier(0);
+        multiply<STEPS, CT>(acc, ring + d * DW, x, place.inside, cols);
+        __builtin_amdgcn_sched_barrier(0);
+        load_w(j + D, d);
+        d = d + 1 == D ? 0 : d + 1;
+        float *red = reds + phase * (WAVES * CT * RED);
+        phase ^= 1;
+#pragma unroll
+        for (int t = 0; t < CT; t++)
+          if (16 * t < cols) put_sums(red + (wave * CT + t) * RED, acc[t]);
+        barrier_lds();
+        for (int token = threadIdx.x >> 4; token * P < cols; token += NT / 16) {
+          const int r = threadIdx.x & 15;
+          p.part[((size_t)slice * slots + sh.slot[c0 + token]) * p.N + (uint32_t)(t0 + j) * 16 + r] =
+              waves_sum<P, CT * RED>(red, token, r);
+        }
       }
     }
-#pragma unroll
-    for (int t = 0; t < TT; t++)
-      if (slot[t] >= 0) acc[t] += part[t];
+    wait_vmcnt<0>();  // nothing is in flight into the ring any more
   }
+}
+
+// y[t] = its routes' sums over the slices, in the order of the routes. A route that goes
+// nowhere, and a later one to an expert that the token has named, has none.
+template <typename YT>
+__global__ __launch_bounds__(256) void fp4_join_kernel(const FewArgs p, YT *__restrict__ y) {
+  const uint32_t t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
+  if (n >= p.N) return;
+  const uint32_t *idx = p.idx + t * p.top_k;
+  const size_t slots = (size_t)p.T * p.top_k;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < p.top_k; j++) {
+    bool use = idx[j] < (uint32_t)p.E;
+    for (int k = 0; k < j; k++) use &= idx[k] != idx[j];
+    if (!use) continue;
+    for (int c = 0; c < p.slices; c++)
+      v += *reinterpret_cast<const f32x4 *>(p.part + (c * slots + t * p.top_k + j) * p.N + n);
+  }
+  YT *d = y + (size_t)t * p.N + n;
 #pragma unroll
-  for (int t = 0; t < TT; t++) red[wave][t][lane] = acc[t];
-  __syncthreads();
-  if (wave >= TT) return;
-  f32x4 v = red[0][wave][lane];
-#pragma unroll
-  for (int i = 1; i < WAVES; i++) v += red[i][wave][lane];
-  const uint32_t n = n0 + 4 * g, m = 16 * wave + l16;
-  if (m >= p.T || n >= p.H) return;
-  YT *d = static_cast<YT *>(p.y) + (size_t)m * p.H + n;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {  // H % 32 == 0: whole quads
+  for (int i = 0; i < 4; i++) {  // N % 32 == 0: whole quads
     if constexpr (sizeof(YT) == 4) d[i] = v[i];
     else d[i] = (uint16_t)bf16_rne_nb(v[i]);
   }
@@ -362,61 +670,98 @@ __global__ __launch_bounds__(WAVES * 64) void fp4_down_kernel(const FewArgs p) {
 template <typename XT>
 hipError_t route_go(const Fp4Moe &p, hipStream_t stream) {
   const XT *x = static_cast<const XT *>(p.x);
-  const int xvec = ((reinterpret_cast<uintptr_t>(p.x)) & 15) == 0, rvec = ((reinterpret_cast<uintptr_t>(p.router)) & 15) == 0;
   if (p.rt_bf16)
-    hipLaunchKernelGGL((fp4_route_kernel<XT, uint16_t>), dim3(p.T), dim3(256), 0, stream, x,
-                       static_cast<const uint16_t *>(p.router), p.H, (int)p.E, (int)p.top_k, p.idx, p.wts, xvec, rvec);
+    hipLaunchKernelGGL((fp4_route_kernel<XT, uint16_t>), dim3(p.T), dim3(NT), 0, stream, x,
+                       static_cast<const uint16_t *>(p.router), p.H, (int)p.E, (int)p.top_k, p.idx, p.wts);
   else
-    hipLaunchKernelGGL((fp4_route_kernel<XT, float>), dim3(p.T), dim3(256), 0, stream, x,
-                       static_cast<const float *>(p.router), p.H, (int)p.E, (int)p.top_k, p.idx, p.wts, xvec, rvec);
+    hipLaunchKernelGGL((fp4_route_kernel<XT, float>), dim3(p.T), dim3(NT), 0, stream, x,
+                       static_cast<const float *>(p.router), p.H, (int)p.E, (int)p.top_k, p.idx, p.wts);
   return hipGetLastError();
 }
 
-template <typename XT, int HP>
-hipError_t gate_up_go(const Fp4Moe &p, const FewArgs &a, hipStream_t stream) {
-  const dim3 grid((p.I + 15) / 16, p.E < p.T * p.top_k ? p.E : p.T * p.top_k);
-  if (p.act == 0) hipLaunchKernelGGL((fp4_gate_up_kernel<XT, HP, 0>), grid, dim3(WAVES * 64), 0, stream, a);
-  else hipLaunchKernelGGL((fp4_gate_up_kernel<XT, HP, 1>), grid, dim3(WAVES * 64), 0, stream, a);
+template <typename Kernel>
+hipError_t few_go(Kernel kernel, std::atomic<uint64_t> &done, int lds, int cus, const FewArgs &a, hipStream_t stream) {
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), lds, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, dim3(cus), dim3(NT), lds, stream, a);
   return hipGetLastError();
 }
 
-template <int HP, typename YT>
-hipError_t down_go(const Fp4Moe &p, const FewArgs &a, hipStream_t stream) {
-  const dim3 grid((p.H + 15) / 16), block(WAVES * 64);
-  if (p.T <= 16) hipLaunchKernelGGL((fp4_down_kernel<1, HP, YT>), grid, block, 0, stream, a);
-  else if (p.T <= 32) hipLaunchKernelGGL((fp4_down_kernel<2, HP, YT>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((fp4_down_kernel<4, HP, YT>), grid, block, 0, stream, a);
-  return hipGetLastError();
+template <typename XT, int STEPS, int CT, int D, int RB, bool CHUNKED>
+hipError_t gate_up_go(const FewArgs &a, int cus, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int lds = WAVES * D * Place<STEPS>::DWORDS * 4 + RB * WAVES * 2 * (CT * RED + 32) * 4;
+  static_assert(lds + sizeof(Shared) <= 160 << 10, "LDS");
+  return few_go(fp4_gate_up_kernel<XT, STEPS, CT, D, RB, CHUNKED>, done, lds, cus, a, stream);
+}
+
+template <typename XT>
+hipError_t gate_up(const FewArgs &a, const Fp4FewPlan &plan, int cus, hipStream_t stream) {
+  if (plan.slices > 1) return gate_up_go<XT, 4, 1, 3, 1, true>(a, cus, stream);
+  if (plan.steps == 4)
+    return plan.tiles == 1 ? gate_up_go<XT, 4, 1, 3, 1, false>(a, cus, stream) : gate_up_go<XT, 4, 2, 2, 1, false>(a, cus, stream);
+  if (plan.tiles == 1) return gate_up_go<XT, 2, 1, 5, 2, false>(a, cus, stream);
+  return plan.tiles == 2 ? gate_up_go<XT, 2, 2, 3, 2, false>(a, cus, stream) : gate_up_go<XT, 2, 3, 4, 1, false>(a, cus, stream);
+}
+
+template <int P, int STEPS, int CT, int D>
+hipError_t down_go(const FewArgs &a, int cus, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int lds = WAVES * D * Place<STEPS>::DWORDS * 4 + 2 * WAVES * CT * RED * 4;
+  static_assert(lds + sizeof(Shared) <= 160 << 10, "LDS");
+  return few_go(fp4_down_kernel<P, STEPS, CT, D>, done, lds, cus, a, stream);
+}
+
+template <int P>
+hipError_t down(const FewArgs &a, const Fp4FewPlan &plan, int cus, hipStream_t stream) {
+  if (plan.tiles == 3) return plan.steps == 2 ? down_go<P, 2, 3, 4>(a, cus, stream) : down_go<P, 3, 3, 3>(a, cus, stream);
+  if (plan.tiles == 2) return plan.steps == 2 ? down_go<P, 2, 2, 5>(a, cus, stream) : down_go<P, 3, 2, 3>(a, cus, stream);
+  if (plan.steps == 2) return down_go<P, 2, 1, 5>(a, cus, stream);
+  return plan.steps == 3 ? down_go<P, 3, 1, 4>(a, cus, stream) : down_go<P, 4, 1, 3>(a, cus, stream);
 }
 
 }  // namespace
 
-size_t fp4_moe_bytes(uint32_t T, uint32_t I, uint32_t top_k, int yt_bf16) {
+size_t fp4_moe_h_bytes(uint32_t T, uint32_t I, uint32_t top_k, int yt_bf16) {
   return (size_t)T * top_k * fp4_moe_planes(yt_bf16) * I * 2;
+}
+size_t fp4_moe_part_bytes(uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32_t top_k, int yt_bf16) {
+  return (size_t)fp4_down_plan(T, I, E, top_k, fp4_moe_planes(yt_bf16)).slices * T * top_k * H * 4;
 }
 
 hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream) {
-  (void)cus;
-  if (p.router) {
+  const bool fused = p.router && p.T <= FUSED_T && p.E <= 32;
+  if (p.router && !fused) {
     const hipError_t e = p.xt_bf16 ? route_go<uint16_t>(p, stream) : route_go<float>(p, stream);
     if (e != hipSuccess) return e;
   }
-  FewArgs a = {p.x, p.idx, p.wts, p.h, p.y, p.T, p.H, p.I, (int)p.E, (int)p.top_k,
-               ((reinterpret_cast<uintptr_t>(p.x)) & 15) == 0, {}, {}};
+  const int planes = fp4_moe_planes(p.yt_bf16);
+  FewArgs a = {p.x,      p.router, p.idx,    p.wts, p.h, p.part, p.T, p.H, p.I, (int)p.E, (int)p.top_k, planes, p.act,
+               p.rt_bf16, fused,    1,        0,     {},  {}};
   for (uint32_t e = 0; e < p.E; e++)
     for (int k = 0; k < 2; k++) {
       a.w[k][e] = p.w[k][e];
       a.s[k][e] = p.s[k][e];
     }
-  hipError_t e;
-  if (p.yt_bf16) e = p.xt_bf16 ? gate_up_go<uint16_t, 2>(p, a, stream) : gate_up_go<float, 2>(p, a, stream);
-  else e = p.xt_bf16 ? gate_up_go<uint16_t, 3>(p, a, stream) : gate_up_go<float, 3>(p, a, stream);
+  const Fp4FewPlan up = fp4_gate_up_plan(p.T, p.H, p.E, p.top_k, p.xt_bf16 ? 1 : 3);
+  hipError_t e = p.xt_bf16 ? gate_up<uint16_t>(a, up, cus, stream) : gate_up<float>(a, up, cus, stream);
   if (e != hipSuccess) return e;
   for (uint32_t i = 0; i < p.E; i++) {
     a.w[0][i] = p.w[2][i];
     a.s[0][i] = p.s[2][i];
   }
-  return p.yt_bf16 ? down_go<2, uint16_t>(p, a, stream) : down_go<3, float>(p, a, stream);
+  const Fp4FewPlan dn = fp4_down_plan(p.T, p.I, p.E, p.top_k, planes);
+  a.route = 0;
+  a.K = p.I;
+  a.N = p.H;
+  a.slices = dn.slices;
+  a.per = dn.per;
+  e = planes == 2 ? down<2>(a, dn, cus, stream) : down<3>(a, dn, cus, stream);
+  if (e != hipSuccess) return e;
+  const dim3 grid((p.H + 1023) / 1024, p.T);
+  if (p.yt_bf16) hipLaunchKernelGGL(fp4_join_kernel<uint16_t>, grid, dim3(256), 0, stream, a, static_cast<uint16_t *>(p.y));
+  else hipLaunchKernelGGL(fp4_join_kernel<float>, grid, dim3(256), 0, stream, a, static_cast<float *>(p.y));
+  return hipGetLastError();
 }
 
 }  // namespace frx

@@ -262,4 +262,40 @@ inline int fp4_grouped_tile(uint32_t R, uint32_t N, uint32_t E, int cus) {
   return FP4_T_64;
 }
 
+// ---- the expert layer for a few tokens -------------------------------------------
+
+// A wave's steps of 128 columns (8 waves split K), column tiles of 16 (token, plane) pairs
+// that it holds, and slices of K with the steps in each: the down projection's are units of
+// their own, the others' follow one another in a workgroup.
+struct Fp4FewPlan {
+  int steps, tiles, slices, per;
+};
+
+// Column tiles that hold half again as many tokens as an expert would have were they spread
+// evenly; a fuller expert's weights are read twice.
+inline int fp4_few_tiles(uint32_t T, uint32_t E, uint32_t top_k, int planes) {
+  const double cols = 1.5 * T * (top_k < E ? top_k : E) / E * planes, most = (double)T * planes;
+  const double c = cols < most ? cols : most;
+  return c <= 16 ? 1 : c <= 32 ? 2 : 3;
+}
+inline Fp4FewPlan fp4_gate_up_plan(uint32_t T, uint32_t H, uint32_t E, uint32_t top_k, int planes) {
+  const int kbs = (int)((H + 127) / 128), tiles = fp4_few_tiles(T, E, top_k, planes);
+  if (kbs > 32) return {4, 1, (kbs + 31) / 32, 32};
+  if (kbs > 16) return {4, tiles == 1 ? 1 : 2, 1, kbs};
+  return {2, tiles, 1, kbs};
+}
+inline Fp4FewPlan fp4_down_plan(uint32_t T, uint32_t I, uint32_t E, uint32_t top_k, int planes) {
+  const int kbs = (int)((I + 127) / 128), tiles = fp4_few_tiles(T, E, top_k, planes);
+  Fp4FewPlan best = {2, tiles, 1, kbs};
+  int least = 1 << 30;
+  for (int steps = tiles == 1 ? 4 : 3; steps >= 2; steps--) {
+    const int slices = (kbs + 8 * steps - 1) / (8 * steps);
+    if (slices * steps < least) {  // the fewest steps of a wave over all slices; of equals the fewest slices
+      least = slices * steps;
+      best = {steps, tiles, slices, (kbs + slices - 1) / slices};
+    }
+  }
+  return best;
+}
+
 }  // namespace frx
