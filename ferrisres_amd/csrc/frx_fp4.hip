@@ -1,7 +1,6 @@
-// frx_fp4.hip — launches of the 4-bit floating-point linears (engines: frx_fp4.hpp,
+// frx_fp4.hip — launches of the 4-bit floating-point linears (engines: frx_fp4_ring.hpp,
 // frx_fp4_skinny.hpp).
-#include <type_traits>
-
+#include "frx_fp4_ring.hpp"
 #include "frx_fp4_skinny.hpp"
 #include "frx_internal.hpp"
 #include "frx_tiles.hpp"
@@ -123,6 +122,25 @@ hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// tokens x weight rows
+using Tile64x128 = Fp4Ring<2, 2, 2, 4, 3>;
+using Tile128x192 = Fp4Ring<2, 4, 4, 3, 3>;
+using Tile128x256 = Fp4Ring<2, 4, 4, 4, 3>;
+using Tile192x256 = Fp4Ring<2, 4, 6, 4, 2>;
+using Tile256x256 = Fp4Ring<2, 4, 8, 4, 2>;
+static_assert(2 * Tile64x128::LDS_BYTES <= 160 << 10, "two workgroups to a compute unit");
+
+template <typename YT>
+hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
+  switch (tile) {
+    case FP4_T_256X256: return dense_go<Tile256x256, YT>(p, S, stream);
+    case FP4_T_192X256: return dense_go<Tile192x256, YT>(p, S, stream);
+    case FP4_T_128X256: return dense_go<Tile128x256, YT>(p, S, stream);
+    case FP4_T_128X192: return dense_go<Tile128x192, YT>(p, S, stream);
+    default: return dense_go<Tile64x128, YT>(p, S, stream);
+  }
+}
+
 template <int RT, int TT, typename XT, typename YT>
 hipError_t skinny_rt(const Fp4Skinny &p, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
@@ -138,17 +156,14 @@ hipError_t skinny_rt(const Fp4Skinny &p, hipStream_t stream) {
 
 template <int TT, typename XT, typename YT>
 hipError_t skinny_go(int rt, const Fp4Skinny &p, hipStream_t stream) {
-  if constexpr (TT <= 2) {
-    if (rt == 4) return skinny_rt<4, TT, XT, YT>(p, stream);
-    if (rt == 3) return skinny_rt<3, TT, XT, YT>(p, stream);
-  }
+  if (rt == 4) return skinny_rt<4, TT, XT, YT>(p, stream);
+  if (rt == 3) return skinny_rt<3, TT, XT, YT>(p, stream);
   if (rt == 2) return skinny_rt<2, TT, XT, YT>(p, stream);
   return skinny_rt<1, TT, XT, YT>(p, stream);
 }
 
 template <typename YT>
 hipError_t skinny_any(int rt, const Fp4Skinny &p, hipStream_t stream) {
-  if (p.M > 32) return skinny_go<4, uint8_t, YT>(rt, p, stream);
   return p.M > 16 ? skinny_go<2, uint8_t, YT>(rt, p, stream) : skinny_go<1, uint8_t, YT>(rt, p, stream);
 }
 
@@ -171,7 +186,8 @@ hipError_t grouped_any(const GroupArgs &p, int tile, hipStream_t stream) {
     hipLaunchKernelGGL((fp4_skinny_grouped_kernel<YT>), grid, block, (int)fp4_skinny_red_bytes(1), stream, p);
     return hipGetLastError();
   }
-  return grouped_go<Fp4Tile<64, 128, 2, 2>, YT>(p, stream);
+  if (tile == FP4_T_256X256) return grouped_go<Tile256x256, YT>(p, stream);
+  return tile == FP4_T_128X256 ? grouped_go<Tile128x256, YT>(p, stream) : grouped_go<Tile64x128, YT>(p, stream);
 }
 
 }  // namespace
@@ -184,8 +200,7 @@ hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, co
     return yt_bf16 ? skinny_any<uint16_t>(plan.per, p, stream) : skinny_any<float>(plan.per, p, stream);
   }
   const DenseArgs p = {a, b, sa, sb, y, plan.S > 1 ? part : nullptr, lda, ldb, M, K, N, plan.per};
-  using T = Fp4Tile<128, 128, 2, 2>;
-  const hipError_t e = yt_bf16 ? dense_go<T, uint16_t>(p, plan.S, stream) : dense_go<T, float>(p, plan.S, stream);
+  const hipError_t e = yt_bf16 ? dense_tile<uint16_t>(plan.tile, p, plan.S, stream) : dense_tile<float>(plan.tile, p, plan.S, stream);
   if (e != hipSuccess || plan.S == 1) return e;
   const size_t n = (size_t)M * N;
   const dim3 grid((unsigned)((n + 1023) / 1024));
@@ -216,7 +231,7 @@ hipError_t launch_fp4_grouped(const uint8_t *a, size_t lda, const uint8_t *sa, c
     p.b[e] = b[e];
     p.sb[e] = sb[e];
   }
-  const int tile = fp4_grouped_tile(R, N, (uint32_t)E, cus);
+  const int tile = fp4_grouped_tile(R, K, N, (uint32_t)E, cus);
   return yt_bf16 ? grouped_any<uint16_t>(p, tile, stream) : grouped_any<float>(p, tile, stream);
 }
 

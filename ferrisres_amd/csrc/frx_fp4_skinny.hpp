@@ -1,4 +1,4 @@
-// frx_fp4_skinny.hpp — the 4-bit product for up to 64 tokens.
+// frx_fp4_skinny.hpp — the 4-bit product for up to 32 tokens.
 //
 // Bound by the weights' bytes: each is read once, straight into registers (a lane of an
 // MFMA operand holds one block of 32 codes of one row, 16 bytes: an instruction reads 64

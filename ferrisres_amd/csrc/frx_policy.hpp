@@ -230,20 +230,35 @@ inline int fp8_grouped_tile(uint32_t R, uint32_t N, uint32_t E, int pipe8, int c
 
 // ---- the 4-bit floating-point linears --------------------------------------------
 
-enum { FP4_T_SKINNY = 0, FP4_T_128 = 1, FP4_T_64 = 2 };
+enum { FP4_T_SKINNY = 0, FP4_T_64X128 = 1, FP4_T_128X192 = 2, FP4_T_128X256 = 3, FP4_T_192X256 = 4, FP4_T_256X256 = 5 };
 struct Fp4Plan {
   int tile;    // FP4_T_*
   int S, per;  // K slices, steps of 256 columns in each (FP4_T_SKINNY: 1, 16-row tiles of a workgroup)
 };
 
+// Tiles of many tokens: height x width, workgroups resident at once on a compute unit, what
+// a tile costs beside its steps, and a step of 256 columns with few tiles and with one on
+// every unit, where the L2s bound (ns). us, 64 x 128 / 128 x 192 / 128 x 256 / 192 x 256 / 256 x
+// 256: 100 x 4096 x 4096 12.1 / 17.3 / 20.5 / 27.3 / 30.9, 1024 x 2048 x 2048 8.8 / 12.6 / 14.5 /
+// 19.1 / 22.2, f32 333 x 5120 x 13824 35 / 26 / 30 / 38 / 44, 1999 x 11008 x 4096 85 / 82 / 57 /
+// 71 / 77, 2048 x 4096 x 11008 100 / 80 / 74 / 68 / 78, f32 11008 x 2016 x 4096 126 / 114 / 106 /
+// 94 / 93, 8192^3 492 / 406 / 360 / 338 / 301 to 325.
+struct Fp4TileCost {
+  int tile, bm, bn, wgs, fix, few, all;
+};
+constexpr Fp4TileCost kFp4Tiles[] = {{FP4_T_64X128, 64, 128, 2, 3000, 410, 740},
+                                     {FP4_T_128X192, 128, 192, 1, 5400, 590, 980},
+                                     {FP4_T_128X256, 128, 256, 1, 6000, 750, 1250},
+                                     {FP4_T_192X256, 192, 256, 1, 8400, 1030, 1700},
+                                     {FP4_T_256X256, 256, 256, 1, 11000, 1090, 2200}};
+
 inline Fp4Plan fp4_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
-  if (M <= 64) {
+  if (M <= 32) {
     // the fewest rounds of row tiles on the fullest compute unit; of equals the most tiles a workgroup
     const uint32_t tiles = (N + 15) / 16;
-    const int most = M <= 32 ? 4 : 2;
     int best = 1;
     uint32_t least = ~0u;
-    for (int rt = 1; rt <= most; rt++) {
+    for (int rt = 1; rt <= 4; rt++) {
       const uint32_t wgs = (tiles + rt - 1) / rt, rounds = (wgs + cus - 1) / cus * rt;
       if (rounds <= least) {
         least = rounds;
@@ -252,14 +267,45 @@ inline Fp4Plan fp4_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
     }
     return {FP4_T_SKINNY, 1, best};
   }
-  return {FP4_T_128, 1, (int)((K + 255) / 256)};
+  const int steps = (int)((K + 255) / 256);
+  Fp4Plan plan = {FP4_T_64X128, 1, steps};
+  double least = 1e30;
+  for (const Fp4TileCost &c : kFp4Tiles) {
+    const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+    // a K slice more: fewer steps, but every part is written and read (4 bytes a value at
+    // about 4 TB/s) and the parts joined by another launch (4 us). Slices begin at even steps.
+    for (int S = 1; S <= 8 && S <= steps; S++) {
+      const int per = S == 1 ? steps : ((steps + S - 1) / S + 1) & ~1;
+      if ((S - 1) * per >= steps) continue;  // an empty slice
+      const double full = (double)c.wgs * cus, n = tiles * S, share = n < full ? n / full : 1.0;
+      const double ns = std::ceil(n / full) * (c.fix + per * (c.few + (c.all - c.few) * share)) +
+                        (S > 1 ? 4000.0 + (double)S * M * N * 8 / 4000 : 0.0);
+      if (ns < least) {
+        least = ns;
+        plan = {c.tile, S, per};
+      }
+    }
+  }
+  return plan;
 }
 
-// Experts' rows: tiles of 16 where R / E is small.
-inline int fp4_grouped_tile(uint32_t R, uint32_t N, uint32_t E, int cus) {
-  (void)cus;
+// Experts' rows: tiles of 16 where R / E is small, else the tile that is cheapest for groups of
+// equal length with half a tile of remainder (the groups' lengths are not known here).
+inline int fp4_grouped_tile(uint32_t R, uint32_t K, uint32_t N, uint32_t E, int cus) {
   if (R <= 8 * E && ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16) < (size_t)1 << 23) return FP4_T_SKINNY;
-  return FP4_T_64;
+  const int steps = (int)((K + 255) / 256);
+  int best = FP4_T_64X128;
+  double least = 1e30;
+  for (const Fp4TileCost &c : kFp4Tiles) {
+    if (c.tile == FP4_T_128X192 || c.tile == FP4_T_192X256) continue;
+    const double tiles = E * ((double)R / E / c.bm + 0.5) * ((N + c.bn - 1) / c.bn), full = (double)c.wgs * cus;
+    const double ns = std::ceil(tiles / full) * (c.fix + steps * (double)c.all);
+    if (ns < least) {
+      least = ns;
+      best = c.tile;
+    }
+  }
+  return best;
 }
 
 // ---- the expert layer for a few tokens -------------------------------------------
