@@ -96,20 +96,6 @@ __global__ __launch_bounds__(FP4_SK_WAVES * 64) void fp4_skinny_kernel(const Fp4
   fp4_skinny<RT, TT, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
-// Sorted rows in tiles of 16 (decode batches: a few rows of each expert).
-template <typename YT>
-__global__ __launch_bounds__(FP4_SK_WAVES * 64) void fp4_skinny_grouped_kernel(const GroupArgs p) {
-  extern __shared__ __align__(16) uint32_t lds[];
-  const uint32_t nts = (p.N + 15) / 16;
-  const uint32_t mt = blockIdx.x / nts, nt = blockIdx.x - mt * nts;
-  uint32_t m0, end;
-  const int e = expert_tile<16>(p.offsets, p.E, p.R, mt, m0, end);
-  if (e < 0) return;
-  const Fp4Skinny q = {p.a + (size_t)m0 * p.lda, p.sa + (size_t)m0 * fp4_scale_bytes(p.K), p.b[e], p.sb[e],
-                       static_cast<YT *>(p.y) + (size_t)m0 * p.N, p.lda, p.ldb, min(16u, end - m0), p.K, p.N, 0};
-  fp4_skinny<1, 1, uint8_t, YT>(q, nt * 16, reinterpret_cast<f32x4 *>(lds));
-}
-
 template <typename Tile, typename YT>
 hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
@@ -123,11 +109,13 @@ hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
 }
 
 // tokens x weight rows
+using Tile64x64 = Fp4Ring<2, 2, 2, 2, 3>;
 using Tile64x128 = Fp4Ring<2, 2, 2, 4, 3>;
 using Tile128x192 = Fp4Ring<2, 4, 4, 3, 3>;
 using Tile128x256 = Fp4Ring<2, 4, 4, 4, 3>;
 using Tile192x256 = Fp4Ring<2, 4, 6, 4, 2>;
 using Tile256x256 = Fp4Ring<2, 4, 8, 4, 2>;
+static_assert(3 * Tile64x64::LDS_BYTES <= 160 << 10, "three workgroups to a compute unit");
 static_assert(2 * Tile64x128::LDS_BYTES <= 160 << 10, "two workgroups to a compute unit");
 
 template <typename YT>
@@ -137,7 +125,8 @@ hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
     case FP4_T_192X256: return dense_go<Tile192x256, YT>(p, S, stream);
     case FP4_T_128X256: return dense_go<Tile128x256, YT>(p, S, stream);
     case FP4_T_128X192: return dense_go<Tile128x192, YT>(p, S, stream);
-    default: return dense_go<Tile64x128, YT>(p, S, stream);
+    case FP4_T_64X128: return dense_go<Tile64x128, YT>(p, S, stream);
+    default: return dense_go<Tile64x64, YT>(p, S, stream);
   }
 }
 
@@ -181,13 +170,12 @@ hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
 
 template <typename YT>
 hipError_t grouped_any(const GroupArgs &p, int tile, hipStream_t stream) {
-  if (tile == FP4_T_SKINNY) {
-    const dim3 grid((unsigned)(((p.R + 15) / 16 + p.E) * ((p.N + 15) / 16))), block(FP4_SK_WAVES * 64);
-    hipLaunchKernelGGL((fp4_skinny_grouped_kernel<YT>), grid, block, (int)fp4_skinny_red_bytes(1), stream, p);
-    return hipGetLastError();
+  switch (tile) {
+    case FP4_T_256X256: return grouped_go<Tile256x256, YT>(p, stream);
+    case FP4_T_128X256: return grouped_go<Tile128x256, YT>(p, stream);
+    case FP4_T_64X128: return grouped_go<Tile64x128, YT>(p, stream);
+    default: return grouped_go<Tile64x64, YT>(p, stream);
   }
-  if (tile == FP4_T_256X256) return grouped_go<Tile256x256, YT>(p, stream);
-  return tile == FP4_T_128X256 ? grouped_go<Tile128x256, YT>(p, stream) : grouped_go<Tile64x128, YT>(p, stream);
 }
 
 }  // namespace

@@ -36,4 +36,14 @@ __device__ __forceinline__ void fp4_mul(f32x4 &acc, const u32x4 &w, uint32_t sw,
   acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, S, (int)sw, S, (int)sx);
 }
 
+// ---- gate and up -------------------------------------------------------------------
+
+// A barrier that waits for this wave's LDS accesses alone: __syncthreads() would wait for the
+// weights on their way too.
+__device__ __forceinline__ void barrier_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 }  // namespace frx

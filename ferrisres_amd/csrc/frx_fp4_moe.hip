@@ -21,8 +21,7 @@
 // instructions for 128 columns, and one exchange of the waves' sums through LDS. The weights
 // of the next tiles are on their way meanwhile, by LDS DMA into a ring that each wave has for
 // itself (held in registers they were waited for at every turn of the loop).
-#include "frx_fp4_codes.hpp"
-#include "frx_fp8.hpp"
+#include "frx_fp4.hpp"
 #include "frx_internal.hpp"
 
 namespace frx {
@@ -386,16 +385,6 @@ __device__ __forceinline__ void multiply(f32x4 (&acc)[CT], const uint32_t *from,
 __device__ __forceinline__ float activate(float g, int act) {
   if (act == 0) return g / (1.0f + expf(-g));
   return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
-}
-
-// ---- gate and up -------------------------------------------------------------------
-
-// A barrier that waits for this wave's LDS accesses alone: __syncthreads() would wait for the
-// weights on their way too.
-__device__ __forceinline__ void barrier_lds() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
 }
 
 // The waves' sums in LDS, floats: 16 x 16 of a column tile as 4 groups of 4 rows, 80 apart, [column]

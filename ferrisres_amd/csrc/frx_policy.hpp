@@ -230,7 +230,7 @@ inline int fp8_grouped_tile(uint32_t R, uint32_t N, uint32_t E, int pipe8, int c
 
 // ---- the 4-bit floating-point linears --------------------------------------------
 
-enum { FP4_T_SKINNY = 0, FP4_T_64X128 = 1, FP4_T_128X192 = 2, FP4_T_128X256 = 3, FP4_T_192X256 = 4, FP4_T_256X256 = 5 };
+enum { FP4_T_SKINNY, FP4_T_64X64, FP4_T_64X128, FP4_T_128X192, FP4_T_128X256, FP4_T_192X256, FP4_T_256X256 };
 struct Fp4Plan {
   int tile;    // FP4_T_*
   int S, per;  // K slices, steps of 256 columns in each (FP4_T_SKINNY: 1, 16-row tiles of a workgroup)
@@ -242,11 +242,14 @@ struct Fp4Plan {
 // 256: 100 x 4096 x 4096 12.1 / 17.3 / 20.5 / 27.3 / 30.9, 1024 x 2048 x 2048 8.8 / 12.6 / 14.5 /
 // 19.1 / 22.2, f32 333 x 5120 x 13824 35 / 26 / 30 / 38 / 44, 1999 x 11008 x 4096 85 / 82 / 57 /
 // 71 / 77, 2048 x 4096 x 11008 100 / 80 / 74 / 68 / 78, f32 11008 x 2016 x 4096 126 / 114 / 106 /
-// 94 / 93, 8192^3 492 / 406 / 360 / 338 / 301 to 325.
+// 94 / 93, 8192^3 492 / 406 / 360 / 338 / 301 to 325. 64 x 64 / 64 x 128: 33 x 2048 x 5632 5.8 / 7.6,
+// 64 x 4096 x 11008 9.4 / 12.4, 333 x 5632 x 2048 11.8 / 15.5, 512 x 8192 x 6144 31.0 / 30.6; experts'
+// rows, 16 of 2048 x 5632: 256 rows 25.0 / 26.7, 2048 rows 55.7 / 51.5.
 struct Fp4TileCost {
   int tile, bm, bn, wgs, fix, few, all;
 };
-constexpr Fp4TileCost kFp4Tiles[] = {{FP4_T_64X128, 64, 128, 2, 3000, 410, 740},
+constexpr Fp4TileCost kFp4Tiles[] = {{FP4_T_64X64, 64, 64, 3, 3000, 320, 860},
+                                     {FP4_T_64X128, 64, 128, 2, 3500, 460, 860},
                                      {FP4_T_128X192, 128, 192, 1, 5400, 590, 980},
                                      {FP4_T_128X256, 128, 256, 1, 6000, 750, 1250},
                                      {FP4_T_192X256, 192, 256, 1, 8400, 1030, 1700},
@@ -268,7 +271,7 @@ inline Fp4Plan fp4_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
     return {FP4_T_SKINNY, 1, best};
   }
   const int steps = (int)((K + 255) / 256);
-  Fp4Plan plan = {FP4_T_64X128, 1, steps};
+  Fp4Plan plan = {FP4_T_64X64, 1, steps};
   double least = 1e30;
   for (const Fp4TileCost &c : kFp4Tiles) {
     const double tiles = (double)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
@@ -289,16 +292,16 @@ inline Fp4Plan fp4_plan(uint32_t M, uint32_t K, uint32_t N, int cus) {
   return plan;
 }
 
-// Experts' rows: tiles of 16 where R / E is small, else the tile that is cheapest for groups of
-// equal length with half a tile of remainder (the groups' lengths are not known here).
+// Experts' rows: the tile that is cheapest for groups of equal length, of half a tile more than
+// they fill where they need more than one (the groups' lengths are not known here).
 inline int fp4_grouped_tile(uint32_t R, uint32_t K, uint32_t N, uint32_t E, int cus) {
-  if (R <= 8 * E && ((size_t)(R + 15) / 16 + E) * ((N + 15) / 16) < (size_t)1 << 23) return FP4_T_SKINNY;
   const int steps = (int)((K + 255) / 256);
-  int best = FP4_T_64X128;
+  int best = FP4_T_64X64;
   double least = 1e30;
   for (const Fp4TileCost &c : kFp4Tiles) {
     if (c.tile == FP4_T_128X192 || c.tile == FP4_T_192X256) continue;
-    const double tiles = E * ((double)R / E / c.bm + 0.5) * ((N + c.bn - 1) / c.bn), full = (double)c.wgs * cus;
+    const double tiles = std::min(E, R) * std::max(1.0, (double)R / E / c.bm + 0.5) * ((N + c.bn - 1) / c.bn);
+    const double full = (double)c.wgs * cus;
     const double ns = std::ceil(tiles / full) * (c.fix + steps * (double)c.all);
     if (ns < least) {
       least = ns;
