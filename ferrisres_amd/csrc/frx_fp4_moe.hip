@@ -34,8 +34,6 @@ constexpr int WAVES = 8, NT = WAVES * 64;
 
 constexpr int MOST_SLOTS = FP4_MOE_MAX_T * 64;
 constexpr int KEPT_SLOTS = 512;
-// Tokens up to which every workgroup of gate_up routes for itself.
-constexpr int FUSED_T = 4;
 
 // Unaligned 16 bytes (a tensor may begin at any element).
 typedef u32x4 __attribute__((aligned(2))) u32x4_u;
@@ -53,7 +51,7 @@ struct FewArgs {
 
 struct Shared {
   const uint8_t *w[2][FP8_MAXE], *s[2][FP8_MAXE];
-  float logit[FUSED_T][64];
+  float logit[64];
   uint8_t expert[MOST_SLOTS];  // of each slot; 255: none
   int count[FP8_MAXE];         // the expert's routes
   float wts[KEPT_SLOTS];       // of each slot, where there are few
@@ -80,31 +78,23 @@ __device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) {
   }
 }
 
-// Logits of up to TM tokens from x on: a wave for each expert.
-template <int TM, typename XT, typename RT>
-__device__ __forceinline__ void router_logits(const XT *x, const RT *router, int T, uint32_t H, int E,
-                                              float (*logit)[64]) {
+// A token's logits: a wave for each expert.
+template <int WAVES, typename XT, typename RT>
+__device__ __forceinline__ void router_logits(const XT *x, const RT *router, uint32_t H, int E, float *logit) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int e = wave; e < E; e += WAVES) {
-    float s[TM] = {};
+    float s = 0.f;
 #pragma unroll 4
     for (uint32_t k = lane * 8; k < H; k += 512) {
-      float r[8];
+      float r[8], v[8];
       load8(router + (size_t)e * H + k, r);
+      load8(x + k, v);
 #pragma unroll
-      for (int t = 0; t < TM; t++) {
-        float v[8];
-        load8(x + (size_t)min(t, T - 1) * H + k, v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) s[t] = __builtin_fmaf(v[i], r[i], s[t]);
-      }
+      for (int i = 0; i < 8; i++) s = __builtin_fmaf(v[i], r[i], s);
     }
 #pragma unroll
-    for (int t = 0; t < TM; t++) {
-#pragma unroll
-      for (int o = 32; o; o >>= 1) s[t] += __shfl_xor(s[t], o);
-      if (lane == 0 && t < T) logit[t][e] = s[t];
-    }
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0) logit[e] = s;
   }
 }
 
@@ -131,18 +121,22 @@ __device__ __forceinline__ int top_experts(const float *logit, int E, int top_k,
   return rank;
 }
 
-// A workgroup per token.
+// A workgroup per token: 8 tokens, 16 experts, H 2048 5.9 us (with 8 waves 8.4). A single token's
+// gate_up routes for itself instead, in every workgroup: 28.2 us a call against 30.2 (32 experts,
+// H 4096: 38 against 43); for 2 and 4 tokens that is dearer, 41 and 54 us against 35 and 46.
+constexpr int ROUTE_WAVES = 16;
 template <typename XT, typename RT>
-__global__ __launch_bounds__(NT) void fp4_route_kernel(const XT *__restrict__ x, const RT *__restrict__ router,
-                                                       uint32_t H, int E, int top_k, uint32_t *__restrict__ idx,
-                                                       float *__restrict__ wts) {
-  __shared__ float logit[1][64];
+__global__ __launch_bounds__(ROUTE_WAVES * 64) void fp4_route_kernel(const XT *__restrict__ x,
+                                                                     const RT *__restrict__ router,
+                                                                     uint32_t H, int E, int top_k, uint32_t *__restrict__ idx,
+                                                                     float *__restrict__ wts) {
+  __shared__ float logit[64];
   const size_t t = blockIdx.x;
-  router_logits<1>(x + t * H, router, 1, H, E, logit);
+  router_logits<ROUTE_WAVES>(x + t * H, router, H, E, logit);
   __syncthreads();
   if (threadIdx.x >= 64) return;
   float w;
-  const int place = top_experts(logit[0], E, top_k, w);
+  const int place = top_experts(logit, E, top_k, w);
   if (place < top_k) {
     idx[t * top_k + place] = threadIdx.x;
     wts[t * top_k + place] = w;
@@ -163,25 +157,19 @@ __device__ __forceinline__ void read_routes(const FewArgs &p, Shared &sh) {
   __syncthreads();
   if (ROUTE && p.route) {
     const XT *x = static_cast<const XT *>(p.x);
-    if (p.T == 1) {
-      if (p.rt_bf16) router_logits<1>(x, static_cast<const uint16_t *>(p.router), 1, p.K, p.E, sh.logit);
-      else router_logits<1>(x, static_cast<const float *>(p.router), 1, p.K, p.E, sh.logit);
-    } else {
-      if (p.rt_bf16) router_logits<FUSED_T>(x, static_cast<const uint16_t *>(p.router), (int)p.T, p.K, p.E, sh.logit);
-      else router_logits<FUSED_T>(x, static_cast<const float *>(p.router), (int)p.T, p.K, p.E, sh.logit);
-    }
+    if (p.rt_bf16) router_logits<WAVES>(x, static_cast<const uint16_t *>(p.router), p.K, p.E, sh.logit);
+    else router_logits<WAVES>(x, static_cast<const float *>(p.router), p.K, p.E, sh.logit);
     __syncthreads();
-    const int t = threadIdx.x >> 6;
-    if (t < (int)p.T) {
+    if (threadIdx.x < 64) {
       float w;
-      const int place = top_experts(sh.logit[t], p.E, p.top_k, w), s = t * p.top_k + place;
+      const int place = top_experts(sh.logit, p.E, p.top_k, w);
       if (place < p.top_k) {
-        sh.expert[s] = lane;
+        sh.expert[place] = lane;
         atomicAdd(&sh.count[lane], 1);
-        sh.wts[s] = w;
+        sh.wts[place] = w;
         if (blockIdx.x == 0) {
-          p.idx[s] = lane;
-          p.wts[s] = w;
+          p.idx[place] = lane;
+          p.wts[place] = w;
         }
       }
     }
@@ -633,7 +621,9 @@ __global__ __launch_bounds__(NT) void fp4_down_kernel(const FewArgs p) {
 }
 
 // y[t] = its routes' sums over the slices, in the order of the routes. A route that goes
-// nowhere, and a later one to an expert that the token has named, has none.
+// nowhere, and a later one to an expert that the token has named, has none. 5 us, most of it a
+// launch's own; joined in down by the last workgroup at each tile 61 tokens took 20 us more, 8
+// two more, 1 as long.
 template <typename YT>
 __global__ __launch_bounds__(256) void fp4_join_kernel(const FewArgs p, YT *__restrict__ y) {
   const uint32_t t = blockIdx.y, n = (blockIdx.x * 256 + threadIdx.x) * 4;
@@ -660,10 +650,10 @@ template <typename XT>
 hipError_t route_go(const Fp4Moe &p, hipStream_t stream) {
   const XT *x = static_cast<const XT *>(p.x);
   if (p.rt_bf16)
-    hipLaunchKernelGGL((fp4_route_kernel<XT, uint16_t>), dim3(p.T), dim3(NT), 0, stream, x,
+    hipLaunchKernelGGL((fp4_route_kernel<XT, uint16_t>), dim3(p.T), dim3(ROUTE_WAVES * 64), 0, stream, x,
                        static_cast<const uint16_t *>(p.router), p.H, (int)p.E, (int)p.top_k, p.idx, p.wts);
   else
-    hipLaunchKernelGGL((fp4_route_kernel<XT, float>), dim3(p.T), dim3(NT), 0, stream, x,
+    hipLaunchKernelGGL((fp4_route_kernel<XT, float>), dim3(p.T), dim3(ROUTE_WAVES * 64), 0, stream, x,
                        static_cast<const float *>(p.router), p.H, (int)p.E, (int)p.top_k, p.idx, p.wts);
   return hipGetLastError();
 }
@@ -719,7 +709,7 @@ size_t fp4_moe_part_bytes(uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32
 }
 
 hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream) {
-  const bool fused = p.router && p.T <= FUSED_T && p.E <= 32;
+  const bool fused = p.router && p.T == 1 && p.E <= 32;
   if (p.router && !fused) {
     const hipError_t e = p.xt_bf16 ? route_go<uint16_t>(p, stream) : route_go<float>(p, stream);
     if (e != hipSuccess) return e;
