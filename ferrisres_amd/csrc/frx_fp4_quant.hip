@@ -1,7 +1,10 @@
 // frx_fp4_quant.hip — codes and scales of the 4-bit floating-point linears, and back.
 //
 // Formulas: frx_fp4_codes.hpp. Bound by memory: 2 or 4 bytes in and 17/32 out a value (the
-// way back the other way round), about 3 VALU operations a value.
+// way back the other way round), about 3 VALU operations a value. 11008 x 4096: f32 along the
+// rows 36.0 us (5.7 TB/s), along the columns 44.9, back 44.7; bf16 24.6, 29.5, 25.4. 2048 x 4096
+// bf16 6.3, 7.4, 5.6. Tried and no faster: two pieces of a row a thread, tiles of 256 x 64 along
+// the columns (whole lines of codes), divisions in 32 bits.
 #include "frx_fp4_codes.hpp"
 #include "frx_internal.hpp"
 
