@@ -34,30 +34,53 @@ __device__ __forceinline__ void fill_operands(Fp4Operands &o, const uint8_t *a, 
   o.K = (int)K;
 }
 
+// A workgroup's tile.
+template <typename Tile, typename YT>
+struct DenseItem {
+  const DenseArgs &p;
+  uint32_t m0, n0, mr, nr;
+  int span, t0, t1;
+  __device__ __forceinline__ DenseItem(const DenseArgs &args) : p(args) {
+    uint32_t mt, nt;
+    xcd_tile<8>(blockIdx.x, (p.M + Tile::BM - 1) / Tile::BM, (p.N + Tile::BN - 1) / Tile::BN, mt, nt);
+    m0 = mt * Tile::BM;
+    n0 = nt * Tile::BN;
+    mr = min((uint32_t)Tile::BM, p.M - m0);
+    nr = min((uint32_t)Tile::BN, p.N - n0);
+    const int steps = (int)((p.K + 255) >> 8);
+    t0 = p.part ? (int)blockIdx.z * p.per : 0;
+    t1 = p.part ? min(t0 + p.per, steps) : steps;
+    span = t1 - t0;
+  }
+  __device__ __forceinline__ bool at(int, Fp4Operands &o) const {
+    fill_operands(o, p.a, p.lda, p.sa, p.b, p.ldb, p.sb, m0, mr, n0, nr, p.K);
+    o.t0 = t0;
+    o.t1 = t1;
+    return true;
+  }
+  __device__ __forceinline__ bool take(int, int &from, int &to) const {
+    from = t0;
+    to = t1;
+    return true;
+  }
+  template <typename Acc>
+  __device__ __forceinline__ void store(const Acc &acc) const {
+    const size_t at = (size_t)m0 * p.N + n0;
+    if (p.part)
+      Tile::template store<float>(acc, p.part + (size_t)blockIdx.z * p.M * p.N + at, p.N, (int)mr, (int)nr,
+                                  (p.N & 3) == 0);
+    else Tile::template store<YT>(acc, (YT *)p.y + at, p.N, (int)mr, (int)nr, quads<YT>(p.y, p.N));
+  }
+};
+
 template <typename Tile, typename YT>
 __global__ __launch_bounds__(Tile::NT, 2) void fp4_dense_kernel(const DenseArgs p) {
   extern __shared__ __align__(16) uint32_t lds[];
-  constexpr int BM = Tile::BM, BN = Tile::BN;
-  uint32_t mt, nt;
-  xcd_tile<8>(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, mt, nt);
-  const uint32_t m0 = mt * BM, n0 = nt * BN;
-  Fp4Operands o;
-  fill_operands(o, p.a, p.lda, p.sa, p.b, p.ldb, p.sb, m0, min((uint32_t)BM, p.M - m0), n0, min((uint32_t)BN, p.N - n0),
-                p.K);
-  const int steps = (int)((p.K + 255) >> 8);
-  o.t0 = p.part ? (int)blockIdx.z * p.per : 0;
-  o.t1 = p.part ? min(o.t0 + p.per, steps) : steps;
-  f32x4 acc[Tile::FN][Tile::FM];
-  Tile::run(lds, o, acc);
-  const size_t at = (size_t)m0 * p.N + n0;
-  if (p.part)
-    Tile::template store<float>(acc, p.part + (size_t)blockIdx.z * p.M * p.N + at, p.N, o.a_rows, o.b_rows,
-                                (p.N & 3) == 0);
-  else Tile::template store<YT>(acc, (YT *)p.y + at, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
+  DenseItem<Tile, YT> item(p);
+  Tile::template run<false>(lds, item);
 }
 
-// Rows sorted by expert: blockIdx.x runs over the tiles of all experts (each expert's
-// rows in tiles of their own; workgroups past the last tile end).
+// Rows sorted by expert, each expert's in tiles of their own.
 struct GroupArgs {
   const uint8_t *a, *sa;
   void *y;
@@ -68,26 +91,58 @@ struct GroupArgs {
   const uint8_t *b[FP8_MAXE], *sb[FP8_MAXE];
 };
 
-// mts: tiles of rows there may be. An XCD's run of tiles goes down the rows first: the
-// tiles of an expert's rows share its weights in that L2.
+// A workgroup's tiles: every gridDim.x-th of all. An XCD's run of them goes down the rows
+// first: the tiles of an expert's rows share its weights in that L2.
 template <typename Tile, typename YT>
-__global__ __launch_bounds__(Tile::NT, 2) void fp4_grouped_kernel(const GroupArgs p, uint32_t mts) {
+struct GroupItems {
+  const GroupArgs &p;
+  const ExpertTiles<Tile::BM> rows;
+  const uint32_t mts, nts;
+  const int steps, span;
+  uint32_t m0, end, n0;  // of the tile whose sums come next
+  __device__ __forceinline__ GroupItems(const GroupArgs &args)
+      : p(args), rows(p.offsets, p.E, p.R), mts(rows.total()), nts((p.N + Tile::BN - 1) / Tile::BN),
+        steps((int)((p.K + 255) >> 8)), span((steps + 1) & ~1) {}
+  __device__ __forceinline__ int where(int i, uint32_t &first, uint32_t &last, uint32_t &col) const {
+    const uint32_t at = blockIdx.x + (uint32_t)i * gridDim.x;
+    if (at >= mts * nts) return -1;
+    uint32_t mt, nt;
+    xcd_tile<0x40000000>(at, mts, nts, mt, nt);
+    col = nt * Tile::BN;
+    return rows.find(mt, first, last);
+  }
+  __device__ __forceinline__ bool at(int i, Fp4Operands &o) const {
+    uint32_t first, last, col;
+    const int e = where(i, first, last, col);
+    if (e < 0) return false;
+    fill_operands(o, p.a, p.lda, p.sa, p.b[e], p.ldb, p.sb[e], first, min((uint32_t)Tile::BM, last - first), col,
+                  min((uint32_t)Tile::BN, p.N - col), p.K);
+    o.t0 = 0;
+    o.t1 = steps;
+    return true;
+  }
+  __device__ __forceinline__ bool take(int i, int &from, int &to) {
+    from = 0;
+    to = steps;
+    return where(i, m0, end, n0) >= 0;
+  }
+  template <typename Acc>
+  __device__ __forceinline__ void store(const Acc &acc) const {
+    Tile::template store<YT>(acc, (YT *)p.y + (size_t)m0 * p.N + n0, p.N, (int)min((uint32_t)Tile::BM, end - m0),
+                             (int)min((uint32_t)Tile::BN, p.N - n0), quads<YT>(p.y, p.N));
+  }
+};
+
+// MANY: as many workgroups as are resident at once take tiles in turn. Rows of 16 experts, 2048 x
+// 5632, 1024 rows of uneven experts 37.6 -> 32.8 us, 2048 rows 45.3 -> 41.7, 64 rows in four
+// experts 12.1 -> 10.2. Not for 256 x 256, which then spills 76 registers (a dense 4096^3 43 -> 164
+// us), nor for the dense product, whose prologue looks up no expert (1024 x 4096 x 4096 20.0 -> 21.1,
+// 1999 x 11008 x 4096 58 -> 68).
+template <typename Tile, typename YT, bool MANY>
+__global__ __launch_bounds__(Tile::NT, 2) void fp4_grouped_kernel(const GroupArgs p) {
   extern __shared__ __align__(16) uint32_t lds[];
-  constexpr int BM = Tile::BM, BN = Tile::BN;
-  uint32_t mt, nt;
-  xcd_tile<0x40000000>(blockIdx.x, mts, (p.N + BN - 1) / BN, mt, nt);
-  uint32_t m0, end;
-  const int e = expert_tile<BM>(p.offsets, p.E, p.R, mt, m0, end);
-  if (e < 0) return;
-  const uint32_t n0 = nt * BN;
-  Fp4Operands o;
-  fill_operands(o, p.a, p.lda, p.sa, p.b[e], p.ldb, p.sb[e], m0, min((uint32_t)BM, end - m0), n0,
-                min((uint32_t)BN, p.N - n0), p.K);
-  o.t0 = 0;
-  o.t1 = (int)((p.K + 255) >> 8);
-  f32x4 acc[Tile::FN][Tile::FM];
-  Tile::run(lds, o, acc);
-  Tile::template store<YT>(acc, (YT *)p.y + (size_t)m0 * p.N + n0, p.N, o.a_rows, o.b_rows, quads<YT>(p.y, p.N));
+  GroupItems<Tile, YT> items(p);
+  Tile::template run<MANY>(lds, items);
 }
 
 template <int RT, int TT, typename XT, typename YT>
@@ -96,8 +151,15 @@ __global__ __launch_bounds__(FP4_SK_WAVES * 64) void fp4_skinny_kernel(const Fp4
   fp4_skinny<RT, TT, XT, YT>(p, blockIdx.x * 16 * RT, reinterpret_cast<f32x4 *>(lds));
 }
 
+// Workgroups for so many tiles: as many as are resident at once, a multiple of the XCDs.
+template <typename Tile>
+unsigned resident(size_t tiles, int cus) {
+  const size_t most = max(8, (160 << 10) / Tile::LDS_BYTES * cus & ~7);
+  return (unsigned)min(tiles, most);
+}
+
 template <typename Tile, typename YT>
-hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
+hipError_t dense_go(const DenseArgs &p, int S, int cus, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const size_t tiles = (size_t)((p.M + Tile::BM - 1) / Tile::BM) * ((p.N + Tile::BN - 1) / Tile::BN);
   if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
@@ -119,14 +181,14 @@ static_assert(3 * Tile64x64::LDS_BYTES <= 160 << 10, "three workgroups to a comp
 static_assert(2 * Tile64x128::LDS_BYTES <= 160 << 10, "two workgroups to a compute unit");
 
 template <typename YT>
-hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
+hipError_t dense_tile(int tile, const DenseArgs &p, int S, int cus, hipStream_t stream) {
   switch (tile) {
-    case FP4_T_256X256: return dense_go<Tile256x256, YT>(p, S, stream);
-    case FP4_T_192X256: return dense_go<Tile192x256, YT>(p, S, stream);
-    case FP4_T_128X256: return dense_go<Tile128x256, YT>(p, S, stream);
-    case FP4_T_128X192: return dense_go<Tile128x192, YT>(p, S, stream);
-    case FP4_T_64X128: return dense_go<Tile64x128, YT>(p, S, stream);
-    default: return dense_go<Tile64x64, YT>(p, S, stream);
+    case FP4_T_256X256: return dense_go<Tile256x256, YT>(p, S, cus, stream);
+    case FP4_T_192X256: return dense_go<Tile192x256, YT>(p, S, cus, stream);
+    case FP4_T_128X256: return dense_go<Tile128x256, YT>(p, S, cus, stream);
+    case FP4_T_128X192: return dense_go<Tile128x192, YT>(p, S, cus, stream);
+    case FP4_T_64X128: return dense_go<Tile64x128, YT>(p, S, cus, stream);
+    default: return dense_go<Tile64x64, YT>(p, S, cus, stream);
   }
 }
 
@@ -156,25 +218,25 @@ hipError_t skinny_any(int rt, const Fp4Skinny &p, hipStream_t stream) {
   return p.M > 16 ? skinny_go<2, uint8_t, YT>(rt, p, stream) : skinny_go<1, uint8_t, YT>(rt, p, stream);
 }
 
-template <typename Tile, typename YT>
-hipError_t grouped_go(const GroupArgs &p, hipStream_t stream) {
+template <typename Tile, typename YT, bool MANY>
+hipError_t grouped_go(const GroupArgs &p, int cus, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const size_t mts = (size_t)(p.R + Tile::BM - 1) / Tile::BM + p.E, tiles = mts * ((p.N + Tile::BN - 1) / Tile::BN);
   if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
-  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(fp4_grouped_kernel<Tile, YT>), Tile::LDS_BYTES, done);
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(fp4_grouped_kernel<Tile, YT, MANY>), Tile::LDS_BYTES, done);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((fp4_grouped_kernel<Tile, YT>), dim3((unsigned)tiles), dim3(Tile::NT), Tile::LDS_BYTES, stream, p,
-                     (uint32_t)mts);
+  hipLaunchKernelGGL((fp4_grouped_kernel<Tile, YT, MANY>), dim3(MANY ? resident<Tile>(tiles, cus) : (unsigned)tiles), dim3(Tile::NT), Tile::LDS_BYTES,
+                     stream, p);
   return hipGetLastError();
 }
 
 template <typename YT>
-hipError_t grouped_any(const GroupArgs &p, int tile, hipStream_t stream) {
+hipError_t grouped_any(const GroupArgs &p, int tile, int cus, hipStream_t stream) {
   switch (tile) {
-    case FP4_T_256X256: return grouped_go<Tile256x256, YT>(p, stream);
-    case FP4_T_128X256: return grouped_go<Tile128x256, YT>(p, stream);
-    case FP4_T_64X128: return grouped_go<Tile64x128, YT>(p, stream);
-    default: return grouped_go<Tile64x64, YT>(p, stream);
+    case FP4_T_256X256: return grouped_go<Tile256x256, YT, false>(p, cus, stream);
+    case FP4_T_128X256: return grouped_go<Tile128x256, YT, true>(p, cus, stream);
+    case FP4_T_64X128: return grouped_go<Tile64x128, YT, true>(p, cus, stream);
+    default: return grouped_go<Tile64x64, YT, true>(p, cus, stream);
   }
 }
 
@@ -182,13 +244,14 @@ hipError_t grouped_any(const GroupArgs &p, int tile, hipStream_t stream) {
 
 hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
                              const uint8_t *sb, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
-                             const Fp4Plan &plan, float *part, hipStream_t stream) {
+                             const Fp4Plan &plan, float *part, int cus, hipStream_t stream) {
   if (plan.tile == FP4_T_SKINNY) {
     const Fp4Skinny p = {a, sa, b, sb, y, lda, ldb, M, K, N, 0};
     return yt_bf16 ? skinny_any<uint16_t>(plan.per, p, stream) : skinny_any<float>(plan.per, p, stream);
   }
   const DenseArgs p = {a, b, sa, sb, y, plan.S > 1 ? part : nullptr, lda, ldb, M, K, N, plan.per};
-  const hipError_t e = yt_bf16 ? dense_tile<uint16_t>(plan.tile, p, plan.S, stream) : dense_tile<float>(plan.tile, p, plan.S, stream);
+  const hipError_t e = yt_bf16 ? dense_tile<uint16_t>(plan.tile, p, plan.S, cus, stream)
+                                  : dense_tile<float>(plan.tile, p, plan.S, cus, stream);
   if (e != hipSuccess || plan.S == 1) return e;
   const size_t n = (size_t)M * N;
   const dim3 grid((unsigned)((n + 1023) / 1024));
@@ -220,7 +283,7 @@ hipError_t launch_fp4_grouped(const uint8_t *a, size_t lda, const uint8_t *sa, c
     p.sb[e] = sb[e];
   }
   const int tile = fp4_grouped_tile(R, K, N, (uint32_t)E, cus);
-  return yt_bf16 ? grouped_any<uint16_t>(p, tile, stream) : grouped_any<float>(p, tile, stream);
+  return yt_bf16 ? grouped_any<uint16_t>(p, tile, cus, stream) : grouped_any<float>(p, tile, cus, stream);
 }
 
 }  // namespace frx

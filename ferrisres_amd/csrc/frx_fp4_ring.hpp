@@ -47,22 +47,23 @@ struct Fp4Ring {
     uint32_t av[2], bv[2], at[2], bt[2], sv;
     uint32_t lda8, ldb8, sld64, a_last, b_last, s_a_last, s_b_last;
     int wave, last;  // last: K's last step
+    int t, t1;       // the step that is loaded next, and the item's end
   };
   struct Step {
     uint32_t *data, *scales;
     int t;
     uint32_t av[2], bv[2];
   };
-  // Step t into stage `stage`. A step past K's last one is zeros.
-  __device__ __forceinline__ static Step step(uint32_t *lds, const Ctx &c, int stage, int t) {
+  // The next step, g-th of all, into stage `stage`. A step past its item's last one is zeros.
+  __device__ __forceinline__ static Step step(uint32_t *lds, const Ctx &c, int stage, int g) {
     Step s;
     s.data = lds + stage;
-    s.scales = lds + NS * DATA + ((t >> 1) & 1) * SCALES;
-    s.t = t;
+    s.scales = lds + NS * DATA + ((g >> 1) & 1) * SCALES;
+    s.t = c.t;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      s.av[h] = t < c.last ? c.av[h] : t == c.last ? c.at[h] : FP4_OUTSIDE;
-      s.bv[h] = t < c.last ? c.bv[h] : t == c.last ? c.bt[h] : FP4_OUTSIDE;
+      s.av[h] = c.t >= c.t1 ? FP4_OUTSIDE : c.t < c.last ? c.av[h] : c.at[h];
+      s.bv[h] = c.t >= c.t1 ? FP4_OUTSIDE : c.t < c.last ? c.bv[h] : c.bt[h];
     }
     return s;
   }
@@ -94,9 +95,17 @@ struct Fp4Ring {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (0x7 << 4));
   }
 
-  // o.t0 is even: the scales come in pairs of steps.
-  __device__ static void run(uint32_t *lds, const Fp4Operands &o, f32x4 (&acc)[FN][FM]) {
+  // The workgroup's items (tiles, or slices of K of tiles) one after the other, through one ring:
+  // the next item's first steps are on their way while one's last are multiplied and its
+  // sums stored. items.at(i, o): operands of the i-th, false behind the last; items.take(i, t0,
+  // t1): the steps of the i-th, whose sums items.store(acc) takes; items.span: steps of an item,
+  // even, as the scales come in pairs (an item's last step may be zeros). !MANY: one item.
+  template <bool MANY, typename Items>
+  __device__ static void run(uint32_t *lds, Items &items) {
     const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    Fp4Operands o;
+    int item = 0, loading = 0;
+    if (!items.at(0, o)) return;
     Ctx c;
     c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     c.last = (o.K + 255) / 256 - 1;
@@ -114,19 +123,35 @@ struct Fp4Ring {
     c.lda8 = 8 * o.lda;
     c.ldb8 = 8 * o.ldb;
     c.sld64 = 64 * o.s_ld;
-    c.a_last = (uint32_t)((o.a_rows - 1) >> 3) * c.lda8;
-    c.b_last = (uint32_t)((o.b_rows - 1) >> 3) * c.ldb8;
-    c.s_a_last = (uint32_t)((o.a_rows - 1) >> 6) * c.sld64;
-    c.s_b_last = (uint32_t)((o.b_rows - 1) >> 6) * c.sld64;
-    c.ra = buffer_rsrc(o.a, (uint32_t)(o.a_rows - 1) * o.lda + (uint32_t)o.K / 2);
-    c.rb = buffer_rsrc(o.b, (uint32_t)(o.b_rows - 1) * o.ldb + (uint32_t)o.K / 2);
-    c.rsa = buffer_rsrc(o.sa, (uint32_t)o.a_rows * o.s_ld);
-    c.rsb = buffer_rsrc(o.sb, (uint32_t)o.b_rows * o.s_ld);
+    const auto begin = [&](const Fp4Operands &q) {
+      c.a_last = (uint32_t)((q.a_rows - 1) >> 3) * c.lda8;
+      c.b_last = (uint32_t)((q.b_rows - 1) >> 3) * c.ldb8;
+      c.s_a_last = (uint32_t)((q.a_rows - 1) >> 6) * c.sld64;
+      c.s_b_last = (uint32_t)((q.b_rows - 1) >> 6) * c.sld64;
+      c.ra = buffer_rsrc(q.a, (uint32_t)(q.a_rows - 1) * q.lda + (uint32_t)q.K / 2);
+      c.rb = buffer_rsrc(q.b, (uint32_t)(q.b_rows - 1) * q.ldb + (uint32_t)q.K / 2);
+      c.rsa = buffer_rsrc(q.sa, (uint32_t)q.a_rows * q.s_ld);
+      c.rsb = buffer_rsrc(q.sb, (uint32_t)q.b_rows * q.s_ld);
+      c.t = q.t0;
+      c.t1 = q.t1;
+    };
+    begin(o);
+    const int span = items.span;
+    int to_load = span;
+    const auto loaded = [&]() {  // one more step is
+      c.t++;
+      if (MANY && --to_load == 0) {
+        to_load = span;
+        Fp4Operands q;
+        if (items.at(++loading, q)) begin(q);
+        else c.t = c.t1 = 0;  // zeros, and scales that do not matter
+      }
+    };
+    f32x4 acc[FN][FM];
 #pragma unroll
     for (int fn = 0; fn < FN; fn++)
 #pragma unroll
       for (int fm = 0; fm < FM; fm++) acc[fn][fm] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (o.t0 >= o.t1) return;
 
     const int xo = (wm * TM + l16) * 32, wo = (BM + wn * TN + l16) * 32;  // dwords of a stage
     const int p0 = ((2 * g) ^ xswz(l16)) * 4, p1 = ((2 * g + 1) ^ xswz(l16)) * 4;
@@ -137,20 +162,21 @@ struct Fp4Ring {
     };
     const uint32_t keep = (64 * g < left ? 0xFFu : 0) | (64 * g + 32 < left ? 0xFF00u : 0);
 
-    // (steps from o.t1 on are loaded as well: the waits go by the number of loads)
+    // (steps behind the last item are loaded as well: the waits go by the number of loads)
 #pragma unroll
     for (int i = 0; i < NS; i++) {
-      const Step s = step(lds, c, i * DATA, o.t0 + i);
+      const Step s = step(lds, c, i * DATA, i);
       if (i % 2 == 0) load_scales(c, s);
 #pragma unroll
       for (int j = 0; j < CODES; j++) load(j, c, s);
+      loaded();
     }
     wait_vmcnt<(NS - 1) * CODES + (NS == 3 ? SPW : 0)>();
     barrier_nofence();
     u32x4 w[2][FN], x[2][FM];
     uint32_t sw[FN], sx[FM], swn[FN], sxn[FM];
     {
-      const uint32_t *sc = lds + NS * DATA + ((o.t0 >> 1) & 1) * SCALES;
+      const uint32_t *sc = lds + NS * DATA;
 #pragma unroll
       for (int f = 0; f < FN; f++) {
         w[0][f] = op(lds, wo + f * 512 + p0);
@@ -162,17 +188,19 @@ struct Fp4Ring {
         sx[f] = scale(sc, 0, so + f * 128);
       }
     }
-    int here = 0;
-    for (int t = o.t0; t < o.t1; t++) {
+    int here = 0, t, t1, to_do = span;
+    items.take(0, t, t1);
+    for (int n = 0;; n++) {
       uint32_t *cur = lds + here;
       const int stage = here;
       here = here == (NS - 1) * DATA ? 0 : here + DATA;
       uint32_t *nxt = lds + here;
-      if (t == c.last) {  // scales past a row's blocks, whatever they are: none that is a NaN
+      if (t >= c.last || t >= t1) {  // scales past a row's blocks, whatever they are: none that is a NaN
+        const uint32_t mask = t >= t1 ? 0 : keep;
 #pragma unroll
-        for (int f = 0; f < FN; f++) sw[f] &= keep;
+        for (int f = 0; f < FN; f++) sw[f] &= mask;
 #pragma unroll
-        for (int f = 0; f < FM; f++) sx[f] &= keep;
+        for (int f = 0; f < FM; f++) sx[f] &= mask;
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -186,23 +214,24 @@ struct Fp4Ring {
         __builtin_amdgcn_sched_barrier(0);
       }
       // every wave is done with this stage, the next one has landed; in flight behind it NS - 2 steps
-      const bool even = ((t + NS) & 1) == 0;  // the step that is loaded now
+      // (and an item's stores: waited for with the loads before them)
+      const bool even = ((n + NS) & 1) == 0;  // the step that is loaded now
       if (NS == 2) wait_all_but<0>();
       else if (even) wait_all_but<(NS - 2) * CODES>();  // (the step before, an odd one)
       else wait_all_but<(NS - 2) * CODES + SPW>();
       barrier_nofence();
       __builtin_amdgcn_sched_barrier(0);
-      const Step s = step(lds, c, stage, t + NS);
-      const uint32_t *sc = lds + NS * DATA + (((t + 1) >> 1) & 1) * SCALES;
+      const Step s = step(lds, c, stage, n + NS);
+      const uint32_t *sc = lds + NS * DATA + (((n + 1) >> 1) & 1) * SCALES;
       if (even) load_scales(c, s);
 #pragma unroll
       for (int fm = 0; fm < FM; fm++) {
         x[0][fm] = op(nxt, xo + fm * 512 + p0);
-        sxn[fm] = scale(sc, t + 1, so + fm * 128);
+        sxn[fm] = scale(sc, n + 1, so + fm * 128);
 #pragma unroll
         for (int f = fm * FN / FM; f < (fm + 1) * FN / FM; f++) {
           w[0][f] = op(nxt, wo + f * 512 + p0);
-          swn[f] = scale(sc, t + 1, bo + f * 128);
+          swn[f] = scale(sc, n + 1, bo + f * 128);
         }
 #pragma unroll
         for (int j = fm * CODES / FM; j < (fm + 1) * CODES / FM; j++) load(j, c, s);
@@ -215,6 +244,17 @@ struct Fp4Ring {
       for (int f = 0; f < FN; f++) sw[f] = swn[f];
 #pragma unroll
       for (int f = 0; f < FM; f++) sx[f] = sxn[f];
+      loaded();
+      t++;
+      if (MANY ? --to_do == 0 : t == t1) {
+        items.store(acc);
+        if (!MANY || !items.take(++item, t, t1)) break;
+        to_do = span;
+#pragma unroll
+        for (int fn = 0; fn < FN; fn++)
+#pragma unroll
+          for (int fm = 0; fm < FM; fm++) acc[fn][fm] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      }
     }
     wait_vmcnt<0>();  // nothing is in flight into LDS any more
   }

@@ -378,7 +378,7 @@ hipError_t launch_fp4_dequantize(const uint8_t *q, size_t ldq, const uint8_t *sc
 // [S][M][N] in part, added in order.
 hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
                              const uint8_t *sb, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
-                             const Fp4Plan &plan, float *part, hipStream_t stream);
+                             const Fp4Plan &plan, float *part, int cus, hipStream_t stream);
 // x f32 or bf16 [M][K], quantised on the way by every workgroup for itself
 // (FP4_T_SKINNY plans whose activations fit: fp4_act_fits).
 constexpr uint32_t FP4_ACT_MAX_M = 4;

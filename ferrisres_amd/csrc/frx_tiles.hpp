@@ -33,29 +33,39 @@ __device__ __forceinline__ void expert_rows(const uint32_t *offsets, int e, uint
   end = max(min(offsets[e + 1], R), first);
 }
 
-// The expert of tile mt when every expert's rows are cut into tiles of BM, and
-// the tile's first row and its expert's last + 1; -1 past the last tile.
-// Lane e counts expert e's tiles; the expert is the first whose running count
-// passes mt.
+// Every expert's rows cut into tiles of BM. Lane e holds expert e's; the expert of a tile is
+// the first whose running count passes it.
+template <int BM>
+struct ExpertTiles {
+  uint32_t first, last, before, upto;
+  __device__ __forceinline__ ExpertTiles(const uint32_t *offsets, int E, uint32_t R) {
+    const int lane = threadIdx.x & 63;
+    first = last = 0;
+    if (lane < E) expert_rows(offsets, lane, R, first, last);
+    const uint32_t tiles = (last - first + BM - 1) / BM;
+    upto = tiles;
+    for (int s = 1; s < 64; s <<= 1) {
+      const uint32_t v = (uint32_t)__shfl_up((int)upto, s);
+      if (lane >= s) upto += v;
+    }
+    before = upto - tiles;
+  }
+  __device__ __forceinline__ uint32_t total() const { return (uint32_t)__builtin_amdgcn_readlane((int)upto, 63); }
+  // Tile mt's expert, its first row and its expert's last + 1; -1 past the last tile.
+  __device__ __forceinline__ int find(uint32_t mt, uint32_t &m0, uint32_t &end) const {
+    const unsigned long long past = __ballot(upto > mt);
+    if (past == 0) return -1;
+    const int e = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+    m0 = (uint32_t)__builtin_amdgcn_readlane((int)first, e) + (mt - (uint32_t)__builtin_amdgcn_readlane((int)before, e)) * BM;
+    end = (uint32_t)__builtin_amdgcn_readlane((int)last, e);
+    return e;
+  }
+};
+
 template <int BM>
 __device__ __forceinline__ int expert_tile(const uint32_t *offsets, int E, uint32_t R, uint32_t mt, uint32_t &m0,
                                            uint32_t &end) {
-  const int lane = threadIdx.x & 63;
-  uint32_t first = 0, last = 0;
-  if (lane < E) expert_rows(offsets, lane, R, first, last);
-  const uint32_t tiles = (last - first + BM - 1) / BM;
-  uint32_t incl = tiles;
-  for (int s = 1; s < 64; s <<= 1) {
-    const uint32_t v = (uint32_t)__shfl_up((int)incl, s);
-    if (lane >= s) incl += v;
-  }
-  const unsigned long long past = __ballot(lane < E && incl > mt);
-  if (past == 0) return -1;
-  const int e = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
-  const uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)(incl - tiles), e);
-  m0 = (uint32_t)__builtin_amdgcn_readlane((int)first, e) + (mt - before) * BM;
-  end = (uint32_t)__builtin_amdgcn_readlane((int)last, e);
-  return e;
+  return ExpertTiles<BM>(offsets, E, R).find(mt, m0, end);
 }
 
 // y = the parts added in order, four values a thread (n of them, parts n apart).
