@@ -1780,7 +1780,7 @@ static frx_status fp4_run(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint
     if (st != FRX_OK) return st;
   }
   const hipError_t e = frx::launch_fp4_linear(a, lda, sa, b, ldb, sb, y, yt == FRX_BF16, M, K, N, plan,
-                                              reinterpret_cast<float *>(ctx->gk_ws), ctx->cus, ctx->stream);
+                                              reinterpret_cast<float *>(ctx->gk_ws), ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "fp4 linear launch");
   return FRX_OK;
 }

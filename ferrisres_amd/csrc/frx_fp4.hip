@@ -159,7 +159,7 @@ unsigned resident(size_t tiles, int cus) {
 }
 
 template <typename Tile, typename YT>
-hipError_t dense_go(const DenseArgs &p, int S, int cus, hipStream_t stream) {
+hipError_t dense_go(const DenseArgs &p, int S, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const size_t tiles = (size_t)((p.M + Tile::BM - 1) / Tile::BM) * ((p.N + Tile::BN - 1) / Tile::BN);
   if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
@@ -181,14 +181,14 @@ static_assert(3 * Tile64x64::LDS_BYTES <= 160 << 10, "three workgroups to a comp
 static_assert(2 * Tile64x128::LDS_BYTES <= 160 << 10, "two workgroups to a compute unit");
 
 template <typename YT>
-hipError_t dense_tile(int tile, const DenseArgs &p, int S, int cus, hipStream_t stream) {
+hipError_t dense_tile(int tile, const DenseArgs &p, int S, hipStream_t stream) {
   switch (tile) {
-    case FP4_T_256X256: return dense_go<Tile256x256, YT>(p, S, cus, stream);
-    case FP4_T_192X256: return dense_go<Tile192x256, YT>(p, S, cus, stream);
-    case FP4_T_128X256: return dense_go<Tile128x256, YT>(p, S, cus, stream);
-    case FP4_T_128X192: return dense_go<Tile128x192, YT>(p, S, cus, stream);
-    case FP4_T_64X128: return dense_go<Tile64x128, YT>(p, S, cus, stream);
-    default: return dense_go<Tile64x64, YT>(p, S, cus, stream);
+    case FP4_T_256X256: return dense_go<Tile256x256, YT>(p, S, stream);
+    case FP4_T_192X256: return dense_go<Tile192x256, YT>(p, S, stream);
+    case FP4_T_128X256: return dense_go<Tile128x256, YT>(p, S, stream);
+    case FP4_T_128X192: return dense_go<Tile128x192, YT>(p, S, stream);
+    case FP4_T_64X128: return dense_go<Tile64x128, YT>(p, S, stream);
+    default: return dense_go<Tile64x64, YT>(p, S, stream);
   }
 }
 
@@ -197,8 +197,8 @@ hipError_t skinny_rt(const Fp4Skinny &p, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   constexpr size_t red = fp4_skinny_red_bytes(RT * TT);
   const auto kernel = fp4_skinny_kernel<RT, TT, XT, YT>;
-  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel),
-                                  (int)(red + (sizeof(XT) == 1 ? 0 : FP4_ACT_MAX_BYTES)), done);
+  constexpr size_t most = FP4_ACT_MAX_VALUES / 2 + FP4_ACT_MAX_VALUES / 32 + 4 * FP4_ACT_MAX_M;  // fp4_skinny_act_bytes
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), (int)(red + (sizeof(XT) == 1 ? 0 : most)), done);
   if (e != hipSuccess) return e;
   const size_t lds = red + (sizeof(XT) == 1 ? 0 : fp4_skinny_act_bytes(p.M, p.K));
   hipLaunchKernelGGL(kernel, dim3((p.N + 16 * RT - 1) / (16 * RT)), dim3(FP4_SK_WAVES * 64), lds, stream, p);
@@ -244,14 +244,14 @@ hipError_t grouped_any(const GroupArgs &p, int tile, int cus, hipStream_t stream
 
 hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
                              const uint8_t *sb, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
-                             const Fp4Plan &plan, float *part, int cus, hipStream_t stream) {
+                             const Fp4Plan &plan, float *part, hipStream_t stream) {
   if (plan.tile == FP4_T_SKINNY) {
     const Fp4Skinny p = {a, sa, b, sb, y, lda, ldb, M, K, N, 0};
     return yt_bf16 ? skinny_any<uint16_t>(plan.per, p, stream) : skinny_any<float>(plan.per, p, stream);
   }
   const DenseArgs p = {a, b, sa, sb, y, plan.S > 1 ? part : nullptr, lda, ldb, M, K, N, plan.per};
-  const hipError_t e = yt_bf16 ? dense_tile<uint16_t>(plan.tile, p, plan.S, cus, stream)
-                                  : dense_tile<float>(plan.tile, p, plan.S, cus, stream);
+  const hipError_t e = yt_bf16 ? dense_tile<uint16_t>(plan.tile, p, plan.S, stream)
+                                  : dense_tile<float>(plan.tile, p, plan.S, stream);
   if (e != hipSuccess || plan.S == 1) return e;
   const size_t n = (size_t)M * N;
   const dim3 grid((unsigned)((n + 1023) / 1024));
@@ -261,7 +261,7 @@ hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, co
 }
 
 bool fp4_act_fits(uint32_t M, uint32_t K) {
-  return M <= FP4_ACT_MAX_M && fp4_skinny_act_bytes(M, K) <= FP4_ACT_MAX_BYTES;
+  return M <= FP4_ACT_MAX_M && (uint64_t)M * K <= FP4_ACT_MAX_VALUES;
 }
 
 hipError_t launch_fp4_linear_act(const void *x, int xt_bf16, const uint8_t *b, size_t ldb, const uint8_t *sb, void *y,

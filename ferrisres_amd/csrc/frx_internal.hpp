@@ -378,11 +378,12 @@ hipError_t launch_fp4_dequantize(const uint8_t *q, size_t ldq, const uint8_t *sc
 // [S][M][N] in part, added in order.
 hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
                              const uint8_t *sb, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
-                             const Fp4Plan &plan, float *part, int cus, hipStream_t stream);
-// x f32 or bf16 [M][K], quantised on the way by every workgroup for itself
-// (FP4_T_SKINNY plans whose activations fit: fp4_act_fits).
-constexpr uint32_t FP4_ACT_MAX_M = 4;
-constexpr size_t FP4_ACT_MAX_BYTES = 64 << 10;
+                             const Fp4Plan &plan, float *part, hipStream_t stream);
+// x f32 or bf16 [M][K], quantised on the way by every workgroup for itself, where that is few
+// values (fp4_act_fits). us against the two launches, bf16: 1 x 2048 x 5632 4.4 / 5.8, 8 x 2048 x
+// 2048 5.4 / 5.6, 4 x 4096 x 11008 9.3 / 9.3, 1 x 11008 x 4096 8.5 / 8.9; beyond 2 x 11008 x 4096
+// 10.3 / 9.3, 16 x 2048 x 5632 8.6 / 6.4.
+constexpr uint32_t FP4_ACT_MAX_M = 16, FP4_ACT_MAX_VALUES = 16384;
 bool fp4_act_fits(uint32_t M, uint32_t K);
 hipError_t launch_fp4_linear_act(const void *x, int xt_bf16, const uint8_t *b, size_t ldb, const uint8_t *sb, void *y,
                                  int yt_bf16, uint32_t M, uint32_t K, uint32_t N, const Fp4Plan &plan,

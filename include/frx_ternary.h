@@ -467,9 +467,9 @@ frx_status frx_fp4_linear(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint
 
 /* y = x w^T for activations x [M][K] (f32 or bf16, contiguous): frx_fp4_quantize
  * (ROWS) and frx_fp4_linear in one call, with the two calls' result bit for bit.
- * Where M <= 4 and M * (K / 2 + 4 * ceil(K / 128)) <= 65536 it is one launch, the
- * codes in LDS; else they lie in a context workspace (which must be there before a
- * graph capture: FRX_ERR_UNSUPPORTED otherwise). K % 32 == 0. */
+ * Where M <= 16 and M * K <= 16384 it is one launch, the codes in LDS; else they lie
+ * in a context workspace (which must be there before a graph capture:
+ * FRX_ERR_UNSUPPORTED otherwise). K % 32 == 0. */
 frx_status frx_fp4_linear_act(frx_ctx *ctx, const void *x, frx_dtype xt, const uint8_t *b, size_t ldb,
                               const uint8_t *sb, void *y, frx_dtype yt, uint32_t M, uint32_t K, uint32_t N);
 

@@ -182,13 +182,13 @@ static void check_workspaces(frx_ctx *c, uint8_t *zeros, void *out) {
   uint32_t allocs = 1;
   const uint8_t *one[1] = {zeros};
   EXPECT(linear(c, zeros, 16, zeros, zeros, 16, zeros, out, FRX_F32, 40, 32, 8) == FRX_OK);
-  EXPECT(act(c, zeros, FRX_F32, zeros, 16, zeros, out, FRX_F32, 4, 32, 8) == FRX_OK);
+  EXPECT(act(c, zeros, FRX_F32, zeros, 16, zeros, out, FRX_F32, 16, 32, 8) == FRX_OK);
   EXPECT(grouped(c, zeros, 16, zeros, one, 16, one, (const uint32_t *)(void *)zeros, 1, out, FRX_F32, 8, 32, 8) == FRX_OK);
   EXPECT(frx_synchronize(c) == FRX_OK);
   EXPECT(frx_workspace_stats(c, &live, &retired, &allocs) == FRX_OK && live == 0 && allocs == 0);
-  EXPECT(act(c, zeros, FRX_F32, zeros, 16, zeros, out, FRX_F32, 5, 32, 8) == FRX_OK);
+  EXPECT(act(c, zeros, FRX_F32, zeros, 16, zeros, out, FRX_F32, 17, 32, 8) == FRX_OK);
   EXPECT(frx_workspace_stats(c, &live, &retired, &allocs) == FRX_OK && allocs == 1);
-  EXPECT(act(c, zeros, FRX_BF16, zeros, 16, zeros, out, FRX_F32, 5, 32, 8) == FRX_OK);
+  EXPECT(act(c, zeros, FRX_BF16, zeros, 16, zeros, out, FRX_F32, 17, 32, 8) == FRX_OK);
   EXPECT(frx_workspace_stats(c, &live, &retired, &allocs) == FRX_OK && allocs == 1);
   EXPECT(ffn(c, zeros, FRX_F32, NULL, FRX_F32, one, one, one, one, one, one, 2, 32, 32, 1, 1, FRX_ACT_SILU, out, FRX_F32,
              (uint32_t *)(void *)zeros, (float *)(void *)zeros) == FRX_OK);

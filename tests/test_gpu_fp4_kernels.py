@@ -71,7 +71,8 @@ def test_few_tokens(ctx, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("xt", ["bf16", "f32"])
-@pytest.mark.parametrize("M,K,N", [(1, 4128, 40), (4, 160, 8300), (3, 1056, 16300), (2, 12320, 5000)])
+@pytest.mark.parametrize("M,K,N", [(1, 4128, 40), (4, 160, 8300), (3, 1056, 16300), (2, 12320, 5000),
+                                   (16, 1024, 90), (16, 1056, 90), (9, 1760, 8300), (5, 3264, 16300), (11, 32, 20)])
 def test_few_activations(ctx, M, K, N, xt):
     """The launch that makes the codes itself against the two calls, bit for bit."""
     g = torch.Generator(device=DEV).manual_seed(K)
