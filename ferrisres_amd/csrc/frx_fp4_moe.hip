@@ -21,6 +21,12 @@
 // instructions for 128 columns, and one exchange of the waves' sums through LDS. The weights
 // of the next tiles are on their way meanwhile, by LDS DMA into a ring that each wave has for
 // itself (held in registers they were waited for at every turn of the loop).
+//
+// 16 experts, top 2, H 2048, I 5632, route + gate and up + down + join, us: 1 token bf16 14.6 + 9.4
+// + 5.0 (its weights' bytes 7.1 at a copy's rate; a workgroup's way to its first tile is 5 to 6,
+// much of it instructions that are fetched for the first time), 8 tokens 6.0 + 31.4 + 20.2 + 4.6
+// (37; the weights at 4.1 TB/s), 61 tokens f32 78.6 + 42.2 + 5.0 (57; a tile's exchange). Waits that leave
+// out a wave's own stores gained nothing.
 #include "frx_fp4.hpp"
 #include "frx_internal.hpp"
 
@@ -677,8 +683,11 @@ hipError_t gate_up_go(const FewArgs &a, int cus, hipStream_t stream) {
 template <typename XT>
 hipError_t gate_up(const FewArgs &a, const Fp4FewPlan &plan, int cus, hipStream_t stream) {
   if (plan.slices > 1) return gate_up_go<XT, 4, 1, 3, 1, true>(a, cus, stream);
-  if (plan.steps == 4)
-    return plan.tiles == 1 ? gate_up_go<XT, 4, 1, 3, 1, false>(a, cus, stream) : gate_up_go<XT, 4, 2, 2, 1, false>(a, cus, stream);
+  if (plan.steps == 4) {
+    if constexpr (sizeof(XT) == 2)
+      if (plan.tiles == 2) return gate_up_go<XT, 4, 2, 2, 1, false>(a, cus, stream);
+    return gate_up_go<XT, 4, 1, 3, 1, false>(a, cus, stream);
+  }
   if (plan.tiles == 1) return gate_up_go<XT, 2, 1, 5, 2, false>(a, cus, stream);
   return plan.tiles == 2 ? gate_up_go<XT, 2, 2, 3, 2, false>(a, cus, stream) : gate_up_go<XT, 2, 3, 4, 1, false>(a, cus, stream);
 }

@@ -70,7 +70,7 @@ def test_every_grouped_tile_has_its_shape(rules):
 @pytest.mark.parametrize("planes", [1, 3])
 def test_every_gate_up_kernel_has_a_layer(rules, planes):
     got = {(s, t, slices > 1) for s, t, slices, _ in (rules.few(T, H, E, k, planes, 0) for T, H, _, E, k in LAYERS)}
-    assert got == GATE_UP
+    assert got == (GATE_UP if planes == 1 else GATE_UP - {(4, 2, False)})
 
 
 @pytest.mark.parametrize("planes", [2, 3])
