@@ -246,7 +246,7 @@ hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, co
                              const uint8_t *sb, void *y, int yt_bf16, uint32_t M, uint32_t K, uint32_t N,
                              const Fp4Plan &plan, float *part, hipStream_t stream) {
   if (plan.tile == FP4_T_SKINNY) {
-    const Fp4Skinny p = {a, sa, b, sb, y, lda, ldb, M, K, N, 0};
+    const Fp4Skinny p = {a, sa, b, sb, y, lda, ldb, M, K, N};
     return yt_bf16 ? skinny_any<uint16_t>(plan.per, p, stream) : skinny_any<float>(plan.per, p, stream);
   }
   const DenseArgs p = {a, b, sa, sb, y, plan.S > 1 ? part : nullptr, lda, ldb, M, K, N, plan.per};
@@ -267,8 +267,7 @@ bool fp4_act_fits(uint32_t M, uint32_t K) {
 hipError_t launch_fp4_linear_act(const void *x, int xt_bf16, const uint8_t *b, size_t ldb, const uint8_t *sb, void *y,
                                  int yt_bf16, uint32_t M, uint32_t K, uint32_t N, const Fp4Plan &plan,
                                  hipStream_t stream) {
-  const int vec = ((reinterpret_cast<uintptr_t>(x) | (size_t)K * (xt_bf16 ? 2 : 4)) & 15) == 0;
-  const Fp4Skinny p = {x, nullptr, b, sb, y, K, ldb, M, K, N, vec};
+  const Fp4Skinny p = {x, nullptr, b, sb, y, K, ldb, M, K, N};
   if (xt_bf16)
     return yt_bf16 ? skinny_go<1, uint16_t, uint16_t>(plan.per, p, stream) : skinny_go<1, uint16_t, float>(plan.per, p, stream);
   return yt_bf16 ? skinny_go<1, float, uint16_t>(plan.per, p, stream) : skinny_go<1, float, float>(plan.per, p, stream);

@@ -26,6 +26,27 @@ __device__ __forceinline__ float fp4_power(uint32_t b) {
   return __uint_as_float(b == 0 ? 0x00400000u : b == 255 ? 0x7FC00000u : b << 23);
 }
 
+// Unaligned 16 bytes (a tensor may begin at any element).
+typedef u32x4 __attribute__((aligned(2))) u32x4_u;
+
+// Eight values from p on, which may be any element.
+__device__ __forceinline__ void ld8u(const float *p, float (&v)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4_u *>(p), b = *reinterpret_cast<const u32x4_u *>(p + 4);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[i] = __uint_as_float(a[i]);
+    v[4 + i] = __uint_as_float(b[i]);
+  }
+}
+__device__ __forceinline__ void ld8u(const uint16_t *p, float (&v)[8]) {
+  const u32x4 a = *reinterpret_cast<const u32x4_u *>(p);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[2 * i] = __uint_as_float(a[i] << 16);
+    v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
+  }
+}
+
 // Eight values times inv as eight codes, the first in the lowest bits; zeros under b = 255.
 __device__ __forceinline__ uint32_t fp4_pack8(const float (&v)[8], float inv, uint32_t b) {
   uint32_t c = 0;

@@ -41,9 +41,6 @@ constexpr int WAVES = 8, NT = WAVES * 64;
 constexpr int MOST_SLOTS = FP4_MOE_MAX_T * 64;
 constexpr int KEPT_SLOTS = 512;
 
-// Unaligned 16 bytes (a tensor may begin at any element).
-typedef u32x4 __attribute__((aligned(2))) u32x4_u;
-
 struct FewArgs {
   const void *x, *router;
   uint32_t *idx;
@@ -66,24 +63,6 @@ struct Shared {
   uint8_t token[64];           // and which they are
 };
 
-// Eight values from p on.
-__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
-  const u32x4 a = *reinterpret_cast<const u32x4_u *>(p), b = *reinterpret_cast<const u32x4_u *>(p + 4);
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    v[i] = __uint_as_float(a[i]);
-    v[4 + i] = __uint_as_float(b[i]);
-  }
-}
-__device__ __forceinline__ void load8(const uint16_t *p, float (&v)[8]) {
-  const u32x4 a = *reinterpret_cast<const u32x4_u *>(p);
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    v[2 * i] = __uint_as_float(a[i] << 16);
-    v[2 * i + 1] = __uint_as_float(a[i] & 0xFFFF0000u);
-  }
-}
-
 // A token's logits: a wave for each expert.
 template <int WAVES, typename XT, typename RT>
 __device__ __forceinline__ void router_logits(const XT *x, const RT *router, uint32_t H, int E, float *logit) {
@@ -93,8 +72,8 @@ __device__ __forceinline__ void router_logits(const XT *x, const RT *router, uin
 #pragma unroll 4
     for (uint32_t k = lane * 8; k < H; k += 512) {
       float r[8], v[8];
-      load8(router + (size_t)e * H + k, r);
-      load8(x + k, v);
+      ld8u(router + (size_t)e * H + k, r);
+      ld8u(x + k, v);
 #pragma unroll
       for (int i = 0; i < 8; i++) s = __builtin_fmaf(v[i], r[i], s);
     }
@@ -304,7 +283,7 @@ __device__ __forceinline__ float cut8(float v, uint32_t &plane) {
 __device__ __forceinline__ u32x4 act8(const uint16_t *p, int) { return *reinterpret_cast<const u32x4_u *>(p); }
 __device__ __forceinline__ u32x4 act8(const float *p, int plane) {
   float v[8];
-  load8(p, v);
+  ld8u(p, v);
   uint32_t h[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) {

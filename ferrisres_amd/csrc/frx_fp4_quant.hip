@@ -3,7 +3,8 @@
 // Formulas: frx_fp4_codes.hpp. Bound by memory: 2 or 4 bytes in and 17/32 out a value (the
 // way back the other way round), about 3 VALU operations a value. 11008 x 4096: f32 along the
 // rows 36.0 us (5.7 TB/s), along the columns 44.9, back 44.7; bf16 24.6, 29.5, 25.4. 2048 x 4096
-// bf16 6.3, 7.4, 5.6. Tried and no faster: two pieces of a row a thread, tiles of 256 x 64 along
+// bf16 6.3, 7.4, 5.6. Loads and stores of 16 bytes at any element's address: 2458 x 12829 f32 along
+// the columns and back 38.6 + 37.7 (by single values 144 in all). Tried and no faster: two pieces of a row a thread, tiles of 256 x 64 along
 // the columns (whole lines of codes), divisions in 32 bits.
 #include "frx_fp4_codes.hpp"
 #include "frx_internal.hpp"
@@ -14,8 +15,7 @@ namespace {
 
 // Blocks along the rows: 16 lanes hold 128 columns, 8 values a lane, and write 64 bytes of
 // codes and a dword of scales. A block past K has zero codes and the smallest scale.
-// VEC: x rows 16-byte aligned.
-template <typename XT, bool VEC>
+template <typename XT>
 __global__ __launch_bounds__(256) void fp4_rows_kernel(const XT *__restrict__ x, uint32_t M, uint32_t K, size_t ldx,
                                                        uint32_t kb, uint8_t *__restrict__ q, size_t ldq,
                                                        uint32_t *__restrict__ scale) {
@@ -25,8 +25,8 @@ __global__ __launch_bounds__(256) void fp4_rows_kernel(const XT *__restrict__ x,
   const uint32_t k = b * 128 + (threadIdx.x & 15) * 8;
   const XT *src = x + (size_t)m * ldx + k;
   float v[8];
-  if (VEC && k + 8 <= K) {
-    ld8v(src, v);
+  if (k + 8 <= K) {
+    ld8u(src, v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = k + i < K ? ld1(src + i) : 0.0f;
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void fp4_rows_kernel(const XT *__restrict__ x,
 // Thread (wave w, lane group h of 16, lane c of it) holds rows 32w + 8h .. + 7 of columns
 // 8c .. 8c + 7, so a wave holds whole blocks. A column's 8 rows are a dword of codes; 16
 // of them, swizzled by column / 8, make its 64 bytes in LDS.
-template <typename XT, bool VEC>
+template <typename XT>
 __global__ __launch_bounds__(256) void fp4_cols_kernel(const XT *__restrict__ x, uint32_t M, uint32_t K, size_t ldx,
                                                        uint8_t *__restrict__ q, size_t ldq,
                                                        uint32_t *__restrict__ scale) {
@@ -56,8 +56,8 @@ __global__ __launch_bounds__(256) void fp4_cols_kernel(const XT *__restrict__ x,
   for (int i = 0; i < 8; i++) {
     const XT *src = x + (size_t)(m0 + i) * ldx + k;
     float r[8];
-    if (m0 + i < M && VEC && k + 8 <= K) {
-      ld8v(src, r);
+    if (m0 + i < M && k + 8 <= K) {
+      ld8u(src, r);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; j++) r[j] = m0 + i < M && k + j < K ? ld1(src + j) : 0.0f;
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void fp4_cols_kernel(const XT *__restrict__ x,
 }
 
 // The values of 8 codes a thread.
-template <typename YT, bool VEC>
+template <typename YT>
 __global__ __launch_bounds__(256) void fp4_values_kernel(const uint8_t *__restrict__ q, size_t ldq,
                                                          const uint8_t *__restrict__ scale, uint32_t M, uint32_t K,
                                                          uint32_t groups, YT *__restrict__ y, size_t ldy) {
@@ -112,9 +112,12 @@ __global__ __launch_bounds__(256) void fp4_values_kernel(const uint8_t *__restri
 #undef FRX_FP4_PAIR
   YT *d = y + (size_t)m * ldy + k;
   if constexpr (sizeof(YT) == 4) {
-    if (VEC && k + 8 <= K) {
-      reinterpret_cast<f32x4 *>(d)[0] = (f32x4){v[0], v[1], v[2], v[3]};
-      reinterpret_cast<f32x4 *>(d)[1] = (f32x4){v[4], v[5], v[6], v[7]};
+    if (k + 8 <= K) {
+      uint32_t h[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) h[j] = __float_as_uint(v[j]);
+      reinterpret_cast<u32x4_u *>(d)[0] = (u32x4){h[0], h[1], h[2], h[3]};
+      reinterpret_cast<u32x4_u *>(d)[1] = (u32x4){h[4], h[5], h[6], h[7]};
     } else {
       for (uint32_t j = 0; j < 8 && k + j < K; j++) d[j] = v[j];
     }
@@ -122,9 +125,9 @@ __global__ __launch_bounds__(256) void fp4_values_kernel(const uint8_t *__restri
     uint32_t h[8];  // (exact: two bits of significand)
 #pragma unroll
     for (int j = 0; j < 8; j++) h[j] = __float_as_uint(v[j]) >> 16;
-    if (VEC && k + 8 <= K) {
-      *reinterpret_cast<u32x4 *>(d) = (u32x4){h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16),
-                                             h[6] | (h[7] << 16)};
+    if (k + 8 <= K) {
+      *reinterpret_cast<u32x4_u *>(d) = (u32x4){h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16),
+                                               h[6] | (h[7] << 16)};
     } else {
       for (uint32_t j = 0; j < 8 && k + j < K; j++) d[j] = (uint16_t)h[j];
     }
@@ -135,15 +138,12 @@ template <typename XT>
 hipError_t quantize_t(const XT *x, uint32_t M, uint32_t K, size_t ldx, int cols, uint8_t *q, size_t ldq,
                       uint32_t *scale, hipStream_t stream) {
   const uint32_t kb = (K + 127) / 128, mb = (M + 127) / 128;
-  const bool vec = ((reinterpret_cast<uintptr_t>(x) | (ldx * sizeof(XT))) & 15) == 0;
   const size_t wgs = cols ? (size_t)kb * mb : ((size_t)M * kb + 15) / 16;
   if (wgs > 0xFFFFFFu) return hipErrorInvalidValue;
   if (cols) {
-    const auto fn = vec ? fp4_cols_kernel<XT, true> : fp4_cols_kernel<XT, false>;
-    hipLaunchKernelGGL(fn, dim3((unsigned)wgs), dim3(256), 0, stream, x, M, K, ldx, q, ldq, scale);
+    hipLaunchKernelGGL(fp4_cols_kernel<XT>, dim3((unsigned)wgs), dim3(256), 0, stream, x, M, K, ldx, q, ldq, scale);
   } else {
-    const auto fn = vec ? fp4_rows_kernel<XT, true> : fp4_rows_kernel<XT, false>;
-    hipLaunchKernelGGL(fn, dim3((unsigned)wgs), dim3(256), 0, stream, x, M, K, ldx, kb, q, ldq, scale);
+    hipLaunchKernelGGL(fp4_rows_kernel<XT>, dim3((unsigned)wgs), dim3(256), 0, stream, x, M, K, ldx, kb, q, ldq, scale);
   }
   return hipGetLastError();
 }
@@ -154,9 +154,7 @@ hipError_t values_t(const uint8_t *q, size_t ldq, const uint8_t *scale, uint32_t
   const uint32_t groups = (K + 7) / 8;
   const size_t wgs = ((size_t)M * groups + 255) / 256;
   if (wgs > 0xFFFFFFu) return hipErrorInvalidValue;
-  const bool vec = ((reinterpret_cast<uintptr_t>(y) | (ldy * sizeof(YT))) & 15) == 0;
-  const auto fn = vec ? fp4_values_kernel<YT, true> : fp4_values_kernel<YT, false>;
-  hipLaunchKernelGGL(fn, dim3((unsigned)wgs), dim3(256), 0, stream, q, ldq, scale, M, K, groups, y, ldy);
+  hipLaunchKernelGGL(fp4_values_kernel<YT>, dim3((unsigned)wgs), dim3(256), 0, stream, q, ldq, scale, M, K, groups, y, ldy);
   return hipGetLastError();
 }
 

@@ -27,7 +27,6 @@ struct Fp4Skinny {
   size_t lda;             // bytes of codes, elements of activations
   size_t ldb;
   uint32_t M, K, N;       // M: 1 to 16 * TT
-  int vec;                // activations: rows 16-byte aligned
 };
 
 constexpr int FP4_SK_WAVES = 8;
@@ -48,8 +47,8 @@ __device__ __forceinline__ void fp4_skinny_quantize(const Fp4Skinny &p, uint8_t 
     const int m = b / kbs, k = (b - m * kbs) * 128 + 8 * l;
     const XT *src = static_cast<const XT *>(p.a) + (size_t)m * p.lda + k;
     float v[8];
-    if (p.vec && k + 8 <= K) {
-      ld8v(src, v);
+    if (k + 8 <= K) {
+      ld8u(src, v);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] = k + i < K ? ld1(src + i) : 0.0f;
