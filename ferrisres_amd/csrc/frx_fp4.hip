@@ -67,9 +67,8 @@ struct DenseItem {
   __device__ __forceinline__ void store(const Acc &acc) const {
     const size_t at = (size_t)m0 * p.N + n0;
     if (p.part)
-      Tile::template store<float>(acc, p.part + (size_t)blockIdx.z * p.M * p.N + at, p.N, (int)mr, (int)nr,
-                                  (p.N & 3) == 0);
-    else Tile::template store<YT>(acc, (YT *)p.y + at, p.N, (int)mr, (int)nr, quads<YT>(p.y, p.N));
+      Tile::template store<float>(acc, p.part + (size_t)blockIdx.z * p.M * p.N + at, p.N, (int)mr, (int)nr);
+    else Tile::template store<YT>(acc, (YT *)p.y + at, p.N, (int)mr, (int)nr);
   }
 };
 
@@ -129,7 +128,7 @@ struct GroupItems {
   template <typename Acc>
   __device__ __forceinline__ void store(const Acc &acc) const {
     Tile::template store<YT>(acc, (YT *)p.y + (size_t)m0 * p.N + n0, p.N, (int)min((uint32_t)Tile::BM, end - m0),
-                             (int)min((uint32_t)Tile::BN, p.N - n0), quads<YT>(p.y, p.N));
+                             (int)min((uint32_t)Tile::BN, p.N - n0));
   }
 };
 

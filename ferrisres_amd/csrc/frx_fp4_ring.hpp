@@ -260,11 +260,19 @@ struct Fp4Ring {
   }
 
   template <typename YT>
-  __device__ __forceinline__ static void store(const f32x4 (&acc)[FN][FM], YT *y, size_t ldy, int m_rows, int n_rows,
-                                               bool vec) {
+  __device__ __forceinline__ static void store(const f32x4 (&acc)[FN][FM], YT *y, size_t ldy, int m_rows, int n_rows) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    fp8_store<FN, FM>(acc, y, ldy, (wave % WM) * TM + (lane & 15), (wave / WM) * TN + 4 * (lane >> 4), m_rows, n_rows,
-                      vec);
+    const int m0 = (wave % WM) * TM + (lane & 15), n0 = (wave / WM) * TN + 4 * (lane >> 4);
+#pragma unroll
+    for (int fm = 0; fm < FM; fm++) {
+      const int m = m0 + fm * 16;
+      if (m >= m_rows) continue;
+#pragma unroll
+      for (int fn = 0; fn < FN; fn++) {
+        const int n = n0 + fn * 16;
+        if (n < n_rows) fp4_store4(y + (size_t)m * ldy + n, acc[fn][fm], (uint32_t)(n_rows - n));
+      }
+    }
   }
 };
 

@@ -164,20 +164,7 @@ __device__ __forceinline__ void fp4_skinny(const Fp4Skinny &p, uint32_t n0, f32x
   for (int i = 1; i < FP4_SK_WAVES; i++) v += red[(i * RT * TT + wave) * 64 + lane];
   const uint32_t n = n0 + 16 * (wave / TT) + 4 * g, m = 16 * (wave % TT) + l16;
   if (m >= p.M || n >= p.N) return;
-  YT *d = static_cast<YT *>(p.y) + (size_t)m * p.N + n;
-  const bool vec = ((reinterpret_cast<uintptr_t>(p.y) & (4 * sizeof(YT) - 1)) | (p.N & 3)) == 0;
-  if constexpr (sizeof(YT) == 4) {
-    if (vec) *reinterpret_cast<f32x4 *>(d) = v;
-    else
-      for (uint32_t e = 0; e < 4 && n + e < p.N; e++) d[e] = v[e];
-  } else {
-    uint32_t h[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) h[e] = bf16_rne_nb(v[e]);
-    if (vec) *reinterpret_cast<u32x2 *>(d) = (u32x2){h[0] | (h[1] << 16), h[2] | (h[3] << 16)};
-    else
-      for (uint32_t e = 0; e < 4 && n + e < p.N; e++) d[e] = (uint16_t)h[e];
-  }
+  fp4_store4(static_cast<YT *>(p.y) + (size_t)m * p.N + n, v, p.N - n);
 }
 
 }  // namespace frx
