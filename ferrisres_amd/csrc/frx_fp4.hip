@@ -221,7 +221,7 @@ template <typename Tile, typename YT, bool MANY>
 hipError_t grouped_go(const GroupArgs &p, int cus, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const size_t mts = (size_t)(p.R + Tile::BM - 1) / Tile::BM + p.E, tiles = mts * ((p.N + Tile::BN - 1) / Tile::BN);
-  if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
+  if ((MANY ? tiles : tiles * Tile::NT) > 0xF0000000u) return hipErrorInvalidValue;  // (counted in 32 bits)
   const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(fp4_grouped_kernel<Tile, YT, MANY>), Tile::LDS_BYTES, done);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((fp4_grouped_kernel<Tile, YT, MANY>), dim3(MANY ? resident<Tile>(tiles, cus) : (unsigned)tiles), dim3(Tile::NT), Tile::LDS_BYTES,

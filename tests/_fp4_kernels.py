@@ -20,6 +20,12 @@ GROUPED = {
     "64-one-step": ([3, 0, 5], 4, 32, 90, T64),
     "64x128": ([1, 0, 2, 1, 1, 0, 1, 3, 1, 1], 2, 736, 5010, T64X128),
     "128x256": ([60, 1, 0, 33, 129, 30, 40, 2, 31, 50], 8, 352, 5900, T128X256),
+    # several tiles for a workgroup, of one step to three
+    "64-turns-1": ([7 * i % 10 for i in range(40)], 5, 32, 2200, T64),
+    "64-turns-2": ([7 * i % 10 for i in range(40)], 0, 480, 2190, T64),
+    "64-turns-3": ([7 * i % 10 for i in range(40)], 5, 544, 2210, T64),
+    "64x128-turns-1": ([1 + 3 * i % 9 for i in range(64)], 3, 32, 1900, T64X128),
+    "64x128-turns-3": ([1 + 3 * i % 9 for i in range(64)], 0, 608, 1890, T64X128),
     "256": ([140, 0, 257, 1, 256, 90, 255, 100, 200, 140], 9, 800, 5900, T256),
 }
 

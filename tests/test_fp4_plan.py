@@ -9,7 +9,8 @@ import subprocess
 
 import pytest
 
-from _fp4_kernels import DOWN, FEW, GATE_UP, GROUPED, KS, LAYERS, ROWS16, ROWS16_K, SPLIT, T128X256, T256, T64, T64X128, TILES
+from _fp4_kernels import (DOWN, FEW, GATE_UP, GROUPED, KS, LAYERS, ROWS16, ROWS16_K, SPLIT, T128X192, T128X256, T192X256,
+                          T256, T64, T64X128, TILES)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CUS = 256
@@ -94,6 +95,18 @@ def test_rules_over_many_shapes(rules):
         assert T64 <= tile <= T256
         assert 1 <= S <= 8 and (S - 1) * per < steps <= S * per
         assert S == 1 or per % 2 == 0
+    # what frx_fp4_linear accepts fits a launch, or (experts' rows, whose workgroups take tiles in turn) a count in 32 bits
+    sides = {T64: (64, 64, 256), T64X128: (64, 128, 256), T128X192: (128, 192, 512), T128X256: (128, 256, 512),
+             T192X256: (192, 256, 512), T256: (256, 256, 512)}
+    for _ in range(20000):
+        M, N, K, E = log(33, 1 << 31), log(1, (1 << 27) - 16), log(1, 1 << 18) * 32, rng.randint(1, 64)
+        if (-(-M // 64) + 64) * -(-N // 128) >= 1 << 24:
+            continue
+        h, w, threads = sides[rules.plan(M, K, N)[0]]
+        assert -(-M // h) * -(-N // w) * threads < 1 << 32
+        tile = rules.grouped(M, K, N, E)
+        h, w, threads = sides[tile]
+        assert (-(-M // h) + E) * -(-N // w) * (threads if tile == T256 else 1) <= 0xF0000000
     for _ in range(5000):
         assert rules.grouped(log(1, 1 << 20), log(1, 4096) * 32, log(1, 1 << 16), rng.randint(1, 64)) in (
             T64, T64X128, T128X256, T256)

@@ -116,6 +116,95 @@ def test_layers(ctx, T, H, I, E, top_k, t):
     check(y, *reference(x.double().numpy(), [v for _, v in w], idx, wt, frx.ACT_SILU, t))
 
 
+def test_offsets_that_are_no_sort(ctx):
+    """Offsets that go down, or pass the rows there are: rows of some expert or left alone, none outside y."""
+    R, K, N, E = 70, 96, 40, 3
+    a, b = operand(1, R, K), operand(2, E * N, K)
+    for off in ([0, 40, 20, 70], [100, 200, 300, 400], [70, 0, 0, 2 ** 31 - 1], [-1, 5, -1, 60]):
+        out = torch.full((R + 16, N), 7.0, device=DEV)
+        ctx.fp4_linear_grouped(*a, b[0].view(E, N, -1), b[1].view(E, N, -1),
+                               torch.tensor(off, dtype=torch.int32, device=DEV), out[8:R + 8])
+        assert bool((out[:8] == 7).all()) and bool((out[R + 8:] == 7).all())
+
+
+def test_first_calls_under_capture():
+    """A product that would split K runs whole, the experts' and the small calls need nothing; a call whose codes have no
+    place is refused and the capture goes on."""
+    c, side = frx.Context(0), torch.cuda.Stream()
+    c.set_stream(side)
+    M, K, N = SPLIT[0][:3]
+    a, b = operand(1, M, K), operand(2, N, K)
+    x, few = torch.randn((M, K), device=DEV), torch.randn((3, K), device=DEV)
+    y, z, g = torch.zeros((M, N), device=DEV), torch.zeros((3, N), device=DEV), torch.zeros((M, N), device=DEV)
+    off = torch.tensor([0, M], dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        c.fp4_linear(*a, *b, y)
+        with pytest.raises(frx.FrxError, match="captured"):
+            c.fp4_linear_act(x, *b, y)
+        c.fp4_linear_act(few, *b, z)
+        c.fp4_linear_grouped(*a, b[0][None], b[1][None], off, g)
+    e = frx.Context(0)
+    for i in range(3):
+        few.normal_()
+        for t in (y, z, g):
+            t.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        close(y, values(*a), values(*b))
+        assert torch.equal(y, g)
+        want = torch.zeros_like(z)
+        e.fp4_linear_act(few, *b, want)
+        assert torch.equal(z, want) and bool(z.any())
+        if i == 0:  # an eager call grows the workspace that the graph does without
+            c.fp4_linear(*a, *b, torch.zeros((M, N), device=DEV))
+            torch.cuda.synchronize()
+    del graph
+    c.set_stream(None)
+    c.close()
+    e.close()
+
+
+def test_two_contexts_at_once():
+    """Products, experts' rows and layers of two contexts on two streams, both queued before either is waited for, against
+    the same calls alone; one operand on both sides of a product."""
+    M, K, N, E, T = 300, 1120, 5010, 8, 7
+    n = N // 10
+    a, b = operand(1, M, K), operand(2, E * n, K)
+    w = [t[None].expand(E, *t.shape).contiguous() for k in ((3, 352, K), (4, 352, K), (5, K, 352)) for t in operand(*k)]
+    x, idx = torch.randn((T, K), device=DEV), torch.arange(2 * T, dtype=torch.int32, device=DEV).view(T, 2) % (E + 1)
+    off = torch.linspace(0, M, E + 1, device=DEV).int()
+    wt, router = torch.rand((T, 2), device=DEV), torch.randn((E, K), device=DEV)
+
+    def calls(c, outs):
+        for _ in range(3):
+            c.fp4_linear(*a, *a, outs[0])
+            c.fp4_linear_grouped(*a, b[0].view(E, n, -1), b[1].view(E, n, -1), off, outs[1])
+            c.fp4_moe_ffn(x, None, *w, outs[2], idx, wt)
+            c.fp4_moe_ffn(x, router, *w, outs[3], top_k=2)
+
+    want, *got = [[torch.zeros(d, device=DEV) for d in ((M, M), (M, n), (T, K), (T, K))] for _ in range(3)]
+    alone = frx.Context(0)
+    calls(alone, want)
+    torch.cuda.synchronize()
+    pairs = [(frx.Context(0), torch.cuda.Stream()) for _ in range(2)]
+    for c, stream in pairs:
+        c.set_stream(stream)
+    for (c, _), outs in zip(pairs, got):
+        calls(c, outs)
+    torch.cuda.synchronize()
+    for outs in got:
+        for u, v in zip(outs, want):
+            assert torch.equal(u, v) and bool(v.any())
+    close(want[0], values(*a), values(*a))
+    for c in (alone, *(c for c, _ in pairs)):
+        c.set_stream(None)
+        c.close()
+
+
 # ---- past 4 GiB ----------------------------------------------------------------------
 
 
