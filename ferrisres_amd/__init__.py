@@ -120,6 +120,7 @@ _SIGS = {
     "frx_fp4_linear": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _int, _u32, _u32, _u32]),
     "frx_fp4_linear_act": (_int, [_vp, _vp, _int, _vp, _sz, _vp, _vp, _int, _u32, _u32, _u32]),
     "frx_fp4_linear_grouped": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _u32, _vp, _int, _u32, _u32, _u32]),
+    "frx_fp4_grad_weight_grouped": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _vp, _vp, _u32, _vp, _int, _u32, _u32, _u32]),
     "frx_fp4_moe_ffn": (_int, [_vp, _vp, _int, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32,
                                _int, _vp, _int, _vp, _vp]),
     "frx_moe_rows_capacity": (_sz, [_u32, _u32, _u32, _u32]),
@@ -917,6 +918,27 @@ class Context:
                                             sp.buffer_info()[0], offsets.data_ptr(), E, y.data_ptr(), _dtype_code(y),
                                             R, 2 * kh, N), self._h)
         return y
+
+    def fp4_grad_weight_grouped(self, a, sa, b, sb, offsets, dw):
+        """frx_fp4_grad_weight_grouped: dw[e] [N][K] = the sum over expert e's
+        rows of dy (a [N][R/2], sa, FP4_COLS) times x (b [K][R/2], sb, FP4_COLS),
+        R rounded up to a multiple of 32; dw a stacked tensor or a list of E."""
+        torch = _torch or _tt()
+        N, rh, lda = _fp4_codes(a, "a")
+        K, r_, ldb = _fp4_codes(b, "b")
+        if r_ != rh:
+            raise _shape_err(f"b has {r_} bytes a row, a {rh}")
+        E = int(offsets.numel()) - 1
+        _dense(offsets, (E + 1,), torch.int32, "offsets")
+        _fp4_scales(sa, N, 2 * rh, "sa")
+        _fp4_scales(sb, K, 2 * rh, "sb")
+        dt = dw[0].dtype if len(dw) else None
+        dp, _ = _per_expert(dw, E, (N, K), dt, "dw", out=True, dev=self._dev)
+        _here(self._dev, a, sa, b, sb, offsets)
+        _check(lib().frx_fp4_grad_weight_grouped(self._h, a.data_ptr(), lda, sa.data_ptr(), b.data_ptr(), ldb,
+                                                 sb.data_ptr(), offsets.data_ptr(), E, dp.buffer_info()[0],
+                                                 _dtype_code(dw[0]), 2 * rh, N, K), self._h)
+        return dw
 
     def fp4_moe_ffn(self, x, router, w_gate, s_gate, w_up, s_up, w_down, s_down, y, topk_idx=None, topk_w=None,
                     top_k=None, act: int = ACT_SILU):

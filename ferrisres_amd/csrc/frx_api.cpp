@@ -1671,6 +1671,16 @@ frx_status frx_fp8_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, fr
   return FRX_OK;
 }
 
+// Two experts' workgroups must not write one place.
+static frx_status check_apart(frx_ctx *ctx, void *const *dw, uint32_t E, size_t bytes) {
+  uintptr_t to[frx::FP8_MAXE];
+  for (uint32_t e = 0; e < E; e++) to[e] = reinterpret_cast<uintptr_t>(dw[e]);
+  std::sort(to, to + E);
+  for (uint32_t e = 1; e < E; e++)
+    if (to[e] - to[e - 1] < bytes) return fail(ctx, FRX_ERR_SHAPE, "two experts' dw overlap");
+  return FRX_OK;
+}
+
 frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, frx_fp8 at, const float *sa,
                                        const uint8_t *b, size_t ldb, const float *sb, const uint32_t *offsets,
                                        uint32_t E, void *const *dw, frx_dtype yt, uint32_t R, uint32_t N, uint32_t K) {
@@ -1681,12 +1691,7 @@ frx_status frx_fp8_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t ld
   if ((st = check_fp8(ctx, a, lda, at, sa, ldb, yt, N, R, K)) != FRX_OK) return st;
   for (uint32_t e = 0; e < E; e++)
     if ((st = check_fp8_side(ctx, b, sb, dw[e], yt)) != FRX_OK) return st;
-  // two experts' workgroups must not write one place
-  uintptr_t to[frx::FP8_MAXE];
-  for (uint32_t e = 0; e < E; e++) to[e] = reinterpret_cast<uintptr_t>(dw[e]);
-  std::sort(to, to + E);
-  for (uint32_t e = 1; e < E; e++)
-    if (to[e] - to[e - 1] < (size_t)N * K * dtype_bytes(yt)) return fail(ctx, FRX_ERR_SHAPE, "two experts' dw overlap");
+  if ((st = check_apart(ctx, dw, E, (size_t)N * K * dtype_bytes(yt))) != FRX_OK) return st;
   if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
   const hipError_t e = frx::launch_fp8_grad_weight(a, lda, at == FRX_FP8_E5M2, sa, b, ldb, sb, offsets, (int)E, dw,
                                                    yt == FRX_BF16, fp8_pipe8(ctx, yt), R, N, K, ctx->stream);
@@ -1838,6 +1843,24 @@ frx_status frx_fp4_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, co
   const hipError_t e = frx::launch_fp4_grouped(a, lda, sa, b, ldb, sb, offsets, (int)E, y, yt == FRX_BF16, R, K, N,
                                                ctx->cus, ctx->stream);
   if (e != hipSuccess) return hip_fail(ctx, e, "fp4 grouped linear launch");
+  return FRX_OK;
+}
+
+frx_status frx_fp4_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b,
+                                       size_t ldb, const uint8_t *sb, const uint32_t *offsets, uint32_t E,
+                                       void *const *dw, frx_dtype yt, uint32_t R, uint32_t N, uint32_t K) {
+  frx_status st = enter(ctx);
+  if (st != FRX_OK) return st;
+  if (E == 0 || E > (uint32_t)frx::FP8_MAXE) return fail(ctx, FRX_ERR_SHAPE, "E=%u must be in [1, %d]", E, frx::FP8_MAXE);
+  if (!dw || !offsets) return fail(ctx, FRX_ERR_SHAPE, "null pointer argument");
+  if ((st = check_fp4(ctx, a, lda, sa, ldb, yt, N, R, K)) != FRX_OK) return st;
+  for (uint32_t e = 0; e < E; e++)
+    if ((st = check_fp4_side(ctx, b, sb, dw[e], yt)) != FRX_OK) return st;
+  if ((st = check_apart(ctx, dw, E, (size_t)N * K * dtype_bytes(yt))) != FRX_OK) return st;
+  if (!aligned_to(offsets, 4)) return fail(ctx, FRX_ERR_SHAPE, "offsets must be 4-byte aligned");
+  const hipError_t e = frx::launch_fp4_grad_weight(a, lda, sa, b, ldb, sb, offsets, (int)E, dw, yt == FRX_BF16, R, N, K,
+                                                   ctx->cus, ctx->stream);
+  if (e != hipSuccess) return hip_fail(ctx, e, "fp4 weight gradient launch");
   return FRX_OK;
 }
 

@@ -144,6 +144,67 @@ __global__ __launch_bounds__(Tile::NT, 2) void fp4_grouped_kernel(const GroupArg
   Tile::template run<MANY>(lds, items);
 }
 
+// Weight gradients: expert blockIdx.y's sums over its rows, whose columns of the codes begin at
+// a multiple of 128 (so codes and scales begin at whole 64 and 4 bytes). Here the engine's tokens are
+// dw's rows (dy's columns) and its weight rows x's columns.
+struct GradArgs {
+  const uint8_t *a, *b, *sa, *sb;
+  const uint32_t *offsets;
+  size_t lda, ldb;
+  uint32_t R, N, K;
+  void *dw[FP8_MAXE];
+};
+
+template <typename Tile, typename YT>
+struct GradItem {
+  const GradArgs &p;
+  uint32_t m0, n0, mr, nr, first, len;
+  int span;
+  __device__ __forceinline__ GradItem(const GradArgs &args) : p(args) {
+    uint32_t mt, nt, end;
+    xcd_tile<8>(blockIdx.x, (p.N + Tile::BM - 1) / Tile::BM, (p.K + Tile::BN - 1) / Tile::BN, mt, nt);
+    m0 = mt * Tile::BM;
+    n0 = nt * Tile::BN;
+    mr = min((uint32_t)Tile::BM, p.N - m0);
+    nr = min((uint32_t)Tile::BN, p.K - n0);
+    expert_rows(p.offsets, blockIdx.y, p.R, first, end);
+    first &= ~127u;
+    len = (end - first) & ~31u;
+    span = (int)((len + 255) >> 8);
+  }
+  __device__ __forceinline__ bool at(int, Fp4Operands &o) const {
+    o.s_ld = fp4_scale_bytes(p.R);
+    o.a = p.a + (size_t)m0 * p.lda + first / 2;
+    o.b = p.b + (size_t)n0 * p.ldb + first / 2;
+    o.sa = p.sa + (size_t)m0 * o.s_ld + first / 32;
+    o.sb = p.sb + (size_t)n0 * o.s_ld + first / 32;
+    o.lda = (uint32_t)p.lda;
+    o.ldb = (uint32_t)p.ldb;
+    o.a_rows = (int)mr;
+    o.b_rows = (int)nr;
+    o.K = (int)len;
+    o.t0 = 0;
+    o.t1 = span;
+    return true;
+  }
+  __device__ __forceinline__ bool take(int, int &from, int &to) const {
+    from = 0;
+    to = span;
+    return true;
+  }
+  template <typename Acc>
+  __device__ __forceinline__ void store(const Acc &acc) const {
+    Tile::template store<YT>(acc, static_cast<YT *>(p.dw[blockIdx.y]) + (size_t)m0 * p.K + n0, p.K, (int)mr, (int)nr);
+  }
+};
+
+template <typename Tile, typename YT>
+__global__ __launch_bounds__(Tile::NT, 2) void fp4_grad_kernel(const GradArgs p) {
+  extern __shared__ __align__(16) uint32_t lds[];
+  GradItem<Tile, YT> item(p);
+  Tile::template run<false>(lds, item);
+}
+
 template <int RT, int TT, typename XT, typename YT>
 __global__ __launch_bounds__(FP4_SK_WAVES * 64) void fp4_skinny_kernel(const Fp4Skinny p) {
   extern __shared__ __align__(16) uint32_t lds[];
@@ -239,6 +300,24 @@ hipError_t grouped_any(const GroupArgs &p, int tile, int cus, hipStream_t stream
   }
 }
 
+template <typename Tile, typename YT>
+hipError_t grad_go(const GradArgs &p, int E, hipStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  const size_t tiles = (size_t)((p.N + Tile::BM - 1) / Tile::BM) * ((p.K + Tile::BN - 1) / Tile::BN);
+  if (tiles * Tile::NT > 0xFFFFFFFFu) return hipErrorInvalidValue;
+  const auto kernel = fp4_grad_kernel<Tile, YT>;
+  const hipError_t e = opt_in_lds(reinterpret_cast<const void *>(kernel), Tile::LDS_BYTES, done);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, E), dim3(Tile::NT), Tile::LDS_BYTES, stream, p);
+  return hipGetLastError();
+}
+
+template <typename YT>
+hipError_t grad_any(const GradArgs &p, int tile, int E, hipStream_t stream) {
+  if (tile == FP4_T_256X256) return grad_go<Tile256x256, YT>(p, E, stream);
+  return tile == FP4_T_128X256 ? grad_go<Tile128x256, YT>(p, E, stream) : grad_go<Tile64x128, YT>(p, E, stream);
+}
+
 }  // namespace
 
 hipError_t launch_fp4_linear(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
@@ -282,6 +361,15 @@ hipError_t launch_fp4_grouped(const uint8_t *a, size_t lda, const uint8_t *sa, c
   }
   const int tile = fp4_grouped_tile(R, K, N, (uint32_t)E, cus);
   return yt_bf16 ? grouped_any<uint16_t>(p, tile, cus, stream) : grouped_any<float>(p, tile, cus, stream);
+}
+
+hipError_t launch_fp4_grad_weight(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
+                                  const uint8_t *sb, const uint32_t *offsets, int E, void *const *dw, int yt_bf16,
+                                  uint32_t R, uint32_t N, uint32_t K, int cus, hipStream_t stream) {
+  GradArgs p = {a, b, sa, sb, offsets, lda, ldb, R, N, K, {}};
+  for (int e = 0; e < E; e++) p.dw[e] = dw[e];
+  const int tile = fp4_grad_tile(R, N, K, (uint32_t)E, cus);
+  return yt_bf16 ? grad_any<uint16_t>(p, tile, E, stream) : grad_any<float>(p, tile, E, stream);
 }
 
 }  // namespace frx

@@ -130,8 +130,8 @@ struct Fp4Ring {
       c.s_b_last = (uint32_t)((q.b_rows - 1) >> 6) * c.sld64;
       c.ra = buffer_rsrc(q.a, (uint32_t)(q.a_rows - 1) * q.lda + (uint32_t)q.K / 2);
       c.rb = buffer_rsrc(q.b, (uint32_t)(q.b_rows - 1) * q.ldb + (uint32_t)q.K / 2);
-      c.rsa = buffer_rsrc(q.sa, (uint32_t)q.a_rows * q.s_ld);
-      c.rsb = buffer_rsrc(q.sb, (uint32_t)q.b_rows * q.s_ld);
+      c.rsa = buffer_rsrc(q.sa, (uint32_t)(q.a_rows - 1) * q.s_ld + fp4_scale_bytes((uint32_t)q.K));
+      c.rsb = buffer_rsrc(q.sb, (uint32_t)(q.b_rows - 1) * q.s_ld + fp4_scale_bytes((uint32_t)q.K));
       c.t = q.t0;
       c.t1 = q.t1;
     };
@@ -246,7 +246,7 @@ struct Fp4Ring {
       for (int f = 0; f < FM; f++) sx[f] = sxn[f];
       loaded();
       t++;
-      if (MANY ? --to_do == 0 : t == t1) {
+      if (MANY ? --to_do == 0 : t >= t1) {
         items.store(acc);
         if (!MANY || !items.take(++item, t, t1)) break;
         to_do = span;

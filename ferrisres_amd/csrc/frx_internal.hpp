@@ -392,6 +392,10 @@ hipError_t launch_fp4_grouped(const uint8_t *a, size_t lda, const uint8_t *sa, c
                               const uint8_t *const *sb, const uint32_t *offsets, int E, void *y, int yt_bf16,
                               uint32_t R, uint32_t K, uint32_t N, int cus, hipStream_t stream);
 
+hipError_t launch_fp4_grad_weight(const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b, size_t ldb,
+                                  const uint8_t *sb, const uint32_t *offsets, int E, void *const *dw, int yt_bf16,
+                                  uint32_t R, uint32_t N, uint32_t K, int cus, hipStream_t stream);
+
 // ---- experts in 4 bits for a few tokens (frx_fp4_moe.hip) --------------------
 constexpr uint32_t FP4_MOE_MAX_T = 64;
 struct Fp4Moe {

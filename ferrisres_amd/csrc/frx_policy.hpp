@@ -311,6 +311,23 @@ inline int fp4_grouped_tile(uint32_t R, uint32_t K, uint32_t N, uint32_t E, int 
   return best;
 }
 
+// Gradients of E experts' weights [N][K] over R rows in all.
+inline int fp4_grad_tile(uint32_t R, uint32_t N, uint32_t K, uint32_t E, int cus) {
+  const double steps = std::ceil((double)R / E / 256);
+  int best = FP4_T_64X128;
+  double least = 1e30;
+  for (const Fp4TileCost &c : kFp4Tiles) {
+    if (c.tile != FP4_T_64X128 && c.tile != FP4_T_128X256 && c.tile != FP4_T_256X256) continue;
+    const double tiles = (double)E * ((N + c.bm - 1) / c.bm) * ((K + c.bn - 1) / c.bn);
+    const double ns = std::ceil(tiles / ((double)c.wgs * cus)) * (c.fix + steps * c.all);
+    if (ns < least) {
+      least = ns;
+      best = c.tile;
+    }
+  }
+  return best;
+}
+
 // ---- the expert layer for a few tokens -------------------------------------------
 
 // A wave's steps of 128 columns (8 waves split K), column tiles of 16 (token, plane) pairs

@@ -487,6 +487,19 @@ frx_status frx_fp4_linear_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, co
                                   const uint32_t *offsets, uint32_t E, void *y, frx_dtype yt, uint32_t R, uint32_t K,
                                   uint32_t N);
 
+/* Gradients of the experts' weights: for each expert e
+ *   dw[e][n][k] = sum over its rows r of dy[r][n] * x[r][k]
+ * from both operands in FRX_FP4_COLS over the sorted rows:
+ *   a [N][lda] (dy), sa [N][4 * ceil(R / 128)]; b [K][ldb] (x), sb [K][4 * ceil(R / 128)];
+ *   offsets [E + 1] as above, multiples of 128 (a sort with align = 128); dw[e] [N][K] yt
+ *   (host array of E device pointers, of matrices that do not overlap; zeros for an expert
+ *   without rows). R % 32 == 0, R <= 2^23, 1 <= E <= 64; otherwise as frx_fp4_linear. No
+ *   allocation. The gradient of x is frx_fp4_linear_grouped over dy in FRX_FP4_ROWS and the
+ *   experts' weights in FRX_FP4_COLS. */
+frx_status frx_fp4_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t lda, const uint8_t *sa, const uint8_t *b,
+                                       size_t ldb, const uint8_t *sb, const uint32_t *offsets, uint32_t E,
+                                       void *const *dw, frx_dtype yt, uint32_t R, uint32_t N, uint32_t K);
+
 /* An expert layer for a few tokens, whose experts' weights are codes and scales in
  * the layout of FRX_FP4_ROWS:
  *   y[t] = sum_j topk_w[t][j] * down_e(act(gate_e x_t) * up_e x_t),  e = topk_idx[t][j]

@@ -29,6 +29,15 @@ GROUPED = {
     "256": ([140, 0, 257, 1, 256, 90, 255, 100, 200, 140], 9, 800, 5900, T256),
 }
 
+# experts' rows (whole blocks of 128), rows behind, N, K, tile of the weights' gradients
+GRADS = {
+    "64x128": ([128, 0, 256, 512], 128, 90, 71, T64X128),
+    "64x128-one": ([896], 0, 330, 129, T64X128),
+    "64x128-none": ([0, 0], 256, 40, 33, T64X128),
+    "128x256": ([256, 128, 0, 512], 0, 2050, 1990, T128X256),
+    "256": ([128, 0, 384, 256], 128, 1500, 2050, T256),
+}
+
 # T, H, I, E, top_k
 LAYERS = [(8, 2080, 96, 4, 2), (33, 2080, 96, 4, 2), (64, 96, 128, 4, 2), (33, 160, 96, 4, 2), (9, 4128, 64, 4, 2),
           (3, 8320, 32, 2, 1), (8, 64, 2080, 4, 2), (16, 64, 2080, 4, 2), (33, 64, 2080, 4, 2), (8, 64, 4064, 16, 2),

@@ -37,6 +37,9 @@ static frx_status (*const act)(frx_ctx *, const void *, frx_dtype, const uint8_t
 static frx_status (*const grouped)(frx_ctx *, const uint8_t *, size_t, const uint8_t *, const uint8_t *const *, size_t,
                                    const uint8_t *const *, const uint32_t *, uint32_t, void *, frx_dtype, uint32_t,
                                    uint32_t, uint32_t) = frx_fp4_linear_grouped;
+static frx_status (*const grad)(frx_ctx *, const uint8_t *, size_t, const uint8_t *, const uint8_t *, size_t,
+                                const uint8_t *, const uint32_t *, uint32_t, void *const *, frx_dtype, uint32_t, uint32_t,
+                                uint32_t) = frx_fp4_grad_weight_grouped;
 static frx_status (*const ffn)(frx_ctx *, const void *, frx_dtype, const void *, frx_dtype, const uint8_t *const *,
                                const uint8_t *const *, const uint8_t *const *, const uint8_t *const *,
                                const uint8_t *const *, const uint8_t *const *, uint32_t, uint32_t, uint32_t, uint32_t,
@@ -49,6 +52,7 @@ static void check_host(void) {
   EXPECT(linear(NULL, NULL, 16, NULL, NULL, 16, NULL, NULL, FRX_F32, 1, 32, 1) == D);
   EXPECT(act(NULL, NULL, FRX_F32, NULL, 16, NULL, NULL, FRX_F32, 1, 32, 1) == D);
   EXPECT(grouped(NULL, NULL, 16, NULL, NULL, 16, NULL, NULL, 1, NULL, FRX_F32, 1, 32, 1) == D);
+  EXPECT(grad(NULL, NULL, 16, NULL, NULL, 16, NULL, NULL, 1, NULL, FRX_F32, 32, 1, 1) == D);
   EXPECT(ffn(NULL, NULL, FRX_F32, NULL, FRX_F32, NULL, NULL, NULL, NULL, NULL, NULL, 1, 32, 32, 1, 1, FRX_ACT_SILU, NULL,
              FRX_F32, NULL, NULL) == D);
 }
@@ -129,6 +133,29 @@ static void check_products(frx_ctx *c, void *mem) {
   sb[0] = q + 2;
   EXPECT(G(q, 16, q, b, 16, sb, o, E, f, 0, R, K, N) == S);
   free(b), free(sb);
+  void **dw = malloc(E * sizeof(*dw));
+  if (!dw) abort();
+  for (int e = 0; e < E; e++) dw[e] = q + 4096 * (E - e);
+#define W(a, lda, sa, bq, ldb, sbq, off, e, out, yt, r, n, k) \
+  grad(c, a, lda, sa, bq, ldb, sbq, off, e, out, (frx_dtype)(yt), r, n, k)
+  EXPECT(W(q, 16, q, q, 16, q, o, 0, dw, 0, 32, N, K) == S && W(q, 16, q, q, 16, q, o, 65, dw, 0, 32, N, K) == S);
+  EXPECT(W(q, 16, q, q, 16, q, NULL, E, dw, 0, 32, N, K) == S && W(q, 16, q, q, 16, q, o, E, NULL, 0, 32, N, K) == S);
+  EXPECT(W(NULL, 16, q, q, 16, q, o, E, dw, 0, 32, N, K) == S && W(q, 16, NULL, q, 16, q, o, E, dw, 0, 32, N, K) == S);
+  EXPECT(W(q, 16, q, NULL, 16, q, o, E, dw, 0, 32, N, K) == S && W(q, 16, q, q, 16, NULL, o, E, dw, 0, 32, N, K) == S);
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 0, 0, N, K) == S && W(q, 16, q, q, 16, q, o, E, dw, 0, 16, N, K) == S);
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 0, 64, N, K) == S && W(q, 24, q, q, 16, q, o, E, dw, 0, 32, N, K) == S);
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 2, 32, N, K) == U && W(q + 8, 16, q, q, 16, q, o, E, dw, 0, 32, N, K) == S);
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 0, 32, 0, K) == S && W(q, 16, q, q, 16, q, o, E, dw, 0, 32, N, 0) == S);
+  EXPECT(W(q, 16, q, q, 16, q, (const uint32_t *)(q + 2), E, dw, 0, 32, N, K) == S);
+  dw[1] = q + 1;
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 1, 32, N, K) == S);
+  dw[1] = NULL;
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 0, 32, N, K) == S);
+  dw[1] = dw[2];
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 0, 32, N, K) == S); /* two of one matrix */
+  dw[1] = (char *)dw[2] + N * K * 4 - 4;
+  EXPECT(W(q, 16, q, q, 16, q, o, E, dw, 0, 32, N, K) == S); /* one element of two */
+  free(dw);
 }
 
 static void check_layer(frx_ctx *c, void *mem) {
@@ -222,6 +249,7 @@ static void check_device(void) {
     EXPECT(linear(c, NULL, 0, NULL, NULL, 0, NULL, NULL, FRX_F32, 0, 0, 0) == O);
     EXPECT(act(c, NULL, FRX_F32, NULL, 0, NULL, NULL, FRX_F32, 0, 0, 0) == O);
     EXPECT(grouped(c, NULL, 0, NULL, NULL, 0, NULL, NULL, 0, NULL, FRX_F32, 0, 0, 0) == O);
+    EXPECT(grad(c, NULL, 0, NULL, NULL, 0, NULL, NULL, 0, NULL, FRX_F32, 0, 0, 0) == O);
     EXPECT(ffn(c, NULL, FRX_F32, NULL, FRX_F32, NULL, NULL, NULL, NULL, NULL, NULL, 0, 0, 0, 0, 0, FRX_ACT_SILU, NULL,
                FRX_F32, NULL, NULL) == O);
     EXPECT(frx_force_status(c, FRX_OK) == FRX_OK);

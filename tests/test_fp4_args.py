@@ -19,6 +19,7 @@ def test_null_context():
     assert L.frx_fp4_linear(None, None, 16, None, None, 16, None, None, 0, 1, 32, 1) == 3
     assert L.frx_fp4_linear_act(None, None, 0, None, 16, None, None, 0, 1, 32, 1) == 3
     assert L.frx_fp4_linear_grouped(None, None, 16, None, None, 16, None, None, 1, None, 0, 1, 32, 1) == 3
+    assert L.frx_fp4_grad_weight_grouped(None, None, 16, None, None, 16, None, None, 1, None, 0, 32, 1, 1) == 3
     assert L.frx_fp4_moe_ffn(None, None, 0, None, 0, None, None, None, None, None, None, 1, 32, 32, 1, 1, 0, None, 0,
                              None, None) == 3
 
@@ -92,6 +93,21 @@ def test_binding_checks_groups(ctx):  # noqa: F811
         refuses(frx.FrxError, bad)
     refuses(TypeError, lambda: ctx.fp4_linear_grouped(a, sa, b, sb, off.long(), y))
     refuses(TypeError, lambda: ctx.fp4_linear_grouped(a, sa, b.int(), sb, off, y))
+
+
+def test_binding_checks_weight_gradients(ctx):  # noqa: F811
+    a, sa, b, sb, off = z(40, 128), z(40, 8), z(70, 128), z(70, 8), torch.zeros(4, dtype=torch.int32)
+    dw = torch.zeros((3, 40, 70))
+    call = ctx.fp4_grad_weight_grouped
+    reaches_the_library(lambda: call(a, sa, b, sb, off, dw))
+    reaches_the_library(lambda: call(a.view(F4), sa.view(E8), b, sb, off, list(dw.bfloat16())))
+    for bad in (lambda: call(a, sa, b[:, :112], sb, off, dw), lambda: call(a, sa[:39], b, sb, off, dw),
+                lambda: call(a, sa, b, sb[:, :4], off, dw), lambda: call(a, sa, b, sb, off, dw[:2]),
+                lambda: call(a, sa, b, sb, off, dw[:, :, :69]), lambda: call(a, sa, b, sb, off, dw[:1].expand(3, 40, 70)),
+                lambda: call(a, sa, b, sb, off[:1], dw[:0])):
+        refuses(frx.FrxError, bad)
+    refuses(TypeError, lambda: call(a, sa, b, sb, off.long(), dw))
+    refuses(TypeError, lambda: call(a, sa, b, sb, off, dw.double()))
 
 
 def test_binding_checks_the_layer(ctx):  # noqa: F811

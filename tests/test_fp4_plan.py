@@ -9,7 +9,7 @@ import subprocess
 
 import pytest
 
-from _fp4_kernels import (DOWN, FEW, GATE_UP, GROUPED, KS, LAYERS, ROWS16, ROWS16_K, SPLIT, T128X192, T128X256, T192X256,
+from _fp4_kernels import (DOWN, FEW, GATE_UP, GRADS, GROUPED, KS, LAYERS, ROWS16, ROWS16_K, SPLIT, T128X192, T128X256, T192X256,
                           T256, T64, T64X128, TILES)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -28,6 +28,7 @@ def rules(tmp_path_factory):
     h, out = ctypes.CDLL(str(so)), (ctypes.c_int * 4)()
     h.fp4_plan_of.argtypes = [ctypes.c_uint32] * 3 + [ctypes.c_int, ctypes.c_void_p]
     h.fp4_grouped_tile_of.argtypes = [ctypes.c_uint32] * 4 + [ctypes.c_int]
+    h.fp4_grad_tile_of.argtypes = [ctypes.c_uint32] * 4 + [ctypes.c_int]
     h.fp4_few_of.argtypes = [ctypes.c_uint32] * 4 + [ctypes.c_int] * 2 + [ctypes.c_void_p]
 
     class Rules:
@@ -39,6 +40,10 @@ def rules(tmp_path_factory):
         @staticmethod
         def grouped(R, K, N, E, cus=CUS):
             return h.fp4_grouped_tile_of(R, K, N, E, cus)
+
+        @staticmethod
+        def grad(R, N, K, E, cus=CUS):
+            return h.fp4_grad_tile_of(R, N, K, E, cus)
 
         @staticmethod
         def few(T, K, E, top_k, planes, down):
@@ -66,6 +71,12 @@ def test_every_grouped_tile_has_its_shape(rules):
     for sizes, behind, K, N, tile in GROUPED.values():
         assert rules.grouped(sum(sizes) + behind, K, N, len(sizes)) == tile
     assert {c[4] for c in GROUPED.values()} == {T64, T64X128, T128X256, T256}
+
+
+def test_every_gradient_tile_has_its_shape(rules):
+    for sizes, behind, N, K, tile in GRADS.values():
+        assert rules.grad(sum(sizes) + behind, N, K, len(sizes)) == tile
+    assert {c[4] for c in GRADS.values()} == {T64X128, T128X256, T256}
 
 
 @pytest.mark.parametrize("planes", [1, 3])
@@ -107,6 +118,8 @@ def test_rules_over_many_shapes(rules):
         tile = rules.grouped(M, K, N, E)
         h, w, threads = sides[tile]
         assert (-(-M // h) + E) * -(-N // w) * (threads if tile == T256 else 1) <= 0xF0000000
+        h, w, threads = sides[rules.grad(K, M, N, E)]
+        assert -(-M // h) * -(-N // w) * threads < 1 << 32
     for _ in range(5000):
         assert rules.grouped(log(1, 1 << 20), log(1, 4096) * 32, log(1, 1 << 16), rng.randint(1, 64)) in (
             T64, T64X128, T128X256, T256)
