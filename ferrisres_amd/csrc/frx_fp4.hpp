@@ -55,6 +55,22 @@ __device__ __forceinline__ void fp4_store4(uint16_t *d, const f32x4 &v, uint32_t
     for (uint32_t e = 0; e < left; e++) d[e] = (uint16_t)h[e];
 }
 
+// Two pieces of 16 sums of a row that 4 lane groups hold, 4 of each a group, as bf16: group g gets the 8
+// from 8 g on, which lie behind one another in y.
+__device__ __forceinline__ u32x4 fp4_join8(const f32x4 &v, const f32x4 &w) {
+  u32x4 o;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const uint32_t p = bf16_rne_nb(v[2 * i]) | (bf16_rne_nb(v[2 * i + 1]) << 16);
+    const uint32_t q = bf16_rne_nb(w[2 * i]) | (bf16_rne_nb(w[2 * i + 1]) << 16);
+    const auto a = __builtin_amdgcn_permlane32_swap(p, q, false, false);        // groups 2, 3 of p with 0, 1 of q
+    const auto b = __builtin_amdgcn_permlane16_swap(a[0], a[1], false, false);  // groups 1, 3 with 0, 2
+    o[i] = b[0];
+    o[2 + i] = b[1];
+  }
+  return o;
+}
+
 // A barrier that waits for this wave's LDS accesses alone: __syncthreads() would wait for the
 // weights on their way too.
 __device__ __forceinline__ void barrier_lds() {
