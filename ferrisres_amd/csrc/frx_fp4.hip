@@ -146,7 +146,9 @@ __global__ __launch_bounds__(Tile::NT, 2) void fp4_grouped_kernel(const GroupArg
 
 // Weight gradients: expert blockIdx.y's sums over its rows, whose columns of the codes begin at
 // a multiple of 128 (so codes and scales begin at whole 64 and 4 bytes). Here the engine's tokens are
-// dw's rows (dy's columns) and its weight rows x's columns.
+// dw's rows (dy's columns) and its weight rows x's columns. Bound by writing dw where experts have few
+// rows: 16 x 128 rows, 5632 x 2048, f32 166 us (738 MB, 4.4 TB/s), bf16 122; 8 x 1024 rows, 2048 x 5632
+// 142 and 104. Tiles in turn gained nothing (128 x 256 176 us, 256 x 256 spills).
 struct GradArgs {
   const uint8_t *a, *b, *sa, *sb;
   const uint32_t *offsets;

@@ -311,7 +311,9 @@ inline int fp4_grouped_tile(uint32_t R, uint32_t K, uint32_t N, uint32_t E, int 
   return best;
 }
 
-// Gradients of E experts' weights [N][K] over R rows in all.
+// Gradients of E experts' weights [N][K] over R rows in all. us f32, 64 x 128 / 128 x 256 / 256 x 256: 16 x
+// 128 rows, 5632 x 2048 217 / 181 / 165, 8 x 128 rows, 1024 x 704 12.5 / 12.2 / 15.9, 4 x 2048 rows,
+// 4096 x 4096 174 / 150 / 120.
 inline int fp4_grad_tile(uint32_t R, uint32_t N, uint32_t K, uint32_t E, int cus) {
   const double steps = std::ceil((double)R / E / 256);
   int best = FP4_T_64X128;
