@@ -170,8 +170,8 @@ struct GradItem {
     mr = min((uint32_t)Tile::BM, p.N - m0);
     nr = min((uint32_t)Tile::BN, p.K - n0);
     expert_rows(p.offsets, blockIdx.y, p.R, first, end);
+    len = end > first ? (end - (first & ~127u)) & ~31u : 0;
     first &= ~127u;
-    len = (end - first) & ~31u;
     span = (int)((len + 255) >> 8);
   }
   __device__ __forceinline__ bool at(int, Fp4Operands &o) const {

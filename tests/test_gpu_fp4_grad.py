@@ -51,6 +51,18 @@ def test_weight_gradients(ctx, name, dtype):
     assert all(torch.equal(x, y) for x, y in zip(lists, dw))
 
 
+def test_rows_that_end_inside_a_block(ctx):
+    """R is a multiple of 32: the last expert's rows end there, and experts behind it have none."""
+    N, K, R = 50, 70, 288
+    a, b = operand(1, N, R), operand(2, K, R)
+    dw = torch.full((4, N, K), float("nan"), device=DEV)
+    ctx.fp4_grad_weight_grouped(*a, *b, torch.tensor([0, 256, 288, 288, 384], dtype=torch.int32, device=DEV), dw)
+    va, vb = values(*a), values(*b)
+    close(dw[0], va[:, :256], vb[:, :256])
+    close(dw[1], va[:, 256:], vb[:, 256:])
+    assert not bool(dw[2:].any())
+
+
 def test_an_odd_address(ctx):
     """dw from any element on."""
     a, b = operand(1, 70, 256), operand(2, 45, 256)
