@@ -25,8 +25,9 @@
 // 16 experts, top 2, H 2048, I 5632, route + gate and up + down + join, us: 1 token bf16 14.6 + 9.4
 // + 5.0 (its weights' bytes 7.1 at a copy's rate; a workgroup's way to its first tile is 5 to 6,
 // much of it instructions that are fetched for the first time), 8 tokens 6.0 + 31.4 + 20.2 + 4.6
-// (37; the weights at 4.1 TB/s), 61 tokens f32 78.6 + 42.2 + 5.0 (57; a tile's exchange). Waits that leave
-// out a wave's own stores gained nothing.
+// (37; the weights at 4.1 TB/s), 61 tokens f32 77.3 + 41.7 + 5.0 (57; of the
+// first 46 are the weights' way alone, 10 the products, 17 a tile's sums, activation and stores). Waits that
+// leave out a wave's own stores gained nothing, nor did sums by lanes of eight.
 #include "frx_fp4.hpp"
 #include "frx_internal.hpp"
 
