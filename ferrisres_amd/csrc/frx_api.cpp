@@ -1896,8 +1896,8 @@ frx_status frx_fp4_moe_ffn(frx_ctx *ctx, const void *x, frx_dtype xt, const void
       p.w[k][e] = w[2 * k][e];
       p.s[k][e] = w[2 * k + 1][e];
     }
-  const size_t h = a256(frx::fp4_moe_h_bytes(T, I, top_k, yt == FRX_BF16));
-  const size_t part = a256(frx::fp4_moe_part_bytes(T, H, I, E, top_k, yt == FRX_BF16));
+  const size_t h = a256(frx::fp4_moe_h_bytes(T, I, top_k));
+  const size_t part = a256(frx::fp4_moe_part_bytes(T, H, I, E, top_k));
   const size_t routes = a256((size_t)T * top_k * 4), need = h + part + (router ? 2 * routes : 0);
   if (!may_grow(ctx, ctx->few_ws_bytes, need))
     return fail(ctx, FRX_ERR_UNSUPPORTED, "the first call at this size allocates and cannot be captured into a graph");

@@ -8,7 +8,7 @@
 // an f32 x as three bf16 planes that add up to it exactly; sums in fp32.
 //
 //   route     the router's logits, top-k and softmax, where the caller has none
-//   gate, up  h = act(g) * u times the route's weight, as bf16 planes, a row for each route
+//   gate, up  h = act(g) * u times the route's weight, as three bf16 planes, a row for each route
 //   down      a row of f32 sums for each route (and slice of I)
 //   combine   the routes of each token, in order
 //
@@ -21,6 +21,9 @@
 // instructions for 128 columns, and one exchange of the waves' sums through LDS. The weights
 // of the next tiles are on their way meanwhile, by LDS DMA into a ring that each wave has for
 // itself (held in registers they were waited for at every turn of the loop).
+//
+// h keeps the 24 bits of an f32 number whatever y is: two planes (2^-17 of h) saved a bf16 layer 0.4 us of
+// 65 at 8 tokens, 3 of 93 at 64 and 8 of 109 at 64 of 32 experts, and flipped last bits of its outputs.
 //
 // 16 experts, top 2, H 2048, I 5632, route + gate and up + down + join, us: 1 token bf16 14.6 + 9.4
 // + 5.0 (its weights' bytes 7.1 at a copy's rate; a workgroup's way to its first tile is 5 to 6,
@@ -46,11 +49,11 @@ struct FewArgs {
   const void *x, *router;
   uint32_t *idx;
   float *wts;
-  uint16_t *h;  // [slot][planes][I]
+  uint16_t *h;  // [slot][plane][I]
   float *part;  // [slice][slot][H]
   uint32_t T, K, N;  // columns of a weight row, rows
-  int E, top_k, planes, act, rt_bf16, route, slices, per;  // slices of K, steps of 128 in each (down)
-  const uint8_t *w[2][FP8_MAXE], *s[2][FP8_MAXE];          // gate, up; or down
+  int E, top_k, act, rt_bf16, route, slices, per;  // slices of K, steps of 128 in each (down)
+  const uint8_t *w[2][FP8_MAXE], *s[2][FP8_MAXE];  // gate, up; or down
 };
 
 struct Shared {
@@ -274,8 +277,10 @@ __device__ __forceinline__ u32x4 widen8(uint32_t c, float s) {
                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
 }
 
-// A value as bf16 planes of which each holds the next 8 bits: three add up to it.
+// A value as bf16 planes of which each holds the next 8 bits: three add up to it. (Of the f32 number
+// v, not of a product that v is the rounding of, as a fused multiply-subtract would have it.)
 __device__ __forceinline__ float cut8(float v, uint32_t &plane) {
+#pragma clang fp contract(off)
   plane = __float_as_uint(v) & 0xFFFF0000u;
   return v - __uint_as_float(plane);
 }
@@ -491,20 +496,14 @@ __global__ __launch_bounds__(NT) void fp4_gate_up_kernel(const FewArgs p) {
           const float other = __shfl_xor(sum, 16);
           if (m) continue;
           const float v = activate(sum, p.act) * other * sh.share[c0 + token];
-          uint16_t *to = p.h + (size_t)sh.slot[c0 + token] * p.planes * p.N + (uint32_t)tile * 16 + r;
-          if (p.planes == 2) {
-            const uint32_t hi = bf16_rne_nb(v);
-            to[0] = (uint16_t)hi;
-            to[p.N] = (uint16_t)bf16_rne_nb(v - __uint_as_float(hi << 16));
-          } else {
-            uint32_t u;
-            float left = cut8(v, u);
-            to[0] = (uint16_t)(u >> 16);
-            left = cut8(left, u);
-            to[p.N] = (uint16_t)(u >> 16);
-            (void)cut8(left, u);
-            to[2 * (size_t)p.N] = (uint16_t)(u >> 16);
-          }
+          uint16_t *to = p.h + (size_t)sh.slot[c0 + token] * FP4_MOE_PLANES * p.N + (uint32_t)tile * 16 + r;
+          uint32_t u;
+          float left = cut8(v, u);
+          to[0] = (uint16_t)(u >> 16);
+          left = cut8(left, u);
+          to[p.N] = (uint16_t)(u >> 16);
+          (void)cut8(left, u);
+          to[2 * (size_t)p.N] = (uint16_t)(u >> 16);
         }
         tile++;
       }
@@ -515,10 +514,10 @@ __global__ __launch_bounds__(NT) void fp4_gate_up_kernel(const FewArgs p) {
 
 // ---- down --------------------------------------------------------------------------
 
-// A unit is a group of an expert's tokens and a slice of K; P planes of h; D tiles' weights on their way.
-template <int P, int STEPS, int CT, int D>
+// A unit is a group of an expert's tokens and a slice of K; D tiles' weights on their way.
+template <int STEPS, int CT, int D>
 __global__ __launch_bounds__(NT) void fp4_down_kernel(const FewArgs p) {
-  constexpr int TOKENS = 16 * CT / P;
+  constexpr int P = FP4_MOE_PLANES, TOKENS = 16 * CT / P;
   extern __shared__ __align__(16) uint32_t lds[];
   __shared__ Shared sh;
   read_routes<uint16_t, false>(p, sh);
@@ -672,29 +671,28 @@ hipError_t gate_up(const FewArgs &a, const Fp4FewPlan &plan, int cus, hipStream_
   return plan.tiles == 2 ? gate_up_go<XT, 2, 2, 3, 2, false>(a, cus, stream) : gate_up_go<XT, 2, 3, 4, 1, false>(a, cus, stream);
 }
 
-template <int P, int STEPS, int CT, int D>
+template <int STEPS, int CT, int D>
 hipError_t down_go(const FewArgs &a, int cus, hipStream_t stream) {
   static std::atomic<uint64_t> done{0};
   constexpr int lds = WAVES * D * Place<STEPS>::DWORDS * 4 + 2 * WAVES * CT * RED * 4;
   static_assert(lds + sizeof(Shared) <= 160 << 10, "LDS");
-  return few_go(fp4_down_kernel<P, STEPS, CT, D>, done, lds, cus, a, stream);
+  return few_go(fp4_down_kernel<STEPS, CT, D>, done, lds, cus, a, stream);
 }
 
-template <int P>
 hipError_t down(const FewArgs &a, const Fp4FewPlan &plan, int cus, hipStream_t stream) {
-  if (plan.tiles == 3) return plan.steps == 2 ? down_go<P, 2, 3, 4>(a, cus, stream) : down_go<P, 3, 3, 3>(a, cus, stream);
-  if (plan.tiles == 2) return plan.steps == 2 ? down_go<P, 2, 2, 5>(a, cus, stream) : down_go<P, 3, 2, 3>(a, cus, stream);
-  if (plan.steps == 2) return down_go<P, 2, 1, 5>(a, cus, stream);
-  return plan.steps == 3 ? down_go<P, 3, 1, 4>(a, cus, stream) : down_go<P, 4, 1, 3>(a, cus, stream);
+  if (plan.tiles == 3) return plan.steps == 2 ? down_go<2, 3, 4>(a, cus, stream) : down_go<3, 3, 3>(a, cus, stream);
+  if (plan.tiles == 2) return plan.steps == 2 ? down_go<2, 2, 5>(a, cus, stream) : down_go<3, 2, 3>(a, cus, stream);
+  if (plan.steps == 2) return down_go<2, 1, 5>(a, cus, stream);
+  return plan.steps == 3 ? down_go<3, 1, 4>(a, cus, stream) : down_go<4, 1, 3>(a, cus, stream);
 }
 
 }  // namespace
 
-size_t fp4_moe_h_bytes(uint32_t T, uint32_t I, uint32_t top_k, int yt_bf16) {
-  return (size_t)T * top_k * fp4_moe_planes(yt_bf16) * I * 2;
+size_t fp4_moe_h_bytes(uint32_t T, uint32_t I, uint32_t top_k) {
+  return (size_t)T * top_k * FP4_MOE_PLANES * I * 2;
 }
-size_t fp4_moe_part_bytes(uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32_t top_k, int yt_bf16) {
-  return (size_t)fp4_down_plan(T, I, E, top_k, fp4_moe_planes(yt_bf16)).slices * T * top_k * H * 4;
+size_t fp4_moe_part_bytes(uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32_t top_k) {
+  return (size_t)fp4_down_plan(T, I, E, top_k, FP4_MOE_PLANES).slices * T * top_k * H * 4;
 }
 
 hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream) {
@@ -703,8 +701,7 @@ hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream) {
     const hipError_t e = p.xt_bf16 ? route_go<uint16_t>(p, stream) : route_go<float>(p, stream);
     if (e != hipSuccess) return e;
   }
-  const int planes = fp4_moe_planes(p.yt_bf16);
-  FewArgs a = {p.x,      p.router, p.idx,    p.wts, p.h, p.part, p.T, p.H, p.I, (int)p.E, (int)p.top_k, planes, p.act,
+  FewArgs a = {p.x,      p.router, p.idx,    p.wts, p.h, p.part, p.T, p.H, p.I, (int)p.E, (int)p.top_k, p.act,
                p.rt_bf16, fused,    1,        0,     {},  {}};
   for (uint32_t e = 0; e < p.E; e++)
     for (int k = 0; k < 2; k++) {
@@ -718,13 +715,13 @@ hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream) {
     a.w[0][i] = p.w[2][i];
     a.s[0][i] = p.s[2][i];
   }
-  const Fp4FewPlan dn = fp4_down_plan(p.T, p.I, p.E, p.top_k, planes);
+  const Fp4FewPlan dn = fp4_down_plan(p.T, p.I, p.E, p.top_k, FP4_MOE_PLANES);
   a.route = 0;
   a.K = p.I;
   a.N = p.H;
   a.slices = dn.slices;
   a.per = dn.per;
-  e = planes == 2 ? down<2>(a, dn, cus, stream) : down<3>(a, dn, cus, stream);
+  e = down(a, dn, cus, stream);
   if (e != hipSuccess) return e;
   const dim3 grid((p.H + 1023) / 1024, p.T);
   if (p.yt_bf16) hipLaunchKernelGGL(fp4_join_kernel<uint16_t>, grid, dim3(256), 0, stream, a, static_cast<uint16_t *>(p.y));

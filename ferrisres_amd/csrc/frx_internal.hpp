@@ -398,20 +398,20 @@ hipError_t launch_fp4_grad_weight(const uint8_t *a, size_t lda, const uint8_t *s
 
 // ---- experts in 4 bits for a few tokens (frx_fp4_moe.hip) --------------------
 constexpr uint32_t FP4_MOE_MAX_T = 64;
+constexpr int FP4_MOE_PLANES = 3;  // of an f32 number
 struct Fp4Moe {
   const void *x, *router;  // router: null, the routes are given
   void *y;
   uint32_t *idx;           // [T][top_k]
   float *wts;              // [T][top_k]
-  uint16_t *h;             // [T * top_k][planes][I] act(g) * u * weight as bf16 planes (fp4_moe_h_bytes)
+  uint16_t *h;             // [T * top_k][FP4_MOE_PLANES][I] act(g) * u * weight as bf16 planes (fp4_moe_h_bytes)
   float *part;             // [slices][T * top_k][H] (fp4_moe_part_bytes)
   uint32_t T, H, I, E, top_k;
   int xt_bf16, rt_bf16, yt_bf16, act;
   const uint8_t *w[3][FP8_MAXE], *s[3][FP8_MAXE];  // gate, up, down
 };
-constexpr int fp4_moe_planes(int yt_bf16) { return yt_bf16 ? 2 : 3; }
-size_t fp4_moe_h_bytes(uint32_t T, uint32_t I, uint32_t top_k, int yt_bf16);
-size_t fp4_moe_part_bytes(uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32_t top_k, int yt_bf16);
+size_t fp4_moe_h_bytes(uint32_t T, uint32_t I, uint32_t top_k);
+size_t fp4_moe_part_bytes(uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32_t top_k);
 hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream);
 
 // ---- tokens sorted by expert, and back (frx_route.hip) -----------------------

@@ -1,0 +1,110 @@
+"""The expert layer for a few tokens (frx_fp4_moe_ffn) on inputs for which every step has one right f32 result, over the
+shapes that reach each of its kernels: compared bit for bit, so that a lost plane of an activation or a lost or doubled
+block of K cannot hide in a tolerance.
+
+Both activations are the identity from 20 on: exp(-20) < 2^-28 beside 1, and tanh of 0.79 * (20 + 0.04 * 20^3) is 1."""
+import numpy as np
+import pytest
+import torch
+
+import ferrisres_amd as frx
+from _fp4_kernels import LAYERS
+from _fp4_ref import DT, TABLE, pack, up
+from _gpu import DEV, host
+
+HALF_, ONE, TWO, FOUR = 1, 2, 4, 6  # code numbers of powers of two
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    assert torch.cuda.is_available(), "GPU tests need a gfx950 device"
+    c = frx.Context(0)
+    yield c
+    c.close()
+
+
+def layer(code, byte):
+    """One matrix of all experts: (codes, scales, values) of code numbers [E][n][k], scale bytes [E][n][k / 32]; 255 behind
+    the bytes of a row."""
+    E, n, k = code.shape
+    pad = np.full((E, n, up(k, 128) // 32), 255, np.uint8)
+    pad[:, :, :k // 32] = byte
+    v = TABLE[code] * np.repeat(np.ldexp(1.0, byte.astype(np.int64) - 127), 32, axis=-1)
+    return pack(code.reshape(E * n, k)).reshape(E, n, k // 2), pad, v
+
+
+def on_dev(w):
+    return [torch.from_numpy(t).to(DEV) for code, pad, _ in w for t in (code, pad)]
+
+
+def distinct(rng, T, E, top_k):
+    return np.stack([rng.permutation(E)[:top_k] for _ in range(T)]).astype(np.int32)
+
+
+# ---- 24 bits: every plane decides -----------------------------------------------------
+
+
+def one_hot(rng, E, n, k, positive):
+    """A code of a power of two in each row, its blocks taken in turn; scales of their own."""
+    col = (np.arange(E * n) % (k // 32)) * 32 + rng.integers(0, 32, E * n)
+    number = rng.choice((HALF_, ONE, TWO, FOUR), E * n)
+    if not positive:
+        number = number + 8 * rng.integers(0, 2, E * n)
+    code = np.zeros((E * n, k), np.uint8)
+    code[np.arange(E * n), col] = number
+    byte = rng.integers(124, 131, (E * n, k // 32)).astype(np.uint8)
+    byte[np.arange(E * n), col // 32] = rng.integers(128, 131, E * n)
+    v = TABLE[number] * np.ldexp(1.0, byte[np.arange(E * n), col // 32].astype(np.int64) - 127)
+    return layer(code.reshape(E, n, k), byte.reshape(E, n, -1)), col.reshape(E, n), v.reshape(E, n).astype(np.float32)
+
+
+def planes_case(T, H, I, E, top_k, xt):
+    rng = np.random.default_rng(T + H + I + top_k)
+    mats = [one_hot(rng, E, I, H, True), one_hot(rng, E, I, H, False), one_hot(rng, E, H, I, False)]
+    x = rng.integers(1 << 23, 1 << 24, (T, H)).astype(np.float32) * np.float32(2.0 ** -18)  # 24 bits from 32 to 64
+    if xt == "bf16":
+        x = torch.from_numpy(x).bfloat16().float().numpy()
+    idx = distinct(rng, T, E, top_k)
+    wt = (rng.integers(1 << 23, 1 << 24, (T, top_k)).astype(np.float32) * np.float32(2.0 ** -24))
+    return x, mats, idx, wt
+
+
+def planes_reference(x, mats, idx, wt, cut=lambda h: h):
+    """y in f32: one product to a sum, so that what is rounded is the product of g and u, its product with the weight, and
+    the sum over the routes in order."""
+    y = np.zeros(x.shape, np.float32)
+    (_, kg, cg), (_, ku, cu), (_, kd, cd) = mats
+    for t in range(len(x)):
+        for j, e in enumerate(idx[t]):
+            g, u = x[t, kg[e]] * cg[e], x[t, ku[e]] * cu[e]
+            h = cut(g * u * wt[t, j])
+            y[t] += h[kd[e]] * cd[e]
+    return y
+
+
+def cut(v, bits):
+    return (v.view(np.uint32) & np.uint32(0xFFFFFFFF << bits & 0xFFFFFFFF)).view(np.float32)
+
+
+@pytest.mark.parametrize("T,H,I,E,top_k", LAYERS)
+def test_a_plane_left_out_shows(T, H, I, E, top_k):
+    """What the next test can tell apart, on the CPU: the last 8 bits of x, or of the intermediate, change the result."""
+    x, mats, idx, wt = planes_case(T, H, I, E, top_k, "f32")
+    y = planes_reference(x, mats, idx, wt)
+    assert (y != 0).all()
+    assert (planes_reference(cut(x, 8), mats, idx, wt) != y).mean() > 0.5
+    assert (planes_reference(x, mats, idx, wt, cut=lambda h: cut(h, 8)) != y).mean() > 0.5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt,yt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("T,H,I,E,top_k", LAYERS)
+def test_every_bit(ctx, T, H, I, E, top_k, xt, yt):
+    """All 24 bits of x, of the intermediate and of the weights reach y; a bf16 y is the f32 one, rounded once."""
+    x, mats, idx, wt = planes_case(T, H, I, E, top_k, xt)
+    want = torch.from_numpy(planes_reference(x, mats, idx, wt)).to(DT[yt])
+    y = torch.full((T, H), float("nan"), dtype=DT[yt], device=DEV)
+    act = frx.ACT_GELU_TANH if T % 2 else frx.ACT_SILU
+    ctx.fp4_moe_ffn(torch.from_numpy(x).to(DT[xt]).to(DEV), None, *on_dev([m[0] for m in mats]), y,
+                    torch.from_numpy(idx).to(DEV), torch.from_numpy(wt).to(DEV), act=act)
+    assert torch.equal(y.cpu(), want)
