@@ -41,6 +41,79 @@ def distinct(rng, T, E, top_k):
     return np.stack([rng.permutation(E)[:top_k] for _ in range(T)]).astype(np.int32)
 
 
+# ---- whole numbers: every block of K decides ------------------------------------------
+
+
+def whole_codes(rng, E, n, k, a_block, signed):
+    """a_block codes of 1 or 2 in every block of 32, zeros elsewhere."""
+    place = rng.random((E, n, k // 32, 32)).argsort(axis=-1) < a_block
+    code = np.where(place, rng.choice((ONE, TWO), place.shape), 0)
+    if signed:
+        code = np.where(place & (rng.random(place.shape) < 0.5), code + 8, code)
+    return layer(code.reshape(E, n, k).astype(np.uint8), np.full((E, n, k // 32), 127, np.uint8))
+
+
+def whole_case(T, H, I, E, top_k):
+    rng = np.random.default_rng(T + H + I)
+    w = [whole_codes(rng, E, I, H, -(-20 // (H // 32)), False), whole_codes(rng, E, I, H, 1, True),
+         whole_codes(rng, E, H, I, 1, True)]
+    x = rng.integers(1, 4, (T, H)).astype(np.float64)
+    idx = distinct(rng, T, E, top_k)
+    wt = rng.choice((0.5, 1.0, 2.0), (T, top_k))
+    return x, w, idx, wt
+
+
+def whole_reference(x, wv, idx, wt):
+    """y, and the sum of what its terms' magnitudes can reach."""
+    y, most = np.zeros(x.shape), np.zeros(x.shape)
+    for e in range(len(wv[0])):
+        t, j = np.nonzero(idx == e)
+        if len(t):
+            g, u = x[t] @ wv[0][e].T, x[t] @ wv[1][e].T
+            assert g.min() >= 20
+            h = g * u * wt[t, j, None]
+            np.add.at(y, t, h @ wv[2][e].T)
+            np.add.at(most, t, np.abs(h) @ np.abs(wv[2][e]).T + (x[t] @ np.abs(wv[1][e]).T).max())
+    return y, most
+
+
+@pytest.mark.parametrize("T,H,I,E,top_k", LAYERS)
+def test_a_block_left_out_shows(T, H, I, E, top_k):
+    """What the next test can tell apart, on the CPU: leaving any block of a matrix out, here the first, the last and one
+    between, changes the layer's result; every sum is of multiples of 1/2 below 2^23, whatever its order."""
+    x, w, idx, wt = whole_case(T, H, I, E, top_k)
+    wv = [v for _, _, v in w]
+    y, most = whole_reference(x, wv, idx, wt)
+    assert most.max() < 2 ** 23
+    for m in range(3):
+        n = wv[m].shape[2] // 32
+        for b in sorted({0, n - 1, *np.random.default_rng(m).integers(0, n, 1)}):
+            less = [v.copy() if i == m else v for i, v in enumerate(wv)]
+            if m == 0:  # (what is left may be an activation's argument below 20: g as it is, then)
+                less[0][:, :, 32 * b:32 * b + 32] = 0
+                got = np.zeros_like(y)
+                for e in range(E):
+                    t, j = np.nonzero(idx == e)
+                    np.add.at(got, t, (x[t] @ less[0][e].T * (x[t] @ wv[1][e].T) * wt[t, j, None]) @ wv[2][e].T)
+            else:
+                less[m][:, :, 32 * b:32 * b + 32] = 0
+                got = whole_reference(x, less, idx, wt)[0]
+            assert (got != y).any(), (m, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt,yt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("T,H,I,E,top_k", LAYERS)
+def test_whole_numbers(ctx, T, H, I, E, top_k, xt, yt):
+    x, w, idx, wt = whole_case(T, H, I, E, top_k)
+    want = torch.from_numpy(whole_reference(x, [v for _, _, v in w], idx, wt)[0]).to(DT[yt])
+    y = torch.full((T, H), float("nan"), dtype=DT[yt], device=DEV)
+    act = frx.ACT_GELU_TANH if T % 2 == 0 else frx.ACT_SILU
+    ctx.fp4_moe_ffn(torch.from_numpy(x).to(DT[xt]).to(DEV), None, *on_dev(w), y, torch.from_numpy(idx).to(DEV),
+                    torch.from_numpy(wt).float().to(DEV), act=act)
+    assert torch.equal(y.cpu(), want)
+
+
 # ---- 24 bits: every plane decides -----------------------------------------------------
 
 
