@@ -507,10 +507,10 @@ frx_status frx_fp4_grad_weight_grouped(frx_ctx *ctx, const uint8_t *a, size_t ld
  *   w_down[e] [H][I / 2], s_down[e] [H][4 * ceil(I / 128)] (contiguous; host arrays of E
  *   device pointers); y [T][H] yt; act: FRX_ACT_SILU or FRX_ACT_GELU_TANH.
  * The activations stay as they are, neither x nor the intermediate becomes codes:
- * products with the weights' values are exact, sums are fp32, the intermediate and its
- * product with its route's weight are f32 numbers, and y is rounded once: a bf16 y is the
- * f32 one, rounded. (frx_fp4_linear_grouped quantises, for many tokens, where the products
- * bound.)
+ * products with the weights' values are exact (of f32 numbers but for their last 2^-149;
+ * a weight past the largest f32 number is an infinity), sums are fp32, the intermediate
+ * and its product with its route's weight are f32 numbers, and a bf16 y is the f32 one,
+ * rounded. (frx_fp4_linear_grouped quantises, for many tokens, where the products bound.)
  * Routes:
  *   router [E][H] rt: the top_k experts of the largest logits x router^T (fp32 sums),
  *     ties to the lowest index, a NaN below every number, in that order; weights are the

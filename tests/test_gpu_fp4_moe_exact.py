@@ -181,3 +181,70 @@ def test_every_bit(ctx, T, H, I, E, top_k, xt, yt):
     ctx.fp4_moe_ffn(torch.from_numpy(x).to(DT[xt]).to(DEV), None, *on_dev([m[0] for m in mats]), y,
                     torch.from_numpy(idx).to(DEV), torch.from_numpy(wt).to(DEV), act=act)
     assert torch.equal(y.cpu(), want)
+
+
+# ---- either end of the range ----------------------------------------------------------
+
+
+def range_case(H, I, xt, end):
+    """x [2][H] and the three matrices: gate takes column 0 of x, row i of up column i % 8 under a scale that suits it, row
+    n of down row n % I of the intermediate and brings it back to an ordinary size."""
+    rng = np.random.default_rng(H + I)
+    m = lambda: rng.integers(1 << 23, 1 << 24, 2) * 2.0 ** -23  # noqa: E731  (24 bits, 1 to 2)
+    x = np.zeros((2, H))
+    if end == "small":
+        x[:, 0] = 64.0
+        x[:, 1] = m() * 2.0 ** 126
+        x[:, 2] = rng.integers(1, 128, 2) * 2.0 ** -133  # a bf16's denormal numbers
+        x[:, 3] = rng.integers(1 << 20, 1 << 23, 2) * 2.0 ** -148  # f32's
+        x[:, 4], x[:, 5], x[:, 6], x[:, 7] = m() * 2.0 ** -118, m(), m() * 8, m() * 2.0 ** -100
+        scale = {1: (0, 1, 2, 3), 2: (247,), 3: (247,), 4: (240, 128), 5: (2, 5), 6: (10, 127), 7: (127,)}
+    else:  # the intermediate below 2^128
+        x[:, 0] = 2.0 ** 64
+        scale = {1: (247,), 2: (130, 160), 3: (127,), 4: (100,), 5: (70,), 6: (3,), 7: (190,)}
+        for c, b in scale.items():
+            x[:, c] = m() * 2.0 ** min(126, 127 - 64 - (max(b) - 127) - 2)
+    t = torch.from_numpy(x).to(DT[xt])
+    x = t.double().numpy()
+    cols = np.arange(I) % 8
+    byte = np.array([rng.choice(scale.get(c, (127,))) for c in cols])
+    byte[cols == 0] = 60  # (column 0 is gate's)
+    number = rng.choice((HALF_, ONE, TWO, FOUR), I)
+    with np.errstate(over="raise"):
+        h = (x[:, :1] * (x[:, cols] * TABLE[number] * np.ldexp(1.0, byte - 127))).astype(np.float32)
+    r = np.arange(H) % I
+    size = np.abs(h[0, r].astype(np.float64))
+    back = np.clip(127 - np.frexp(np.where(size > 0, size, 1.0))[1], 0, 252)
+    want = (h[:, r] * np.ldexp(1.0, back - 127)).astype(np.float32)
+
+    def matrix(n, k, col, number, byte):
+        code, by = np.zeros((1, n, k), np.uint8), np.full((1, n, k // 32), 127, np.uint8)
+        code[0, np.arange(n), col] = number
+        by[0, np.arange(n), col // 32] = byte
+        return layer(code, by)
+
+    return t, [matrix(I, H, 0 * cols, ONE, 127), matrix(I, H, cols, number, byte), matrix(H, I, r, ONE, back)], h, want
+
+
+@pytest.mark.parametrize("xt", ["bf16", "f32"])
+@pytest.mark.parametrize("end", ["small", "large"])
+def test_what_the_range_holds(end, xt):
+    """On the CPU: the intermediates reach the ends that the next test is about, and y is finite and not zero."""
+    _, _, h, want = range_case(32, 32, xt, end)
+    size = np.abs(h)
+    assert np.isfinite(want).all() and (want != 0).all()
+    assert size.max() > 2.0 ** 126 if end == "large" else size.min() < 2.0 ** -110
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt,yt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("end", ["small", "large"])
+@pytest.mark.parametrize("H,I", [(32, 32), (2080, 96), (4128, 2080)])
+def test_either_end_of_the_range(ctx, H, I, end, xt, yt):
+    """Weights, activations and intermediates that bf16 holds as denormal numbers or not at all, and the largest
+    intermediates: nothing of an f32 number is lost on the way but 2^-149."""
+    x, w, _, want = range_case(H, I, xt, end)
+    y = torch.full((2, H), float("nan"), dtype=DT[yt], device=DEV)
+    ctx.fp4_moe_ffn(x.to(DEV), None, *on_dev(w), y, torch.zeros((2, 1), dtype=torch.int32, device=DEV),
+                    torch.ones((2, 1), device=DEV))
+    assert torch.equal(y.cpu(), torch.from_numpy(want).to(DT[yt]))
