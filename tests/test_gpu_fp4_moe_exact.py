@@ -248,3 +248,45 @@ def test_either_end_of_the_range(ctx, H, I, end, xt, yt):
     ctx.fp4_moe_ffn(x.to(DEV), None, *on_dev(w), y, torch.zeros((2, 1), dtype=torch.int32, device=DEV),
                     torch.ones((2, 1), device=DEV))
     assert torch.equal(y.cpu(), torch.from_numpy(want).to(DT[yt]))
+
+
+# ---- past 4 GiB -----------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("bf16", "bf16")])
+def test_a_long_expert_bit_for_bit(ctx, xt, yt):
+    """Gate, up and down of more than 2^32 bytes each, one code to a row: row i of gate and of up takes a column of x of its
+    own, row n of down a column of the intermediate, the rows together one of every 135 columns. A row whose address wrapped
+    at 4 GiB would take another's, a slice left out would give zeros, and no value of y is one."""
+    H, I = 8192, 32 * 34400
+    g = torch.Generator(device=DEV).manual_seed(3)
+    draw = lambda lo, hi, n: torch.randint(lo, hi, (n,), device=DEV, generator=g)  # noqa: E731
+
+    def matrix(n, k, col, number):
+        code = torch.zeros((1, n, k // 2), dtype=torch.uint8, device=DEV)
+        code[0, torch.arange(n, device=DEV), col // 2] = torch.where(col % 2 == 1, number * 16, number).to(torch.uint8)
+        return code, torch.full((1, n, k // 32), 127, dtype=torch.uint8, device=DEV)
+
+    x = (draw(1 << 23, 1 << 24, H).float() * 2.0 ** -18).to(DT[xt])  # 32 to 64
+    value = torch.tensor(TABLE, device=DEV, dtype=torch.float32)
+    powers = torch.tensor([ONE, TWO, FOUR], device=DEV)
+    kg, ku, ng, nu = draw(0, H, I), draw(0, H, I), powers[draw(0, 3, I)], powers[draw(0, 3, I)] + 8 * draw(0, 2, I)
+    part = torch.arange(H, device=DEV) * I // H
+    kd, nd = torch.clamp_max(part + draw(0, I // H, H), I - 1), powers[draw(0, 3, H)]
+    kd[H - 1] = I - 1
+    w = [t for m in (matrix(I, H, kg, ng), matrix(I, H, ku, nu), matrix(H, I, kd, nd)) for t in m]
+    assert all(w[m].numel() > 1 << 32 for m in (0, 2, 4))
+    xf = x.float()
+    h = (xf[kg] * value[ng]) * (xf[ku] * value[nu])  # one f32 rounding
+    # what a wrapped row would give differs: rows 2^32 bytes apart, for every row past the mark
+    far = (1 << 32) // (H // 2)
+    assert bool((h[far:] != h[:I - far]).float().mean() > 0.99) and int((kd >= far).sum()) > 300
+    want = h[kd] * value[nd]
+    far = -(-(1 << 32) // (I // 2))
+    assert bool((want[far:] != want[:H - far]).float().mean() > 0.99)
+    assert bool((want != 0).all())
+    y = torch.full((1, H), float("nan"), dtype=DT[yt], device=DEV)
+    ctx.fp4_moe_ffn(x[None], None, *w, y, torch.zeros((1, 1), dtype=torch.int32, device=DEV),
+                    torch.ones((1, 1), device=DEV))
+    assert torch.equal(y[0], want.to(DT[yt]))
