@@ -110,9 +110,8 @@ __device__ __forceinline__ int top_experts(const float *logit, int E, int top_k,
   return rank;
 }
 
-// A workgroup per token: 8 tokens, 16 experts, H 2048 5.9 us (with 8 waves 8.4). A single token's
-// gate_up routes for itself instead, in every workgroup: 28.2 us a call against 30.2 (32 experts,
-// H 4096: 38 against 43); for 2 and 4 tokens that is dearer, 41 and 54 us against 35 and 46.
+// A workgroup per token: 8 tokens, 16 experts, H 2048 5.9 us (with 8 waves 8.4). Not for a single
+// token, whose gate_up routes for itself (fp4_routes_inside).
 constexpr int ROUTE_WAVES = 16;
 template <typename XT, typename RT>
 __global__ __launch_bounds__(ROUTE_WAVES * 64) void fp4_route_kernel(const XT *__restrict__ x,
@@ -702,7 +701,7 @@ size_t fp4_moe_part_bytes(uint32_t T, uint32_t H, uint32_t I, uint32_t E, uint32
 }
 
 hipError_t launch_fp4_moe(const Fp4Moe &p, int cus, hipStream_t stream) {
-  const bool fused = p.router && p.T == 1 && p.E <= 32;
+  const bool fused = p.router && fp4_routes_inside(p.T);
   if (p.router && !fused) {
     const hipError_t e = p.xt_bf16 ? route_go<uint16_t>(p, stream) : route_go<float>(p, stream);
     if (e != hipSuccess) return e;

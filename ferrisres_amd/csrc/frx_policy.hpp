@@ -339,6 +339,14 @@ struct Fp4FewPlan {
   int steps, tiles, slices, per;
 };
 
+// Whether every workgroup of gate and up finds the routes for itself, a launch less but the router read
+// by each of them: for one token. us a call, inside / in a launch of its own, H / I, experts: bf16 1024 / 352, 8
+// 18.1 / 19.4, 2048 / 5632, 16 27.6 / 29.7, 4096 / 1408, 32 27.3 / 31.7, of 64 experts 2048 / 1408 26.2 / 28.0,
+// 4096 / 1408 33.8 / 41.7, 8192 / 704 46.5 / 58.6, f32 29.6 / 32.1, 43.0 / 44.7, 66.8 / 66.4; the other way round
+// only where 64 experts meet little else (1024 / 352, 8 chosen, 29.4 / 28.1). For 2 and 4 tokens (16 experts,
+// 2048 / 5632) it is dearer, 41 and 54 against 35 and 46.
+constexpr bool fp4_routes_inside(uint32_t T) { return T == 1; }
+
 // Column tiles that hold half again as many tokens as an expert would have were they spread
 // evenly; a fuller expert's weights are read twice.
 inline int fp4_few_tiles(uint32_t T, uint32_t E, uint32_t top_k, int planes) {
