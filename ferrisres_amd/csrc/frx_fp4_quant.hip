@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void fp4_cols_kernel(const XT *__restrict__ x,
                                                        uint8_t *__restrict__ q, size_t ldq,
                                                        uint32_t *__restrict__ scale) {
   __shared__ __align__(16) uint32_t st[128 * 16];
-  __shared__ uint8_t sc[128 * 4];
+  __shared__ uint32_t sc[128];  // a column's scales, a byte from each wave
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 4, c = lane & 15;
   const uint32_t kb = (K + 127) / 128, mb = (M + 127) / 128;
   const uint32_t mt = blockIdx.x / kb, kt = blockIdx.x - mt * kb;
@@ -73,13 +73,13 @@ __global__ __launch_bounds__(256) void fp4_cols_kernel(const XT *__restrict__ x,
     mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
     mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
     const uint32_t b = fp4_scale(mx);
-    if (h == 0) sc[(8 * c + j) * 4 + wave] = (uint8_t)b;
+    if (h == 0) reinterpret_cast<uint8_t *>(sc)[(8 * c + j) * 4 + wave] = (uint8_t)b;
     st[(8 * c + j) * 16 + ((4 * wave + h) ^ c)] = fp4_pack8(v[j], fp4_inverse(b), b);
   }
   __syncthreads();
   const uint32_t r0 = kt * 128, bytes = fp4_row_bytes(M);
   if (threadIdx.x < 128 && r0 + threadIdx.x < K)
-    scale[(size_t)(r0 + threadIdx.x) * mb + mt] = *reinterpret_cast<const uint32_t *>(&sc[threadIdx.x * 4]);
+    scale[(size_t)(r0 + threadIdx.x) * mb + mt] = sc[threadIdx.x];
 #pragma unroll
   for (int i = 0; i < 2; i++) {
     const uint32_t r = (threadIdx.x >> 2) + 64 * i, p = threadIdx.x & 3, z = r >> 3;
