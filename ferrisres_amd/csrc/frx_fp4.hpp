@@ -36,7 +36,7 @@ __device__ __forceinline__ void fp4_mul(f32x4 &acc, const u32x4 &w, uint32_t sw,
   acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 4, S, (int)sw, S, (int)sx);
 }
 
-// ---- gate and up -------------------------------------------------------------------
+// ---- stores of y, and a barrier ----------------------------------------------------
 
 // Four sums of a row of y, from d on (any element), of which `left` are the row's. One store at
 // any address: with an odd N single values cost 2048 x 4096 x 11010 94 us instead of 71.
