@@ -183,6 +183,22 @@ def test_every_bit(ctx, T, H, I, E, top_k, xt, yt):
     assert torch.equal(y.cpu(), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("xt", ["bf16", "f32"])
+@pytest.mark.parametrize("T,H,I,E,top_k", LAYERS)
+def test_a_bf16_y_is_the_f32_one_rounded(ctx, T, H, I, E, top_k, xt):
+    """Any values: whatever the sums round, y is rounded once more."""
+    rng = np.random.default_rng(T + H)
+    w = [layer(rng.integers(0, 16, (E, n, k)).astype(np.uint8), rng.integers(119, 123, (E, n, k // 32)).astype(np.uint8))
+         for n, k in ((I, H), (I, H), (H, I))]
+    x = torch.from_numpy(rng.standard_normal((T, H)).astype(np.float32)).to(DT[xt]).to(DEV)
+    idx, wt = torch.from_numpy(distinct(rng, T, E, top_k)).to(DEV), torch.from_numpy(rng.random((T, top_k), np.float32)).to(DEV)
+    y, z = torch.zeros((T, H), device=DEV), torch.zeros((T, H), dtype=torch.bfloat16, device=DEV)
+    ctx.fp4_moe_ffn(x, None, *on_dev(w), y, idx, wt)
+    ctx.fp4_moe_ffn(x, None, *on_dev(w), z, idx, wt)
+    assert torch.equal(z, y.bfloat16()) and y.any()
+
+
 # ---- either end of the range ----------------------------------------------------------
 
 
