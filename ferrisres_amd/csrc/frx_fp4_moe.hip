@@ -25,10 +25,10 @@
 // h keeps the 24 bits of an f32 number whatever y is: two planes (2^-17 of h) saved a bf16 layer 0.4 us of
 // 65 at 8 tokens, 3 of 93 at 64 and 8 of 109 at 64 of 32 experts, and flipped last bits of its outputs.
 //
-// 16 experts, top 2, H 2048, I 5632, route + gate and up + down + join, us: 1 token bf16 14.6 + 9.4
+// 16 experts, top 2, H 2048, I 5632, route + gate and up + down + join, us: 1 token bf16 14.5 + 9.6
 // + 5.0 (its weights' bytes 7.1 at a copy's rate; a workgroup's way to its first tile is 5 to 6,
-// much of it instructions that are fetched for the first time), 8 tokens 6.0 + 31.4 + 20.2 + 4.6
-// (37; the weights at 4.1 TB/s), 61 tokens f32 77.3 + 41.7 + 5.0 (57; of the
+// much of it instructions that are fetched for the first time), 8 tokens 6.0 + 31.9 + 20.5 + 4.7
+// (37; gate's and up's weights at 4.0 TB/s, down's at 3.0), 61 tokens f32 78.9 + 42.0 + 5.0 (57; of the
 // first 46 are the weights' way alone, 10 the products, 17 a tile's sums, activation and stores). Waits that
 // leave out a wave's own stores gained nothing, nor did sums by lanes of eight.
 #include "frx_fp4.hpp"
